@@ -13,7 +13,7 @@ from typing import Optional
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("EP_HIP_LIB") or os.path.join(_HERE, "libep_hip.so")   # EP_HIP_LIB: A/B builds only
 
-EP_ABI_VERSION = 26        # include/ep_hip.h EP_ABI_VERSION the ctypes structs below are written for (checked in load())
+EP_ABI_VERSION = 27        # include/ep_hip.h EP_ABI_VERSION the ctypes structs below are written for (checked in load())
 EP_DTYPE_F32 = 0
 EP_DTYPE_BF16 = 1
 EP_DTYPE_F16 = 2          # fp16-stored tokens: forward entry points of the EP head only (ABI v24)
@@ -292,6 +292,21 @@ class EPCbamStep(C.Structure):
     _fields_ = [("dims", EPCbamDims)] + list(EPAimStep._fields_[1:])
 
 
+class EPMx4Tokens(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("codes_bstride", C.c_int64), ("scales_bstride", C.c_int64),
+                ("lengths", C.c_void_p), ("image_index", C.c_void_p), ("M", C.c_int64),
+                ("B", C.c_int32), ("N", C.c_int32), ("D", C.c_int32)]
+
+
+class EPDistillArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int32), ("ldl", C.c_int64),
+                ("B", C.c_int32), ("C", C.c_int32), ("K", C.c_int32), ("R", C.c_int64),
+                ("teacher_values", C.c_void_p), ("ldv", C.c_int64), ("teacher_index", C.c_void_p), ("ldi", C.c_int64),
+                ("teacher_tail", C.c_void_p), ("teacher_rows", C.c_void_p), ("targets", C.c_void_p),
+                ("temperature", C.c_float), ("alpha", C.c_float), ("grad_scale", C.c_float),
+                ("grad_scale_dev", C.c_void_p), ("loss_rows", C.c_void_p), ("dlogits", C.c_void_p), ("ldd", C.c_int64)]
+
+
 class EPDinovitDims(C.Structure):
     _fields_ = [("B", C.c_int32), ("N", C.c_int32), ("D", C.c_int32), ("H", C.c_int32), ("hidden", C.c_int32), ("C", C.c_int32),
                 ("ln_eps", C.c_float)]
@@ -327,6 +342,15 @@ SIGNATURES = {
                                  c_f32p, c_f32p, c_int, c_void, c_size, c_void]),
     "ep_pool_backward_per_image": (c_int, [c_void, c_int, c_i64, c_void, c_int, c_int, c_int, c_int, c_float, c_f32p, c_f32p,
                                            c_f32p, c_f32p, c_void]),
+    "ep_mx4_quantize": (c_int, [c_void, c_int, c_i64, c_i64, c_int, c_int, c_int, c_void, c_void, c_i64, c_i64, c_void]),
+    "ep_mx4_dequantize": (c_int, [C.POINTER(EPMx4Tokens), c_void, c_int, c_void]),
+    "ep_mx4_pool_workspace_bytes": (c_size, [c_int, c_int, c_int, c_int]),
+    "ep_mx4_pool_forward": (c_int, [C.POINTER(EPMx4Tokens), c_f32p, c_i64, c_int, c_float, c_f32p, c_f32p, c_f32p, c_void, c_size,
+                                    c_void]),
+    "ep_mx4_pool_backward": (c_int, [C.POINTER(EPMx4Tokens), c_int, c_float, c_f32p, c_f32p, c_f32p, c_f32p, c_f32p, c_int, c_int,
+                                     c_void, c_size, c_void]),
+    "ep_distill_workspace_bytes": (c_size, [c_int, c_int, c_int]),
+    "ep_distill_topk": (c_int, [C.POINTER(EPDistillArgs), c_void, c_size, c_void]),
     "ep_attention_from_scores": (c_int, [c_f32p, c_f32p, c_int, c_int, c_int, c_f32p, c_void]),
     "ep_project_forward": (c_int, [c_f32p, c_f32p, c_int, c_int, c_int, c_int, c_f32p, c_void]),
     "ep_project_backward": (c_int, [c_f32p, c_f32p, c_f32p, c_f32p, c_int, c_int, c_int, c_int, c_f32p,

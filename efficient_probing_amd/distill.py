@@ -1,0 +1,136 @@
+"""Distillation from a teacher's stored top logits: the loss beside ``functional.cross_entropy`` for a probe that learns from a
+fine-tuned or larger model's K best logits per image instead of (or beside) the labels.
+
+    loss_rows, dlogits = topk_distillation(logits, teacher_values, teacher_index, targets, temperature=2.0, alpha=0.5)
+    loss = distillation_loss(logits, teacher_values, teacher_index, ...)          # mean over rows, differentiable in logits
+
+Per row, with y = logits / T and p = softmax of the teacher's listed logits / T (and, with ``teacher_tail``, of the mass of all
+classes it does not list, as one more outcome on both sides):
+
+    loss = alpha T^2 sum_k p_k (log p_k - log softmax(y)_k)  +  (1 - alpha) cross_entropy(logits, target)
+
+The reference trains on labels alone (main_linprobe.py:589); there is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import _native as N
+from . import functional as F_
+
+MAX_K = 1024
+MAX_CLASSES = 1 << 20
+_DT = {torch.float32: N.EP_DTYPE_F32, torch.bfloat16: N.EP_DTYPE_BF16, torch.float16: N.EP_DTYPE_F16}
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows with contiguous elements that do not overlap, as the kernels read them."""
+    return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def _call(lg, val, idx, tail, rows, tgt, temperature, alpha, grad_scale, grad_scale_dev, grad) -> torch.Tensor:
+    B, C_ = lg.shape
+    R, K = val.shape
+    loss = torch.empty((B,), device=lg.device, dtype=torch.float32)
+    lib = N.load()
+    ws = torch.empty(lib.ep_distill_workspace_bytes(B, C_, K), device=lg.device, dtype=torch.uint8)
+    args = N.EPDistillArgs(logits=lg.data_ptr(), dtype=_DT[lg.dtype], ldl=lg.stride(0), B=B, C=C_, K=K, R=R, teacher_values=val.data_ptr(),
+                           ldv=val.stride(0), teacher_index=idx.data_ptr(), ldi=idx.stride(0), teacher_tail=F_._ptr(tail),
+                           teacher_rows=F_._ptr(rows), targets=F_._ptr(tgt), temperature=temperature, alpha=alpha, grad_scale=grad_scale,
+                           grad_scale_dev=F_._ptr(grad_scale_dev), loss_rows=loss.data_ptr(), dlogits=F_._ptr(grad), ldd=C_)
+    with torch.cuda.device(lg.device):
+        N.check(lib.ep_distill_topk(C.byref(args), ws.data_ptr(), ws.numel(), N.current_stream_ptr(lg.device)), "ep_distill_topk")
+    return loss
+
+
+def _checked(logits, teacher_values, teacher_index, targets, teacher_tail, teacher_rows, temperature, alpha):
+    """The call's arguments as the kernels read them; raises on what they do not take."""
+    N.require_gpu_tensor(logits, "logits")
+    if logits.dim() != 2 or min(logits.shape) < 1:
+        raise ValueError(f"logits must be (B, C), got {tuple(logits.shape)}")
+    if logits.dtype not in _DT:
+        raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    B, C_ = logits.shape
+    if teacher_values.dim() != 2 or teacher_values.shape != teacher_index.shape or min(teacher_values.shape) < 1:
+        raise ValueError(f"teacher_values and teacher_index must be (rows, K), got {tuple(teacher_values.shape)} and {tuple(teacher_index.shape)}")
+    R, K = teacher_values.shape
+    if K > MAX_K or C_ > MAX_CLASSES:
+        raise ValueError(f"at most {MAX_K} teacher entries and {MAX_CLASSES} classes, got {K} and {C_}")
+    if teacher_index.dtype.is_floating_point or teacher_index.dtype == torch.bool:
+        raise ValueError(f"teacher_index must hold integers, got {teacher_index.dtype}")
+    if not (temperature > 0.0 and temperature < float("inf")) or not 0.0 <= alpha <= 1.0:
+        raise ValueError(f"temperature must be positive and alpha within [0, 1], got {temperature} and {alpha}")
+    if alpha < 1.0 and targets is None:
+        raise ValueError("alpha < 1 needs targets")
+    if targets is not None and tuple(targets.shape) != (B,):
+        raise ValueError(f"targets must be ({B},), got {tuple(targets.shape)}")
+    if targets is not None and (targets.dtype.is_floating_point or targets.dtype == torch.bool):
+        raise ValueError(f"targets must hold integers, got {targets.dtype}")
+    if teacher_tail is not None and tuple(teacher_tail.shape) != (R,):
+        raise ValueError(f"teacher_tail must be ({R},), got {tuple(teacher_tail.shape)}")
+    if teacher_rows is None:
+        if R != B:
+            raise ValueError(f"{R} teacher rows for {B} logit rows: give teacher_rows")
+    elif teacher_rows.dtype != torch.int32 or tuple(teacher_rows.shape) != (B,) or not teacher_rows.is_contiguous():
+        raise ValueError(f"teacher_rows must be a contiguous int32 vector of {B}")
+    dev = logits.device
+    for t, name in ((teacher_values, "teacher_values"), (teacher_index, "teacher_index"), (teacher_tail, "teacher_tail"), (teacher_rows, "teacher_rows"),
+                    (targets, "targets")):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the logits on {dev}")
+    lg = _rows(logits.detach())
+    val = _rows(teacher_values.detach().float())
+    idx = teacher_index
+    if idx.dtype != torch.int32:
+        idx = idx.to(torch.int64).clamp(-1, MAX_CLASSES).to(torch.int32)   # (a 64-bit class beyond int32 stays out of range)
+    idx = _rows(idx)
+    tail = None if teacher_tail is None else teacher_tail.detach().float().contiguous()
+    tgt = None if targets is None else targets.to(torch.int64).contiguous()
+    return lg, val, idx, tail, teacher_rows, tgt, float(temperature), float(alpha)
+
+
+def topk_distillation(logits: torch.Tensor, teacher_values: torch.Tensor, teacher_index: torch.Tensor, targets: Optional[torch.Tensor] = None, *,
+                      teacher_tail: Optional[torch.Tensor] = None, teacher_rows: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                      alpha: float = 1.0, grad_scale: float = 1.0, need_grad: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(loss of every row (B,) fp32, d(mean loss)/dlogits * grad_scale in the logits' type, or None without ``need_grad``).
+
+    ``logits`` (B, C) fp32 / bf16 / fp16, any row stride.  ``teacher_values`` / ``teacher_index`` (R, K): the teacher's logits and their
+    classes, in any order; entries with a negative class are skipped, a class listed twice takes both entries.  ``teacher_tail``
+    (R,): log of the sum of exp(logit / temperature) over the classes not listed (-inf: none); without it the listed classes are
+    the teacher's whole distribution.  ``teacher_rows`` (B,) int32: batch row b reads row ``teacher_rows[b]`` of the tables in place
+    (a store's table and the batch's image_index); without it row b.  ``targets`` (B,) class indices for ``alpha`` < 1; a negative
+    one takes no label term.  A row whose teacher lists nothing has no distillation term.  A class, target or row out of range
+    makes that row's loss and gradient NaN."""
+    args = _checked(logits, teacher_values, teacher_index, targets, teacher_tail, teacher_rows, temperature, alpha)
+    grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype) if need_grad else None
+    return _call(*args, float(grad_scale), None, grad), grad
+
+
+class _Distillation(torch.autograd.Function):
+    """The backward pass runs the rows again with the incoming gradient as its scale: no second buffer of the logits' size is kept or
+    rescaled, and a loss scale acts before the gradient is rounded to a 16-bit type."""
+
+    @staticmethod
+    def forward(ctx, logits, values, index, targets, tail, rows, temperature, alpha):
+        args = _checked(logits, values, index, targets, tail, rows, temperature, alpha)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(*args[:6])
+            ctx.t, ctx.alpha = args[6:]
+        return _call(*args, 1.0, None, None).mean()
+
+    @staticmethod
+    def backward(ctx, g):
+        lg = ctx.saved_tensors[0]
+        grad = torch.empty(lg.shape, device=lg.device, dtype=lg.dtype)
+        _call(*ctx.saved_tensors, ctx.t, ctx.alpha, 1.0, g.float().contiguous(), grad)
+        return (grad,) + (None,) * 7
+
+
+def distillation_loss(logits: torch.Tensor, teacher_values: torch.Tensor, teacher_index: torch.Tensor, targets: Optional[torch.Tensor] = None, *,
+                      teacher_tail: Optional[torch.Tensor] = None, teacher_rows: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                      alpha: float = 1.0) -> torch.Tensor:
+    """Mean of ``topk_distillation``'s row losses, differentiable in ``logits`` (the teacher takes no gradient)."""
+    return _Distillation.apply(logits, teacher_values, teacher_index, targets, teacher_tail, teacher_rows, temperature, alpha)

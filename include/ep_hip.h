@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define EP_ABI_VERSION 26
+#define EP_ABI_VERSION 27
 
 #define EP_DTYPE_F32 0
 #define EP_DTYPE_BF16 1
@@ -1160,6 +1160,75 @@ int ep_dinovit_head_train_step(const ep_dinovit_step* step, void* ws, size_t ws_
 int ep_dinovit_head_eval_forward(const ep_dinovit_dims* dims, const void* x, int x_dtype, int64_t x_bstride, const float* params,
                                  const float* running_mean, const float* running_var, float bn_eps, float* logits, int ldl,
                                  void* ws, size_t ws_bytes, ep_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * MX4 token cache (ABI v27): tokens held in 4 bits, the OCP microscaling layout MXFP4 -- E2M1 codes in groups of 32 channels
+ * with one E8M0 scale byte per group (value = e2m1(code) * 2^(byte - 127); byte 255 = the whole group is NaN).
+ *   codes  (M, N, Dp/2)  uint8: two codes per byte, the even channel in the low nibble
+ *   scales (M, N, Dp/32) uint8
+ * with Dp = 128 * ceil(D / 128): a row is whole 128-channel blocks (64 code bytes + 4 scale bytes each), pad channels hold code 0.
+ * Rows of one image are contiguous; the image strides are explicit (bytes), so image and token ranges are views.
+ * codes: 16-byte aligned, codes_bstride a multiple of 16; scales: 4-byte aligned, scales_bstride a multiple of 4.
+ * lengths (optional, (M,) int32): image m holds lengths[m] tokens (clamped to [0, N]); the rest is masked out of the
+ * attention, whatever it holds.  image_index (optional, (B,) int32): image b of the call is cache image image_index[b], read in
+ * place; an index outside [0, M) is never read through: its pooled rows and its read-back are NaN and it takes no gradient.
+ * There is no counterpart in the reference: its token dump is float32 (reference tools/dump_tokens.py:95-98). */
+typedef struct ep_mx4_tokens {
+  const uint8_t* codes; const uint8_t* scales;
+  int64_t codes_bstride, scales_bstride;   /* bytes between two images */
+  const int32_t* lengths;                  /* (M,) or NULL */
+  const int32_t* image_index;              /* (B,) or NULL (then B <= M images 0 .. B-1) */
+  int64_t M;
+  int32_t B, N, D;
+} ep_mx4_tokens;
+
+/* x (B, N, D) fp32 / bf16 / fp16, channels contiguous, strides in elements -> codes / scales of images 0 .. B-1.
+ * A group's exponent is floor(log2(amax)) - 2, one more where amax >= 1.75 * 2^floor(log2(amax)) (the largest value then rounds
+ * into the grid instead of being cut off at 6), kept within [-125, 125]; values round to nearest, ties to the even code.  A group
+ * that holds a NaN or an infinity becomes a NaN group. */
+int ep_mx4_quantize(const void* x, int x_dtype, int64_t x_bstride, int64_t x_tstride, int B, int N, int D, uint8_t* codes,
+                    uint8_t* scales, int64_t codes_bstride, int64_t scales_bstride, ep_stream_t stream);
+/* out (B, N, D) contiguous, fp32 / bf16 (both exact) / fp16 (rounded); `lengths` is not looked at. */
+int ep_mx4_dequantize(const ep_mx4_tokens* t, void* out, int out_dtype, ep_stream_t stream);
+/* Attention pooling over the cache: ep_pool_forward / ep_pool_backward / ep_pool_backward_per_image with x = the cache's
+ * tokens.  queries (Q, D) with q_bstride 0, or (B, Q, D).  P (B, Q, D); ML (B, Q, 4) = {row max, sum exp(S - max), 0, 0};
+ * S (B, Q, N) raw scores (-inf behind an image's length), NULL where no backward pass follows.  An image without tokens has
+ * P = 0, max 0 and sum 0.  D <= 4096. */
+size_t ep_mx4_pool_workspace_bytes(int B, int N, int D, int Q);
+int ep_mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S,
+                        float* ML, void* workspace, size_t workspace_bytes, ep_stream_t stream);
+/* dq (Q, D) summed over the batch in a fixed order, or, with per_image != 0, (B, Q, D).  delta = dP . P per row is computed from
+ * P, or read from ML[..][2] where P is NULL (ep_project_backward leaves it there).  accumulate adds to dq. */
+int ep_mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S, const float* ML, const float* P,
+                         const float* dP, float* dq, int per_image, int accumulate, void* workspace, size_t workspace_bytes,
+                         ep_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Distillation from a teacher's top logits (ABI v27), beside ep_cross_entropy.  Per row b of `logits` (B, C):
+ *   t = {teacher_values[r, k] / T} for teacher_index[r, k] >= 0, and teacher_tail[r] where given (the log of the sum of
+ *   exp(logit / T) over the classes the teacher does not list);   p = softmax(t);   y = logits / T
+ *   log q_k = y[idx_k] - logsumexp(y),   log q_tail = logsumexp(y over the classes not listed) - logsumexp(y)
+ *   loss_rows[b] = alpha * T^2 * sum p (log p - log q)  +  (1 - alpha) * (logsumexp(logits) - logits[target])
+ *   dlogits[b, :] = grad_scale / B * d loss_rows[b] / d logits[b, :]      (grad_scale times *grad_scale_dev where given)
+ * with r = teacher_rows[b] (int32, into a table of R rows read in place), or b.  A class listed more than once takes the sum of
+ * its entries; entries with a negative index are skipped; a row without any entry has no distillation term.  targets may be NULL
+ * when alpha == 1; a negative target takes no label term.  A row index, class or target out of range makes the row's loss and gradient
+ * NaN and is never read through.  K <= 1024.  dlogits (same type and row stride rules as logits) may be NULL. */
+typedef struct ep_distill_args {
+  const void* logits; int32_t dtype; int64_t ldl;       /* fp32 / bf16 / fp16; row stride in elements, >= C */
+  int32_t B, C, K; int64_t R;                           /* R: rows of the teacher's tables */
+  const float* teacher_values; int64_t ldv;             /* (R, K), row stride */
+  const int32_t* teacher_index; int64_t ldi;            /* (R, K), row stride */
+  const float* teacher_tail;                            /* (R,) or NULL */
+  const int32_t* teacher_rows;                          /* (B,) or NULL (then R >= B) */
+  const int64_t* targets;                               /* (B,) or NULL */
+  float temperature, alpha, grad_scale;
+  const float* grad_scale_dev;                          /* one float on the device that grad_scale is multiplied by, or NULL */
+  float* loss_rows;                                     /* (B,) */
+  void* dlogits; int64_t ldd;
+} ep_distill_args;
+size_t ep_distill_workspace_bytes(int B, int C, int K);
+int ep_distill_topk(const ep_distill_args* args, void* workspace, size_t workspace_bytes, ep_stream_t stream);
 
 #ifdef __cplusplus
 }

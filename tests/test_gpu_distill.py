@@ -1,0 +1,225 @@
+"""Distillation from a teacher's top logits against the float64 oracle.
+
+Tolerances (u = 2^-24): an exponential is off by a few u plus u times its argument's size (at most about 40 for a term that
+still counts next to the maximum, and the division by T), a sum by a few u: relative errors of r = 64 u cover every probability.
+Loss: a sum of p (log p - log q) whose logarithms carry r + u |log|.  Gradient: r on each probability, then one rounding to the
+logits' type (half a step, eps / 2 relative; for fp16 also half of the smallest subnormal)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import distill_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+R_ = 64 * U
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
+
+
+def _teacher(R, C, K, seed):
+    rng = np.random.default_rng(seed)
+    idx = np.stack([rng.permutation(C)[:K] for _ in range(R)]).astype(np.int32) if C < 100000 else \
+        np.stack([(rng.integers(C) + (C // K) * rng.permutation(K)) % C for _ in range(R)]).astype(np.int32)
+    return (6 + 3 * rng.standard_normal((R, K))).astype(np.float32), idx, (4 + rng.standard_normal(R)).astype(np.float32)
+
+
+def _check(z, val, idx, tgt=None, tail=None, rows=None, T=1.0, alpha=1.0, gs=1.0):
+    from efficient_probing_amd import distill
+    B, C = z.shape
+    dev = lambda a, dt=None: None if a is None else torch.as_tensor(a, device=DEV) if dt is None else torch.as_tensor(a, device=DEV).to(dt)
+    pick = np.arange(B) if rows is None else np.asarray(rows)
+    zf = z.double().cpu().numpy()
+    want, g = O.distill(zf, val[pick], idx[pick], tgt, None if tail is None else tail[pick], T, alpha)
+    args = dict(targets=dev(tgt), teacher_tail=dev(tail), teacher_rows=dev(rows, torch.int32), temperature=T, alpha=alpha)
+    loss, grad = distill.topk_distillation(z, dev(val), dev(idx), args.pop("targets"), grad_scale=gs, **args)
+    only, none = distill.topk_distillation(z, dev(val), dev(idx), dev(tgt), need_grad=False, **args)
+    assert none is None and torch.equal(only.nan_to_num(7.0), loss.nan_to_num(7.0)) and grad.dtype == z.dtype and grad.shape == z.shape
+    got = loss.double().cpu().numpy()
+    spread = np.nanmax(np.where(np.isfinite(zf), np.abs(zf), 0.0)) / min(T, 1.0) + np.abs(val[idx >= 0]).max(initial=0.0) / T + 20
+    fin = np.isfinite(want)
+    assert np.array_equal(np.isfinite(got), fin) and np.array_equal(got[~fin], want[~fin], equal_nan=True)
+    assert (np.abs(got - want)[fin] <= (1 + alpha * T * T) * (R_ + 4 * U * spread) * 2).all(), np.abs(got - want)[fin].max()
+    scale = gs / B
+    gg = grad.double().cpu().numpy()
+    err = np.abs(gg - g * scale)
+    parts = alpha * T * (1.0 if tail is None else 2.0) + 1.0        # sizes of the probabilities that a component is a difference of
+    lim = scale * parts * (R_ + 4 * U * spread) * np.maximum(np.abs(g).max(), 1e-3) + np.abs(g * scale) * torch.finfo(z.dtype).eps / 2 + TINY[z.dtype]
+    ok = np.isfinite(g)
+    assert np.array_equal(np.isfinite(gg), ok)
+    assert (err <= lim)[ok].all(), float((err / lim)[ok].max())
+    return loss, grad
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,C,K", [(1, 1, 1), (3, 2, 1), (5, 10, 10), (7, 63, 5), (4, 257, 64), (33, 1000, 32), (9, 1003, 8), (3, 4099, 100), (2, 21841, 64),
+                                   (1, 65537, 256), (2, 131071, 1024), (300, 100, 7)])
+@pytest.mark.parametrize("mode", ["soft", "soft+label", "tail", "tail+label"])
+def test_against_float64(B, C, K, dtype, mode):
+    rng = np.random.default_rng(B + C)
+    z = (2 * torch.randn(B, C, generator=torch.Generator().manual_seed(C))).to(dtype).to(DEV)
+    val, idx, tail = _teacher(B, C, K, C + K)
+    if K == C:
+        tail[:] = -np.inf                                          # no class is left for the tail
+    label = "label" in mode
+    _check(z, val, idx, rng.integers(0, C, B) if label else None, tail if "tail" in mode else None, T=2.0 if label else 1.0, alpha=0.4 if label else 1.0)
+
+
+@pytest.mark.parametrize("T", [0.25, 3.0, 10.0])
+@pytest.mark.parametrize("alpha", [0.0, 0.7, 1.0])
+def test_temperatures_and_rows_of_a_table(T, alpha):
+    B, C, K, R = 12, 1000, 16, 40
+    z = torch.randn(B, C, generator=torch.Generator().manual_seed(3)).to(DEV) * 3
+    val, idx, tail = _teacher(R, C, K, 5)
+    rng = np.random.default_rng(1)
+    rows = rng.integers(0, R, B)
+    rows[3] = rows[4]
+    _check(z, val, idx, rng.integers(0, C, B), tail / T, rows, T, alpha, gs=128.0)
+    _check(z, val, idx, rng.integers(0, C, B), None, rows, T, alpha)
+
+
+@pytest.mark.parametrize("tail_on", [False, True])
+@pytest.mark.parametrize("C", [40, 5000])
+def test_repeated_and_skipped_entries(C, tail_on):
+    """A class listed two, three and K times, skipped entries between, a row that lists nothing, labels among the listed classes,
+    labels that are ignored."""
+    B, K = 8, 12
+    z = torch.randn(B, C, generator=torch.Generator().manual_seed(3)).to(DEV) * 2
+    val, idx, tail = _teacher(B, C, K, 2)
+    idx[1, 5] = idx[1, 2]
+    idx[2, [0, 4, 11]] = idx[2, 7]
+    idx[3, :] = idx[3, 0]
+    idx[4, ::2] = -1
+    idx[5, :] = -1
+    idx[6, :] = -5
+    tail[6] = -np.inf
+    tgt = np.array([idx[0, 0], idx[1, 5], idx[2, 7], idx[3, 0], 3, 4, 5, -100])
+    for alpha in (1.0, 0.5):
+        loss, grad = _check(z, val, idx, tgt if alpha < 1 else None, tail if tail_on else None, T=2.0, alpha=alpha)
+        if alpha == 1.0:
+            assert float(loss[6]) == 0 and bool((grad[6] == 0).all())
+            if not tail_on:
+                assert float(loss[5]) == 0 and bool((grad[5] == 0).all())
+        for _ in range(3):
+            l2, g2 = _check(z, val, idx, tgt if alpha < 1 else None, tail if tail_on else None, T=2.0, alpha=alpha)
+            assert torch.equal(loss, l2) and torch.equal(grad, g2)
+
+
+def test_masked_and_extreme_logits():
+    """Classes masked by -inf or the type's lowest value, a row far from zero, a student that gives the teacher's class no mass, a
+    teacher of -inf entries."""
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        B, C, K = 6, 300, 5
+        z = torch.randn(B, C, generator=torch.Generator().manual_seed(3)).to(dtype).to(DEV)
+        val, idx, tail = _teacher(B, C, K, 2)
+        rng = np.random.default_rng(0)
+        for b in range(B):
+            free = np.setdiff1d(np.arange(C), idx[b])
+            z[b, torch.as_tensor(rng.choice(free, 100, False), device=DEV)] = -float("inf") if b % 2 else torch.finfo(dtype).min
+        z[2] += 1000.0 if dtype == torch.float32 else 64.0
+        val[3, :2] = -np.inf
+        z[3, int(idx[3, 0])] = -float("inf")                      # the teacher gives it nothing either
+        tgt = np.array([int(idx[b, 2]) for b in range(B)])
+        _check(z, val, idx, tgt, None, T=1.0, alpha=0.5)
+        _check(z, val, idx, tgt, tail, T=2.0, alpha=0.5)
+    z = torch.randn(2, 50, device=DEV)
+    val, idx, _ = _teacher(2, 50, 4, 2)
+    z[1, int(idx[1, 0])] = -float("inf")                          # the teacher gives it mass: an infinite loss, in its row
+    from efficient_probing_amd import distill
+    loss, grad = distill.topk_distillation(z, torch.as_tensor(val, device=DEV), torch.as_tensor(idx, device=DEV))
+    assert torch.isinf(loss[1]) and torch.isfinite(loss[0]) and bool(torch.isfinite(grad).all())
+
+
+def test_out_of_range_is_not_read():
+    from efficient_probing_amd import distill
+    z = torch.randn(6, 50, device=DEV)
+    val, idx, _ = _teacher(6, 50, 4, 2)
+    clean, cg = distill.topk_distillation(z, torch.as_tensor(val, device=DEV), torch.as_tensor(idx, device=DEV))
+    idx[1, 3] = 50
+    idx[2, 0] = 2 ** 31 - 1
+    tgt = torch.tensor([1, 1, 1, 50, 2 ** 40, -2 ** 40], device=DEV)
+    loss, grad = distill.topk_distillation(z, torch.as_tensor(val, device=DEV), torch.as_tensor(idx, device=DEV), tgt, alpha=0.5)
+    assert torch.isnan(loss).tolist() == [False, True, True, True, True, False]
+    assert torch.isnan(grad).all(1).tolist() == torch.isnan(grad).any(1).tolist() == torch.isnan(loss).tolist()
+    wide = torch.as_tensor(idx, device=DEV).long()
+    wide[4, 1] = 2 ** 40
+    loss, _ = distill.topk_distillation(z, torch.as_tensor(val, device=DEV), wide)
+    assert torch.isnan(loss).tolist() == [False, True, True, False, True, False]
+    assert torch.equal(loss[[0, 3, 5]], clean[[0, 3, 5]])
+    rows = torch.tensor([0, 6, -1, 3, 2 ** 31 - 1, 5], dtype=torch.int32, device=DEV)
+    loss, grad = distill.topk_distillation(z, torch.as_tensor(val, device=DEV), torch.as_tensor(idx, device=DEV), teacher_rows=rows)
+    assert torch.isnan(loss).tolist() == [False, True, True, False, True, False]
+    assert torch.equal(loss[[0, 3, 5]], clean[[0, 3, 5]]) and torch.equal(grad[[0, 3, 5]], cg[[0, 3, 5]])
+
+
+def test_strides_types_and_streams():
+    from efficient_probing_amd import distill
+    big = torch.randn(9, 4003, device=DEV)
+    val, idx, tail = _teacher(9, 1000, 8, 2)
+    v, i, t = (torch.as_tensor(a, device=DEV) for a in (val, idx, tail))
+    for z in (big[:, :1000], big[:, 3:1003], big[:, ::4][:, :1000], big.t()[:1000].t(), big[:1, :1000].expand(9, 1000)):
+        a = distill.topk_distillation(z, v, i, teacher_tail=t)
+        b = distill.topk_distillation(z.contiguous(), v, i, teacher_tail=t)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    vv, ii = torch.zeros(9, 20, device=DEV), torch.zeros(9, 20, device=DEV, dtype=torch.int16)
+    vv[:, 2:10], ii[:, 2:10] = v, i.to(torch.int16)
+    a = distill.topk_distillation(big[:, :1000], vv[:, 2:10], ii[:, 2:10], teacher_tail=t)
+    b = distill.topk_distillation(big[:, :1000], v, i, teacher_tail=t)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c = distill.topk_distillation(big[:, :1000], v, i, teacher_tail=t)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(c[0], b[0]) and torch.equal(c[1], b[1])
+
+
+def test_autograd_and_graphs():
+    from efficient_probing_amd import distill
+    B, C = 16, 1000
+    val, idx, tail = _teacher(B, C, 8, 2)
+    v, i, t = (torch.as_tensor(a, device=DEV) for a in (val, idx, tail))
+    y = torch.randint(0, C, (B,), device=DEV)
+    z0 = torch.randn(B, C, device=DEV)
+    z = z0.clone().requires_grad_(True)
+    loss = distill.distillation_loss(z, v, i, y, teacher_tail=t, temperature=2.0, alpha=0.3)
+    (3.0 * loss).backward()
+    rows, grad = distill.topk_distillation(z0, v, i, y, teacher_tail=t, temperature=2.0, alpha=0.3, grad_scale=3.0)
+    torch.testing.assert_close(loss.detach(), rows.mean(), rtol=1e-6, atol=1e-6)
+    torch.testing.assert_close(z.grad, grad, rtol=1e-6, atol=1e-9)
+    # a loss scale acts before the gradient is rounded to fp16
+    h = (z0 * 0.1).half().requires_grad_(True)
+    (65536.0 * distill.distillation_loss(h, v, i)).backward()
+    f = h.detach().float().requires_grad_(True)
+    (65536.0 * distill.distillation_loss(f, v, i)).backward()
+    assert float((h.grad.float() - f.grad).abs().max()) <= 2.0 ** -11 * float(f.grad.abs().max())
+    zs = z0.clone()
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = distill.topk_distillation(zs, v, i, y, teacher_tail=t, alpha=0.3)
+        graphs.append((gr, out))
+    for k in range(4):
+        zs.copy_(z0 * (1 + k))
+        want = distill.topk_distillation(zs, v, i, y, teacher_tail=t, alpha=0.3)
+        for gr, _ in graphs:
+            gr.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("bad", [
+    dict(logits=(2, 3, 4)), dict(logits=(3, 50)), dict(values=(2, 5)), dict(K=1025), dict(T=0.0), dict(T=float("inf")), dict(alpha=1.5), dict(alpha=0.5),
+    dict(index=torch.float32), dict(tail=3), dict(rows=torch.int64), dict(targets=3), dict(logits_type=torch.float64)])
+def test_refusals(bad):
+    from efficient_probing_amd import distill
+    K = bad.get("K", 4)
+    z = torch.zeros(bad.get("logits", (2, 50)), device=DEV, dtype=bad.get("logits_type", torch.float32))
+    with pytest.raises(ValueError):
+        distill.topk_distillation(z, torch.zeros(bad.get("values", (2, K)), device=DEV), torch.zeros(2, K, device=DEV, dtype=bad.get("index", torch.int32)),
+                                  torch.zeros(bad["targets"], device=DEV, dtype=torch.int64) if "targets" in bad else None,
+                                  teacher_tail=torch.zeros(bad["tail"], device=DEV) if "tail" in bad else None,
+                                  teacher_rows=torch.zeros(2, device=DEV, dtype=bad["rows"]) if "rows" in bad else None,
+                                  temperature=bad.get("T", 1.0), alpha=bad.get("alpha", 1.0))
