@@ -1,133 +1,840 @@
-// Attention pooling over the MX4 token cache, forward and backward (S = scale q.x, A = softmax over the image's tokens, P = A x;
-// dA = dP.x, dS = A (dA - delta), dq = scale sum dS x), x the decoded tokens.
+// Attention pooling over the MX4 token cache, forward and backward (x: the decoded tokens):
+//     S = scale q.x     A = softmax over the image's tokens     P = A x
+//     dA = dP.x         dS = A (dA - dP.P)                       dq = scale sum dS x
 //
-// Plain form: one workgroup per (image, query) row, a wave per token for the dot products, a lane per eight channels for the sums.
+// ONE kernel for both passes: they are the same two contractions with a per-token weight between them.  Every byte of the cache is
+// read once per pass.  A wave owns CPW 128-channel blocks of the row for all tokens and queries (a D-slice); a tile is 32 tokens.
+//
+//   * Tiles come HBM -> LDS by LDS-DMA into a ring of NST stages that the wave keeps to itself (no barrier on the data path).
+//   * First contraction (scores / dA), on the matrix cores in the cache's own format: v_mfma_scale_f32_16x16x128_f8f6f4 takes the
+//     E2M1 codes and their E8M0 scale bytes as they lie in LDS, no decoding.  The fp32 operand (queries, dP) becomes six E2M3
+//     terms with block scales 2^-4 apart: what is left over is below 2^-22 of a block's largest value.  All products are exact,
+//     the sums fp32.
+//   * D-slices are added through LDS, one record per wave and tile, in wave order, one barrier per tile; every wave then holds the
+//     scores in the very lanes in which the second contraction wants its weights.
+//   * Weights (exp(S - max), or dS) are split into three bf16 terms, exactly.
+//   * Second contraction: codes are decoded to bf16 (exact; v_cvt_scalef32_pk_bf16_fp4 applies the token's own scale, which is why
+//     this side cannot stay in 4 bits: the contraction runs over tokens and every token has its own scale), transposed between
+//     token pairs by v_perm, v_mfma_f32_16x16x32_bf16.
+//
+// QM 8: up to 8 queries, rows of a 16-row matrix instruction = 8 queries x 2 terms.  QM 16 / 32: one / two blocks of 16 queries.
 #include "ep_mx4.h"
+#include "ep_mx4_pool.h"
 
 namespace ep {
 
-constexpr int MXP_WAVES = 4;
+typedef int mx_i8 __attribute__((ext_vector_type(8)));
+typedef uint32_t mx_u6 __attribute__((ext_vector_type(6)));
+typedef uint32_t mx_u4 __attribute__((ext_vector_type(4)));
+typedef float mx_f16 __attribute__((ext_vector_type(16)));
+typedef float mx_f32 __attribute__((ext_vector_type(32)));
+typedef __bf16 mx_bf8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* mx_lds_t;
+typedef const __attribute__((address_space(1))) void* mx_gptr_t;
 
-struct MxPool {
-  ep_mx4_tokens t;
-  const float* q; int64_t qb;      // forward: queries; backward: dP (B, Q, D)
-  int Q; float scale;
-  float* P; float* S; float* ML;   // forward outputs (S: never null here)
-  const float* Pin;                // backward: P, or null (delta from ML)
-  float* dS;                       // backward scratch (B, Q, N)
-  float* dq;                       // backward: (B, Q, D) per-image gradients
+constexpr float MX_LOG2E = 1.4426950408889634f;
+constexpr int MX_NT = 2;                         // cache policy of the code loads: streamed once
+constexpr float MX_LAZY = 12.0f;                 // the running maximum follows a score only when it lies this far above it
+
+template <int QM> struct MxDims {
+  static constexpr int NQB = QM == 32 ? 2 : 1;   // blocks of query rows
+  static constexpr int ROWS = QM == 8 ? 8 : 16;  // queries of a block
+  static constexpr int SETS = QM == 8 ? 3 : 6;   // matrix operands of the fp32 rows: six terms, two of them in one operand at QM 8
+  static constexpr int SCB = QM == 8 ? 1 : 2;    // dwords of their scale bytes
+  static constexpr int SV = QM == 8 ? 4 : 8;     // scores per lane, tile and query block
+  static constexpr int PSETS = QM == 8 ? 2 : 3;  // operands of the weights
+  static constexpr int REC = 64 * 4 * SV * NQB;  // bytes of an exchange record
 };
 
-// out[n] = scale * row . x[n] for the image's tokens (waves stride over them)
-__device__ __forceinline__ void mx_dots(const ep_mx4_tokens& t, const uint8_t* codes, const uint8_t* scales, int len, const float* row, float scale,
-                                        float* out) {
-  const int words = (t.D + MX_BLOCK - 1) / MX_BLOCK * 16;
-  const int lane = lane_id(), w = (int)(threadIdx.x >> 6);
-  for (int n = w; n < len; n += MXP_WAVES) {
-    float s = 0.f;
-    for (int j = lane; 8 * j < t.D; j += 64) {
-      float v[8];
-      mx_decode8(*reinterpret_cast<const uint32_t*>(codes + ((int64_t)n * words + j) * 4),
-                 __uint_as_float((uint32_t)scales[(int64_t)n * (words / 4) + j / 4] << 23), v);
+template <int N>
+__device__ __forceinline__ void mx_wait_vm() {
+  static_assert(N >= 0 && N <= 63, "vmcnt");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mx_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ float mx_ror8(float v) { return dpp_f<0x128>(v); }
+__device__ __forceinline__ uint32_t mx_ror8u(uint32_t v) { return __float_as_uint(mx_ror8(__uint_as_float(v))); }
+__device__ __forceinline__ float mx_over_groups_max(float v) {       // over the four 16-lane rows
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float mx_over_groups_sum(float v) {
+  v = fold16(v, v);
+  return fold32(v, v);
+}
+__device__ __forceinline__ f4 mx_mfma(mx_u4 a, mx_u4 b, f4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf8, a), __builtin_bit_cast(mx_bf8, b), c, 0, 0, 0);
+}
+template <int BYTE>
+__device__ __forceinline__ f4 mx_mfma_codes(const mx_u4& codes, uint32_t scale, const mx_u6& row, uint32_t row_scales, f4 c) {
+  const mx_i8 a = {(int)codes[0], (int)codes[1], (int)codes[2], (int)codes[3], 0, 0, 0, 0};
+  const mx_i8 b = {(int)row[0], (int)row[1], (int)row[2], (int)row[3], (int)row[4], (int)row[5], 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4 /* E2M1 */, 2 /* E2M3 */, 0, (int)scale, BYTE, (int)row_scales);
+}
+
+// 32 consecutive fp32 values of an operand row -> six E2M3 terms; term t has scale byte s0 - 4 t.  The conversion's two sources are
+// the even and the odd values.  It and its inverse write their results before they have read all of their sources (the scale among
+// them), which the compiler does not allow for: it may place the result over a source that dies there, and the low terms then differ
+// from run to run.  So every source is kept alive behind the instruction by an empty asm.
+struct MxTerms { mx_u6 t[6]; int s0; };
+__device__ __forceinline__ void mx_terms(mx_f32 v, MxTerms& o) {
+  uint32_t am = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (8 * j + i < t.D) s += row[8 * j + i] * v[i];
+  for (int i = 0; i < 32; ++i) { const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu; am = a > am ? a : am; }
+  const int ex = (int)(am >> 23);
+  o.s0 = ex == 255 ? 255 : (ex - 2 < 24 ? 24 : ex - 2);
+  const int base = o.s0 == 255 ? 252 : o.s0;
+#pragma unroll
+  for (int t = 0; t < 6; ++t) {
+    const float sc = __uint_as_float((uint32_t)(base - 4 * t) << 23);
+    mx_f16 a, b;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { a[i] = v[2 * i]; b[i] = v[2 * i + 1]; }
+    o.t[t] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, sc);
+    asm volatile("" ::"v"(a), "v"(b), "v"(sc), "v"(o.t[t]));
+    if (t < 5) {
+      const mx_f32 d = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(o.t[t], sc);
+      asm volatile("" ::"v"(o.t[t]), "v"(sc), "v"(d));
+      v -= d;
     }
-    s = wave_sum(s);
-    if (lane == 0) out[n] = s * scale;
   }
 }
 
-__device__ __forceinline__ float mx_block_reduce(float v, bool mx, float* lds) {
-  v = mx ? wave_max(v) : wave_sum(v);
-  __syncthreads();
-  if (lane_id() == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = lds[0];
-  for (int i = 1; i < MXP_WAVES; ++i) r = mx ? fmaxf(r, lds[i]) : r + lds[i];
-  return r;
-}
+// the operand of one row block for this lane's column: queries q (QM 8: two terms share an operand, columns 8-15 take the odd ones)
+template <int QM>
+struct MxOperand { mx_u6 b[MxDims<QM>::SETS]; uint32_t sc[MxDims<QM>::SCB]; };
 
-// out[d] = sum_n f(n) x[n][d]
-template <typename F>
-__device__ __forceinline__ void mx_weighted(const ep_mx4_tokens& t, const uint8_t* codes, const uint8_t* scales, int len, F&& f, float mul, float* out) {
-  const int words = (t.D + MX_BLOCK - 1) / MX_BLOCK * 16;
-  for (int j = (int)threadIdx.x; 8 * j < t.D; j += 64 * MXP_WAVES) {
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int n = 0; n < len; ++n) {
-      float v[8];
-      mx_decode8(*reinterpret_cast<const uint32_t*>(codes + ((int64_t)n * words + j) * 4),
-                 __uint_as_float((uint32_t)scales[(int64_t)n * (words / 4) + j / 4] << 23), v);
-      const float a = f(n);
+template <int QM>
+__device__ __forceinline__ void mx_operand(const mx_f32& v, int c, MxOperand<QM>& o) {
+  MxTerms t;
+  mx_terms(v, t);
+  if constexpr (QM == 8) {
+    const bool odd = (c & 8) != 0;
+    uint32_t s = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += a * v[i];
+    for (int k = 0; k < 3; ++k) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) o.b[k][i] = odd ? t.t[2 * k + 1][i] : t.t[2 * k][i];
+      const int e = t.s0 == 255 ? 255 : t.s0 - 4 * (2 * k + (odd ? 1 : 0));
+      s |= (uint32_t)e << (8 * k);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (8 * j + i < t.D) out[8 * j + i] = acc[i] * mul;
-  }
-}
-
-__global__ __launch_bounds__(64 * MXP_WAVES) void ep_mx4_pool_fwd_kernel(MxPool p) {
-  __shared__ float red[MXP_WAVES];
-  const ep_mx4_tokens& t = p.t;
-  const int b = (int)(blockIdx.x / (unsigned)p.Q), q = (int)(blockIdx.x % (unsigned)p.Q);
-  int len;
-  const int img = mx_image(t, b, len);
-  const float bad = img < 0 ? __uint_as_float(0x7fc00000u) : 0.f;
-  const uint8_t* codes = t.codes + (int64_t)(img < 0 ? 0 : img) * t.codes_bstride;
-  const uint8_t* scales = t.scales + (int64_t)(img < 0 ? 0 : img) * t.scales_bstride;
-  const int64_t r = (int64_t)b * p.Q + q;
-  float* S = p.S + r * t.N;
-  mx_dots(t, codes, scales, len, p.q + (int64_t)b * p.qb + (int64_t)q * t.D, p.scale, S);
-  __syncthreads();
-  float m = -INFINITY;
-  for (int n = (int)threadIdx.x; n < len; n += 64 * MXP_WAVES) m = fmaxf(m, S[n]);
-  m = mx_block_reduce(m, true, red);
-  if (m == -INFINITY) m = 0.f;                                // no tokens
-  float l = 0.f;
-  for (int n = (int)threadIdx.x; n < len; n += 64 * MXP_WAVES) l += expf(S[n] - m);
-  l = mx_block_reduce(l, false, red);
-  for (int n = len + (int)threadIdx.x; n < t.N; n += 64 * MXP_WAVES) S[n] = -INFINITY;
-  if (threadIdx.x == 0) *reinterpret_cast<f4*>(p.ML + r * 4) = f4{m + bad, l + bad, 0.f, 0.f};
-  float* out = p.P + r * t.D;
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  mx_weighted(t, codes, scales, len, [&](int n) { return expf(S[n] - m); }, inv + bad, out);
-}
-
-__global__ __launch_bounds__(64 * MXP_WAVES) void ep_mx4_pool_bwd_kernel(MxPool p) {
-  __shared__ float red[MXP_WAVES];
-  const ep_mx4_tokens& t = p.t;
-  const int b = (int)(blockIdx.x / (unsigned)p.Q), q = (int)(blockIdx.x % (unsigned)p.Q);
-  int len;
-  const int img = mx_image(t, b, len);
-  const uint8_t* codes = t.codes + (int64_t)(img < 0 ? 0 : img) * t.codes_bstride;
-  const uint8_t* scales = t.scales + (int64_t)(img < 0 ? 0 : img) * t.scales_bstride;
-  const int64_t r = (int64_t)b * p.Q + q;
-  const float* dP = p.q + r * t.D;
-  float delta;
-  if (p.Pin) {
-    delta = 0.f;
-    for (int d = (int)threadIdx.x; d < t.D; d += 64 * MXP_WAVES) delta += dP[d] * p.Pin[r * t.D + d];
-    delta = mx_block_reduce(delta, false, red);
+    o.sc[0] = s;
   } else {
-    delta = p.ML[r * 4 + 2];
+#pragma unroll
+    for (int k = 0; k < 6; ++k) o.b[k] = t.t[k];
+    uint32_t s[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 6; ++k) s[k / 3] |= (uint32_t)(t.s0 == 255 ? 255 : t.s0 - 4 * k) << (8 * (k % 3));
+    o.sc[0] = s[0]; o.sc[1] = s[1];
   }
-  const float m = p.ML[r * 4], l = p.ML[r * 4 + 1], inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  float* dS = p.dS + r * t.N;
-  mx_dots(t, codes, scales, len, dP, 1.f, dS);
-  __syncthreads();
-  for (int n = (int)threadIdx.x; n < len; n += 64 * MXP_WAVES) dS[n] = expf(p.S[r * t.N + n] - m) * inv * (dS[n] - delta);
-  __syncthreads();
-  mx_weighted(t, codes, scales, len, [&](int n) { return dS[n]; }, p.scale, p.dq + r * t.D);
 }
 
-__global__ __launch_bounds__(256) void ep_mx4_sum_images_kernel(const float* __restrict__ part, int B, int64_t QD, float* __restrict__ dq, int accumulate) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= QD) return;
-  float s = accumulate ? dq[i] : 0.f;
-  for (int b = 0; b < B; ++b) s += part[(int64_t)b * QD + i];
-  dq[i] = s;
+// 32 values of `row` from channel d on, times mul; 0 behind D and where `on` is false.  Addresses are clamped into the row instead of
+// branched around, so that all loads are under way together.
+__device__ __forceinline__ mx_f32 mx_load_row(const float* row, bool on, int d, int D, bool vec, float mul) {
+  mx_f32 v;
+  if (vec) {
+    f4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { const int e = d + 4 * i; x[i] = *reinterpret_cast<const f4*>(row + (e < D ? e : D - 4)); }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool ok = on && d + 4 * i < D;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * i + j] = ok ? x[i][j] * mul : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = row[d + i < D ? d + i : D - 1];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = on && d + i < D ? v[i] * mul : 0.f;
+  }
+  return v;
+}
+
+// a wave's sequence of (unit, tile): units u, u + ustep, ..., of each the tiles t_off, t_off + tstep, ...
+struct MxCursor {
+  int u, ustep, units, tile, hi, len, toff, tstep, tps, splits;
+  int b, img;
+  __device__ __forceinline__ bool valid() const { return u < units; }
+  __device__ __forceinline__ void open(const ep_mx4_tokens& t) {       // first unit from u on that has a tile
+    for (; u < units; u += ustep) {
+      b = u / splits;
+      const int s = u - b * splits;
+      img = __builtin_amdgcn_readfirstlane(mx_image(t, b, len));
+      len = __builtin_amdgcn_readfirstlane(len);
+      const int n = (len + 31) >> 5;
+      hi = (s + 1) * tps < n ? (s + 1) * tps : n;
+      tile = s * tps + toff;
+      if (tile < hi) return;
+    }
+  }
+  __device__ __forceinline__ bool next(const ep_mx4_tokens& t) {       // true: the next tile is another unit's (or there is none)
+    tile += tstep;
+    if (tile < hi) return false;
+    u += ustep;
+    open(t);
+    return true;
+  }
+};
+
+template <int QM, int CPW, int NST, bool BWD>
+__global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
+  typedef MxDims<QM> DM;
+  constexpr int NQB = DM::NQB, SV = DM::SV;
+  constexpr int CODES = 2048 * CPW, STAGE = CODES + 256 * ((CPW + 1) / 2), OPS = 2 * CPW + (CPW + 1) / 2;
+  extern __shared__ __align__(16) char lds[];
+  const int lane = lane_id(), c = lane & 15, g = lane >> 4;
+  const int wave = wave_id_uniform();
+  const int nw = p.nw, groups = p.groups;
+  const int grp = wave / nw, dw = wave - grp * nw;
+  const ep_mx4_tokens& t = p.t;
+  const int nc = p.nc, rowC = nc * 64, rowS = nc * 4;
+  const int chunk0 = dw * CPW;
+  const int q0 = (int)blockIdx.y * p.qblk, qn = p.Q - q0 < p.qblk ? p.Q - q0 : p.qblk;      // queries of this workgroup
+  char* ring = lds + wave * (NST * STAGE);
+  char* exch = lds + nw * groups * (NST * STAGE);                      // [2][groups][nw][REC]
+
+  // ---- lane constants
+  unsigned dma_tok[2], dma_seg = (unsigned)(((lane & 3) ^ g) * 16);
+  dma_tok[0] = 8 * ((lane >> 2) & 3) + g; dma_tok[1] = dma_tok[0] + 4;
+  const int sc_off = (8 * (c >> 2) + (c & 3)) * 4;                     // + 16 h: scale dword of the score row
+  const int a_off = (4 * (c & 3) + (c >> 2)) * 64 + ((g ^ (c & 3)) << 4);
+  int p_off[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p_off[i] = i * 256 + g * 64 + (((c >> 2) ^ i) << 4) + (c & 3) * 4;
+  const uint32_t rot = (uint32_t)(8 * (c >> 2) + 9);
+
+  auto issue = [&](const MxCursor& cu, int slot) {
+    char* st = ring + slot * STAGE;
+    const int t0 = cu.tile << 5, rows = cu.len - t0;                   // rows behind the image's end repeat its last one
+    const uint8_t* src = t.codes + (int64_t)cu.img * t.codes_bstride + (int64_t)t0 * rowC;
+    const uint8_t* scl = t.scales + (int64_t)cu.img * t.scales_bstride + (int64_t)t0 * rowS;
+#pragma unroll
+    for (int k = 0; k < CPW; ++k) {
+      const int ch = chunk0 + k < nc ? chunk0 + k : nc - 1;            // a slice that the row does not fill repeats its last block
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int tok = (int)dma_tok[h] < rows ? (int)dma_tok[h] : rows - 1;
+        __builtin_amdgcn_global_load_lds((mx_gptr_t)(src + (unsigned)(tok * rowC + ch * 64) + dma_seg), (mx_lds_t)(st + k * 2048 + h * 1024), 16, 0, MX_NT);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < CPW; k += 2) {
+      const int kk = k + (lane >> 5) < CPW ? k + (lane >> 5) : CPW - 1;
+      const int ch = chunk0 + kk < nc ? chunk0 + kk : nc - 1;
+      const int tok = (lane & 31) < rows ? (lane & 31) : rows - 1;
+      __builtin_amdgcn_global_load_lds((mx_gptr_t)(scl + (unsigned)(tok * rowS + ch * 4)), (mx_lds_t)(st + CODES + k * 128), 4, 0, 0);
+    }
+  };
+
+  MxCursor cu;                                                          // the tile being worked on
+  cu.units = p.units; cu.splits = p.splits; cu.tps = p.tps;
+  if constexpr (BWD) { cu.u = (int)blockIdx.x * groups + grp; cu.ustep = (int)gridDim.x * groups; cu.toff = 0; cu.tstep = 1; }
+  else { cu.u = (int)blockIdx.x; cu.ustep = (int)gridDim.x; cu.toff = grp; cu.tstep = groups; }
+  MxCursor ahead = cu;                                                  // the next tile to load
+  ahead.open(t);
+  int islot = 0;
+#pragma unroll
+  for (int i = 0; i < NST; ++i) {
+    if (ahead.valid()) { issue(ahead, islot); ahead.next(t); }
+    islot = islot + 1 == NST ? 0 : islot + 1;
+  }
+  if (!ahead.valid()) mx_wait_vm<0>();                                  // fewer tiles than stages: the counted waits assume a full ring
+
+  // ---- operand rows
+  MxOperand<QM> op[NQB][CPW];
+  const bool vecq = p.vecq;
+  auto load_operand = [&](const float* rows, const float* prows, float mul, float (&delta)[NQB]) {
+#pragma unroll
+    for (int qb = 0; qb < NQB; ++qb) {
+      const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+      const bool on = q < qn;
+      const int64_t at = (int64_t)(q0 + (on ? q : 0)) * t.D;
+      float d = 0.f;
+#pragma unroll
+      for (int k = 0; k < CPW; ++k) {
+        const int d0 = (chunk0 + k) * MX_BLOCK + 32 * g;
+        const mx_f32 v = mx_load_row(rows + at, on, d0, t.D, vecq, mul);
+        if (BWD && prows) {
+          const mx_f32 w = mx_load_row(prows + at, on, d0, t.D, vecq, 1.f);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) d = fmaf(v[i], w[i], d);
+        }
+        mx_operand<QM>(v, c, op[qb][k]);
+      }
+      delta[qb] = BWD && prows ? mx_over_groups_sum(d) : 0.f;
+    }
+  };
+  float delta[NQB];
+  if (!BWD && !p.qb) load_operand(p.q, nullptr, p.scale, delta);
+
+  f4 acc[NQB][CPW][8];
+  auto clear = [&]() {
+#pragma unroll
+    for (int qb = 0; qb < NQB; ++qb)
+#pragma unroll
+      for (int k = 0; k < CPW; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[qb][k][j] = f4{0.f, 0.f, 0.f, 0.f};
+  };
+  clear();
+  float m_run[NQB], mz[NQB], l_run[NQB], t_max[NQB], invl[NQB];       // mz: the maximum that weights are taken against
+  const int hh = QM == 8 ? c >> 3 : 0;                                  // QM 8: the lane's half of the 8 tokens
+  const int tok0 = 8 * g + 4 * hh;                                      // first token of the lane's scores in a tile
+  int slot = 0, buf = 0;
+
+  // acc rows 4 g + i of query block qb are queries qrow(i); multiply each by the value that lane (c = query) holds
+  auto scale_rows = [&](int qb, float f) {
+    float r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __shfl(f, QM == 8 ? (4 * g + i) & 7 : 4 * g + i, 64);
+#pragma unroll
+    for (int k = 0; k < CPW; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { acc[qb][k][j].x *= r[0]; acc[qb][k][j].y *= r[1]; acc[qb][k][j].z *= r[2]; acc[qb][k][j].w *= r[3]; }
+  };
+
+  // one tile: `work` false where this wave only keeps the barrier
+  auto tile_step = [&](bool work, int b, int t0, int len) {
+    float s[NQB][SV];
+    float sg[NQB][BWD ? SV : 1];                                        // backward: the saved scores
+    const char* st = ring + slot * STAGE;
+    if (work) {
+      mx_wait_vm<(NST - 1) * OPS>();
+      if constexpr (BWD) {
+#pragma unroll
+        for (int qb = 0; qb < NQB; ++qb) {
+          const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+          const float* sp = p.S + ((int64_t)b * p.Q + q0 + q) * t.N + t0 + tok0;
+#pragma unroll
+          for (int h = 0; h < SV / 4; ++h) {
+            f4 v = {0.f, 0.f, 0.f, 0.f};
+            const int n = t0 + tok0 + 4 * h;
+            if (q < qn) {
+              if (p.vecs) { if (n < t.N) v = *reinterpret_cast<const f4*>(sp + 4 * h); }
+              else {
+                if (n < t.N) v.x = sp[4 * h];
+                if (n + 1 < t.N) v.y = sp[4 * h + 1];
+                if (n + 2 < t.N) v.z = sp[4 * h + 2];
+                if (n + 3 < t.N) v.w = sp[4 * h + 3];
+              }
+            }
+            sg[qb][4 * h] = v.x; sg[qb][4 * h + 1] = v.y; sg[qb][4 * h + 2] = v.z; sg[qb][4 * h + 3] = v.w;
+          }
+        }
+      }
+      // first contraction
+      f4 sa[NQB][2], sl[NQB][2];                                        // leading and lower terms: an addition to a large sum costs its last bit
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) sa[qb][0] = sa[qb][1] = sl[qb][0] = sl[qb][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < CPW; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const mx_u4 w = *reinterpret_cast<const mx_u4*>(st + k * 2048 + h * 1024 + a_off);
+          const uint32_t sc = *reinterpret_cast<const uint32_t*>(st + CODES + k * 128 + h * 16 + sc_off) >> (8 * g);
+#pragma unroll
+          for (int qb = 0; qb < NQB; ++qb) {
+            const MxOperand<QM>& o = op[qb][k];
+            sa[qb][h] = mx_mfma_codes<0>(w, sc, o.b[0], o.sc[0], sa[qb][h]);
+            if constexpr (QM != 8) {
+              sl[qb][h] = mx_mfma_codes<2>(w, sc, o.b[5], o.sc[1], sl[qb][h]);
+              sl[qb][h] = mx_mfma_codes<1>(w, sc, o.b[4], o.sc[1], sl[qb][h]);
+              sl[qb][h] = mx_mfma_codes<0>(w, sc, o.b[3], o.sc[1], sl[qb][h]);
+            }
+            sl[qb][h] = mx_mfma_codes<2>(w, sc, o.b[2], o.sc[0], sl[qb][h]);
+            sl[qb][h] = mx_mfma_codes<1>(w, sc, o.b[1], o.sc[0], sl[qb][h]);
+          }
+        }
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) {
+        sa[qb][0] += sl[qb][0]; sa[qb][1] += sl[qb][1];
+        if constexpr (QM == 8) {                                        // columns q and q + 8 are terms of one query
+          const bool up = (c & 8) != 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float own = up ? sa[qb][1][i] : sa[qb][0][i], oth = up ? sa[qb][0][i] : sa[qb][1][i];
+            s[qb][i] = own + mx_ror8(oth) - (BWD ? delta[qb] : 0.f);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { s[qb][i] = sa[qb][0][i] - (BWD ? delta[qb] : 0.f); s[qb][4 + i] = sa[qb][1][i] - (BWD ? delta[qb] : 0.f); }
+        }
+      }
+    }
+    if (nw > 1) {                                                       // add the D-slices
+      char* ex = exch + (buf * groups + grp) * nw * DM::REC;
+      if (work) {
+#pragma unroll
+        for (int qb = 0; qb < NQB; ++qb)
+#pragma unroll
+          for (int h = 0; h < SV / 4; ++h)
+            *reinterpret_cast<f4*>(ex + dw * DM::REC + ((qb * (SV / 4) + h) * 64 + lane) * 16) = f4{s[qb][4 * h], s[qb][4 * h + 1], s[qb][4 * h + 2], s[qb][4 * h + 3]};
+      }
+      mx_barrier();
+      buf ^= 1;
+      if (work) {
+#pragma unroll
+        for (int qb = 0; qb < NQB; ++qb)
+#pragma unroll
+          for (int h = 0; h < SV / 4; ++h) {
+            f4 v = *reinterpret_cast<const f4*>(ex + ((qb * (SV / 4) + h) * 64 + lane) * 16);
+            for (int o = 1; o < nw; ++o) v += *reinterpret_cast<const f4*>(ex + o * DM::REC + ((qb * (SV / 4) + h) * 64 + lane) * 16);
+            s[qb][4 * h] = v.x; s[qb][4 * h + 1] = v.y; s[qb][4 * h + 2] = v.z; s[qb][4 * h + 3] = v.w;
+          }
+      }
+    }
+    if (!work) return;
+    const bool tail = t0 + 32 > len;
+    // weights
+    mx_u4 wt[NQB][DM::PSETS];
+#pragma unroll
+    for (int qb = 0; qb < NQB; ++qb) {
+      float pv[SV];
+      if constexpr (!BWD) {
+        if (tail) {
+#pragma unroll
+          for (int i = 0; i < SV; ++i) s[qb][i] = t0 + tok0 + i < len ? s[qb][i] : -INFINITY;
+        }
+        if (p.S && dw == 0) {
+          const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+          if (q < qn) {
+            float* sp = p.S + ((int64_t)b * p.Q + q0 + q) * t.N + t0 + tok0;
+#pragma unroll
+            for (int h = 0; h < SV / 4; ++h) {
+              const int n = t0 + tok0 + 4 * h;
+              if (p.vecs) { if (n < t.N) *reinterpret_cast<f4*>(sp + 4 * h) = f4{s[qb][4 * h], s[qb][4 * h + 1], s[qb][4 * h + 2], s[qb][4 * h + 3]}; }
+              else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (n + i < t.N) sp[4 * h + i] = s[qb][4 * h + i];
+              }
+            }
+          }
+        }
+        float mx = s[qb][0];
+#pragma unroll
+        for (int i = 1; i < SV; ++i) mx = fmaxf(mx, s[qb][i]);
+        t_max[qb] = fmaxf(t_max[qb], mx);
+        if (__any(mx > m_run[qb] + MX_LAZY)) {
+          if (QM == 8) mx = fmaxf(mx, mx_ror8(mx));
+          mx = mx_over_groups_max(mx);
+          const float mn = fmaxf(m_run[qb], mx);
+          const float f = mn == m_run[qb] ? 1.f : __builtin_amdgcn_exp2f((m_run[qb] - mn) * MX_LOG2E);
+          m_run[qb] = mn;
+          mz[qb] = mn == -INFINITY ? 0.f : mn;
+          l_run[qb] *= f;
+          scale_rows(qb, f);
+        }
+#pragma unroll
+        for (int i = 0; i < SV; ++i) { pv[i] = __builtin_amdgcn_exp2f((s[qb][i] - mz[qb]) * MX_LOG2E); l_run[qb] += pv[i]; }
+      } else {
+#pragma unroll
+        for (int i = 0; i < SV; ++i) {
+          const float a = __builtin_amdgcn_exp2f((sg[qb][i] - mz[qb]) * MX_LOG2E) * invl[qb];
+          pv[i] = a * s[qb][i];
+        }
+        if (tail) {
+#pragma unroll
+          for (int i = 0; i < SV; ++i) pv[i] = t0 + tok0 + i < len ? pv[i] : 0.f;
+        }
+      }
+      // three bf16 terms, exact: the upper half of the bits, of what is left, and of what is left then
+      uint32_t H[SV / 2], M[SV / 2], L[SV / 2];
+#pragma unroll
+      for (int i = 0; i < SV / 2; ++i) {
+        const float a = pv[2 * i], b2 = pv[2 * i + 1];
+        const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), rb = b2 - __uint_as_float(__float_as_uint(b2) & 0xffff0000u);
+        const float la = ra - __uint_as_float(__float_as_uint(ra) & 0xffff0000u), lb = rb - __uint_as_float(__float_as_uint(rb) & 0xffff0000u);
+        H[i] = __builtin_amdgcn_perm(__float_as_uint(b2), __float_as_uint(a), 0x07060302u);
+        M[i] = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), 0x07060302u);
+        L[i] = __builtin_amdgcn_perm(__float_as_uint(lb), __float_as_uint(la), 0x07060302u);
+      }
+      if constexpr (QM == 8) {                                          // rows 0-7: first and third term, rows 8-15: second; 8 slots = both halves
+        const bool up = (c & 8) != 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t r1 = mx_ror8u(up ? H[i] : M[i]), r2 = mx_ror8u(L[i]);
+          wt[qb][0][i] = up ? r1 : H[i];
+          wt[qb][0][2 + i] = up ? M[i] : r1;
+          wt[qb][1][i] = up ? 0u : L[i];
+          wt[qb][1][2 + i] = up ? 0u : r2;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { wt[qb][0][i] = H[i]; wt[qb][1][i] = M[i]; wt[qb][2][i] = L[i]; }
+      }
+    }
+    // second contraction
+#pragma unroll
+    for (int k = 0; k < CPW; ++k) {
+      uint32_t w[8];
+      float sc[8];
+      const mx_u4 s0 = *reinterpret_cast<const mx_u4*>(st + CODES + k * 128 + g * 32), s1 = *reinterpret_cast<const mx_u4*>(st + CODES + k * 128 + g * 32 + 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = *reinterpret_cast<const uint32_t*>(st + k * 2048 + (i >> 2) * 1024 + p_off[i & 3]);
+        const uint32_t four = i < 4 ? s0[i & 3] : s1[i & 3];
+        sc[i] = __uint_as_float(__builtin_amdgcn_alignbit(four, four, rot));
+      }
+#define EP_MX_PAIR(PR)                                                                                                   \
+  do {                                                                                                                   \
+    uint32_t x[8];                                                                                                       \
+    _Pragma("unroll") for (int i = 0; i < 8; ++i) x[i] = mx_pair<PR>(w[i], sc[i]);                                      \
+    mx_u4 ev, od;                                                                                                        \
+    _Pragma("unroll") for (int i = 0; i < 4; ++i) {                                                                     \
+      ev[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05040100u);                                                \
+      od[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);                                                \
+    }                                                                                                                    \
+    _Pragma("unroll") for (int qb = 0; qb < NQB; ++qb) _Pragma("unroll") for (int z = DM::PSETS - 1; z >= 0; --z) {     \
+      acc[qb][k][2 * PR] = mx_mfma(wt[qb][z], ev, acc[qb][k][2 * PR]);                                                   \
+      acc[qb][k][2 * PR + 1] = mx_mfma(wt[qb][z], od, acc[qb][k][2 * PR + 1]);                                           \
+    }                                                                                                                    \
+  } while (0)
+      EP_MX_PAIR(0); EP_MX_PAIR(1); EP_MX_PAIR(2); EP_MX_PAIR(3);
+#undef EP_MX_PAIR
+    }
+    // the stage is read: load the tile NST further on into it
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (ahead.valid()) { issue(ahead, slot); ahead.next(t); }
+    else mx_wait_vm<0>();                                               // the last tiles: fewer loads are under way than the counted wait assumes
+    slot = slot + 1 == NST ? 0 : slot + 1;
+  };
+
+  // store acc (times r(query)) as rows of out (row stride D): QM 8 adds the two term rows first
+  auto store_rows = [&](float* out, const float (&inv)[NQB]) {
+#pragma unroll
+    for (int qb = 0; qb < NQB; ++qb) {
+      float r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = __shfl(inv[qb], QM == 8 ? 4 * (g & 1) + i : 4 * g + i, 64);
+#pragma unroll
+      for (int k = 0; k < CPW; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int q = QM == 8 ? 4 * (g & 1) + i : qb * 16 + 4 * g + i;
+          float* o = out + (int64_t)(q0 + q) * t.D;
+          constexpr int NV = QM == 8 ? 1 : 2;
+#pragma unroll
+          for (int v = 0; v < NV; ++v) {
+            f4 x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = (QM == 8 ? fold32(acc[qb][k][j][i], acc[qb][k][j + 4][i]) : acc[qb][k][4 * v + j][i]) * r[i];
+            const int d = (chunk0 + k) * MX_BLOCK + 8 * c + (QM == 8 ? 4 * (g >> 1) : 4 * v);
+            if (q < qn && chunk0 + k < nc) {
+              if (p.veco) { if (d < t.D) *reinterpret_cast<f4*>(o + d) = x; }
+              else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if (d + j < t.D) o[d + j] = x[j];
+              }
+            }
+          }
+        }
+    }
+  };
+  // add the groups' accumulators into group 0's (through the ring, which is idle then), half a row block at a time
+  auto add_groups = [&]() {
+    for (int o = 1; o < groups; ++o) {
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb)
+#pragma unroll
+        for (int k = 0; k < CPW; ++k)
+#pragma unroll
+          for (int j0 = 0; j0 < 8; j0 += 4) {
+            if (grp == o) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) *reinterpret_cast<f4*>(lds + (dw * 4 + j) * 1024 + lane * 16) = acc[qb][k][j0 + j];
+            }
+            mx_barrier();
+            if (grp == 0) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[qb][k][j0 + j] += *reinterpret_cast<const f4*>(lds + (dw * 4 + j) * 1024 + lane * 16);
+            }
+            mx_barrier();
+          }
+    }
+  };
+
+  if constexpr (!BWD) {
+    for (int u = (int)blockIdx.x; u < p.units; u += (int)gridDim.x) {
+      const int b = u / p.splits, sp = u - b * p.splits;
+      int len;
+      const int img = __builtin_amdgcn_readfirstlane(mx_image(t, b, len));
+      len = __builtin_amdgcn_readfirstlane(len);
+      const int n = (len + 31) >> 5, lo = sp * p.tps, hi = (sp + 1) * p.tps < n ? (sp + 1) * p.tps : n;
+      if (p.qb) load_operand(p.q + (int64_t)b * p.qb, nullptr, p.scale, delta);
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) { m_run[qb] = t_max[qb] = -INFINITY; mz[qb] = l_run[qb] = 0.f; }
+      clear();
+      for (int tl = lo; tl < hi; tl += groups) tile_step(tl + grp < hi, b, (tl + grp) << 5, len);
+      if (p.S && sp == p.splits - 1 && dw == 0 && grp == 0) {           // scores behind the image's tiles
+        for (int q = 0; q < qn; ++q)
+          for (int i = (n << 5) + lane; i < t.N; i += 64) p.S[((int64_t)b * p.Q + q0 + q) * t.N + i] = img < 0 ? __uint_as_float(0x7fc00000u) : -INFINITY;
+      }
+      float f[NQB];
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) {                                // over the lanes of a query
+        if (QM == 8) { l_run[qb] += mx_ror8(l_run[qb]); t_max[qb] = fmaxf(t_max[qb], mx_ror8(t_max[qb])); }
+        l_run[qb] = mx_over_groups_sum(l_run[qb]);
+        t_max[qb] = mx_over_groups_max(t_max[qb]);
+      }
+      if (groups > 1) {                                                 // (one unit per workgroup then: the ring is idle)
+        float* ml = reinterpret_cast<float*>(exch);                     // [groups][NQB][16][3]
+        mx_barrier();
+        if (dw == 0 && g == 0) {
+#pragma unroll
+          for (int qb = 0; qb < NQB; ++qb) {
+            float* e = ml + ((grp * NQB + qb) * 16 + c) * 3;
+            e[0] = m_run[qb]; e[1] = l_run[qb]; e[2] = t_max[qb];
+          }
+        }
+        mx_barrier();
+#pragma unroll
+        for (int qb = 0; qb < NQB; ++qb) {
+          float M = -INFINITY, T = -INFINITY, l = 0.f;
+          for (int o = 0; o < groups; ++o) { const float* e = ml + ((o * NQB + qb) * 16 + c) * 3; M = fmaxf(M, e[0]); T = fmaxf(T, e[2]); }
+          for (int o = 0; o < groups; ++o) {
+            const float* e = ml + ((o * NQB + qb) * 16 + c) * 3;
+            l += e[0] == M ? e[1] : e[1] * __builtin_amdgcn_exp2f((e[0] - M) * MX_LOG2E);
+          }
+          const float own = m_run[qb] == M ? 1.f : __builtin_amdgcn_exp2f((m_run[qb] - M) * MX_LOG2E);
+          scale_rows(qb, own);
+          m_run[qb] = M; l_run[qb] = l; t_max[qb] = T;
+          mz[qb] = M == -INFINITY ? 0.f : M;
+        }
+        add_groups();
+      }
+      if (grp == 0) {
+        const float bad = img < 0 ? __uint_as_float(0x7fc00000u) : 0.f;
+#pragma unroll
+        for (int qb = 0; qb < NQB; ++qb) {
+          const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+          const bool none = t_max[qb] == -INFINITY && l_run[qb] == 0.f;                       // no token
+          const float m = none ? (p.splits > 1 ? -INFINITY : 0.f) : t_max[qb];
+          const float e = none ? 0.f : __builtin_amdgcn_exp2f((mz[qb] - m) * MX_LOG2E);       // from the running to the true maximum
+          if (dw == 0 && g == 0 && (QM != 8 || c < 8) && q < qn) {
+            if (p.splits > 1) *reinterpret_cast<f2*>(p.part_ml + ((int64_t)u * p.Q + q0 + q) * 2) = f2{m + bad, l_run[qb] * e + bad};
+            else *reinterpret_cast<f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4) = f4{m + bad, l_run[qb] * e + bad, 0.f, 0.f};
+          }
+          f[qb] = (p.splits > 1 ? e : (none ? 0.f : 1.f / l_run[qb])) + bad;
+        }
+        store_rows(p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, f);
+      }
+    }
+  } else {
+    float one[NQB];
+#pragma unroll
+    for (int qb = 0; qb < NQB; ++qb) one[qb] = p.scale;
+    auto open_unit = [&](int b) {
+      load_operand(p.q + (int64_t)b * p.Q * t.D, p.Pin ? p.Pin + (int64_t)b * p.Q * t.D : nullptr, 1.f, delta);
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) {
+        const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+        f4 ml = {0.f, 0.f, 0.f, 0.f};
+        if (q < qn) ml = *reinterpret_cast<const f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4);
+        mz[qb] = ml.x;
+        invl[qb] = ml.y == 0.f ? 0.f : 1.f / ml.y;
+        if (!p.Pin && dw == 0) delta[qb] = ml.z;                        // (each D-slice takes off its own part of delta)
+      }
+    };
+    if (p.per_unit) {                                                   // images (and runs) without a token are not visited below
+      MxCursor z = cu;
+      for (; z.u < z.units; z.u += z.ustep) {
+        const int b = z.u / z.splits;
+        int len;
+        mx_image(t, b, len);
+        if ((z.u - b * z.splits) * z.tps >= (len + 31) >> 5) store_rows(p.part + (int64_t)z.u * p.Q * t.D, one);
+      }
+    }
+    cu.open(t);
+    bool fresh = true;
+    const int iters = nw > 1 ? (int)((p.units + cu.ustep - 1) / cu.ustep) * p.tps : 0;
+    for (int it = 0; nw > 1 ? it < iters : cu.valid(); ++it) {
+      const bool work = cu.valid();
+      if (work && fresh) open_unit(cu.b);
+      tile_step(work, cu.b, cu.tile << 5, cu.len);
+      if (!work) continue;
+      const int u = cu.u;
+      fresh = cu.next(t);
+      if (fresh && p.per_unit) {                                        // one gradient per image (and split)
+        store_rows(p.part + (int64_t)u * p.Q * t.D, one);
+        clear();
+      }
+    }
+    if (!p.per_unit) {
+      if (groups > 1) { mx_wait_vm<0>(); mx_barrier(); add_groups(); }
+      if (grp == 0) store_rows(p.part + (int64_t)blockIdx.x * p.Q * t.D, one);
+    }
+  }
+}
+
+// joins the splits of an image: one workgroup per (image, query)
+__global__ __launch_bounds__(256) void ep_mx4_join_kernel(const float* __restrict__ part, const float* __restrict__ ml, int splits, int Q, int D,
+                                                          float* __restrict__ P, float* __restrict__ ML) {
+  const int b = (int)(blockIdx.x / (unsigned)Q), q = (int)(blockIdx.x % (unsigned)Q);
+  float m = -INFINITY, l = 0.f;
+  bool bad = false;
+  for (int s = 0; s < splits; ++s) {
+    const float v = ml[(((int64_t)b * splits + s) * Q + q) * 2];
+    bad |= v != v;
+    m = fmaxf(m, v);
+  }
+  for (int s = 0; s < splits; ++s) {
+    const float* e = ml + (((int64_t)b * splits + s) * Q + q) * 2;
+    if (e[1] != 0.f) l += e[1] * __builtin_amdgcn_exp2f((e[0] - m) * MX_LOG2E);
+  }
+  if (bad) m = l = __uint_as_float(0x7fc00000u);
+  if (threadIdx.x == 0) *reinterpret_cast<f4*>(ML + ((int64_t)b * Q + q) * 4) = f4{l == 0.f ? 0.f : m, l, 0.f, 0.f};
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  for (int d = (int)threadIdx.x; d < D; d += 256) {
+    float a = 0.f;
+    for (int s = 0; s < splits; ++s) {
+      const int64_t r = ((int64_t)b * splits + s) * Q + q;
+      const float mv = ml[r * 2];
+      if (ml[r * 2 + 1] != 0.f) a += part[r * D + d] * __builtin_amdgcn_exp2f((mv - m) * MX_LOG2E);
+    }
+    P[((int64_t)b * Q + q) * D + d] = a * inv;
+  }
+}
+
+// out[i] (+)= sum over n of part[n][i], in order of n within 16 interleaved chains and then the chains: blockIdx.y selects the output
+__global__ __launch_bounds__(256) void ep_mx4_sum_kernel(const float* __restrict__ part, int n, int64_t len, float* __restrict__ out, int accumulate) {
+  __shared__ float red[16][17];
+  const int x = (int)threadIdx.x & 15, y = (int)threadIdx.x >> 4;
+  const int64_t i = (int64_t)blockIdx.x * 16 + x;
+  const float* src = part + (int64_t)blockIdx.y * n * len;
+  float s = 0.f;
+  if (i < len)
+    for (int r = y; r < n; r += 16) s += src[(int64_t)r * len + i];
+  red[y][x] = s;
+  __syncthreads();
+  if (y == 0 && i < len) {
+    float a = red[0][x];
+    for (int r = 1; r < 16; ++r) a += red[r][x];
+    float* o = out + (int64_t)blockIdx.y * len + i;
+    *o = accumulate ? *o + a : a;
+  }
+}
+
+// ---- plan: which variant, how many waves, groups, splits ----------------------------------------------------------------
+struct MxPlan { int qm, cpw, nw, groups, splits, tps, units, grid, yblk, qblk; size_t lds, ws; };
+
+static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
+  MxPlan p{};
+  const int nc = mx_blocks(D), cus = cu_count(), tiles = (N + 31) / 32;
+  // widest query block that the row width leaves registers for: accumulators and operand of a 128-channel block take 50 / 68 / 136
+  // registers at 8 / 16 / 32 queries, a workgroup is at most 8 waves of 256
+  p.qm = Q <= 8 || nc > 24 ? 8 : (Q <= 16 || nc > 8 ? 16 : 32);
+  const int cmax = p.qm == 8 ? 4 : (p.qm == 16 ? 3 : 1);
+  p.nw = (nc + cmax - 1) / cmax;
+  p.cpw = (nc + p.nw - 1) / p.nw;
+  p.yblk = (Q + p.qm - 1) / p.qm;
+  p.qblk = (Q + p.yblk - 1) / p.yblk;
+  const int gmax = 8 / p.nw;                                            // groups of a workgroup of at most 8 waves
+  p.splits = 1;
+  if (bwd) {
+    p.groups = gmax;
+    const int64_t want = (int64_t)cus * gmax;
+    if (B < want) p.splits = (int)((want + B - 1) / B);
+    const int most = (tiles + 1) / 2;
+    if (p.splits > most) p.splits = most;
+  } else {
+    p.groups = B <= cus ? gmax : 1;
+    if (p.groups > tiles) p.groups = tiles;
+    if (B < cus) p.splits = cus / B;
+    const int most = tiles / (4 * p.groups);
+    if (p.splits > most) p.splits = most;
+  }
+  if (p.splits < 1) p.splits = 1;
+  p.tps = (tiles + p.splits - 1) / p.splits;
+  p.splits = (tiles + p.tps - 1) / p.tps;
+  p.units = B * p.splits;
+  const int stage = 2048 * p.cpw + 256 * ((p.cpw + 1) / 2), rec = 256 * (p.qm == 8 ? 4 : p.qm == 16 ? 8 : 16);
+  const int waves = p.nw * p.groups;
+  p.lds = (size_t)waves * (MX_STAGES * stage) + (p.nw > 1 || p.groups > 1 ? 2 * (size_t)waves * rec : 0);
+  if (bwd) {
+    p.grid = (p.units + p.groups - 1) / p.groups;
+    if (p.grid > cus) p.grid = cus;
+    p.ws = !per_image ? (size_t)p.grid * Q * D * 4 : p.splits > 1 ? (size_t)p.units * Q * D * 4 : 0;
+  } else {
+    int per_cu = 8 / waves;
+    const int by_lds = (int)(160 * 1024 / p.lds);
+    if (per_cu > by_lds) per_cu = by_lds;
+    p.grid = p.groups > 1 ? p.units : (p.units < cus * per_cu ? p.units : cus * per_cu);
+    p.ws = p.splits > 1 ? (size_t)p.units * Q * (D + 2) * 4 : 0;
+  }
+  return p;
+}
+
+template <int QM, int CPW, bool BWD>
+static int mx_launch2(const MxPool& p, const MxPlan& pl, hipStream_t st) {
+  auto* fn = ep_mx4_pool_kernel<QM, CPW, MX_STAGES, BWD>;
+  if (pl.lds > 64 * 1024) EP_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, (int)pl.lds));
+  hipLaunchKernelGGL((ep_mx4_pool_kernel<QM, CPW, MX_STAGES, BWD>), dim3((unsigned)pl.grid, (unsigned)pl.yblk), dim3((unsigned)(64 * pl.nw * pl.groups)), pl.lds, st, p);
+  EP_LAUNCH_CHECK("ep_mx4_pool_kernel");
+  return 0;
+}
+template <bool BWD>
+static int mx_launch(const MxPool& p, const MxPlan& pl, hipStream_t st) {
+  switch (pl.qm * 10 + pl.cpw) {
+    case 81: return mx_launch2<8, 1, BWD>(p, pl, st);
+    case 82: return mx_launch2<8, 2, BWD>(p, pl, st);
+    case 83: return mx_launch2<8, 3, BWD>(p, pl, st);
+    case 84: return mx_launch2<8, 4, BWD>(p, pl, st);
+    case 161: return mx_launch2<16, 1, BWD>(p, pl, st);
+    case 162: return mx_launch2<16, 2, BWD>(p, pl, st);
+    case 163: return mx_launch2<16, 3, BWD>(p, pl, st);
+    default: return mx_launch2<32, 1, BWD>(p, pl, st);
+  }
+}
+
+static MxPool mx_pool_params(const ep_mx4_tokens* t, int Q, float scale, const MxPlan& pl) {
+  MxPool p{};
+  p.t = *t; p.Q = Q; p.scale = scale; p.nc = mx_blocks(t->D);
+  p.nw = pl.nw; p.groups = pl.groups; p.splits = pl.splits; p.tps = pl.tps; p.units = pl.units; p.qblk = pl.qblk;
+  p.vecs = t->N % 4 == 0;
+  return p;
+}
+
+int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S, float* ML, void* ws,
+                     size_t ws_bytes, hipStream_t st) {
+  const MxPlan pl = mx_plan(t->B, t->N, t->D, Q, false, false);
+  EP_REQUIRE(ws_bytes >= pl.ws, EP_E_WORKSPACE, "ep_mx4_pool_forward: workspace %zu < %zu", ws_bytes, pl.ws);
+  MxPool p = mx_pool_params(t, Q, scale, pl);
+  p.q = queries; p.qb = q_bstride; p.P = P; p.S = S; p.ML = ML;
+  p.part = static_cast<float*>(ws); p.part_ml = p.part + (size_t)pl.units * Q * t->D;
+  p.vecq = t->D % 4 == 0 && aligned16(queries) && q_bstride % 4 == 0;
+  p.veco = t->D % 4 == 0 && aligned16(pl.splits > 1 ? (const void*)p.part : (const void*)P);
+  p.vecs = p.vecs && aligned16(S);
+  EP_TRY(mx_launch<false>(p, pl, st));
+  if (pl.splits > 1) {
+    hipLaunchKernelGGL(ep_mx4_join_kernel, dim3((unsigned)t->B * Q), dim3(256), 0, st, p.part, p.part_ml, pl.splits, Q, t->D, P, ML);
+    EP_LAUNCH_CHECK("ep_mx4_join_kernel");
+  }
+  return 0;
+}
+
+int mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S, const float* ML, const float* P, const float* dP, float* dq,
+                      int per_image, int accumulate, void* ws, size_t ws_bytes, hipStream_t st) {
+  const MxPlan pl = mx_plan(t->B, t->N, t->D, Q, true, per_image != 0);
+  EP_REQUIRE(ws_bytes >= pl.ws, EP_E_WORKSPACE, "ep_mx4_pool_backward: workspace %zu < %zu", ws_bytes, pl.ws);
+  MxPool p = mx_pool_params(t, Q, scale, pl);
+  p.q = dP; p.Pin = P; p.S = const_cast<float*>(S); p.ML = const_cast<float*>(ML);
+  p.per_unit = per_image != 0;
+  p.part = per_image && pl.splits == 1 ? dq : static_cast<float*>(ws);
+  p.vecq = t->D % 4 == 0 && aligned16(dP) && aligned16(P);
+  p.veco = t->D % 4 == 0 && aligned16(p.part);
+  p.vecs = p.vecs && aligned16(S);
+  const int64_t QD = (int64_t)Q * t->D;
+  EP_TRY(mx_launch<true>(p, pl, st));
+  if (!per_image || pl.splits > 1) {
+    const int n = per_image ? pl.splits : pl.grid;
+    hipLaunchKernelGGL(ep_mx4_sum_kernel, dim3((unsigned)((QD + 15) / 16), per_image ? (unsigned)t->B : 1u), dim3(256), 0, st, p.part, n, QD, dq, accumulate);
+    EP_LAUNCH_CHECK("ep_mx4_sum_kernel");
+  }
+  return 0;
 }
 
 }  // namespace ep
@@ -137,14 +844,20 @@ using namespace ep;
 extern "C" {
 
 size_t ep_mx4_pool_workspace_bytes(int B, int N, int D, int Q) {
-  if (B <= 0 || N <= 0 || D <= 0 || Q <= 0) return 0;
-  return round_up(((size_t)B * Q * N + (size_t)B * Q * D) * sizeof(float), 256);
+  if (B <= 0 || N <= 0 || D <= 0 || Q <= 0 || D > MX_MAX_D) return 0;
+  size_t n = 256;
+  for (int k = 0; k < 3; ++k) {
+    const size_t w = mx_plan(B, N, D, Q, k > 0, k == 2).ws;
+    n = w > n ? w : n;
+  }
+  return round_up(n, 256);
 }
 
 static int mx_pool_check(const ep_mx4_tokens* t, int Q, void* ws, size_t bytes, const char* what) {
   EP_TRY(mx4_check(t, what));
   EP_REQUIRE(Q > 0, EP_E_ARG, "%s: Q = %d", what, Q);
   EP_REQUIRE(t->D <= MX_MAX_D, EP_E_SHAPE, "%s: D = %d > %d", what, t->D, MX_MAX_D);
+  EP_REQUIRE((int64_t)t->B * Q <= 2147483647, EP_E_SHAPE, "%s: %d x %d rows in one call", what, t->B, Q);
   EP_REQUIRE(ws && aligned16(ws), EP_E_ARG, "%s: the workspace must be given and 16-byte aligned", what);
   const size_t need = ep_mx4_pool_workspace_bytes(t->B, t->N, t->D, Q);
   EP_REQUIRE(bytes >= need, EP_E_WORKSPACE, "%s: workspace %zu < %zu", what, bytes, need);
@@ -157,11 +870,7 @@ int ep_mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_
   EP_REQUIRE(queries && P && ML, EP_E_ARG, "ep_mx4_pool_forward: null pointer");
   EP_REQUIRE(aligned16(ML), EP_E_ALIGN, "ep_mx4_pool_forward: ML must be 16-byte aligned");
   EP_REQUIRE(q_bstride == 0 || q_bstride >= (int64_t)Q * t->D, EP_E_SHAPE, "ep_mx4_pool_forward: query batch stride %lld", (long long)q_bstride);
-  MxPool p{};
-  p.t = *t; p.q = queries; p.qb = q_bstride; p.Q = Q; p.scale = scale; p.P = P; p.S = S ? S : (float*)workspace; p.ML = ML;
-  hipLaunchKernelGGL(ep_mx4_pool_fwd_kernel, dim3((unsigned)t->B * Q), dim3(64 * MXP_WAVES), 0, (hipStream_t)stream, p);
-  EP_LAUNCH_CHECK("ep_mx4_pool_fwd_kernel");
-  return 0;
+  return mx4_pool_forward(t, queries, q_bstride, Q, scale, P, S, ML, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 int ep_mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S, const float* ML, const float* P, const float* dP, float* dq,
@@ -170,19 +879,7 @@ int ep_mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float
   EP_REQUIRE(S && ML && dP && dq, EP_E_ARG, "ep_mx4_pool_backward: null pointer");
   EP_REQUIRE(aligned16(ML), EP_E_ALIGN, "ep_mx4_pool_backward: ML must be 16-byte aligned");
   EP_REQUIRE(!(per_image && accumulate), EP_E_UNSUPPORTED, "ep_mx4_pool_backward: accumulate is for shared queries");
-  MxPool p{};
-  p.t = *t; p.q = dP; p.Q = Q; p.scale = scale; p.S = const_cast<float*>(S); p.ML = const_cast<float*>(ML); p.Pin = P;
-  p.dS = (float*)workspace;
-  p.dq = per_image ? dq : p.dS + (size_t)t->B * Q * t->N;
-  hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(ep_mx4_pool_bwd_kernel, dim3((unsigned)t->B * Q), dim3(64 * MXP_WAVES), 0, st, p);
-  EP_LAUNCH_CHECK("ep_mx4_pool_bwd_kernel");
-  if (!per_image) {
-    const int64_t QD = (int64_t)Q * t->D;
-    hipLaunchKernelGGL(ep_mx4_sum_images_kernel, dim3((unsigned)((QD + 255) / 256)), dim3(256), 0, st, p.dq, t->B, QD, dq, accumulate);
-    EP_LAUNCH_CHECK("ep_mx4_sum_images_kernel");
-  }
-  return 0;
+  return mx4_pool_backward(t, Q, scale, S, ML, P, dP, dq, per_image, accumulate, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"
