@@ -17,7 +17,8 @@ struct MxPool {
   int nc, nw, groups;                    // 128-channel blocks of a row; waves a row is cut over; such groups of waves in a workgroup
   int splits, tps, units;                // an image's tiles are cut into `splits` runs of `tps`; unit = image * splits + run
   int per_unit;                          // backward: a gradient per unit instead of per workgroup
-  int vecq, vecs, veco;                  // 16-byte accesses to the operand rows / scores / outputs
+  int ldq;                               // row stride of the operand rows
+  int vecs, veco;                        // 16-byte accesses to the scores / outputs
 };
 
 int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S, float* ML, void* ws,

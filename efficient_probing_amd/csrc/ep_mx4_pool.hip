@@ -76,80 +76,63 @@ __device__ __forceinline__ f4 mx_mfma_codes(const mx_u4& codes, uint32_t scale, 
 // the even and the odd values.  It and its inverse write their results before they have read all of their sources (the scale among
 // them), which the compiler does not allow for: it may place the result over a source that dies there, and the low terms then differ
 // from run to run.  So every source is kept alive behind the instruction by an empty asm.
-struct MxTerms { mx_u6 t[6]; int s0; };
-__device__ __forceinline__ void mx_terms(mx_f32 v, MxTerms& o) {
-  uint32_t am = 0;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) { const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu; am = a > am ? a : am; }
-  const int ex = (int)(am >> 23);
-  o.s0 = ex == 255 ? 255 : (ex - 2 < 24 ? 24 : ex - 2);
-  const int base = o.s0 == 255 ? 252 : o.s0;
-#pragma unroll
-  for (int t = 0; t < 6; ++t) {
-    const float sc = __uint_as_float((uint32_t)(base - 4 * t) << 23);
-    mx_f16 a, b;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) { a[i] = v[2 * i]; b[i] = v[2 * i + 1]; }
-    o.t[t] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, sc);
-    asm volatile("" ::"v"(a), "v"(b), "v"(sc), "v"(o.t[t]));
-    if (t < 5) {
-      const mx_f32 d = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(o.t[t], sc);
-      asm volatile("" ::"v"(o.t[t]), "v"(sc), "v"(d));
-      v -= d;
-    }
-  }
-}
-
-// the operand of one row block for this lane's column: queries q (QM 8: two terms share an operand, columns 8-15 take the odd ones)
 template <int QM>
 struct MxOperand { mx_u6 b[MxDims<QM>::SETS]; uint32_t sc[MxDims<QM>::SCB]; };
 
+// the operand of one row block for this lane's column; QM 8: two terms share an operand, columns 8-15 take the odd ones
 template <int QM>
-__device__ __forceinline__ void mx_operand(const mx_f32& v, int c, MxOperand<QM>& o) {
-  MxTerms t;
-  mx_terms(v, t);
-  if constexpr (QM == 8) {
-    const bool odd = (c & 8) != 0;
-    uint32_t s = 0;
+__device__ __forceinline__ void mx_operand(mx_f16 a, mx_f16 b, int c, MxOperand<QM>& o) {       // a, b: the row's even and odd channels
+  uint32_t am = 0;
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-#pragma unroll
-      for (int i = 0; i < 6; ++i) o.b[k][i] = odd ? t.t[2 * k + 1][i] : t.t[2 * k][i];
-      const int e = t.s0 == 255 ? 255 : t.s0 - 4 * (2 * k + (odd ? 1 : 0));
-      s |= (uint32_t)e << (8 * k);
-    }
-    o.sc[0] = s;
-  } else {
-#pragma unroll
-    for (int k = 0; k < 6; ++k) o.b[k] = t.t[k];
-    uint32_t s[2] = {0, 0};
-#pragma unroll
-    for (int k = 0; k < 6; ++k) s[k / 3] |= (uint32_t)(t.s0 == 255 ? 255 : t.s0 - 4 * k) << (8 * (k % 3));
-    o.sc[0] = s[0]; o.sc[1] = s[1];
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t x = __float_as_uint(a[i]) & 0x7fffffffu, y = __float_as_uint(b[i]) & 0x7fffffffu;
+    am = x > am ? x : am;
+    am = y > am ? y : am;
   }
+  const int ex = (int)(am >> 23);
+  const bool bad = ex == 255;                                  // an infinity or a NaN in the row: the scale byte 255 makes its scores NaN
+  const int s0 = bad ? 252 : (ex - 2 < 24 ? 24 : ex - 2);
+  const bool odd = QM == 8 && (c & 8) != 0;
+  uint32_t bytes[2] = {0, 0};
+#pragma unroll
+  for (int t = 0; t < 6; ++t) {
+    const float sc = __uint_as_float((uint32_t)(s0 - 4 * t) << 23);
+    const mx_u6 k = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, sc);
+    asm volatile("" ::"v"(a), "v"(b), "v"(sc), "v"(k));
+    if (t < 5) {
+      const mx_f32 d = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(k, sc);
+      asm volatile("" ::"v"(k), "v"(sc), "v"(d));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) { a[i] -= d[2 * i]; b[i] -= d[2 * i + 1]; }
+    }
+    const uint32_t byte = bad ? 255u : (uint32_t)(s0 - 4 * t);
+    if constexpr (QM == 8) {
+      if (t % 2 == 0) { o.b[t / 2] = k; bytes[0] |= (odd ? 0u : byte) << (8 * (t / 2)); }
+      else {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) o.b[t / 2][i] = odd ? k[i] : o.b[t / 2][i];
+        bytes[0] |= (odd ? byte : 0u) << (8 * (t / 2));
+      }
+    } else {
+      o.b[t] = k;
+      bytes[t / 3] |= byte << (8 * (t % 3));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  o.sc[0] = bytes[0];
+  if constexpr (QM != 8) o.sc[1] = bytes[1];
 }
 
-// 32 values of `row` from channel d on, times mul; 0 behind D and where `on` is false.  Addresses are clamped into the row instead of
-// branched around, so that all loads are under way together.
-__device__ __forceinline__ mx_f32 mx_load_row(const float* row, bool on, int d, int D, bool vec, float mul) {
-  mx_f32 v;
-  if (vec) {
-    f4 x[8];
+// 32 values of an operand row (16-byte aligned, whole 128-channel blocks: other rows are padded first), times mul
+__device__ __forceinline__ void mx_load_row(const float* row, float mul, mx_f16& a, mx_f16& b) {
+  f4 x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { const int e = d + 4 * i; x[i] = *reinterpret_cast<const f4*>(row + (e < D ? e : D - 4)); }
+  for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const f4*>(row)[i];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool ok = on && d + 4 * i < D;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * i + j] = ok ? x[i][j] * mul : 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = row[d + i < D ? d + i : D - 1];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = on && d + i < D ? v[i] * mul : 0.f;
+  for (int i = 0; i < 8; ++i) {
+    a[2 * i] = x[i][0] * mul; b[2 * i] = x[i][1] * mul;
+    a[2 * i + 1] = x[i][2] * mul; b[2 * i + 1] = x[i][3] * mul;
   }
-  return v;
 }
 
 // a wave's sequence of (unit, tile): units u, u + ustep, ..., of each the tiles t_off, t_off + tstep, ...
@@ -244,30 +227,32 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
 
   // ---- operand rows
   MxOperand<QM> op[NQB][CPW];
-  const bool vecq = p.vecq;
   auto load_operand = [&](const float* rows, const float* prows, float mul, float (&delta)[NQB]) {
 #pragma unroll
     for (int qb = 0; qb < NQB; ++qb) {
       const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-      const bool on = q < qn;
-      const int64_t at = (int64_t)(q0 + (on ? q : 0)) * t.D;
+      const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * p.ldq + 32 * g;      // (rows without a query: the first one's, times 0)
       float d = 0.f;
 #pragma unroll
       for (int k = 0; k < CPW; ++k) {
-        const int d0 = (chunk0 + k) * MX_BLOCK + 32 * g;
-        const mx_f32 v = mx_load_row(rows + at, on, d0, t.D, vecq, mul);
+        const bool in = chunk0 + k < nc;
+        const int d0 = (in ? chunk0 + k : nc - 1) * MX_BLOCK;
+        mx_f16 ve, vo;
+        mx_load_row(rows + at + d0, in && q < qn ? mul : 0.f, ve, vo);
         if (BWD && prows) {
-          const mx_f32 w = mx_load_row(prows + at, on, d0, t.D, vecq, 1.f);
+          mx_f16 we, wo;
+          mx_load_row(prows + at + d0, 1.f, we, wo);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) d = fmaf(v[i], w[i], d);
+          for (int i = 0; i < 16; ++i) d = fmaf(vo[i], wo[i], fmaf(ve[i], we[i], d));
+          __builtin_amdgcn_sched_barrier(0);
         }
-        mx_operand<QM>(v, c, op[qb][k]);
+        mx_operand<QM>(ve, vo, c, op[qb][k]);
+        __builtin_amdgcn_sched_barrier(0);
       }
       delta[qb] = BWD && prows ? mx_over_groups_sum(d) : 0.f;
     }
   };
   float delta[NQB];
-  if (!BWD && !p.qb) load_operand(p.q, nullptr, p.scale, delta);
 
   f4 acc[NQB][CPW][8];
   auto clear = [&]() {
@@ -363,6 +348,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
         }
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
     if (nw > 1) {                                                       // add the D-slices
       char* ex = exch + (buf * groups + grp) * nw * DM::REC;
       if (work) {
@@ -467,6 +453,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
       }
     }
     // second contraction
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int k = 0; k < CPW; ++k) {
       uint32_t w[8];
@@ -493,6 +480,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
     }                                                                                                                    \
   } while (0)
       EP_MX_PAIR(0); EP_MX_PAIR(1); EP_MX_PAIR(2); EP_MX_PAIR(3);
+      __builtin_amdgcn_sched_barrier(0);
 #undef EP_MX_PAIR
     }
     // the stage is read: load the tile NST further on into it
@@ -564,7 +552,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
       const int img = __builtin_amdgcn_readfirstlane(mx_image(t, b, len));
       len = __builtin_amdgcn_readfirstlane(len);
       const int n = (len + 31) >> 5, lo = sp * p.tps, hi = (sp + 1) * p.tps < n ? (sp + 1) * p.tps : n;
-      if (p.qb) load_operand(p.q + (int64_t)b * p.qb, nullptr, p.scale, delta);
+      if (p.qb || u == (int)blockIdx.x) load_operand(p.q + (int64_t)b * p.qb, nullptr, p.scale, delta);
 #pragma unroll
       for (int qb = 0; qb < NQB; ++qb) { m_run[qb] = t_max[qb] = -INFINITY; mz[qb] = l_run[qb] = 0.f; }
       clear();
@@ -628,7 +616,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
 #pragma unroll
     for (int qb = 0; qb < NQB; ++qb) one[qb] = p.scale;
     auto open_unit = [&](int b) {
-      load_operand(p.q + (int64_t)b * p.Q * t.D, p.Pin ? p.Pin + (int64_t)b * p.Q * t.D : nullptr, 1.f, delta);
+      load_operand(p.q + (int64_t)b * p.Q * p.ldq, p.Pin ? p.Pin + (int64_t)b * p.Q * p.ldq : nullptr, 1.f, delta);
 #pragma unroll
       for (int qb = 0; qb < NQB; ++qb) {
         const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
@@ -719,7 +707,16 @@ __global__ __launch_bounds__(256) void ep_mx4_sum_kernel(const float* __restrict
 }
 
 // ---- plan: which variant, how many waves, groups, splits ----------------------------------------------------------------
-struct MxPlan { int qm, cpw, nw, groups, splits, tps, units, grid, yblk, qblk; size_t lds, ws; };
+// rows of D channels -> rows of whole 128-channel blocks, zero-filled
+__global__ __launch_bounds__(256) void ep_mx4_pad_rows_kernel(const float* __restrict__ src, int64_t rows, int D, int Dp, float* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * Dp) return;
+  const int64_t r = i / Dp;
+  const int d = (int)(i - r * Dp);
+  out[i] = d < D ? src[r * D + d] : 0.f;
+}
+
+struct MxPlan { int qm, cpw, nw, groups, splits, tps, units, grid, yblk, qblk; size_t lds, ws, pad; };     // ws: bytes, of them pad for padded operand rows
 
 static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   MxPlan p{};
@@ -765,7 +762,24 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
     p.grid = p.groups > 1 ? p.units : (p.units < cus * per_cu ? p.units : cus * per_cu);
     p.ws = p.splits > 1 ? (size_t)p.units * Q * (D + 2) * 4 : 0;
   }
+  const size_t rows = (size_t)(bwd ? 2 * (int64_t)B * Q : per_image ? (int64_t)B * Q : Q);
+  p.pad = D % MX_BLOCK ? round_up(rows * nc * MX_BLOCK * 4, 256) : 0;
+  p.ws += p.pad;
   return p;
+}
+
+// operand rows as the kernel reads them
+static int mx_rows(const float* src, int64_t rows, int D, char*& ws, const float** out, hipStream_t st) {
+  *out = src;
+  if (D % MX_BLOCK == 0) return 0;
+  const int Dp = mx_blocks(D) * MX_BLOCK;
+  const int64_t grid = (rows * Dp + 255) / 256;
+  EP_REQUIRE(grid <= 2147483647, EP_E_SHAPE, "MX4 attention: %lld rows of %d channels in one call", (long long)rows, D);
+  hipLaunchKernelGGL(ep_mx4_pad_rows_kernel, dim3((unsigned)grid), dim3(256), 0, st, src, rows, D, Dp, reinterpret_cast<float*>(ws));
+  EP_LAUNCH_CHECK("ep_mx4_pad_rows_kernel");
+  *out = reinterpret_cast<float*>(ws);
+  ws += (size_t)rows * Dp * 4;
+  return 0;
 }
 
 template <int QM, int CPW, bool BWD>
@@ -794,18 +808,19 @@ static MxPool mx_pool_params(const ep_mx4_tokens* t, int Q, float scale, const M
   MxPool p{};
   p.t = *t; p.Q = Q; p.scale = scale; p.nc = mx_blocks(t->D);
   p.nw = pl.nw; p.groups = pl.groups; p.splits = pl.splits; p.tps = pl.tps; p.units = pl.units; p.qblk = pl.qblk;
-  p.vecs = t->N % 4 == 0;
+  p.vecs = t->N % 4 == 0; p.ldq = p.nc * MX_BLOCK;
   return p;
 }
 
 int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S, float* ML, void* ws,
                      size_t ws_bytes, hipStream_t st) {
-  const MxPlan pl = mx_plan(t->B, t->N, t->D, Q, false, false);
+  const MxPlan pl = mx_plan(t->B, t->N, t->D, Q, false, q_bstride != 0);
   EP_REQUIRE(ws_bytes >= pl.ws, EP_E_WORKSPACE, "ep_mx4_pool_forward: workspace %zu < %zu", ws_bytes, pl.ws);
   MxPool p = mx_pool_params(t, Q, scale, pl);
-  p.q = queries; p.qb = q_bstride; p.P = P; p.S = S; p.ML = ML;
-  p.part = static_cast<float*>(ws); p.part_ml = p.part + (size_t)pl.units * Q * t->D;
-  p.vecq = t->D % 4 == 0 && aligned16(queries) && q_bstride % 4 == 0;
+  char* w = static_cast<char*>(ws);
+  p.qb = q_bstride ? (int64_t)Q * p.ldq : 0; p.P = P; p.S = S; p.ML = ML;
+  EP_TRY(mx_rows(queries, q_bstride ? (int64_t)t->B * Q : Q, t->D, w, &p.q, st));
+  p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + pl.pad); p.part_ml = p.part + (size_t)pl.units * Q * t->D;
   p.veco = t->D % 4 == 0 && aligned16(pl.splits > 1 ? (const void*)p.part : (const void*)P);
   p.vecs = p.vecs && aligned16(S);
   EP_TRY(mx_launch<false>(p, pl, st));
@@ -821,10 +836,12 @@ int mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S
   const MxPlan pl = mx_plan(t->B, t->N, t->D, Q, true, per_image != 0);
   EP_REQUIRE(ws_bytes >= pl.ws, EP_E_WORKSPACE, "ep_mx4_pool_backward: workspace %zu < %zu", ws_bytes, pl.ws);
   MxPool p = mx_pool_params(t, Q, scale, pl);
-  p.q = dP; p.Pin = P; p.S = const_cast<float*>(S); p.ML = const_cast<float*>(ML);
+  char* w = static_cast<char*>(ws);
+  EP_TRY(mx_rows(dP, (int64_t)t->B * Q, t->D, w, &p.q, st));
+  if (P) EP_TRY(mx_rows(P, (int64_t)t->B * Q, t->D, w, &p.Pin, st));
+  p.S = const_cast<float*>(S); p.ML = const_cast<float*>(ML);
   p.per_unit = per_image != 0;
-  p.part = per_image && pl.splits == 1 ? dq : static_cast<float*>(ws);
-  p.vecq = t->D % 4 == 0 && aligned16(dP) && aligned16(P);
+  p.part = per_image && pl.splits == 1 ? dq : reinterpret_cast<float*>(static_cast<char*>(ws) + pl.pad);
   p.veco = t->D % 4 == 0 && aligned16(p.part);
   p.vecs = p.vecs && aligned16(S);
   const int64_t QD = (int64_t)Q * t->D;
@@ -846,8 +863,8 @@ extern "C" {
 size_t ep_mx4_pool_workspace_bytes(int B, int N, int D, int Q) {
   if (B <= 0 || N <= 0 || D <= 0 || Q <= 0 || D > MX_MAX_D) return 0;
   size_t n = 256;
-  for (int k = 0; k < 3; ++k) {
-    const size_t w = mx_plan(B, N, D, Q, k > 0, k == 2).ws;
+  for (int k = 0; k < 4; ++k) {
+    const size_t w = mx_plan(B, N, D, Q, (k & 1) != 0, (k & 2) != 0).ws;
     n = w > n ? w : n;
   }
   return round_up(n, 256);
@@ -869,7 +886,8 @@ int ep_mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_
   EP_TRY(mx_pool_check(t, Q, workspace, workspace_bytes, "ep_mx4_pool_forward"));
   EP_REQUIRE(queries && P && ML, EP_E_ARG, "ep_mx4_pool_forward: null pointer");
   EP_REQUIRE(aligned16(ML), EP_E_ALIGN, "ep_mx4_pool_forward: ML must be 16-byte aligned");
-  EP_REQUIRE(q_bstride == 0 || q_bstride >= (int64_t)Q * t->D, EP_E_SHAPE, "ep_mx4_pool_forward: query batch stride %lld", (long long)q_bstride);
+  EP_REQUIRE(q_bstride == 0 || q_bstride == (int64_t)Q * t->D, EP_E_SHAPE, "ep_mx4_pool_forward: query batch stride %lld", (long long)q_bstride);
+  EP_REQUIRE(t->D % MX_BLOCK || aligned16(queries), EP_E_ALIGN, "ep_mx4_pool_forward: queries must be 16-byte aligned");
   return mx4_pool_forward(t, queries, q_bstride, Q, scale, P, S, ML, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
@@ -878,6 +896,7 @@ int ep_mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float
   EP_TRY(mx_pool_check(t, Q, workspace, workspace_bytes, "ep_mx4_pool_backward"));
   EP_REQUIRE(S && ML && dP && dq, EP_E_ARG, "ep_mx4_pool_backward: null pointer");
   EP_REQUIRE(aligned16(ML), EP_E_ALIGN, "ep_mx4_pool_backward: ML must be 16-byte aligned");
+  EP_REQUIRE(t->D % MX_BLOCK || (aligned16(dP) && aligned16(P)), EP_E_ALIGN, "ep_mx4_pool_backward: dP and P must be 16-byte aligned");
   EP_REQUIRE(!(per_image && accumulate), EP_E_UNSUPPORTED, "ep_mx4_pool_backward: accumulate is for shared queries");
   return mx4_pool_backward(t, Q, scale, S, ML, P, dP, dq, per_image, accumulate, workspace, workspace_bytes, (hipStream_t)stream);
 }

@@ -176,7 +176,12 @@ def _queries(cache: Mx4Tokens, queries: torch.Tensor, per_image: bool, B: int) -
         raise ValueError(f"queries must be {want}, got {tuple(queries.shape)}")
     if D > MAX_DIM:
         raise ValueError(f"the attention over a 4-bit cache takes at most {MAX_DIM} channels, got {D}")
-    return q, q.shape[-2]
+    return _aligned(q), q.shape[-2]
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """16-byte aligned storage, as the kernels read operand rows."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _workspace(B: int, n: int, D: int, Q: int, device) -> torch.Tensor:
@@ -211,7 +216,8 @@ def pool_backward(cache: Mx4Tokens, S: torch.Tensor, ML: torch.Tensor, dP: torch
     args = cache._args(image_index)
     B, n, D = args.B, args.N, args.D
     Q = S.shape[1] if S.dim() == 3 else -1
-    dP = F_._f32c(dP, "dP")
+    dP = _aligned(F_._f32c(dP, "dP"))
+    P = None if P is None else _aligned(P)
     for t, name, shape in ((S, "S", (B, Q, n)), (ML, "ML", (B, Q, 4)), (dP, "dP", (B, Q, D)), (P, "P", (B, Q, D))):
         if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float32 or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous float32 {shape}, got {tuple(t.shape)} {t.dtype}")

@@ -1193,7 +1193,7 @@ int ep_mx4_dequantize(const ep_mx4_tokens* t, void* out, int out_dtype, ep_strea
 /* Attention pooling over the cache: ep_pool_forward / ep_pool_backward / ep_pool_backward_per_image with x = the cache's
  * tokens.  queries (Q, D) with q_bstride 0, or (B, Q, D).  P (B, Q, D); ML (B, Q, 4) = {row max, sum exp(S - max), 0, 0};
  * S (B, Q, N) raw scores (-inf behind an image's length), NULL where no backward pass follows.  An image without tokens has
- * P = 0, max 0 and sum 0.  D <= 4096. */
+ * P = 0, max 0 and sum 0.  D <= 4096; where D is a multiple of 128, queries / P / dP are 16-byte aligned. */
 size_t ep_mx4_pool_workspace_bytes(int B, int N, int D, int Q);
 int ep_mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S,
                         float* ML, void* workspace, size_t workspace_bytes, ep_stream_t stream);
