@@ -345,9 +345,9 @@ SIGNATURES = {
     "ep_mx4_quantize": (c_int, [c_void, c_int, c_i64, c_i64, c_int, c_int, c_int, c_void, c_void, c_i64, c_i64, c_void]),
     "ep_mx4_dequantize": (c_int, [C.POINTER(EPMx4Tokens), c_void, c_int, c_void]),
     "ep_mx4_pool_workspace_bytes": (c_size, [c_int, c_int, c_int, c_int]),
-    "ep_mx4_pool_forward": (c_int, [C.POINTER(EPMx4Tokens), c_f32p, c_i64, c_int, c_float, c_f32p, c_f32p, c_f32p, c_void, c_size,
+    "ep_mx4_pool_forward": (c_int, [C.POINTER(EPMx4Tokens), c_f32p, c_i64, c_int, c_float, c_f32p, c_f32p, c_i64, c_f32p, c_void, c_size,
                                     c_void]),
-    "ep_mx4_pool_backward": (c_int, [C.POINTER(EPMx4Tokens), c_int, c_float, c_f32p, c_f32p, c_f32p, c_f32p, c_f32p, c_int, c_int,
+    "ep_mx4_pool_backward": (c_int, [C.POINTER(EPMx4Tokens), c_int, c_float, c_f32p, c_i64, c_f32p, c_f32p, c_f32p, c_f32p, c_int, c_int,
                                      c_void, c_size, c_void]),
     "ep_distill_workspace_bytes": (c_size, [c_int, c_int, c_int]),
     "ep_distill_topk": (c_int, [C.POINTER(EPDistillArgs), c_void, c_size, c_void]),

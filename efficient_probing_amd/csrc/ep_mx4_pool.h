@@ -12,18 +12,19 @@ struct MxPool {
   int Q, qblk;                           // all queries; queries of a blockIdx.y
   float scale;
   float* P; float* S; float* ML;
+  int64_t lds_;                          // row stride of S, a multiple of 4
   const float* Pin;                      // backward: P, or null (delta in ML[..][2])
   float* part; float* part_ml;           // partial results of units (forward splits, backward)
   int nc, nw, groups;                    // 128-channel blocks of a row; waves a row is cut over; such groups of waves in a workgroup
   int splits, tps, units;                // an image's tiles are cut into `splits` runs of `tps`; unit = image * splits + run
   int per_unit;                          // backward: a gradient per unit instead of per workgroup
   int ldq;                               // row stride of the operand rows
-  int vecs, veco;                        // 16-byte accesses to the scores / outputs
+  int veco;                              // 16-byte stores to the outputs
 };
 
-int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S, float* ML, void* ws,
+int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S, int64_t s_stride, float* ML, void* ws,
                      size_t ws_bytes, hipStream_t st);
-int mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S, const float* ML, const float* P, const float* dP, float* dq,
+int mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S, int64_t s_stride, const float* ML, const float* P, const float* dP, float* dq,
                       int per_image, int accumulate, void* ws, size_t ws_bytes, hipStream_t st);
 
 }  // namespace ep

@@ -7,9 +7,9 @@
 //
 //   * Tiles come HBM -> LDS by LDS-DMA into a ring of NST stages that the wave keeps to itself (no barrier on the data path).
 //   * First contraction (scores / dA), on the matrix cores in the cache's own format: v_mfma_scale_f32_16x16x128_f8f6f4 takes the
-//     E2M1 codes and their E8M0 scale bytes as they lie in LDS, no decoding.  The fp32 operand (queries, dP) becomes six E2M3
-//     terms with block scales 2^-4 apart: what is left over is below 2^-22 of a block's largest value.  All products are exact,
-//     the sums fp32.
+//     E2M1 codes and their E8M0 scale bytes as they lie in LDS, no decoding.  The fp32 operand (queries, dP) becomes five E2M3
+//     terms with block scales 2^-5 apart: below 2 that type is a fixed-point grid of 1/8, so every term takes five more bits and
+//     at most 2^-24 of a block's largest value is left over.  All products are exact, the sums fp32.
 //   * D-slices are added through LDS, one record per wave and tile, in wave order, one barrier per tile; every wave then holds the
 //     scores in the very lanes in which the second contraction wants its weights.
 //   * Weights (exp(S - max), or dS) are split into three bf16 terms, exactly.
@@ -39,7 +39,7 @@ constexpr float MX_LAZY = 12.0f;                 // the running maximum follows 
 template <int QM> struct MxDims {
   static constexpr int NQB = QM == 32 ? 2 : 1;   // blocks of query rows
   static constexpr int ROWS = QM == 8 ? 8 : 16;  // queries of a block
-  static constexpr int SETS = QM == 8 ? 3 : 6;   // matrix operands of the fp32 rows: six terms, two of them in one operand at QM 8
+  static constexpr int SETS = QM == 8 ? 3 : 5;   // matrix operands of the fp32 rows: five terms, two of them in one operand at QM 8
   static constexpr int SCB = QM == 8 ? 1 : 2;    // dwords of their scale bytes
   static constexpr int SV = QM == 8 ? 4 : 8;     // scores per lane, tile and query block
   static constexpr int PSETS = QM == 8 ? 2 : 3;  // operands of the weights
@@ -91,21 +91,21 @@ __device__ __forceinline__ void mx_operand(mx_f16 a, mx_f16 b, int c, MxOperand<
   }
   const int ex = (int)(am >> 23);
   const bool bad = ex == 255;                                  // an infinity or a NaN in the row: the scale byte 255 makes its scores NaN
-  const int s0 = bad ? 252 : (ex - 2 < 24 ? 24 : ex - 2);
+  const int s0 = bad ? 252 : (ex < 24 ? 24 : ex);              // the row lies below 2 * 2^(s0 - 127)
   const bool odd = QM == 8 && (c & 8) != 0;
   uint32_t bytes[2] = {0, 0};
 #pragma unroll
-  for (int t = 0; t < 6; ++t) {
-    const float sc = __uint_as_float((uint32_t)(s0 - 4 * t) << 23);
+  for (int t = 0; t < 5; ++t) {
+    const float sc = __uint_as_float((uint32_t)(s0 - 5 * t) << 23);
     const mx_u6 k = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, sc);
     asm volatile("" ::"v"(a), "v"(b), "v"(sc), "v"(k));
-    if (t < 5) {
+    if (t < 4) {
       const mx_f32 d = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(k, sc);
       asm volatile("" ::"v"(k), "v"(sc), "v"(d));
 #pragma unroll
       for (int i = 0; i < 16; ++i) { a[i] -= d[2 * i]; b[i] -= d[2 * i + 1]; }
     }
-    const uint32_t byte = bad ? 255u : (uint32_t)(s0 - 4 * t);
+    const uint32_t byte = bad ? 255u : (uint32_t)(s0 - 5 * t);
     if constexpr (QM == 8) {
       if (t % 2 == 0) { o.b[t / 2] = k; bytes[0] |= (odd ? 0u : byte) << (8 * (t / 2)); }
       else {
@@ -118,6 +118,10 @@ __device__ __forceinline__ void mx_operand(mx_f16 a, mx_f16 b, int c, MxOperand<
       bytes[t / 3] |= byte << (8 * (t % 3));
     }
     __builtin_amdgcn_sched_barrier(0);
+  }
+  if constexpr (QM == 8) {                                     // there is no sixth term
+#pragma unroll
+    for (int i = 0; i < 6; ++i) o.b[2][i] = odd ? 0u : o.b[2][i];
   }
   o.sc[0] = bytes[0];
   if constexpr (QM != 8) o.sc[1] = bytes[1];
@@ -151,6 +155,7 @@ struct MxCursor {
       tile = s * tps + toff;
       if (tile < hi) return;
     }
+    b = img = tile = hi = 0; len = 1;                                   // nothing left: loads go on, from the cache's first row
   }
   __device__ __forceinline__ bool next(const ep_mx4_tokens& t) {       // true: the next tile is another unit's (or there is none)
     tile += tstep;
@@ -179,8 +184,11 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
   char* exch = lds + nw * groups * (NST * STAGE);                      // [2][groups][nw][REC]
 
   // ---- lane constants
-  unsigned dma_tok[2], dma_seg = (unsigned)(((lane & 3) ^ g) * 16);
-  dma_tok[0] = 8 * ((lane >> 2) & 3) + g; dma_tok[1] = dma_tok[0] + 4;
+  const unsigned dma_seg = (unsigned)(((lane & 3) ^ g) * 16);          // LDS row r of a tile holds token 8 (r % 4) + r / 4, its 16-byte
+  const int dma_tok = 8 * ((lane >> 2) & 3) + g;                       // pieces XOR-ed with r / 4: both contractions read all banks
+  const unsigned dma_full = (unsigned)(dma_tok * rowC) + dma_seg;
+  const unsigned scl_full = (unsigned)((lane & 31) * rowS);
+  const int tok0 = 8 * g + (QM == 8 ? 4 * (c >> 3) : 0);               // first token of the lane's scores in a tile
   const int sc_off = (8 * (c >> 2) + (c & 3)) * 4;                     // + 16 h: scale dword of the score row
   const int a_off = (4 * (c & 3) + (c >> 2)) * 64 + ((g ^ (c & 3)) << 4);
   int p_off[4];
@@ -190,24 +198,25 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
 
   auto issue = [&](const MxCursor& cu, int slot) {
     char* st = ring + slot * STAGE;
-    const int t0 = cu.tile << 5, rows = cu.len - t0;                   // rows behind the image's end repeat its last one
+    const int t0 = cu.tile << 5, rows = cu.len - t0;
     const uint8_t* src = t.codes + (int64_t)cu.img * t.codes_bstride + (int64_t)t0 * rowC;
     const uint8_t* scl = t.scales + (int64_t)cu.img * t.scales_bstride + (int64_t)t0 * rowS;
+    unsigned off0 = dma_full, off1 = dma_full + 4 * rowC, offs = scl_full;
+    if (rows < 32) {                                                   // rows behind the image's end repeat its last one
+      off0 = (unsigned)((dma_tok < rows ? dma_tok : rows - 1) * rowC) + dma_seg;
+      off1 = (unsigned)((dma_tok + 4 < rows ? dma_tok + 4 : rows - 1) * rowC) + dma_seg;
+      offs = (unsigned)(((lane & 31) < rows ? (lane & 31) : rows - 1) * rowS);
+    }
 #pragma unroll
     for (int k = 0; k < CPW; ++k) {
       const int ch = chunk0 + k < nc ? chunk0 + k : nc - 1;            // a slice that the row does not fill repeats its last block
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int tok = (int)dma_tok[h] < rows ? (int)dma_tok[h] : rows - 1;
-        __builtin_amdgcn_global_load_lds((mx_gptr_t)(src + (unsigned)(tok * rowC + ch * 64) + dma_seg), (mx_lds_t)(st + k * 2048 + h * 1024), 16, 0, MX_NT);
-      }
+      __builtin_amdgcn_global_load_lds((mx_gptr_t)(src + ch * 64 + off0), (mx_lds_t)(st + k * 2048), 16, 0, MX_NT);
+      __builtin_amdgcn_global_load_lds((mx_gptr_t)(src + ch * 64 + off1), (mx_lds_t)(st + k * 2048 + 1024), 16, 0, MX_NT);
     }
 #pragma unroll
-    for (int k = 0; k < CPW; k += 2) {
-      const int kk = k + (lane >> 5) < CPW ? k + (lane >> 5) : CPW - 1;
-      const int ch = chunk0 + kk < nc ? chunk0 + kk : nc - 1;
-      const int tok = (lane & 31) < rows ? (lane & 31) : rows - 1;
-      __builtin_amdgcn_global_load_lds((mx_gptr_t)(scl + (unsigned)(tok * rowS + ch * 4)), (mx_lds_t)(st + CODES + k * 128), 4, 0, 0);
+    for (int k = 0; k < CPW; k += 2) {                                 // lanes 32-63: the second block
+      const int ch0 = chunk0 + k < nc ? chunk0 + k : nc - 1, ch1 = k + 1 < CPW && ch0 + 1 < nc ? ch0 + 1 : ch0;
+      __builtin_amdgcn_global_load_lds((mx_gptr_t)(scl + (offs + (unsigned)(lane < 32 ? ch0 : ch1) * 4u)), (mx_lds_t)(st + CODES + k * 128), 4, 0, 0);
     }
   };
 
@@ -217,13 +226,23 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
   else { cu.u = (int)blockIdx.x; cu.ustep = (int)gridDim.x; cu.toff = grp; cu.tstep = groups; }
   MxCursor ahead = cu;                                                  // the next tile to load
   ahead.open(t);
-  int islot = 0;
+  float sg[NQB][SV];                                                    // backward: saved scores of the next tile
+  auto load_scores = [&](const MxCursor& cu) {
 #pragma unroll
-  for (int i = 0; i < NST; ++i) {
-    if (ahead.valid()) { issue(ahead, islot); ahead.next(t); }
-    islot = islot + 1 == NST ? 0 : islot + 1;
-  }
-  if (!ahead.valid()) mx_wait_vm<0>();                                  // fewer tiles than stages: the counted waits assume a full ring
+    for (int qb = 0; qb < NQB; ++qb) {
+      const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+      const float* row = p.S + ((int64_t)cu.b * p.Q + q0) * p.lds_;
+#pragma unroll
+      for (int h = 0; h < SV / 4; ++h) {
+        const int n = (cu.tile << 5) + tok0 + 4 * h;
+        const f4 v = *reinterpret_cast<const f4*>(row + (unsigned)((q < qn ? q : 0) * (int)p.lds_ + (n < p.lds_ ? n : (int)p.lds_ - 4)));
+        sg[qb][4 * h] = v.x; sg[qb][4 * h + 1] = v.y; sg[qb][4 * h + 2] = v.z; sg[qb][4 * h + 3] = v.w;
+      }
+    }
+  };
+  if constexpr (BWD) load_scores(ahead);
+#pragma unroll
+  for (int i = 0; i < NST; ++i) { issue(ahead, i); ahead.next(t); }
 
   // ---- operand rows
   MxOperand<QM> op[NQB][CPW];
@@ -254,6 +273,24 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
   };
   float delta[NQB];
 
+  float m_run[NQB], mz[NQB], l_run[NQB], t_max[NQB], invl[NQB];         // mz: the maximum that weights are taken against
+  auto open_unit = [&](int b) {                                         // backward: dP's rows and the saved statistics
+    load_operand(p.q + (int64_t)b * p.Q * p.ldq, p.Pin ? p.Pin + (int64_t)b * p.Q * p.ldq : nullptr, 1.f, delta);
+#pragma unroll
+    for (int qb = 0; qb < NQB; ++qb) {
+      const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+      f4 ml = {0.f, 0.f, 0.f, 0.f};
+      if (q < qn) ml = *reinterpret_cast<const f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4);
+      mz[qb] = ml.x;
+      invl[qb] = ml.y == 0.f ? 0.f : 1.f / ml.y;
+      if (!p.Pin && dw == 0) delta[qb] = ml.z;                          // (each D-slice takes off its own part of delta)
+    }
+  };
+  if constexpr (BWD) {
+    cu.open(t);
+    if (cu.valid()) open_unit(cu.b);                                    // in front of the accumulators: most launches have one unit a wave
+  }
+
   f4 acc[NQB][CPW][8];
   auto clear = [&]() {
 #pragma unroll
@@ -264,9 +301,6 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
         for (int j = 0; j < 8; ++j) acc[qb][k][j] = f4{0.f, 0.f, 0.f, 0.f};
   };
   clear();
-  float m_run[NQB], mz[NQB], l_run[NQB], t_max[NQB], invl[NQB];       // mz: the maximum that weights are taken against
-  const int hh = QM == 8 ? c >> 3 : 0;                                  // QM 8: the lane's half of the 8 tokens
-  const int tok0 = 8 * g + 4 * hh;                                      // first token of the lane's scores in a tile
   int slot = 0, buf = 0;
 
   // acc rows 4 g + i of query block qb are queries qrow(i); multiply each by the value that lane (c = query) holds
@@ -283,32 +317,9 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
   // one tile: `work` false where this wave only keeps the barrier
   auto tile_step = [&](bool work, int b, int t0, int len) {
     float s[NQB][SV];
-    float sg[NQB][BWD ? SV : 1];                                        // backward: the saved scores
     const char* st = ring + slot * STAGE;
     if (work) {
       mx_wait_vm<(NST - 1) * OPS>();
-      if constexpr (BWD) {
-#pragma unroll
-        for (int qb = 0; qb < NQB; ++qb) {
-          const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-          const float* sp = p.S + ((int64_t)b * p.Q + q0 + q) * t.N + t0 + tok0;
-#pragma unroll
-          for (int h = 0; h < SV / 4; ++h) {
-            f4 v = {0.f, 0.f, 0.f, 0.f};
-            const int n = t0 + tok0 + 4 * h;
-            if (q < qn) {
-              if (p.vecs) { if (n < t.N) v = *reinterpret_cast<const f4*>(sp + 4 * h); }
-              else {
-                if (n < t.N) v.x = sp[4 * h];
-                if (n + 1 < t.N) v.y = sp[4 * h + 1];
-                if (n + 2 < t.N) v.z = sp[4 * h + 2];
-                if (n + 3 < t.N) v.w = sp[4 * h + 3];
-              }
-            }
-            sg[qb][4 * h] = v.x; sg[qb][4 * h + 1] = v.y; sg[qb][4 * h + 2] = v.z; sg[qb][4 * h + 3] = v.w;
-          }
-        }
-      }
       // first contraction
       f4 sa[NQB][2], sl[NQB][2];                                        // leading and lower terms: an addition to a large sum costs its last bit
 #pragma unroll
@@ -324,7 +335,6 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
             const MxOperand<QM>& o = op[qb][k];
             sa[qb][h] = mx_mfma_codes<0>(w, sc, o.b[0], o.sc[0], sa[qb][h]);
             if constexpr (QM != 8) {
-              sl[qb][h] = mx_mfma_codes<2>(w, sc, o.b[5], o.sc[1], sl[qb][h]);
               sl[qb][h] = mx_mfma_codes<1>(w, sc, o.b[4], o.sc[1], sl[qb][h]);
               sl[qb][h] = mx_mfma_codes<0>(w, sc, o.b[3], o.sc[1], sl[qb][h]);
             }
@@ -386,17 +396,10 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
         if (p.S && dw == 0) {
           const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
           if (q < qn) {
-            float* sp = p.S + ((int64_t)b * p.Q + q0 + q) * t.N + t0 + tok0;
+            float* sp = p.S + ((int64_t)b * p.Q + q0 + q) * p.lds_ + t0 + tok0;
 #pragma unroll
-            for (int h = 0; h < SV / 4; ++h) {
-              const int n = t0 + tok0 + 4 * h;
-              if (p.vecs) { if (n < t.N) *reinterpret_cast<f4*>(sp + 4 * h) = f4{s[qb][4 * h], s[qb][4 * h + 1], s[qb][4 * h + 2], s[qb][4 * h + 3]}; }
-              else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (n + i < t.N) sp[4 * h + i] = s[qb][4 * h + i];
-              }
-            }
+            for (int h = 0; h < SV / 4; ++h)
+              if (t0 + tok0 + 4 * h < t.N) *reinterpret_cast<f4*>(sp + 4 * h) = f4{s[qb][4 * h], s[qb][4 * h + 1], s[qb][4 * h + 2], s[qb][4 * h + 3]};
           }
         }
         float mx = s[qb][0];
@@ -483,10 +486,15 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
       __builtin_amdgcn_sched_barrier(0);
 #undef EP_MX_PAIR
     }
-    // the stage is read: load the tile NST further on into it
+  };
+  // the stage is read: load the tile NST further on into it.  The loads always are the same number (at the end of the sequence they
+  // repeat one row), so a counted wait means the same everywhere; the next tile's scores are asked for in front of them, so that
+  // waiting for the scores does not wait for the tile.
+  auto refill = [&]() {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (ahead.valid()) { issue(ahead, slot); ahead.next(t); }
-    else mx_wait_vm<0>();                                               // the last tiles: fewer loads are under way than the counted wait assumes
+    if constexpr (BWD) load_scores(cu);
+    issue(ahead, slot);
+    ahead.next(t);
     slot = slot + 1 == NST ? 0 : slot + 1;
   };
 
@@ -556,10 +564,14 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
 #pragma unroll
       for (int qb = 0; qb < NQB; ++qb) { m_run[qb] = t_max[qb] = -INFINITY; mz[qb] = l_run[qb] = 0.f; }
       clear();
-      for (int tl = lo; tl < hi; tl += groups) tile_step(tl + grp < hi, b, (tl + grp) << 5, len);
+      for (int tl = lo; tl < hi; tl += groups) {
+        const bool work = tl + grp < hi;
+        tile_step(work, b, (tl + grp) << 5, len);
+        if (work) refill();
+      }
       if (p.S && sp == p.splits - 1 && dw == 0 && grp == 0) {           // scores behind the image's tiles
         for (int q = 0; q < qn; ++q)
-          for (int i = (n << 5) + lane; i < t.N; i += 64) p.S[((int64_t)b * p.Q + q0 + q) * t.N + i] = img < 0 ? __uint_as_float(0x7fc00000u) : -INFINITY;
+          for (int i = (n << 5) + lane; i < t.N; i += 64) p.S[((int64_t)b * p.Q + q0 + q) * p.lds_ + i] = img < 0 ? __uint_as_float(0x7fc00000u) : -INFINITY;
       }
       float f[NQB];
 #pragma unroll
@@ -569,6 +581,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
         t_max[qb] = mx_over_groups_max(t_max[qb]);
       }
       if (groups > 1) {                                                 // (one unit per workgroup then: the ring is idle)
+        mx_wait_vm<0>();
         float* ml = reinterpret_cast<float*>(exch);                     // [groups][NQB][16][3]
         mx_barrier();
         if (dw == 0 && g == 0) {
@@ -615,20 +628,9 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
     float one[NQB];
 #pragma unroll
     for (int qb = 0; qb < NQB; ++qb) one[qb] = p.scale;
-    auto open_unit = [&](int b) {
-      load_operand(p.q + (int64_t)b * p.Q * p.ldq, p.Pin ? p.Pin + (int64_t)b * p.Q * p.ldq : nullptr, 1.f, delta);
-#pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) {
-        const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-        f4 ml = {0.f, 0.f, 0.f, 0.f};
-        if (q < qn) ml = *reinterpret_cast<const f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4);
-        mz[qb] = ml.x;
-        invl[qb] = ml.y == 0.f ? 0.f : 1.f / ml.y;
-        if (!p.Pin && dw == 0) delta[qb] = ml.z;                        // (each D-slice takes off its own part of delta)
-      }
-    };
     if (p.per_unit) {                                                   // images (and runs) without a token are not visited below
       MxCursor z = cu;
+      z.u = (int)blockIdx.x * groups + grp;
       for (; z.u < z.units; z.u += z.ustep) {
         const int b = z.u / z.splits;
         int len;
@@ -636,8 +638,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
         if ((z.u - b * z.splits) * z.tps >= (len + 31) >> 5) store_rows(p.part + (int64_t)z.u * p.Q * t.D, one);
       }
     }
-    cu.open(t);
-    bool fresh = true;
+    bool fresh = false;
     const int iters = nw > 1 ? (int)((p.units + cu.ustep - 1) / cu.ustep) * p.tps : 0;
     for (int it = 0; nw > 1 ? it < iters : cu.valid(); ++it) {
       const bool work = cu.valid();
@@ -646,6 +647,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
       if (!work) continue;
       const int u = cu.u;
       fresh = cu.next(t);
+      refill();
       if (fresh && p.per_unit) {                                        // one gradient per image (and split)
         store_rows(p.part + (int64_t)u * p.Q * t.D, one);
         clear();
@@ -656,53 +658,72 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
       if (grp == 0) store_rows(p.part + (int64_t)blockIdx.x * p.Q * t.D, one);
     }
   }
+  mx_wait_vm<0>();                                                      // no load into LDS outlives its wave
 }
 
-// joins the splits of an image: one workgroup per (image, query)
+// joins the splits of an image: blockIdx.x = (image, query), blockIdx.y = 64 channels; 16 chains of splits side by side
 __global__ __launch_bounds__(256) void ep_mx4_join_kernel(const float* __restrict__ part, const float* __restrict__ ml, int splits, int Q, int D,
                                                           float* __restrict__ P, float* __restrict__ ML) {
+  __shared__ float red[16][64 + 4];
   const int b = (int)(blockIdx.x / (unsigned)Q), q = (int)(blockIdx.x % (unsigned)Q);
+  const float* e = ml + ((int64_t)b * splits * Q + q) * 2;             // {maximum, sum} of split s at e[s * 2 Q]
+  const int lane = lane_id();
   float m = -INFINITY, l = 0.f;
   bool bad = false;
-  for (int s = 0; s < splits; ++s) {
-    const float v = ml[(((int64_t)b * splits + s) * Q + q) * 2];
-    bad |= v != v;
-    m = fmaxf(m, v);
+  for (int s = lane; s < splits; s += 64) { const float v = e[(int64_t)s * 2 * Q]; bad |= v != v; m = fmaxf(m, v); }
+  m = wave_max(m);
+  for (int s = lane; s < splits; s += 64) {
+    const float v = e[(int64_t)s * 2 * Q + 1];
+    if (v != 0.f) l += v * __builtin_amdgcn_exp2f((e[(int64_t)s * 2 * Q] - m) * MX_LOG2E);
   }
-  for (int s = 0; s < splits; ++s) {
-    const float* e = ml + (((int64_t)b * splits + s) * Q + q) * 2;
-    if (e[1] != 0.f) l += e[1] * __builtin_amdgcn_exp2f((e[0] - m) * MX_LOG2E);
+  l = wave_sum(l);
+  if (__any(bad)) m = l = __uint_as_float(0x7fc00000u);
+  if (threadIdx.x == 0 && blockIdx.y == 0) *reinterpret_cast<f4*>(ML + ((int64_t)b * Q + q) * 4) = f4{l == 0.f ? 0.f : m, l, 0.f, 0.f};
+  const int x = (int)threadIdx.x & 15, y = (int)threadIdx.x >> 4, d0 = (int)blockIdx.y * 64;
+  f4 a = {0.f, 0.f, 0.f, 0.f};
+  for (int s = y; s < splits; s += 16) {
+    if (e[(int64_t)s * 2 * Q + 1] == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f((e[(int64_t)s * 2 * Q] - m) * MX_LOG2E);
+    const float* row = part + (((int64_t)b * splits + s) * Q + q) * D + d0 + 4 * x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (d0 + 4 * x + j < D) a[j] += f * row[j];
   }
-  if (bad) m = l = __uint_as_float(0x7fc00000u);
-  if (threadIdx.x == 0) *reinterpret_cast<f4*>(ML + ((int64_t)b * Q + q) * 4) = f4{l == 0.f ? 0.f : m, l, 0.f, 0.f};
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  for (int d = (int)threadIdx.x; d < D; d += 256) {
-    float a = 0.f;
-    for (int s = 0; s < splits; ++s) {
-      const int64_t r = ((int64_t)b * splits + s) * Q + q;
-      const float mv = ml[r * 2];
-      if (ml[r * 2 + 1] != 0.f) a += part[r * D + d] * __builtin_amdgcn_exp2f((mv - m) * MX_LOG2E);
-    }
-    P[((int64_t)b * Q + q) * D + d] = a * inv;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) red[y][4 * x + j] = a[j];
+  __syncthreads();
+  if (threadIdx.x < 64 && d0 + (int)threadIdx.x < D) {
+    float r = red[0][threadIdx.x];
+    for (int k = 1; k < 16; ++k) r += red[k][threadIdx.x];
+    P[((int64_t)b * Q + q) * D + d0 + threadIdx.x] = r * (l == 0.f ? 0.f : 1.f / l);
   }
 }
 
-// out[i] (+)= sum over n of part[n][i], in order of n within 16 interleaved chains and then the chains: blockIdx.y selects the output
+// out[i] (+)= sum over n of part[n][i], 16 interleaved chains and then these in order; blockIdx.y selects the output
 __global__ __launch_bounds__(256) void ep_mx4_sum_kernel(const float* __restrict__ part, int n, int64_t len, float* __restrict__ out, int accumulate) {
-  __shared__ float red[16][17];
+  __shared__ float red[16][64 + 4];
   const int x = (int)threadIdx.x & 15, y = (int)threadIdx.x >> 4;
-  const int64_t i = (int64_t)blockIdx.x * 16 + x;
+  const int64_t i = (int64_t)blockIdx.x * 64 + 4 * x;
   const float* src = part + (int64_t)blockIdx.y * n * len;
-  float s = 0.f;
-  if (i < len)
-    for (int r = y; r < n; r += 16) s += src[(int64_t)r * len + i];
-  red[y][x] = s;
+  f4 s = {0.f, 0.f, 0.f, 0.f};
+  if (len % 4 == 0) {
+    if (i < len)
+      for (int r = y; r < n; r += 16) s += *reinterpret_cast<const f4*>(src + (int64_t)r * len + i);
+  } else {
+    for (int r = y; r < n; r += 16)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j < len) s[j] += src[(int64_t)r * len + i + j];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) red[y][4 * x + j] = s[j];
   __syncthreads();
-  if (y == 0 && i < len) {
-    float a = red[0][x];
-    for (int r = 1; r < 16; ++r) a += red[r][x];
-    float* o = out + (int64_t)blockIdx.y * len + i;
-    *o = accumulate ? *o + a : a;
+  const int64_t o = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  if (threadIdx.x < 64 && o < len) {
+    float a = red[0][threadIdx.x];
+    for (int k = 1; k < 16; ++k) a += red[k][threadIdx.x];
+    float* dst = out + (int64_t)blockIdx.y * len + o;
+    *dst = accumulate ? *dst + a : a;
   }
 }
 
@@ -808,11 +829,11 @@ static MxPool mx_pool_params(const ep_mx4_tokens* t, int Q, float scale, const M
   MxPool p{};
   p.t = *t; p.Q = Q; p.scale = scale; p.nc = mx_blocks(t->D);
   p.nw = pl.nw; p.groups = pl.groups; p.splits = pl.splits; p.tps = pl.tps; p.units = pl.units; p.qblk = pl.qblk;
-  p.vecs = t->N % 4 == 0; p.ldq = p.nc * MX_BLOCK;
+  p.ldq = p.nc * MX_BLOCK;
   return p;
 }
 
-int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S, float* ML, void* ws,
+int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S, int64_t s_stride, float* ML, void* ws,
                      size_t ws_bytes, hipStream_t st) {
   const MxPlan pl = mx_plan(t->B, t->N, t->D, Q, false, q_bstride != 0);
   EP_REQUIRE(ws_bytes >= pl.ws, EP_E_WORKSPACE, "ep_mx4_pool_forward: workspace %zu < %zu", ws_bytes, pl.ws);
@@ -822,16 +843,16 @@ int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bst
   EP_TRY(mx_rows(queries, q_bstride ? (int64_t)t->B * Q : Q, t->D, w, &p.q, st));
   p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + pl.pad); p.part_ml = p.part + (size_t)pl.units * Q * t->D;
   p.veco = t->D % 4 == 0 && aligned16(pl.splits > 1 ? (const void*)p.part : (const void*)P);
-  p.vecs = p.vecs && aligned16(S);
+  p.lds_ = s_stride;
   EP_TRY(mx_launch<false>(p, pl, st));
   if (pl.splits > 1) {
-    hipLaunchKernelGGL(ep_mx4_join_kernel, dim3((unsigned)t->B * Q), dim3(256), 0, st, p.part, p.part_ml, pl.splits, Q, t->D, P, ML);
+    hipLaunchKernelGGL(ep_mx4_join_kernel, dim3((unsigned)t->B * Q, (unsigned)((t->D + 63) / 64)), dim3(256), 0, st, p.part, p.part_ml, pl.splits, Q, t->D, P, ML);
     EP_LAUNCH_CHECK("ep_mx4_join_kernel");
   }
   return 0;
 }
 
-int mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S, const float* ML, const float* P, const float* dP, float* dq,
+int mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S, int64_t s_stride, const float* ML, const float* P, const float* dP, float* dq,
                       int per_image, int accumulate, void* ws, size_t ws_bytes, hipStream_t st) {
   const MxPlan pl = mx_plan(t->B, t->N, t->D, Q, true, per_image != 0);
   EP_REQUIRE(ws_bytes >= pl.ws, EP_E_WORKSPACE, "ep_mx4_pool_backward: workspace %zu < %zu", ws_bytes, pl.ws);
@@ -843,12 +864,12 @@ int mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S
   p.per_unit = per_image != 0;
   p.part = per_image && pl.splits == 1 ? dq : reinterpret_cast<float*>(static_cast<char*>(ws) + pl.pad);
   p.veco = t->D % 4 == 0 && aligned16(p.part);
-  p.vecs = p.vecs && aligned16(S);
+  p.lds_ = s_stride;
   const int64_t QD = (int64_t)Q * t->D;
   EP_TRY(mx_launch<true>(p, pl, st));
   if (!per_image || pl.splits > 1) {
     const int n = per_image ? pl.splits : pl.grid;
-    hipLaunchKernelGGL(ep_mx4_sum_kernel, dim3((unsigned)((QD + 15) / 16), per_image ? (unsigned)t->B : 1u), dim3(256), 0, st, p.part, n, QD, dq, accumulate);
+    hipLaunchKernelGGL(ep_mx4_sum_kernel, dim3((unsigned)((QD + 63) / 64), per_image ? (unsigned)t->B : 1u), dim3(256), 0, st, p.part, n, QD, dq, accumulate);
     EP_LAUNCH_CHECK("ep_mx4_sum_kernel");
   }
   return 0;
@@ -881,24 +902,28 @@ static int mx_pool_check(const ep_mx4_tokens* t, int Q, void* ws, size_t bytes, 
   return 0;
 }
 
-int ep_mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S, float* ML, void* workspace,
+int ep_mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S, int64_t s_stride, float* ML, void* workspace,
                         size_t workspace_bytes, ep_stream_t stream) {
   EP_TRY(mx_pool_check(t, Q, workspace, workspace_bytes, "ep_mx4_pool_forward"));
   EP_REQUIRE(queries && P && ML, EP_E_ARG, "ep_mx4_pool_forward: null pointer");
+  EP_REQUIRE(!S || (aligned16(S) && s_stride % 4 == 0 && s_stride >= t->N && Q * s_stride <= 2147483647), EP_E_ALIGN,
+             "ep_mx4_pool_forward: S must be 16-byte aligned, its row stride (%lld) a multiple of 4, at least N", (long long)s_stride);
   EP_REQUIRE(aligned16(ML), EP_E_ALIGN, "ep_mx4_pool_forward: ML must be 16-byte aligned");
   EP_REQUIRE(q_bstride == 0 || q_bstride == (int64_t)Q * t->D, EP_E_SHAPE, "ep_mx4_pool_forward: query batch stride %lld", (long long)q_bstride);
   EP_REQUIRE(t->D % MX_BLOCK || aligned16(queries), EP_E_ALIGN, "ep_mx4_pool_forward: queries must be 16-byte aligned");
-  return mx4_pool_forward(t, queries, q_bstride, Q, scale, P, S, ML, workspace, workspace_bytes, (hipStream_t)stream);
+  return mx4_pool_forward(t, queries, q_bstride, Q, scale, P, S, s_stride, ML, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
-int ep_mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S, const float* ML, const float* P, const float* dP, float* dq,
+int ep_mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S, int64_t s_stride, const float* ML, const float* P, const float* dP, float* dq,
                          int per_image, int accumulate, void* workspace, size_t workspace_bytes, ep_stream_t stream) {
   EP_TRY(mx_pool_check(t, Q, workspace, workspace_bytes, "ep_mx4_pool_backward"));
   EP_REQUIRE(S && ML && dP && dq, EP_E_ARG, "ep_mx4_pool_backward: null pointer");
+  EP_REQUIRE(aligned16(S) && s_stride % 4 == 0 && s_stride >= t->N && Q * s_stride <= 2147483647, EP_E_ALIGN,
+             "ep_mx4_pool_backward: S must be 16-byte aligned, its row stride (%lld) a multiple of 4, at least N", (long long)s_stride);
   EP_REQUIRE(aligned16(ML), EP_E_ALIGN, "ep_mx4_pool_backward: ML must be 16-byte aligned");
   EP_REQUIRE(t->D % MX_BLOCK || (aligned16(dP) && aligned16(P)), EP_E_ALIGN, "ep_mx4_pool_backward: dP and P must be 16-byte aligned");
   EP_REQUIRE(!(per_image && accumulate), EP_E_UNSUPPORTED, "ep_mx4_pool_backward: accumulate is for shared queries");
-  return mx4_pool_backward(t, Q, scale, S, ML, P, dP, dq, per_image, accumulate, workspace, workspace_bytes, (hipStream_t)stream);
+  return mx4_pool_backward(t, Q, scale, S, s_stride, ML, P, dP, dq, per_image, accumulate, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -184,6 +184,11 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _padded(n: int) -> int:
+    """Row stride of saved scores: whole 16-byte pieces."""
+    return (n + 3) // 4 * 4
+
+
 def _workspace(B: int, n: int, D: int, Q: int, device) -> torch.Tensor:
     return torch.empty(N.load().ep_mx4_pool_workspace_bytes(B, n, D, Q), device=device, dtype=torch.uint8)
 
@@ -191,19 +196,19 @@ def _workspace(B: int, n: int, D: int, Q: int, device) -> torch.Tensor:
 def pool_forward(cache: Mx4Tokens, queries: torch.Tensor, scale: float, per_image_queries: bool = False,
                  image_index: Optional[torch.Tensor] = None, need_scores: bool = True):
     """``functional.pool_forward`` over a 4-bit cache: P (B, Q, D), S (B, Q, N) or None without ``need_scores``, ML (B, Q, 4) with the
-    row maximum and the sum of exponentials.  ``queries`` (Q, D) / (1, Q, D), or (B, Q, D) with ``per_image_queries``.  Tokens behind an
+    row maximum and the sum of exponentials (S is a view of rows padded to a multiple of 4).  ``queries`` (Q, D) / (1, Q, D), or (B, Q, D) with ``per_image_queries``.  Tokens behind an
     image's length have score -inf; an image without tokens pools to 0; an index outside the cache gives NaN."""
     args = cache._args(image_index)
     B, n, D = args.B, args.N, args.D
     q, Q = _queries(cache, queries, per_image_queries, B)
     dev = _on(cache.codes, q, image_index)
     P = torch.empty((B, Q, D), device=dev, dtype=torch.float32)
-    S = torch.empty((B, Q, n), device=dev, dtype=torch.float32) if need_scores else None
+    S = torch.empty((B, Q, _padded(n)), device=dev, dtype=torch.float32)[:, :, :n] if need_scores else None
     ML = torch.empty((B, Q, 4), device=dev, dtype=torch.float32)
     ws = _workspace(B, n, D, Q, dev)
     with torch.cuda.device(dev):
         N.check(N.load().ep_mx4_pool_forward(C.byref(args), q.data_ptr(), Q * D if per_image_queries else 0, Q, float(scale), P.data_ptr(),
-                                             F_._ptr(S), ML.data_ptr(), ws.data_ptr(), ws.numel(), N.current_stream_ptr(dev)), "ep_mx4_pool_forward")
+                                             F_._ptr(S), _padded(n), ML.data_ptr(), ws.data_ptr(), ws.numel(), N.current_stream_ptr(dev)), "ep_mx4_pool_forward")
     return P, S, ML
 
 
@@ -218,7 +223,11 @@ def pool_backward(cache: Mx4Tokens, S: torch.Tensor, ML: torch.Tensor, dP: torch
     Q = S.shape[1] if S.dim() == 3 else -1
     dP = _aligned(F_._f32c(dP, "dP"))
     P = None if P is None else _aligned(P)
-    for t, name, shape in ((S, "S", (B, Q, n)), (ML, "ML", (B, Q, 4)), (dP, "dP", (B, Q, D)), (P, "P", (B, Q, D))):
+    if tuple(S.shape) != (B, Q, n) or S.dtype != torch.float32:
+        raise ValueError(f"S must be float32 {(B, Q, n)}, got {tuple(S.shape)} {S.dtype}")
+    if S.stride(2) != 1 or S.stride(1) % 4 or S.stride(1) < n or S.stride(0) != Q * S.stride(1) or S.data_ptr() % 16:
+        S = torch.nn.functional.pad(S, (0, _padded(n) - n)).contiguous()      # not as pool_forward left it
+    for t, name, shape in ((ML, "ML", (B, Q, 4)), (dP, "dP", (B, Q, D)), (P, "P", (B, Q, D))):
         if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float32 or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous float32 {shape}, got {tuple(t.shape)} {t.dtype}")
     if D > MAX_DIM:
@@ -235,7 +244,7 @@ def pool_backward(cache: Mx4Tokens, S: torch.Tensor, ML: torch.Tensor, dP: torch
     dev = _on(cache.codes, S, ML, dP, P, dq, image_index)
     ws = _workspace(B, n, D, Q, dev)
     with torch.cuda.device(dev):
-        N.check(N.load().ep_mx4_pool_backward(C.byref(args), Q, float(scale), S.data_ptr(), ML.data_ptr(), F_._ptr(P), dP.data_ptr(),
+        N.check(N.load().ep_mx4_pool_backward(C.byref(args), Q, float(scale), S.data_ptr(), S.stride(1), ML.data_ptr(), F_._ptr(P), dP.data_ptr(),
                                               dq.data_ptr(), int(per_image_queries), int(accumulate), ws.data_ptr(), ws.numel(),
                                               N.current_stream_ptr(dev)), "ep_mx4_pool_backward")
     return dq

@@ -1192,14 +1192,15 @@ int ep_mx4_quantize(const void* x, int x_dtype, int64_t x_bstride, int64_t x_tst
 int ep_mx4_dequantize(const ep_mx4_tokens* t, void* out, int out_dtype, ep_stream_t stream);
 /* Attention pooling over the cache: ep_pool_forward / ep_pool_backward / ep_pool_backward_per_image with x = the cache's
  * tokens.  queries (Q, D) with q_bstride 0, or (B, Q, D).  P (B, Q, D); ML (B, Q, 4) = {row max, sum exp(S - max), 0, 0};
- * S (B, Q, N) raw scores (-inf behind an image's length), NULL where no backward pass follows.  An image without tokens has
+ * S raw scores, rows (b, q) s_stride floats apart (a multiple of 4, at least N; -inf behind an image's length), NULL where no
+ * backward pass follows.  An image without tokens has
  * P = 0, max 0 and sum 0.  D <= 4096; where D is a multiple of 128, queries / P / dP are 16-byte aligned. */
 size_t ep_mx4_pool_workspace_bytes(int B, int N, int D, int Q);
 int ep_mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bstride, int Q, float scale, float* P, float* S,
-                        float* ML, void* workspace, size_t workspace_bytes, ep_stream_t stream);
+                        int64_t s_stride, float* ML, void* workspace, size_t workspace_bytes, ep_stream_t stream);
 /* dq (Q, D) summed over the batch in a fixed order, or, with per_image != 0, (B, Q, D).  delta = dP . P per row is computed from
  * P, or read from ML[..][2] where P is NULL (ep_project_backward leaves it there).  accumulate adds to dq. */
-int ep_mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S, const float* ML, const float* P,
+int ep_mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S, int64_t s_stride, const float* ML, const float* P,
                          const float* dP, float* dq, int per_image, int accumulate, void* workspace, size_t workspace_bytes,
                          ep_stream_t stream);
 

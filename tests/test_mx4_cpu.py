@@ -75,7 +75,7 @@ def test_c_entries_refuse_on_the_host():
 
     def fwd(q=buf.data_ptr(), Q=3, ws=buf.data_ptr() // 16 * 16, nb=need, **over):
         t = N.EPMx4Tokens(**{**ok, **over})
-        return lib.ep_mx4_pool_forward(C.byref(t), q, 0, Q, 1.0, buf.data_ptr(), 0, buf.data_ptr() // 16 * 16, ws, nb, 0)
+        return lib.ep_mx4_pool_forward(C.byref(t), q, 0, Q, 1.0, buf.data_ptr(), 0, 0, buf.data_ptr() // 16 * 16, ws, nb, 0)
 
     assert fwd(codes=0) == -1 and fwd(q=0) == -1 and fwd(Q=0) == -1 and fwd(N=0) == -1
     assert fwd(B=3) == -1                                          # three images of a cache of two, without an index
@@ -85,9 +85,9 @@ def test_c_entries_refuse_on_the_host():
     t = N.EPMx4Tokens(**ok)
     assert lib.ep_mx4_dequantize(C.byref(t), buf.data_ptr() // 16 * 16, 7, 0) == -5
     assert lib.ep_mx4_quantize(buf.data_ptr(), 9, 500, 100, 2, 5, 100, ok["codes"], ok["scales"], 320, 20, 0) == -5
-    bwd = lambda per, acc: lib.ep_mx4_pool_backward(C.byref(t), 3, 1.0, buf.data_ptr(), buf.data_ptr() // 16 * 16, 0, buf.data_ptr(), buf.data_ptr(),
+    bwd = lambda per, acc, sst=8: lib.ep_mx4_pool_backward(C.byref(t), 3, 1.0, buf.data_ptr() // 16 * 16, sst, buf.data_ptr() // 16 * 16, 0, buf.data_ptr(), buf.data_ptr(),
                                                     per, acc, buf.data_ptr() // 16 * 16, need, 0)
-    assert bwd(1, 1) == -5
+    assert bwd(1, 1) == -5 and bwd(0, 0, 6) == -3 and bwd(0, 0, 4) == -3
     d = dict(logits=buf.data_ptr(), dtype=0, ldl=10, B=2, C=10, K=3, R=2, teacher_values=buf.data_ptr(), ldv=3, teacher_index=buf.data_ptr(), ldi=3,
              temperature=1.0, alpha=1.0, grad_scale=1.0, loss_rows=buf.data_ptr())
     dist = lambda **over: lib.ep_distill_topk(C.byref(N.EPDistillArgs(**{**d, **over})), buf.data_ptr(), 1 << 20, 0)
