@@ -31,6 +31,16 @@ __device__ __forceinline__ void mx_decode8(uint32_t w, float scale, float (&v)[8
   }
 }
 
+// A word of a per-image table at a wave-uniform place, through the scalar cache: a vector load would have to wait for every tile load
+// in front of it.  (Nothing writes these tables while the kernel runs.)
+__device__ __forceinline__ int mx_uniform_load(const int32_t* p) {
+  int v;
+  const uint64_t a = (uint64_t)p;
+  const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) << 32;
+  asm volatile("s_load_dword %0, %1, 0x0\n\ts_waitcnt lgkmcnt(0)" : "=s"(v) : "s"(u) : "memory");
+  return v;
+}
+
 // image of the call -> image of the cache (-1: an index outside the cache) and its token count
 __device__ __forceinline__ int mx_image(const ep_mx4_tokens& t, int b, int& len) {
   int64_t img = t.image_index ? (int64_t)t.image_index[b] : (int64_t)b;
@@ -39,6 +49,16 @@ __device__ __forceinline__ int mx_image(const ep_mx4_tokens& t, int b, int& len)
   len = t.lengths ? t.lengths[img] : t.N;
   len = len < 0 ? 0 : (len > t.N ? t.N : len);
   return (int)img;
+}
+
+// the same for a wave-uniform b
+__device__ __forceinline__ int mx_image_uniform(const ep_mx4_tokens& t, int b, int& len) {
+  const int img = t.image_index ? mx_uniform_load(t.image_index + b) : b;
+  len = 0;
+  if (img < 0 || (int64_t)img >= t.M) return -1;
+  len = t.lengths ? mx_uniform_load(t.lengths + img) : t.N;
+  len = len < 0 ? 0 : (len > t.N ? t.N : len);
+  return img;
 }
 
 int mx4_check(const ep_mx4_tokens* t, const char* what);

@@ -46,6 +46,12 @@ template <int QM> struct MxDims {
   static constexpr int REC = 64 * 4 * SV * NQB;  // bytes of an exchange record
 };
 
+// the lane number once more, opaque to the compiler: what is derived from it is made where it is used and not kept in registers
+// across the tile loop, where they are scarce
+__device__ __forceinline__ int mx_fresh(int lane) {
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
 template <int N>
 __device__ __forceinline__ void mx_wait_vm() {
   static_assert(N >= 0 && N <= 63, "vmcnt");
@@ -148,8 +154,7 @@ struct MxCursor {
     for (; u < units; u += ustep) {
       b = u / splits;
       const int s = u - b * splits;
-      img = __builtin_amdgcn_readfirstlane(mx_image(t, b, len));
-      len = __builtin_amdgcn_readfirstlane(len);
+      img = mx_image_uniform(t, b, len);
       const int n = (len + 31) >> 5;
       hi = (s + 1) * tps < n ? (s + 1) * tps : n;
       tile = s * tps + toff;
@@ -183,17 +188,12 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
   char* ring = lds + wave * (NST * STAGE);
   char* exch = lds + nw * groups * (NST * STAGE);                      // [2][groups][nw][REC]
 
-  // ---- lane constants
-  const unsigned dma_seg = (unsigned)(((lane & 3) ^ g) * 16);          // LDS row r of a tile holds token 8 (r % 4) + r / 4, its 16-byte
-  const int dma_tok = 8 * ((lane >> 2) & 3) + g;                       // pieces XOR-ed with r / 4: both contractions read all banks
-  const unsigned dma_full = (unsigned)(dma_tok * rowC) + dma_seg;
-  const unsigned scl_full = (unsigned)((lane & 31) * rowS);
+  // ---- lane constants.  LDS row r of a tile holds token 8 (r % 4) + r / 4, its 16-byte pieces XOR-ed with r / 4: both contractions
+  // then read all banks.
   const int tok0 = 8 * g + (QM == 8 ? 4 * (c >> 3) : 0);               // first token of the lane's scores in a tile
   const int sc_off = (8 * (c >> 2) + (c & 3)) * 4;                     // + 16 h: scale dword of the score row
   const int a_off = (4 * (c & 3) + (c >> 2)) * 64 + ((g ^ (c & 3)) << 4);
-  int p_off[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) p_off[i] = i * 256 + g * 64 + (((c >> 2) ^ i) << 4) + (c & 3) * 4;
+  const int p_off = g * 64 + c * 4;                                    // slot i: (p_off ^ 16 (i % 4)) + 256 i
   const uint32_t rot = (uint32_t)(8 * (c >> 2) + 9);
 
   auto issue = [&](const MxCursor& cu, int slot) {
@@ -201,12 +201,11 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
     const int t0 = cu.tile << 5, rows = cu.len - t0;
     const uint8_t* src = t.codes + (int64_t)cu.img * t.codes_bstride + (int64_t)t0 * rowC;
     const uint8_t* scl = t.scales + (int64_t)cu.img * t.scales_bstride + (int64_t)t0 * rowS;
-    unsigned off0 = dma_full, off1 = dma_full + 4 * rowC, offs = scl_full;
-    if (rows < 32) {                                                   // rows behind the image's end repeat its last one
-      off0 = (unsigned)((dma_tok < rows ? dma_tok : rows - 1) * rowC) + dma_seg;
-      off1 = (unsigned)((dma_tok + 4 < rows ? dma_tok + 4 : rows - 1) * rowC) + dma_seg;
-      offs = (unsigned)(((lane & 31) < rows ? (lane & 31) : rows - 1) * rowS);
-    }
+    const int ln = mx_fresh(lane);
+    const int tok = 8 * ((ln >> 2) & 3) + (ln >> 4), last = rows - 1;  // rows behind the image's end repeat its last one
+    const unsigned seg = (unsigned)(((ln & 3) ^ (ln >> 4)) * 16);
+    const unsigned off0 = (unsigned)((tok < last ? tok : last) * rowC) + seg, off1 = (unsigned)((tok + 4 < last ? tok + 4 : last) * rowC) + seg;
+    const unsigned offs = (unsigned)(((ln & 31) < last ? (ln & 31) : last) * rowS);
 #pragma unroll
     for (int k = 0; k < CPW; ++k) {
       const int ch = chunk0 + k < nc ? chunk0 + k : nc - 1;            // a slice that the row does not fill repeats its last block
@@ -216,7 +215,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
 #pragma unroll
     for (int k = 0; k < CPW; k += 2) {                                 // lanes 32-63: the second block
       const int ch0 = chunk0 + k < nc ? chunk0 + k : nc - 1, ch1 = k + 1 < CPW && ch0 + 1 < nc ? ch0 + 1 : ch0;
-      __builtin_amdgcn_global_load_lds((mx_gptr_t)(scl + (offs + (unsigned)(lane < 32 ? ch0 : ch1) * 4u)), (mx_lds_t)(st + CODES + k * 128), 4, 0, 0);
+      __builtin_amdgcn_global_load_lds((mx_gptr_t)(scl + (offs + (unsigned)(ln < 32 ? ch0 : ch1) * 4u)), (mx_lds_t)(st + CODES + k * 128), 4, 0, 0);
     }
   };
 
@@ -228,6 +227,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
   ahead.open(t);
   float sg[NQB][SV];                                                    // backward: saved scores of the next tile
   auto load_scores = [&](const MxCursor& cu) {
+    const int ln = mx_fresh(lane), c = ln & 15, tok0 = 8 * (ln >> 4) + (QM == 8 ? 4 * (c >> 3) : 0);
 #pragma unroll
     for (int qb = 0; qb < NQB; ++qb) {
       const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
@@ -247,6 +247,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
   // ---- operand rows
   MxOperand<QM> op[NQB][CPW];
   auto load_operand = [&](const float* rows, const float* prows, float mul, float (&delta)[NQB]) {
+    const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
 #pragma unroll
     for (int qb = 0; qb < NQB; ++qb) {
       const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
@@ -275,6 +276,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
 
   float m_run[NQB], mz[NQB], l_run[NQB], t_max[NQB], invl[NQB];         // mz: the maximum that weights are taken against
   auto open_unit = [&](int b) {                                         // backward: dP's rows and the saved statistics
+    const int c = mx_fresh(lane) & 15;
     load_operand(p.q + (int64_t)b * p.Q * p.ldq, p.Pin ? p.Pin + (int64_t)b * p.Q * p.ldq : nullptr, 1.f, delta);
 #pragma unroll
     for (int qb = 0; qb < NQB; ++qb) {
@@ -286,11 +288,6 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
       if (!p.Pin && dw == 0) delta[qb] = ml.z;                          // (each D-slice takes off its own part of delta)
     }
   };
-  if constexpr (BWD) {
-    cu.open(t);
-    if (cu.valid()) open_unit(cu.b);                                    // in front of the accumulators: most launches have one unit a wave
-  }
-
   f4 acc[NQB][CPW][8];
   auto clear = [&]() {
 #pragma unroll
@@ -305,6 +302,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
 
   // acc rows 4 g + i of query block qb are queries qrow(i); multiply each by the value that lane (c = query) holds
   auto scale_rows = [&](int qb, float f) {
+    const int g = mx_fresh(lane) >> 4;
     float r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = __shfl(f, QM == 8 ? (4 * g + i) & 7 : 4 * g + i, 64);
@@ -314,11 +312,10 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
       for (int j = 0; j < 8; ++j) { acc[qb][k][j].x *= r[0]; acc[qb][k][j].y *= r[1]; acc[qb][k][j].z *= r[2]; acc[qb][k][j].w *= r[3]; }
   };
 
-  // one tile: `work` false where this wave only keeps the barrier
-  auto tile_step = [&](bool work, int b, int t0, int len) {
+  auto tile_step = [&](int b, int t0, int len) {
     float s[NQB][SV];
     const char* st = ring + slot * STAGE;
-    if (work) {
+    {
       mx_wait_vm<(NST - 1) * OPS>();
       // first contraction
       f4 sa[NQB][2], sl[NQB][2];                                        // leading and lower terms: an addition to a large sum costs its last bit
@@ -361,7 +358,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
     __builtin_amdgcn_sched_barrier(0);
     if (nw > 1) {                                                       // add the D-slices
       char* ex = exch + (buf * groups + grp) * nw * DM::REC;
-      if (work) {
+      {
 #pragma unroll
         for (int qb = 0; qb < NQB; ++qb)
 #pragma unroll
@@ -370,7 +367,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
       }
       mx_barrier();
       buf ^= 1;
-      if (work) {
+      {
 #pragma unroll
         for (int qb = 0; qb < NQB; ++qb)
 #pragma unroll
@@ -381,7 +378,6 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
           }
       }
     }
-    if (!work) return;
     const bool tail = t0 + 32 > len;
     // weights
     mx_u4 wt[NQB][DM::PSETS];
@@ -461,11 +457,10 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
     for (int k = 0; k < CPW; ++k) {
       uint32_t w[8];
       float sc[8];
-      const mx_u4 s0 = *reinterpret_cast<const mx_u4*>(st + CODES + k * 128 + g * 32), s1 = *reinterpret_cast<const mx_u4*>(st + CODES + k * 128 + g * 32 + 16);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        w[i] = *reinterpret_cast<const uint32_t*>(st + k * 2048 + (i >> 2) * 1024 + p_off[i & 3]);
-        const uint32_t four = i < 4 ? s0[i & 3] : s1[i & 3];
+        w[i] = *reinterpret_cast<const uint32_t*>(st + k * 2048 + i * 256 + (p_off ^ ((i & 3) << 4)));
+        const uint32_t four = *reinterpret_cast<const uint32_t*>(st + CODES + k * 128 + g * 32 + i * 4);
         sc[i] = __uint_as_float(__builtin_amdgcn_alignbit(four, four, rot));
       }
 #define EP_MX_PAIR(PR)                                                                                                   \
@@ -498,8 +493,9 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
     slot = slot + 1 == NST ? 0 : slot + 1;
   };
 
-  // store acc (times r(query)) as rows of out (row stride D): QM 8 adds the two term rows first
-  auto store_rows = [&](float* out, const float (&inv)[NQB]) {
+  // store (or add) acc times r(query) as rows of out (row stride D): QM 8 adds the two term rows first
+  auto store_rows = [&](float* out, const float (&inv)[NQB], bool add) {
+    const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
 #pragma unroll
     for (int qb = 0; qb < NQB; ++qb) {
       float r[4];
@@ -511,6 +507,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
         for (int i = 0; i < 4; ++i) {
           const int q = QM == 8 ? 4 * (g & 1) + i : qb * 16 + 4 * g + i;
           float* o = out + (int64_t)(q0 + q) * t.D;
+          __builtin_amdgcn_sched_barrier(0);                             // row by row: the added values of all rows at once would not fit
           constexpr int NV = QM == 8 ? 1 : 2;
 #pragma unroll
           for (int v = 0; v < NV; ++v) {
@@ -519,19 +516,25 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
             for (int j = 0; j < 4; ++j) x[j] = (QM == 8 ? fold32(acc[qb][k][j][i], acc[qb][k][j + 4][i]) : acc[qb][k][4 * v + j][i]) * r[i];
             const int d = (chunk0 + k) * MX_BLOCK + 8 * c + (QM == 8 ? 4 * (g >> 1) : 4 * v);
             if (q < qn && chunk0 + k < nc) {
-              if (p.veco) { if (d < t.D) *reinterpret_cast<f4*>(o + d) = x; }
-              else {
+              if (p.veco) {
+                if (d < t.D) {
+                  if (BWD && add) x += *reinterpret_cast<const f4*>(o + d);
+                  *reinterpret_cast<f4*>(o + d) = x;
+                }
+              } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                  if (d + j < t.D) o[d + j] = x[j];
+                  if (d + j < t.D) o[d + j] = BWD && add ? o[d + j] + x[j] : x[j];
               }
             }
           }
         }
     }
   };
-  // add the groups' accumulators into group 0's (through the ring, which is idle then), half a row block at a time
+  // add the groups' accumulators into group 0's, half a row block at a time, through the exchange records (2 groups nw of them, at
+  // least 4 KiB a wave of a group)
   auto add_groups = [&]() {
+    const int ln = mx_fresh(lane);
     for (int o = 1; o < groups; ++o) {
 #pragma unroll
       for (int qb = 0; qb < NQB; ++qb)
@@ -541,12 +544,12 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
           for (int j0 = 0; j0 < 8; j0 += 4) {
             if (grp == o) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) *reinterpret_cast<f4*>(lds + (dw * 4 + j) * 1024 + lane * 16) = acc[qb][k][j0 + j];
+              for (int j = 0; j < 4; ++j) *reinterpret_cast<f4*>(exch + (dw * 4 + j) * 1024 + ln * 16) = acc[qb][k][j0 + j];
             }
             mx_barrier();
             if (grp == 0) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) acc[qb][k][j0 + j] += *reinterpret_cast<const f4*>(lds + (dw * 4 + j) * 1024 + lane * 16);
+              for (int j = 0; j < 4; ++j) acc[qb][k][j0 + j] += *reinterpret_cast<const f4*>(exch + (dw * 4 + j) * 1024 + ln * 16);
             }
             mx_barrier();
           }
@@ -557,21 +560,22 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
     for (int u = (int)blockIdx.x; u < p.units; u += (int)gridDim.x) {
       const int b = u / p.splits, sp = u - b * p.splits;
       int len;
-      const int img = __builtin_amdgcn_readfirstlane(mx_image(t, b, len));
-      len = __builtin_amdgcn_readfirstlane(len);
+      const int img = mx_image_uniform(t, b, len);
       const int n = (len + 31) >> 5, lo = sp * p.tps, hi = (sp + 1) * p.tps < n ? (sp + 1) * p.tps : n;
       if (p.qb || u == (int)blockIdx.x) load_operand(p.q + (int64_t)b * p.qb, nullptr, p.scale, delta);
 #pragma unroll
       for (int qb = 0; qb < NQB; ++qb) { m_run[qb] = t_max[qb] = -INFINITY; mz[qb] = l_run[qb] = 0.f; }
       clear();
-      for (int tl = lo; tl < hi; tl += groups) {
-        const bool work = tl + grp < hi;
-        tile_step(work, b, (tl + grp) << 5, len);
-        if (work) refill();
+      int tl = lo;
+      for (; tl + grp < hi; tl += groups) {
+        tile_step(b, (tl + grp) << 5, len);
+        refill();
       }
+      if (tl < hi && nw > 1) mx_barrier();                              // a group without a tile in the last round keeps the others' barrier
+      const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
       if (p.S && sp == p.splits - 1 && dw == 0 && grp == 0) {           // scores behind the image's tiles
         for (int q = 0; q < qn; ++q)
-          for (int i = (n << 5) + lane; i < t.N; i += 64) p.S[((int64_t)b * p.Q + q0 + q) * p.lds_ + i] = img < 0 ? __uint_as_float(0x7fc00000u) : -INFINITY;
+          for (int i = (n << 5) + ln; i < t.N; i += 64) p.S[((int64_t)b * p.Q + q0 + q) * p.lds_ + i] = img < 0 ? __uint_as_float(0x7fc00000u) : -INFINITY;
       }
       float f[NQB];
 #pragma unroll
@@ -580,8 +584,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
         l_run[qb] = mx_over_groups_sum(l_run[qb]);
         t_max[qb] = mx_over_groups_max(t_max[qb]);
       }
-      if (groups > 1) {                                                 // (one unit per workgroup then: the ring is idle)
-        mx_wait_vm<0>();
+      if (groups > 1) {
         float* ml = reinterpret_cast<float*>(exch);                     // [groups][NQB][16][3]
         mx_barrier();
         if (dw == 0 && g == 0) {
@@ -621,41 +624,33 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
           }
           f[qb] = (p.splits > 1 ? e : (none ? 0.f : 1.f / l_run[qb])) + bad;
         }
-        store_rows(p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, f);
+        store_rows(p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, f, false);
       }
     }
   } else {
     float one[NQB];
 #pragma unroll
     for (int qb = 0; qb < NQB; ++qb) one[qb] = p.scale;
-    if (p.per_unit) {                                                   // images (and runs) without a token are not visited below
-      MxCursor z = cu;
-      z.u = (int)blockIdx.x * groups + grp;
-      for (; z.u < z.units; z.u += z.ustep) {
-        const int b = z.u / z.splits;
-        int len;
-        mx_image(t, b, len);
-        if ((z.u - b * z.splits) * z.tps >= (len + 31) >> 5) store_rows(p.part + (int64_t)z.u * p.Q * t.D, one);
+    const int rounds = (p.units + cu.ustep - 1) / cu.ustep;
+    int u = cu.u;
+    cu.open(t);
+    for (int r = 0; r < rounds; ++r, u += cu.ustep) {                   // a group's r-th unit; the sum over rounds and groups is in a fixed order
+      if (cu.valid() && cu.u == u) open_unit(cu.b);
+      clear();
+      int it = 0;
+      for (; cu.u == u && u < p.units; ++it) {
+        tile_step(cu.b, cu.tile << 5, cu.len);
+        cu.next(t);
+        refill();
       }
-    }
-    bool fresh = false;
-    const int iters = nw > 1 ? (int)((p.units + cu.ustep - 1) / cu.ustep) * p.tps : 0;
-    for (int it = 0; nw > 1 ? it < iters : cu.valid(); ++it) {
-      const bool work = cu.valid();
-      if (work && fresh) open_unit(cu.b);
-      tile_step(work, cu.b, cu.tile << 5, cu.len);
-      if (!work) continue;
-      const int u = cu.u;
-      fresh = cu.next(t);
-      refill();
-      if (fresh && p.per_unit) {                                        // one gradient per image (and split)
-        store_rows(p.part + (int64_t)u * p.Q * t.D, one);
-        clear();
+      if (nw > 1)
+        for (; it < p.tps; ++it) mx_barrier();                          // groups with fewer tiles keep the others' barriers
+      if (p.per_unit) {                                                 // one gradient per image (and split)
+        if (u < p.units) store_rows(p.part + (int64_t)u * p.Q * t.D, one, false);
+      } else {
+        if (groups > 1) { mx_barrier(); add_groups(); }
+        if (grp == 0) store_rows(p.part + (int64_t)blockIdx.x * p.Q * t.D, one, r > 0);
       }
-    }
-    if (!p.per_unit) {
-      if (groups > 1) { mx_wait_vm<0>(); mx_barrier(); add_groups(); }
-      if (grp == 0) store_rows(p.part + (int64_t)blockIdx.x * p.Q * t.D, one);
     }
   }
   mx_wait_vm<0>();                                                      // no load into LDS outlives its wave
