@@ -656,10 +656,452 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
   mx_wait_vm<0>();                                                      // no load into LDS outlives its wave
 }
 
-// joins the splits of an image: blockIdx.x = (image, query), blockIdx.y = 64 channels; 16 chains of splits side by side
+// ---- the pipelined form --------------------------------------------------------------------------------------------------
+// One 128-channel block per wave (nw pool waves) and one wave more that makes the weights.  Per tile j of the workgroup's sequence:
+//     pool waves   first contraction of tile j -> record j | barrier j | second contraction of tile j - 1, refill its stage
+//     weight wave                                          | barrier j | sums the records of tile j, softmax (or dS), weights j
+// so that the long chain exchange -> maximum -> exponentials -> split runs beside the contractions of other tiles, once per tile
+// instead of once per wave, and the pool waves' registers (accumulators and operand of one block) leave room for 3 - 4 waves a SIMD.
+template <int QM> constexpr int mx_pipe_waves() { return QM == 32 ? 12 : 16; }
+
+template <int QM, int NST, bool BWD>
+__global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) void ep_mx4_pipe_kernel(MxPool p) {
+  typedef MxDims<QM> DM;
+  constexpr int NQB = DM::NQB, SV = DM::SV;
+  constexpr int STAGE = 2048 + 128, OPS = 3;
+  constexpr int WREC = NQB * DM::PSETS * 1024, WALL = WREC + 2 * NQB * 64 + 64;      // weights, rescaling factors, row factors, flags
+  extern __shared__ __align__(16) char lds[];
+  const int lane = lane_id(), c = lane & 15, g = lane >> 4;
+  const int wave = wave_id_uniform();
+  const ep_mx4_tokens& t = p.t;
+  const int nw = p.nw, rowC = p.nc * 64, rowS = p.nc * 4;
+  const int q0 = (int)blockIdx.y * p.qblk, qn = p.Q - q0 < p.qblk ? p.Q - q0 : p.qblk;      // queries of this workgroup
+  char* recs = lds + nw * (NST * STAGE);                                // [2][nw][REC]
+  char* wbuf = recs + 2 * nw * DM::REC;                                 // [2][WALL]
+  const int tok0 = 8 * g + (QM == 8 ? 4 * (c >> 3) : 0);                // first token of the lane's scores in a tile
+  const float NANF = __uint_as_float(0x7fc00000u);
+
+  MxCursor start;
+  start.units = p.units; start.splits = p.splits; start.tps = p.tps;
+  start.u = (int)blockIdx.x; start.ustep = (int)gridDim.x; start.toff = 0; start.tstep = 1;
+
+  if (wave < nw) {                                                      // ================= pool waves
+    char* ring = lds + wave * (NST * STAGE);
+    const int sc_off = (8 * (c >> 2) + (c & 3)) * 4;                    // + 16 h: scale dword of the score row
+    const int a_off = (4 * (c & 3) + (c >> 2)) * 64 + ((g ^ (c & 3)) << 4);
+    const int p_off = g * 64 + c * 4;                                   // slot i: (p_off ^ 16 (i % 4)) + 256 i
+    const uint32_t rot = (uint32_t)(8 * (c >> 2) + 9);
+
+    auto issue = [&](const MxCursor& cu, int slot) {
+      char* st = ring + slot * STAGE;
+      const int t0 = cu.tile << 5, last = cu.len - t0 - 1;              // rows behind the image's end repeat its last one
+      const uint8_t* src = t.codes + (int64_t)cu.img * t.codes_bstride + (int64_t)t0 * rowC + wave * 64;
+      const uint8_t* scl = t.scales + (int64_t)cu.img * t.scales_bstride + (int64_t)t0 * rowS + wave * 4;
+      const int ln = mx_fresh(lane);
+      const int tok = 8 * ((ln >> 2) & 3) + (ln >> 4);
+      const unsigned seg = (unsigned)(((ln & 3) ^ (ln >> 4)) * 16);
+      const unsigned off0 = (unsigned)((tok < last ? tok : last) * rowC) + seg, off1 = (unsigned)((tok + 4 < last ? tok + 4 : last) * rowC) + seg;
+      __builtin_amdgcn_global_load_lds((mx_gptr_t)(src + off0), (mx_lds_t)st, 16, 0, MX_NT);
+      __builtin_amdgcn_global_load_lds((mx_gptr_t)(src + off1), (mx_lds_t)(st + 1024), 16, 0, MX_NT);
+      if (ln < 32) __builtin_amdgcn_global_load_lds((mx_gptr_t)(scl + (unsigned)((ln < last ? ln : last) * rowS)), (mx_lds_t)(st + 2048), 4, 0, 0);
+    };
+
+    MxCursor cs = start, ahead;                                         // the tile to score, the tile to load
+    cs.open(t);
+    ahead = cs;
+#pragma unroll
+    for (int i = 0; i < NST; ++i) { issue(ahead, i); ahead.next(t); }
+    MxCursor cp = cs;                                                   // the tile to pool
+
+    MxOperand<QM> op[NQB];
+    float delta[NQB];
+    auto open_unit = [&](int b) {                                       // the operand rows; backward: this block's part of delta = dP . P
+      const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
+      const float* rows = p.q + (BWD ? (int64_t)b * p.Q * p.ldq : (int64_t)b * p.qb);
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) {
+        const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+        const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * p.ldq + wave * MX_BLOCK + 32 * g;    // (rows without a query: the first one's, times 0)
+        mx_f16 ve, vo;
+        mx_load_row(rows + at, q < qn ? (BWD ? 1.f : p.scale) : 0.f, ve, vo);
+        float d = 0.f;
+        if (BWD && p.Pin) {
+          mx_f16 we, wo;
+          mx_load_row(p.Pin + (int64_t)b * p.Q * p.ldq + at, 1.f, we, wo);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) d = fmaf(vo[i], wo[i], fmaf(ve[i], we[i], d));
+          d = mx_over_groups_sum(d);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        delta[qb] = d;
+        mx_operand<QM>(ve, vo, c, op[qb]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+
+    f4 acc[NQB][8];
+    auto clear = [&]() {
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[qb][j] = f4{0.f, 0.f, 0.f, 0.f};
+    };
+    // acc times r (one factor per row 4 g + i) as rows of out: QM 8 adds the two term rows first
+    auto store_rows = [&](float* out, const f4 (&r)[NQB]) {
+      const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int q = QM == 8 ? 4 * (g & 1) + i : qb * 16 + 4 * g + i;
+          float* o = out + (int64_t)(q0 + q) * t.D;
+          __builtin_amdgcn_sched_barrier(0);
+          constexpr int NV = QM == 8 ? 1 : 2;
+#pragma unroll
+          for (int v = 0; v < NV; ++v) {
+            f4 x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = (QM == 8 ? fold32(acc[qb][j][i], acc[qb][j + 4][i]) : acc[qb][4 * v + j][i]) * r[qb][i];
+            const int d = wave * MX_BLOCK + 8 * c + (QM == 8 ? 4 * (g >> 1) : 4 * v);
+            if (q < qn) {
+              if (p.veco) { if (d < t.D) *reinterpret_cast<f4*>(o + d) = x; }
+              else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if (d + j < t.D) o[d + j] = x[j];
+              }
+            }
+          }
+        }
+    };
+    int sslot = 0, pslot = 0, buf = 0;
+
+    auto scores = [&]() {                                               // first contraction of the ring's stage sslot -> record
+      mx_wait_vm<(NST - 2) * OPS>();
+      const char* st = ring + sslot * STAGE;
+      char* rec = recs + (buf * nw + wave) * DM::REC;
+      f4 sa[NQB][2], sl[NQB][2];                                        // leading and lower terms: an addition to a large sum costs its last bit
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) sa[qb][0] = sa[qb][1] = sl[qb][0] = sl[qb][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const mx_u4 w = *reinterpret_cast<const mx_u4*>(st + h * 1024 + a_off);
+        const uint32_t sc = *reinterpret_cast<const uint32_t*>(st + 2048 + h * 16 + sc_off) >> (8 * g);
+#pragma unroll
+        for (int qb = 0; qb < NQB; ++qb) {
+          const MxOperand<QM>& o = op[qb];
+          sa[qb][h] = mx_mfma_codes<0>(w, sc, o.b[0], o.sc[0], sa[qb][h]);
+          if constexpr (QM != 8) {
+            sl[qb][h] = mx_mfma_codes<1>(w, sc, o.b[4], o.sc[1], sl[qb][h]);
+            sl[qb][h] = mx_mfma_codes<0>(w, sc, o.b[3], o.sc[1], sl[qb][h]);
+          }
+          sl[qb][h] = mx_mfma_codes<2>(w, sc, o.b[2], o.sc[0], sl[qb][h]);
+          sl[qb][h] = mx_mfma_codes<1>(w, sc, o.b[1], o.sc[0], sl[qb][h]);
+        }
+      }
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) {
+        sa[qb][0] += sl[qb][0]; sa[qb][1] += sl[qb][1];
+        const float dl = BWD ? delta[qb] : 0.f;
+        if constexpr (QM == 8) {                                        // columns q and q + 8 are terms of one query
+          const bool up = (c & 8) != 0;
+          f4 s;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float own = up ? sa[qb][1][i] : sa[qb][0][i], oth = up ? sa[qb][0][i] : sa[qb][1][i];
+            s[i] = own + mx_ror8(oth) - dl;
+          }
+          *reinterpret_cast<f4*>(rec + lane * 16) = s;
+        } else {
+          *reinterpret_cast<f4*>(rec + (2 * qb) * 1024 + lane * 16) = sa[qb][0] - dl;
+          *reinterpret_cast<f4*>(rec + (2 * qb + 1) * 1024 + lane * 16) = sa[qb][1] - dl;
+        }
+      }
+      sslot = sslot + 1 == NST ? 0 : sslot + 1;
+    };
+
+    auto pool = [&]() {                                                 // second contraction of stage pslot with the weights of buffer buf
+      const char* st = ring + pslot * STAGE;
+      const char* wr = wbuf + buf * WALL;
+      mx_u4 wt[NQB][DM::PSETS];
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb)
+#pragma unroll
+        for (int z = 0; z < DM::PSETS; ++z) wt[qb][z] = *reinterpret_cast<const mx_u4*>(wr + (qb * DM::PSETS + z) * 1024 + lane * 16);
+      if constexpr (!BWD) {
+        if (__builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(wr + WREC + 2 * NQB * 64))) {        // the running maximum has moved
+#pragma unroll
+          for (int qb = 0; qb < NQB; ++qb) {
+            const f4 r = *reinterpret_cast<const f4*>(wr + WREC + qb * 64 + (QM == 8 ? 16 * (g & 1) : 16 * g));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[qb][j] *= r;
+          }
+        }
+      }
+      uint32_t w[8];
+      float sc[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = *reinterpret_cast<const uint32_t*>(st + i * 256 + (p_off ^ ((i & 3) << 4)));
+        const uint32_t four = *reinterpret_cast<const uint32_t*>(st + 2048 + g * 32 + i * 4);
+        sc[i] = __uint_as_float(__builtin_amdgcn_alignbit(four, four, rot));
+      }
+#define EP_MX_PAIR(PR)                                                                                                   \
+  do {                                                                                                                   \
+    uint32_t x[8];                                                                                                       \
+    _Pragma("unroll") for (int i = 0; i < 8; ++i) x[i] = mx_pair<PR>(w[i], sc[i]);                                      \
+    mx_u4 ev, od;                                                                                                        \
+    _Pragma("unroll") for (int i = 0; i < 4; ++i) {                                                                     \
+      ev[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05040100u);                                                \
+      od[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);                                                \
+    }                                                                                                                    \
+    _Pragma("unroll") for (int qb = 0; qb < NQB; ++qb) _Pragma("unroll") for (int z = DM::PSETS - 1; z >= 0; --z) {     \
+      acc[qb][2 * PR] = mx_mfma(wt[qb][z], ev, acc[qb][2 * PR]);                                                         \
+      acc[qb][2 * PR + 1] = mx_mfma(wt[qb][z], od, acc[qb][2 * PR + 1]);                                                 \
+    }                                                                                                                    \
+  } while (0)
+      EP_MX_PAIR(0); EP_MX_PAIR(1); EP_MX_PAIR(2); EP_MX_PAIR(3);
+#undef EP_MX_PAIR
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                // the stage is read
+      issue(ahead, pslot);
+      ahead.next(t);
+      pslot = pslot + 1 == NST ? 0 : pslot + 1;
+    };
+
+    clear();
+    f4 one[NQB];
+#pragma unroll
+    for (int qb = 0; qb < NQB; ++qb) one[qb] = f4{p.scale, p.scale, p.scale, p.scale};
+    if (cs.valid()) {
+      open_unit(cs.b);
+      bool fresh = false;
+      scores();
+      buf ^= 1;
+      fresh = cs.next(t);
+      mx_barrier();
+      for (;;) {
+        const bool more = cs.valid();
+        if (more) {
+          if (fresh && (BWD || p.qb)) open_unit(cs.b);
+          scores();
+        }
+        mx_barrier();
+        buf ^= 1;                                                       // weights of the tile before, at the other parity than its record's successor
+        pool();
+        const int u = cp.u, b = cp.b;
+        if (cp.next(t)) {                                               // the unit's last tile
+          if constexpr (!BWD) {
+            f4 r[NQB];
+#pragma unroll
+            for (int qb = 0; qb < NQB; ++qb) r[qb] = *reinterpret_cast<const f4*>(wbuf + buf * WALL + WREC + NQB * 64 + qb * 64 + (QM == 8 ? 16 * (g & 1) : 16 * g));
+            store_rows(p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, r);
+            clear();
+          } else if (p.per_unit) {
+            store_rows(p.part + (int64_t)u * p.Q * t.D, one);
+            clear();
+          }
+        }
+        if (!more) break;
+        fresh = cs.next(t);
+      }
+    } else {
+      mx_barrier();
+    }
+    if (BWD && !p.per_unit) store_rows(p.part + (int64_t)blockIdx.x * p.Q * t.D, one);
+    else {                                                              // units without a token
+      clear();
+      for (int u = (int)blockIdx.x; u < p.units; u += (int)gridDim.x) {
+        const int b = u / p.splits, sp = u - b * p.splits;
+        int len;
+        const int img = mx_image_uniform(t, b, len);
+        if (sp * p.tps < (len + 31) >> 5) continue;
+        const float f = !BWD && img < 0 ? NANF : 0.f;
+        f4 r[NQB];
+#pragma unroll
+        for (int qb = 0; qb < NQB; ++qb) r[qb] = f4{f, f, f, f};
+        store_rows(BWD || p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, r);
+      }
+    }
+    mx_wait_vm<0>();                                                    // no load into LDS outlives its wave
+  } else {                                                              // ================= weight wave
+    MxCursor cw = start;
+    cw.open(t);
+    float m_run[NQB], mz[NQB], l_run[NQB], t_max[NQB], invl[NQB], dml[NQB], sg[NQB][SV];
+    auto load_scores = [&](const MxCursor& cu) {                        // backward: the saved scores of a tile
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) {
+        const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+        const float* row = p.S + ((int64_t)cu.b * p.Q + q0) * p.lds_;
+#pragma unroll
+        for (int h = 0; h < SV / 4; ++h) {
+          const int n = (cu.tile << 5) + tok0 + 4 * h;
+          const f4 v = *reinterpret_cast<const f4*>(row + (unsigned)((q < qn ? q : 0) * (int)p.lds_ + (n < p.lds_ ? n : (int)p.lds_ - 4)));
+          sg[qb][4 * h] = v.x; sg[qb][4 * h + 1] = v.y; sg[qb][4 * h + 2] = v.z; sg[qb][4 * h + 3] = v.w;
+        }
+      }
+    };
+    auto open_unit = [&](int b) {
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) {
+        m_run[qb] = t_max[qb] = -INFINITY; mz[qb] = l_run[qb] = 0.f;
+        if constexpr (BWD) {
+          const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+          f4 ml = {0.f, 0.f, 0.f, 0.f};
+          if (q < qn) ml = *reinterpret_cast<const f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4);
+          mz[qb] = ml.x;
+          invl[qb] = ml.y == 0.f ? 0.f : 1.f / ml.y;
+          dml[qb] = p.Pin ? 0.f : ml.z;
+        }
+      }
+    };
+    bool fresh = true;
+    int buf = 0;
+    if (BWD) load_scores(cw);
+    for (;;) {
+      const bool more = cw.valid();
+      if (more && fresh) open_unit(cw.b);
+      mx_barrier();
+      if (!more) break;
+      const int b = cw.b, u = cw.u, t0 = cw.tile << 5, len = cw.len;
+      const bool tail = t0 + 32 > len;
+      char* wr = wbuf + buf * WALL;
+      bool moved = false;
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) {
+        const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+        float s[SV], pv[SV];
+#pragma unroll
+        for (int h = 0; h < SV / 4; ++h) {                              // the blocks' parts, in their order
+          const char* r = recs + buf * nw * DM::REC + (qb * (SV / 4) + h) * 1024 + lane * 16;
+          f4 v = *reinterpret_cast<const f4*>(r);
+#pragma unroll 4
+          for (int o = 1; o < nw; ++o) v += *reinterpret_cast<const f4*>(r + o * DM::REC);
+          s[4 * h] = v.x; s[4 * h + 1] = v.y; s[4 * h + 2] = v.z; s[4 * h + 3] = v.w;
+        }
+        if constexpr (!BWD) {
+          if (tail) {
+#pragma unroll
+            for (int i = 0; i < SV; ++i) s[i] = t0 + tok0 + i < len ? s[i] : -INFINITY;
+          }
+          if (p.S && q < qn) {
+            float* sp = p.S + ((int64_t)b * p.Q + q0 + q) * p.lds_ + t0 + tok0;
+#pragma unroll
+            for (int h = 0; h < SV / 4; ++h)
+              if (t0 + tok0 + 4 * h < t.N) *reinterpret_cast<f4*>(sp + 4 * h) = f4{s[4 * h], s[4 * h + 1], s[4 * h + 2], s[4 * h + 3]};
+          }
+          float mx = s[0];
+#pragma unroll
+          for (int i = 1; i < SV; ++i) mx = fmaxf(mx, s[i]);
+          t_max[qb] = fmaxf(t_max[qb], mx);
+          float f = 1.f;
+          if (__any(mx > m_run[qb] + MX_LAZY)) {
+            if (QM == 8) mx = fmaxf(mx, mx_ror8(mx));
+            mx = mx_over_groups_max(mx);
+            const float mn = fmaxf(m_run[qb], mx);
+            f = mn == m_run[qb] ? 1.f : __builtin_amdgcn_exp2f((m_run[qb] - mn) * MX_LOG2E);
+            m_run[qb] = mn;
+            mz[qb] = mn == -INFINITY ? 0.f : mn;
+            l_run[qb] *= f;
+            moved = !fresh;                                             // (nothing is accumulated in front of the first tile)
+          }
+          if (g == 0 && (QM != 8 || c < 8)) *reinterpret_cast<float*>(wr + WREC + qb * 64 + c * 4) = f;
+#pragma unroll
+          for (int i = 0; i < SV; ++i) { pv[i] = __builtin_amdgcn_exp2f((s[i] - mz[qb]) * MX_LOG2E); l_run[qb] += pv[i]; }
+        } else {
+#pragma unroll
+          for (int i = 0; i < SV; ++i) {
+            const float a = __builtin_amdgcn_exp2f((sg[qb][i] - mz[qb]) * MX_LOG2E) * invl[qb];
+            pv[i] = a * (s[i] - dml[qb]);
+          }
+          if (tail) {
+#pragma unroll
+            for (int i = 0; i < SV; ++i) pv[i] = t0 + tok0 + i < len ? pv[i] : 0.f;
+          }
+        }
+        // three bf16 terms, exact: the upper half of the bits, of what is left, and of what is left then
+        uint32_t H[SV / 2], M[SV / 2], L[SV / 2];
+#pragma unroll
+        for (int i = 0; i < SV / 2; ++i) {
+          const float x = pv[2 * i], y = pv[2 * i + 1];
+          const float rx = x - __uint_as_float(__float_as_uint(x) & 0xffff0000u), ry = y - __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+          const float lx = rx - __uint_as_float(__float_as_uint(rx) & 0xffff0000u), ly = ry - __uint_as_float(__float_as_uint(ry) & 0xffff0000u);
+          H[i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+          M[i] = __builtin_amdgcn_perm(__float_as_uint(ry), __float_as_uint(rx), 0x07060302u);
+          L[i] = __builtin_amdgcn_perm(__float_as_uint(ly), __float_as_uint(lx), 0x07060302u);
+        }
+        mx_u4 wt[DM::PSETS];
+        if constexpr (QM == 8) {                                        // rows 0-7: first and third term, rows 8-15: second; 8 slots = both halves
+          const bool up = (c & 8) != 0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t r1 = mx_ror8u(up ? H[i] : M[i]), r2 = mx_ror8u(L[i]);
+            wt[0][i] = up ? r1 : H[i];
+            wt[0][2 + i] = up ? M[i] : r1;
+            wt[1][i] = up ? 0u : L[i];
+            wt[1][2 + i] = up ? 0u : r2;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { wt[0][i] = H[i]; wt[1][i] = M[i]; wt[DM::PSETS - 1][i] = L[i]; }
+        }
+#pragma unroll
+        for (int z = 0; z < DM::PSETS; ++z) *reinterpret_cast<mx_u4*>(wr + (qb * DM::PSETS + z) * 1024 + lane * 16) = wt[z];
+      }
+      fresh = cw.next(t);
+      if constexpr (BWD) load_scores(cw);
+      else {
+        if (lane == 0) *reinterpret_cast<int*>(wr + WREC + 2 * NQB * 64) = moved;
+        if (fresh) {                                                    // the unit is done: statistics, row factors, the scores behind its tiles
+          const int spl = u - b * p.splits;
+#pragma unroll
+          for (int qb = 0; qb < NQB; ++qb) {
+            const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
+            float l = l_run[qb], tm = t_max[qb];
+            if (QM == 8) { l += mx_ror8(l); tm = fmaxf(tm, mx_ror8(tm)); }
+            l = mx_over_groups_sum(l);
+            tm = mx_over_groups_max(tm);
+            const float e = __builtin_amdgcn_exp2f((mz[qb] - tm) * MX_LOG2E);               // from the running to the true maximum
+            if (g == 0 && (QM != 8 || c < 8)) {
+              if (q < qn) {
+                if (p.splits > 1) *reinterpret_cast<f2*>(p.part_ml + ((int64_t)u * p.Q + q0 + q) * 2) = f2{tm, l * e};
+                else *reinterpret_cast<f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4) = f4{tm, l * e, 0.f, 0.f};
+              }
+              *reinterpret_cast<float*>(wr + WREC + NQB * 64 + qb * 64 + c * 4) = p.splits > 1 ? e : 1.f / l;
+            }
+          }
+          if (p.S && spl == p.splits - 1)
+            for (int q = 0; q < qn; ++q)
+              for (int i = (((len + 31) >> 5) << 5) + lane; i < t.N; i += 64) p.S[((int64_t)b * p.Q + q0 + q) * p.lds_ + i] = -INFINITY;
+        }
+      }
+      buf ^= 1;
+    }
+    if constexpr (!BWD) {                                               // units without a token
+      for (int u = (int)blockIdx.x; u < p.units; u += (int)gridDim.x) {
+        const int b = u / p.splits, sp = u - b * p.splits;
+        int len;
+        const int img = mx_image_uniform(t, b, len);
+        const int n = (len + 31) >> 5;
+        if (sp * p.tps < n) continue;
+        const float bad = img < 0 ? NANF : 0.f;
+        for (int q = lane; q < qn; q += 64) {
+          if (p.splits > 1) *reinterpret_cast<f2*>(p.part_ml + ((int64_t)u * p.Q + q0 + q) * 2) = f2{img < 0 ? NANF : -INFINITY, bad};
+          else *reinterpret_cast<f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4) = f4{bad, bad, 0.f, 0.f};
+        }
+        if (p.S && sp == p.splits - 1)
+          for (int q = 0; q < qn; ++q)
+            for (int i = (n << 5) + lane; i < t.N; i += 64) p.S[((int64_t)b * p.Q + q0 + q) * p.lds_ + i] = img < 0 ? NANF : -INFINITY;
+      }
+    }
+  }
+}
+
+// joins the splits of an image: blockIdx.x = (image, query); CH chains of splits side by side, 1024 / CH channels a workgroup
+template <int CH>
 __global__ __launch_bounds__(256) void ep_mx4_join_kernel(const float* __restrict__ part, const float* __restrict__ ml, int splits, int Q, int D,
                                                           float* __restrict__ P, float* __restrict__ ML) {
-  __shared__ float red[16][64 + 4];
+  constexpr int LN = 256 / CH;
+  __shared__ f4 red[CH][LN + 1];
   const int b = (int)(blockIdx.x / (unsigned)Q), q = (int)(blockIdx.x % (unsigned)Q);
   const float* e = ml + ((int64_t)b * splits * Q + q) * 2;             // {maximum, sum} of split s at e[s * 2 Q]
   const int lane = lane_id();
@@ -674,24 +1116,27 @@ __global__ __launch_bounds__(256) void ep_mx4_join_kernel(const float* __restric
   l = wave_sum(l);
   if (__any(bad)) m = l = __uint_as_float(0x7fc00000u);
   if (threadIdx.x == 0 && blockIdx.y == 0) *reinterpret_cast<f4*>(ML + ((int64_t)b * Q + q) * 4) = f4{l == 0.f ? 0.f : m, l, 0.f, 0.f};
-  const int x = (int)threadIdx.x & 15, y = (int)threadIdx.x >> 4, d0 = (int)blockIdx.y * 64;
+  const int x = (int)threadIdx.x % LN, y = (int)threadIdx.x / LN, d = ((int)blockIdx.y * LN + x) * 4;
   f4 a = {0.f, 0.f, 0.f, 0.f};
-  for (int s = y; s < splits; s += 16) {
+  for (int s = y; s < splits; s += CH) {
     if (e[(int64_t)s * 2 * Q + 1] == 0.f) continue;
     const float f = __builtin_amdgcn_exp2f((e[(int64_t)s * 2 * Q] - m) * MX_LOG2E);
-    const float* row = part + (((int64_t)b * splits + s) * Q + q) * D + d0 + 4 * x;
+    const float* row = part + (((int64_t)b * splits + s) * Q + q) * D + d;
+    if (D % 4 == 0) { if (d < D) a += f * *reinterpret_cast<const f4*>(row); }
+    else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (d0 + 4 * x + j < D) a[j] += f * row[j];
+      for (int j = 0; j < 4; ++j)
+        if (d + j < D) a[j] += f * row[j];
+    }
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) red[y][4 * x + j] = a[j];
+  red[y][x] = a;
   __syncthreads();
-  if (threadIdx.x < 64 && d0 + (int)threadIdx.x < D) {
-    float r = red[0][threadIdx.x];
-    for (int k = 1; k < 16; ++k) r += red[k][threadIdx.x];
-    P[((int64_t)b * Q + q) * D + d0 + threadIdx.x] = r * (l == 0.f ? 0.f : 1.f / l);
-  }
+  if (y) return;
+  for (int k = 1; k < CH; ++k) a += red[k][x];
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (d + j < D) P[((int64_t)b * Q + q) * D + d + j] = a[j] * inv;
 }
 
 // out[i] (+)= sum over n of part[n][i], 16 interleaved chains and then these in order; blockIdx.y selects the output
@@ -732,52 +1177,58 @@ __global__ __launch_bounds__(256) void ep_mx4_pad_rows_kernel(const float* __res
   out[i] = d < D ? src[r * D + d] : 0.f;
 }
 
-struct MxPlan { int qm, cpw, nw, groups, splits, tps, units, grid, yblk, qblk; size_t lds, ws, pad; };     // ws: bytes, of them pad for padded operand rows
+struct MxPlan {
+  int qm, cpw, nw, groups, splits, tps, units, grid, yblk, qblk;
+  int stages;                                                           // of the pipelined form, or 0: the wide-row form
+  size_t lds, ws, pad;                                                  // ws: bytes, of them pad for padded operand rows
+};
+
+static size_t mx_pipe_lds(int qm, int nw, int stages) {
+  const size_t rec = 256 * (qm == 8 ? 4 : qm == 16 ? 8 : 16), nqb = qm == 32 ? 2 : 1, wall = nqb * (qm == 8 ? 2 : 3) * 1024 + 2 * nqb * 64 + 64;
+  return (size_t)nw * stages * 2176 + 2 * (size_t)nw * rec + 2 * wall;
+}
 
 static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   MxPlan p{};
   const int nc = mx_blocks(D), cus = cu_count(), tiles = (N + 31) / 32;
-  // widest query block that the row width leaves registers for: accumulators and operand of a 128-channel block take 50 / 68 / 136
-  // registers at 8 / 16 / 32 queries, a workgroup is at most 8 waves of 256
-  p.qm = Q <= 8 || nc > 24 ? 8 : (Q <= 16 || nc > 8 ? 16 : 32);
-  const int cmax = p.qm == 8 ? 4 : (p.qm == 16 ? 3 : 1);
-  p.nw = (nc + cmax - 1) / cmax;
-  p.cpw = (nc + p.nw - 1) / p.nw;
+  constexpr int LDS = 160 * 1024;
+  int cap;                                                              // workgroups that run at the same time
+  if (nc <= 15) {                                                       // a wave per block and the weight wave: at most 16 (12 at 32 queries)
+    p.qm = Q <= 8 ? 8 : (Q <= 16 || nc > 11 ? 16 : 32);
+    p.nw = nc; p.cpw = 1; p.groups = 1;
+    const int waves = p.qm == 32 ? 12 : 16;
+    auto fit = [&](int st) { const int n = (int)(LDS / mx_pipe_lds(p.qm, nc, st)); return waves / (nc + 1) < n ? waves / (nc + 1) : n; };
+    p.stages = fit(4) == fit(3) ? 4 : 3;
+    p.lds = mx_pipe_lds(p.qm, nc, p.stages);
+    cap = cus * fit(p.stages);
+  } else {                                                              // four blocks per wave
+    p.qm = 8;
+    p.nw = (nc + 3) / 4; p.cpw = 4;
+    p.groups = bwd || B <= cus ? 8 / p.nw : 1;
+    const int waves = p.nw * p.groups;
+    p.lds = (size_t)waves * (MX_STAGES * (2048 * 4 + 512)) + 2 * (size_t)waves * 1024;
+    const int n = (int)(LDS / p.lds);
+    cap = cus * (8 / waves < n ? 8 / waves : n);
+  }
   p.yblk = (Q + p.qm - 1) / p.qm;
   p.qblk = (Q + p.yblk - 1) / p.yblk;
-  const int gmax = 8 / p.nw;                                            // groups of a workgroup of at most 8 waves
-  p.splits = 1;
-  if (bwd) {
-    p.groups = gmax;
-    const int64_t want = (int64_t)cus * gmax;
-    if (B < want) p.splits = (int)((want + B - 1) / B);
-    const int most = (tiles + 1) / 2;
-    if (p.splits > most) p.splits = most;
-  } else {
-    p.groups = B <= cus ? gmax : 1;
-    if (p.groups > tiles) p.groups = tiles;
-    if (B < cus) p.splits = cus / B;
-    const int most = tiles / (4 * p.groups);
-    if (p.splits > most) p.splits = most;
-  }
+  // few images: their token axis is cut into runs.  Forward the runs have to be joined by a second launch, so they are kept longer.
+  const int per = p.stages ? 1 : p.groups, least = bwd ? 2 : (p.stages ? 8 : 2 * per);
+  p.splits = B < cap * (bwd ? per : 1) ? (cap * (bwd ? per : 1)) / B : 1;
+  if (p.splits > tiles / least) p.splits = tiles / least;
   if (p.splits < 1) p.splits = 1;
   p.tps = (tiles + p.splits - 1) / p.splits;
   p.splits = (tiles + p.tps - 1) / p.tps;
   p.units = B * p.splits;
-  const int stage = 2048 * p.cpw + 256 * ((p.cpw + 1) / 2), rec = 256 * (p.qm == 8 ? 4 : p.qm == 16 ? 8 : 16);
-  const int waves = p.nw * p.groups;
-  p.lds = (size_t)waves * (MX_STAGES * stage) + (p.nw > 1 || p.groups > 1 ? 2 * (size_t)waves * rec : 0);
-  if (bwd) {
-    p.grid = (p.units + p.groups - 1) / p.groups;
-    if (p.grid > cus) p.grid = cus;
-    p.ws = !per_image ? (size_t)p.grid * Q * D * 4 : p.splits > 1 ? (size_t)p.units * Q * D * 4 : 0;
+  if (p.stages) {
+    p.grid = p.units < cap ? p.units : cap;
+  } else if (bwd) {
+    p.grid = (p.units + p.groups - 1) / p.groups < cap ? (p.units + p.groups - 1) / p.groups : cap;
   } else {
-    int per_cu = 8 / waves;
-    const int by_lds = (int)(160 * 1024 / p.lds);
-    if (per_cu > by_lds) per_cu = by_lds;
-    p.grid = p.groups > 1 ? p.units : (p.units < cus * per_cu ? p.units : cus * per_cu);
-    p.ws = p.splits > 1 ? (size_t)p.units * Q * (D + 2) * 4 : 0;
+    p.grid = p.groups > 1 || p.units < cap ? p.units : cap;             // several groups share one unit: a workgroup each
   }
+  if (bwd) p.ws = !per_image ? (size_t)p.grid * Q * D * 4 : p.splits > 1 ? (size_t)p.units * Q * D * 4 : 0;
+  else p.ws = p.splits > 1 ? (size_t)p.units * Q * (D + 2) * 4 : 0;
   const size_t rows = (size_t)(bwd ? 2 * (int64_t)B * Q : per_image ? (int64_t)B * Q : Q);
   p.pad = D % MX_BLOCK ? round_up(rows * nc * MX_BLOCK * 4, 256) : 0;
   p.ws += p.pad;
@@ -798,25 +1249,24 @@ static int mx_rows(const float* src, int64_t rows, int D, char*& ws, const float
   return 0;
 }
 
-template <int QM, int CPW, bool BWD>
-static int mx_launch2(const MxPool& p, const MxPlan& pl, hipStream_t st) {
-  auto* fn = ep_mx4_pool_kernel<QM, CPW, MX_STAGES, BWD>;
+template <typename K>
+static int mx_launch_kernel(K* fn, const MxPool& p, const MxPlan& pl, int threads, hipStream_t st) {
   if (pl.lds > 64 * 1024) EP_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, (int)pl.lds));
-  hipLaunchKernelGGL((ep_mx4_pool_kernel<QM, CPW, MX_STAGES, BWD>), dim3((unsigned)pl.grid, (unsigned)pl.yblk), dim3((unsigned)(64 * pl.nw * pl.groups)), pl.lds, st, p);
+  hipLaunchKernelGGL(fn, dim3((unsigned)pl.grid, (unsigned)pl.yblk), dim3((unsigned)threads), pl.lds, st, p);
   EP_LAUNCH_CHECK("ep_mx4_pool_kernel");
   return 0;
 }
 template <bool BWD>
 static int mx_launch(const MxPool& p, const MxPlan& pl, hipStream_t st) {
-  switch (pl.qm * 10 + pl.cpw) {
-    case 81: return mx_launch2<8, 1, BWD>(p, pl, st);
-    case 82: return mx_launch2<8, 2, BWD>(p, pl, st);
-    case 83: return mx_launch2<8, 3, BWD>(p, pl, st);
-    case 84: return mx_launch2<8, 4, BWD>(p, pl, st);
-    case 161: return mx_launch2<16, 1, BWD>(p, pl, st);
-    case 162: return mx_launch2<16, 2, BWD>(p, pl, st);
-    case 163: return mx_launch2<16, 3, BWD>(p, pl, st);
-    default: return mx_launch2<32, 1, BWD>(p, pl, st);
+  const int threads = 64 * (pl.nw + 1);
+  switch (pl.stages * 100 + pl.qm) {
+    case 308: return mx_launch_kernel(ep_mx4_pipe_kernel<8, 3, BWD>, p, pl, threads, st);
+    case 408: return mx_launch_kernel(ep_mx4_pipe_kernel<8, 4, BWD>, p, pl, threads, st);
+    case 316: return mx_launch_kernel(ep_mx4_pipe_kernel<16, 3, BWD>, p, pl, threads, st);
+    case 416: return mx_launch_kernel(ep_mx4_pipe_kernel<16, 4, BWD>, p, pl, threads, st);
+    case 332: return mx_launch_kernel(ep_mx4_pipe_kernel<32, 3, BWD>, p, pl, threads, st);
+    case 432: return mx_launch_kernel(ep_mx4_pipe_kernel<32, 4, BWD>, p, pl, threads, st);
+    default: return mx_launch_kernel(ep_mx4_pool_kernel<8, 4, MX_STAGES, BWD>, p, pl, 64 * pl.nw * pl.groups, st);
   }
 }
 
@@ -841,7 +1291,10 @@ int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bst
   p.lds_ = s_stride;
   EP_TRY(mx_launch<false>(p, pl, st));
   if (pl.splits > 1) {
-    hipLaunchKernelGGL(ep_mx4_join_kernel, dim3((unsigned)t->B * Q, (unsigned)((t->D + 63) / 64)), dim3(256), 0, st, p.part, p.part_ml, pl.splits, Q, t->D, P, ML);
+    if (pl.splits <= 4)
+      hipLaunchKernelGGL(ep_mx4_join_kernel<1>, dim3((unsigned)t->B * Q, (unsigned)((t->D + 1023) / 1024)), dim3(256), 0, st, p.part, p.part_ml, pl.splits, Q, t->D, P, ML);
+    else
+      hipLaunchKernelGGL(ep_mx4_join_kernel<16>, dim3((unsigned)t->B * Q, (unsigned)((t->D + 63) / 64)), dim3(256), 0, st, p.part, p.part_ml, pl.splits, Q, t->D, P, ML);
     EP_LAUNCH_CHECK("ep_mx4_join_kernel");
   }
   return 0;
