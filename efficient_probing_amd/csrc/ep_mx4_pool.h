@@ -4,7 +4,8 @@
 
 namespace ep {
 
-constexpr int MX_STAGES = 2;             // tiles of a wave's ring
+constexpr int MX_STAGES = 2;             // tiles of a wave's ring: wide-row form
+constexpr int MX_PIPE_STAGES = 3;        // ... and pipelined form
 
 struct MxPool {
   ep_mx4_tokens t;

@@ -664,11 +664,12 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
 // instead of once per wave, and the pool waves' registers (accumulators and operand of one block) leave room for 3 - 4 waves a SIMD.
 template <int QM> constexpr int mx_pipe_waves() { return QM == 32 ? 12 : 16; }
 
-template <int QM, int NST, bool BWD>
+// OPENS: the operand rows change with the image (backward, per-image queries); else they are made once.
+template <int QM, bool BWD, bool OPENS>
 __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) void ep_mx4_pipe_kernel(MxPool p) {
   typedef MxDims<QM> DM;
-  constexpr int NQB = DM::NQB, SV = DM::SV;
-  constexpr int STAGE = 2048 + 128, OPS = 3;
+  constexpr int NQB = DM::NQB, SV = DM::SV, PREC = 2048 * NQB;            // a record: the accumulators as they are
+  constexpr int NST = MX_PIPE_STAGES, STAGE = 2048 + 128, OPS = 3;
   constexpr int WREC = NQB * DM::PSETS * 1024, WALL = WREC + 2 * NQB * 64 + 64;      // weights, rescaling factors, row factors, flags
   extern __shared__ __align__(16) char lds[];
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
@@ -677,7 +678,8 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
   const int nw = p.nw, rowC = p.nc * 64, rowS = p.nc * 4;
   const int q0 = (int)blockIdx.y * p.qblk, qn = p.Q - q0 < p.qblk ? p.Q - q0 : p.qblk;      // queries of this workgroup
   char* recs = lds + nw * (NST * STAGE);                                // [2][nw][REC]
-  char* wbuf = recs + 2 * nw * DM::REC;                                 // [2][WALL]
+  char* wbuf = recs + 2 * nw * PREC;                                 // [2][WALL]
+  float* dbuf = reinterpret_cast<float*>(wbuf + 2 * WALL);              // [2][nw][NQB][16]: the blocks' parts of delta, by parity of the unit
   const int tok0 = 8 * g + (QM == 8 ? 4 * (c >> 3) : 0);                // first token of the lane's scores in a tile
   const float NANF = __uint_as_float(0x7fc00000u);
 
@@ -692,29 +694,43 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
     const int p_off = g * 64 + c * 4;                                   // slot i: (p_off ^ 16 (i % 4)) + 256 i
     const uint32_t rot = (uint32_t)(8 * (c >> 2) + 9);
 
-    auto issue = [&](const MxCursor& cu, int slot) {
+    // lane offsets of a whole tile; rows behind an image's end repeat its last one
+    const int dtok = 8 * ((lane >> 2) & 3) + g;
+    const unsigned dseg = (unsigned)(((lane & 3) ^ g) * 16);
+    const unsigned full0 = (unsigned)(dtok * rowC) + dseg, fulls = (unsigned)((lane & 31) * rowS);
+    MxCursor ahead;                                                     // the tile to load, and where it lies
+    const uint8_t *src, *scl;
+    auto locate = [&]() {
+      const int64_t t0 = (int64_t)ahead.tile << 5;
+      src = t.codes + (int64_t)ahead.img * t.codes_bstride + t0 * rowC + wave * 64;
+      scl = t.scales + (int64_t)ahead.img * t.scales_bstride + t0 * rowS + wave * 4;
+    };
+    auto load_tile = [&](int slot) {                                    // ... into the ring; and on to the next
       char* st = ring + slot * STAGE;
-      const int t0 = cu.tile << 5, last = cu.len - t0 - 1;              // rows behind the image's end repeat its last one
-      const uint8_t* src = t.codes + (int64_t)cu.img * t.codes_bstride + (int64_t)t0 * rowC + wave * 64;
-      const uint8_t* scl = t.scales + (int64_t)cu.img * t.scales_bstride + (int64_t)t0 * rowS + wave * 4;
-      const int ln = mx_fresh(lane);
-      const int tok = 8 * ((ln >> 2) & 3) + (ln >> 4);
-      const unsigned seg = (unsigned)(((ln & 3) ^ (ln >> 4)) * 16);
-      const unsigned off0 = (unsigned)((tok < last ? tok : last) * rowC) + seg, off1 = (unsigned)((tok + 4 < last ? tok + 4 : last) * rowC) + seg;
+      const int last = ahead.len - (ahead.tile << 5) - 1;
+      unsigned off0 = full0, off1 = full0 + 4 * rowC, offs = fulls;
+      if (last < 31) {
+        off0 = (unsigned)((dtok < last ? dtok : last) * rowC) + dseg;
+        off1 = (unsigned)((dtok + 4 < last ? dtok + 4 : last) * rowC) + dseg;
+        offs = (unsigned)(((lane & 31) < last ? (lane & 31) : last) * rowS);
+      }
       __builtin_amdgcn_global_load_lds((mx_gptr_t)(src + off0), (mx_lds_t)st, 16, 0, MX_NT);
       __builtin_amdgcn_global_load_lds((mx_gptr_t)(src + off1), (mx_lds_t)(st + 1024), 16, 0, MX_NT);
-      if (ln < 32) __builtin_amdgcn_global_load_lds((mx_gptr_t)(scl + (unsigned)((ln < last ? ln : last) * rowS)), (mx_lds_t)(st + 2048), 4, 0, 0);
+      if (lane < 32) __builtin_amdgcn_global_load_lds((mx_gptr_t)(scl + offs), (mx_lds_t)(st + 2048), 4, 0, 0);
+      src += 32 * rowC; scl += 32 * rowS;
+      if (ahead.next(t)) locate();
     };
 
-    MxCursor cs = start, ahead;                                         // the tile to score, the tile to load
+    MxCursor cs = start;                                                // the tile to score
     cs.open(t);
     ahead = cs;
+    locate();
 #pragma unroll
-    for (int i = 0; i < NST; ++i) { issue(ahead, i); ahead.next(t); }
+    for (int i = 0; i < NST; ++i) load_tile(i);
     MxCursor cp = cs;                                                   // the tile to pool
 
     MxOperand<QM> op[NQB];
-    float delta[NQB];
+    int parity = 0;
     auto open_unit = [&](int b) {                                       // the operand rows; backward: this block's part of delta = dP . P
       const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
       const float* rows = p.q + (BWD ? (int64_t)b * p.Q * p.ldq : (int64_t)b * p.qb);
@@ -724,19 +740,20 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
         const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * p.ldq + wave * MX_BLOCK + 32 * g;    // (rows without a query: the first one's, times 0)
         mx_f16 ve, vo;
         mx_load_row(rows + at, q < qn ? (BWD ? 1.f : p.scale) : 0.f, ve, vo);
-        float d = 0.f;
         if (BWD && p.Pin) {
+          float d = 0.f;
           mx_f16 we, wo;
           mx_load_row(p.Pin + (int64_t)b * p.Q * p.ldq + at, 1.f, we, wo);
 #pragma unroll
           for (int i = 0; i < 16; ++i) d = fmaf(vo[i], wo[i], fmaf(ve[i], we[i], d));
           d = mx_over_groups_sum(d);
+          if (g == 0) dbuf[((parity * nw + wave) * NQB + qb) * 16 + c] = d;
           __builtin_amdgcn_sched_barrier(0);
         }
-        delta[qb] = d;
         mx_operand<QM>(ve, vo, c, op[qb]);
         __builtin_amdgcn_sched_barrier(0);
       }
+      parity ^= 1;
     };
 
     f4 acc[NQB][8];
@@ -779,10 +796,8 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
     auto scores = [&]() {                                               // first contraction of the ring's stage sslot -> record
       mx_wait_vm<(NST - 2) * OPS>();
       const char* st = ring + sslot * STAGE;
-      char* rec = recs + (buf * nw + wave) * DM::REC;
-      f4 sa[NQB][2], sl[NQB][2];                                        // leading and lower terms: an addition to a large sum costs its last bit
-#pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) sa[qb][0] = sa[qb][1] = sl[qb][0] = sl[qb][1] = f4{0.f, 0.f, 0.f, 0.f};
+      char* rec = recs + (buf * nw + wave) * PREC;
+      // lower terms first: only the last addition, the leading term's, rounds at the size of the score
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const mx_u4 w = *reinterpret_cast<const mx_u4*>(st + h * 1024 + a_off);
@@ -790,31 +805,15 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
 #pragma unroll
         for (int qb = 0; qb < NQB; ++qb) {
           const MxOperand<QM>& o = op[qb];
-          sa[qb][h] = mx_mfma_codes<0>(w, sc, o.b[0], o.sc[0], sa[qb][h]);
+          f4 s = {0.f, 0.f, 0.f, 0.f};
           if constexpr (QM != 8) {
-            sl[qb][h] = mx_mfma_codes<1>(w, sc, o.b[4], o.sc[1], sl[qb][h]);
-            sl[qb][h] = mx_mfma_codes<0>(w, sc, o.b[3], o.sc[1], sl[qb][h]);
+            s = mx_mfma_codes<1>(w, sc, o.b[4], o.sc[1], s);
+            s = mx_mfma_codes<0>(w, sc, o.b[3], o.sc[1], s);
           }
-          sl[qb][h] = mx_mfma_codes<2>(w, sc, o.b[2], o.sc[0], sl[qb][h]);
-          sl[qb][h] = mx_mfma_codes<1>(w, sc, o.b[1], o.sc[0], sl[qb][h]);
-        }
-      }
-#pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) {
-        sa[qb][0] += sl[qb][0]; sa[qb][1] += sl[qb][1];
-        const float dl = BWD ? delta[qb] : 0.f;
-        if constexpr (QM == 8) {                                        // columns q and q + 8 are terms of one query
-          const bool up = (c & 8) != 0;
-          f4 s;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float own = up ? sa[qb][1][i] : sa[qb][0][i], oth = up ? sa[qb][0][i] : sa[qb][1][i];
-            s[i] = own + mx_ror8(oth) - dl;
-          }
-          *reinterpret_cast<f4*>(rec + lane * 16) = s;
-        } else {
-          *reinterpret_cast<f4*>(rec + (2 * qb) * 1024 + lane * 16) = sa[qb][0] - dl;
-          *reinterpret_cast<f4*>(rec + (2 * qb + 1) * 1024 + lane * 16) = sa[qb][1] - dl;
+          s = mx_mfma_codes<2>(w, sc, o.b[2], o.sc[0], s);
+          s = mx_mfma_codes<1>(w, sc, o.b[1], o.sc[0], s);
+          s = mx_mfma_codes<0>(w, sc, o.b[0], o.sc[0], s);
+          *reinterpret_cast<f4*>(rec + (2 * qb + h) * 1024 + lane * 16) = s;
         }
       }
       sslot = sslot + 1 == NST ? 0 : sslot + 1;
@@ -863,8 +862,7 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
       EP_MX_PAIR(0); EP_MX_PAIR(1); EP_MX_PAIR(2); EP_MX_PAIR(3);
 #undef EP_MX_PAIR
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                // the stage is read
-      issue(ahead, pslot);
-      ahead.next(t);
+      load_tile(pslot);
       pslot = pslot + 1 == NST ? 0 : pslot + 1;
     };
 
@@ -882,7 +880,7 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
       for (;;) {
         const bool more = cs.valid();
         if (more) {
-          if (fresh && (BWD || p.qb)) open_unit(cs.b);
+          if (OPENS && fresh) open_unit(cs.b);
           scores();
         }
         mx_barrier();
@@ -950,12 +948,12 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
           if (q < qn) ml = *reinterpret_cast<const f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4);
           mz[qb] = ml.x;
           invl[qb] = ml.y == 0.f ? 0.f : 1.f / ml.y;
-          dml[qb] = p.Pin ? 0.f : ml.z;
+          dml[qb] = ml.z;
         }
       }
     };
     bool fresh = true;
-    int buf = 0;
+    int buf = 0, parity = 0;
     if (BWD) load_scores(cw);
     for (;;) {
       const bool more = cw.valid();
@@ -963,6 +961,15 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
       mx_barrier();
       if (!more) break;
       const int b = cw.b, u = cw.u, t0 = cw.tile << 5, len = cw.len;
+      if (BWD && fresh && p.Pin) {                                      // delta from the blocks' parts
+#pragma unroll
+        for (int qb = 0; qb < NQB; ++qb) {
+          float d = 0.f;
+          for (int o = 0; o < nw; ++o) d += dbuf[((parity * nw + o) * NQB + qb) * 16 + c];
+          dml[qb] = d;
+        }
+        parity ^= 1;
+      }
       const bool tail = t0 + 32 > len;
       char* wr = wbuf + buf * WALL;
       bool moved = false;
@@ -970,13 +977,25 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
       for (int qb = 0; qb < NQB; ++qb) {
         const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
         float s[SV], pv[SV];
+        f4 v[2];
 #pragma unroll
-        for (int h = 0; h < SV / 4; ++h) {                              // the blocks' parts, in their order
-          const char* r = recs + buf * nw * DM::REC + (qb * (SV / 4) + h) * 1024 + lane * 16;
-          f4 v = *reinterpret_cast<const f4*>(r);
+        for (int h = 0; h < 2; ++h) v[h] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-          for (int o = 1; o < nw; ++o) v += *reinterpret_cast<const f4*>(r + o * DM::REC);
-          s[4 * h] = v.x; s[4 * h + 1] = v.y; s[4 * h + 2] = v.z; s[4 * h + 3] = v.w;
+        for (int o = 0; o < nw; ++o) {                                  // the blocks' parts, in their order
+          const char* r = recs + (buf * nw + o) * PREC + qb * 2048 + lane * 16;
+          v[0] += *reinterpret_cast<const f4*>(r);
+          v[1] += *reinterpret_cast<const f4*>(r + 1024);
+        }
+        if constexpr (QM == 8) {                                        // columns q and q + 8 are terms of one query; a lane keeps one half
+          const bool up = (c & 8) != 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float own = up ? v[1][i] : v[0][i], oth = up ? v[0][i] : v[1][i];
+            s[i] = own + mx_ror8(oth);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < SV; ++i) s[i] = v[i / 4][i % 4];
         }
         if constexpr (!BWD) {
           if (tail) {
@@ -1179,13 +1198,13 @@ __global__ __launch_bounds__(256) void ep_mx4_pad_rows_kernel(const float* __res
 
 struct MxPlan {
   int qm, cpw, nw, groups, splits, tps, units, grid, yblk, qblk;
-  int stages;                                                           // of the pipelined form, or 0: the wide-row form
+  bool pipe;                                                            // the pipelined form, or the wide-row form
   size_t lds, ws, pad;                                                  // ws: bytes, of them pad for padded operand rows
 };
 
-static size_t mx_pipe_lds(int qm, int nw, int stages) {
-  const size_t rec = 256 * (qm == 8 ? 4 : qm == 16 ? 8 : 16), nqb = qm == 32 ? 2 : 1, wall = nqb * (qm == 8 ? 2 : 3) * 1024 + 2 * nqb * 64 + 64;
-  return (size_t)nw * stages * 2176 + 2 * (size_t)nw * rec + 2 * wall;
+static size_t mx_pipe_lds(int qm, int nw) {
+  const size_t nqb = qm == 32 ? 2 : 1, rec = 2048 * nqb, wall = nqb * (qm == 8 ? 2 : 3) * 1024 + 2 * nqb * 64 + 64;
+  return (size_t)nw * MX_PIPE_STAGES * 2176 + 2 * (size_t)nw * rec + 2 * wall + 2 * (size_t)nw * nqb * 64;
 }
 
 static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
@@ -1197,10 +1216,10 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
     p.qm = Q <= 8 ? 8 : (Q <= 16 || nc > 11 ? 16 : 32);
     p.nw = nc; p.cpw = 1; p.groups = 1;
     const int waves = p.qm == 32 ? 12 : 16;
-    auto fit = [&](int st) { const int n = (int)(LDS / mx_pipe_lds(p.qm, nc, st)); return waves / (nc + 1) < n ? waves / (nc + 1) : n; };
-    p.stages = fit(4) == fit(3) ? 4 : 3;
-    p.lds = mx_pipe_lds(p.qm, nc, p.stages);
-    cap = cus * fit(p.stages);
+    p.pipe = true;
+    p.lds = mx_pipe_lds(p.qm, nc);
+    const int n = (int)(LDS / p.lds);
+    cap = cus * (waves / (nc + 1) < n ? waves / (nc + 1) : n);
   } else {                                                              // four blocks per wave
     p.qm = 8;
     p.nw = (nc + 3) / 4; p.cpw = 4;
@@ -1213,14 +1232,14 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   p.yblk = (Q + p.qm - 1) / p.qm;
   p.qblk = (Q + p.yblk - 1) / p.yblk;
   // few images: their token axis is cut into runs.  Forward the runs have to be joined by a second launch, so they are kept longer.
-  const int per = p.stages ? 1 : p.groups, least = bwd ? 2 : (p.stages ? 8 : 2 * per);
+  const int per = p.pipe ? 1 : p.groups, least = bwd ? 2 : (p.pipe ? 8 : 2 * per);
   p.splits = B < cap * (bwd ? per : 1) ? (cap * (bwd ? per : 1)) / B : 1;
   if (p.splits > tiles / least) p.splits = tiles / least;
   if (p.splits < 1) p.splits = 1;
   p.tps = (tiles + p.splits - 1) / p.splits;
   p.splits = (tiles + p.tps - 1) / p.tps;
   p.units = B * p.splits;
-  if (p.stages) {
+  if (p.pipe) {
     p.grid = p.units < cap ? p.units : cap;
   } else if (bwd) {
     p.grid = (p.units + p.groups - 1) / p.groups < cap ? (p.units + p.groups - 1) / p.groups : cap;
@@ -1259,15 +1278,11 @@ static int mx_launch_kernel(K* fn, const MxPool& p, const MxPlan& pl, int thread
 template <bool BWD>
 static int mx_launch(const MxPool& p, const MxPlan& pl, hipStream_t st) {
   const int threads = 64 * (pl.nw + 1);
-  switch (pl.stages * 100 + pl.qm) {
-    case 308: return mx_launch_kernel(ep_mx4_pipe_kernel<8, 3, BWD>, p, pl, threads, st);
-    case 408: return mx_launch_kernel(ep_mx4_pipe_kernel<8, 4, BWD>, p, pl, threads, st);
-    case 316: return mx_launch_kernel(ep_mx4_pipe_kernel<16, 3, BWD>, p, pl, threads, st);
-    case 416: return mx_launch_kernel(ep_mx4_pipe_kernel<16, 4, BWD>, p, pl, threads, st);
-    case 332: return mx_launch_kernel(ep_mx4_pipe_kernel<32, 3, BWD>, p, pl, threads, st);
-    case 432: return mx_launch_kernel(ep_mx4_pipe_kernel<32, 4, BWD>, p, pl, threads, st);
-    default: return mx_launch_kernel(ep_mx4_pool_kernel<8, 4, MX_STAGES, BWD>, p, pl, 64 * pl.nw * pl.groups, st);
-  }
+  if (!pl.pipe) return mx_launch_kernel(ep_mx4_pool_kernel<8, 4, MX_STAGES, BWD>, p, pl, 64 * pl.nw * pl.groups, st);
+  const bool opens = BWD || p.qb;
+  if (pl.qm == 8) return opens ? mx_launch_kernel(ep_mx4_pipe_kernel<8, BWD, true>, p, pl, threads, st) : mx_launch_kernel(ep_mx4_pipe_kernel<8, BWD, BWD>, p, pl, threads, st);
+  if (pl.qm == 16) return opens ? mx_launch_kernel(ep_mx4_pipe_kernel<16, BWD, true>, p, pl, threads, st) : mx_launch_kernel(ep_mx4_pipe_kernel<16, BWD, BWD>, p, pl, threads, st);
+  return opens ? mx_launch_kernel(ep_mx4_pipe_kernel<32, BWD, true>, p, pl, threads, st) : mx_launch_kernel(ep_mx4_pipe_kernel<32, BWD, BWD>, p, pl, threads, st);
 }
 
 static MxPool mx_pool_params(const ep_mx4_tokens* t, int Q, float scale, const MxPlan& pl) {
