@@ -662,11 +662,9 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
 //     weight wave                                          | barrier j | sums the records of tile j, softmax (or dS), weights j
 // so that the long chain exchange -> maximum -> exponentials -> split runs beside the contractions of other tiles, once per tile
 // instead of once per wave, and the pool waves' registers (accumulators and operand of one block) leave room for 3 - 4 waves a SIMD.
-template <int QM> constexpr int mx_pipe_waves() { return QM == 32 ? 12 : 16; }
-
 // OPENS: the operand rows change with the image (backward, per-image queries); else they are made once.
 template <int QM, bool BWD, bool OPENS>
-__global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) void ep_mx4_pipe_kernel(MxPool p) {
+__global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
   typedef MxDims<QM> DM;
   constexpr int NQB = DM::NQB, SV = DM::SV, PREC = 2048 * NQB;            // a record: the accumulators as they are
   constexpr int NST = MX_PIPE_STAGES, STAGE = 2048 + 128, OPS = 3;
@@ -764,7 +762,7 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
         for (int j = 0; j < 8; ++j) acc[qb][j] = f4{0.f, 0.f, 0.f, 0.f};
     };
     // acc times r (one factor per row 4 g + i) as rows of out: QM 8 adds the two term rows first
-    auto store_rows = [&](float* out, const f4 (&r)[NQB]) {
+    auto store_rows = [&](float* out, const f4 (&r)[NQB], bool add) {
       const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
 #pragma unroll
       for (int qb = 0; qb < NQB; ++qb)
@@ -781,11 +779,15 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
             for (int j = 0; j < 4; ++j) x[j] = (QM == 8 ? fold32(acc[qb][j][i], acc[qb][j + 4][i]) : acc[qb][4 * v + j][i]) * r[qb][i];
             const int d = wave * MX_BLOCK + 8 * c + (QM == 8 ? 4 * (g >> 1) : 4 * v);
             if (q < qn) {
-              if (p.veco) { if (d < t.D) *reinterpret_cast<f4*>(o + d) = x; }
-              else {
+              if (p.veco) {
+                if (d < t.D) {
+                  if (BWD && add) x += *reinterpret_cast<const f4*>(o + d);
+                  *reinterpret_cast<f4*>(o + d) = x;
+                }
+              } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                  if (d + j < t.D) o[d + j] = x[j];
+                  if (d + j < t.D) o[d + j] = BWD && add ? o[d + j] + x[j] : x[j];
               }
             }
           }
@@ -866,47 +868,47 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
       pslot = pslot + 1 == NST ? 0 : pslot + 1;
     };
 
-    clear();
-    f4 one[NQB];
-#pragma unroll
-    for (int qb = 0; qb < NQB; ++qb) one[qb] = f4{p.scale, p.scale, p.scale, p.scale};
-    if (cs.valid()) {
+    // The sequence of tiles; where the operand changes with the image, one sequence per unit: the accumulators are written out (added to
+    // the workgroup's partial gradient) before the next rows are made, for which there would be no registers beside them.
+    bool first = true;
+    while (cs.valid()) {
       open_unit(cs.b);
-      bool fresh = false;
+      clear();
+      const int unit = cs.u;
       scores();
       buf ^= 1;
-      fresh = cs.next(t);
+      cs.next(t);
       mx_barrier();
       for (;;) {
-        const bool more = cs.valid();
-        if (more) {
-          if (OPENS && fresh) open_unit(cs.b);
-          scores();
-        }
+        const bool more = cs.valid() && (!OPENS || cs.u == unit);
+        if (more) scores();
         mx_barrier();
-        buf ^= 1;                                                       // weights of the tile before, at the other parity than its record's successor
+        buf ^= 1;                                                       // (the parity of the tile before)
         pool();
         const int u = cp.u, b = cp.b;
-        if (cp.next(t)) {                                               // the unit's last tile
-          if constexpr (!BWD) {
+        const bool done = cp.next(t);                                   // that was the unit's last tile
+        if constexpr (!BWD) {
+          if (done) {
             f4 r[NQB];
 #pragma unroll
             for (int qb = 0; qb < NQB; ++qb) r[qb] = *reinterpret_cast<const f4*>(wbuf + buf * WALL + WREC + NQB * 64 + qb * 64 + (QM == 8 ? 16 * (g & 1) : 16 * g));
-            store_rows(p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, r);
-            clear();
-          } else if (p.per_unit) {
-            store_rows(p.part + (int64_t)u * p.Q * t.D, one);
-            clear();
+            store_rows(p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, r, false);
+            if (!OPENS) clear();
           }
         }
         if (!more) break;
-        fresh = cs.next(t);
+        cs.next(t);
       }
-    } else {
-      mx_barrier();
+      buf ^= 1;
+      if constexpr (BWD) {
+        f4 one[NQB];
+#pragma unroll
+        for (int qb = 0; qb < NQB; ++qb) one[qb] = f4{p.scale, p.scale, p.scale, p.scale};
+        store_rows(p.part + (int64_t)(p.per_unit ? unit : (int)blockIdx.x) * p.Q * t.D, one, !p.per_unit && !first);
+      }
+      first = false;
     }
-    if (BWD && !p.per_unit) store_rows(p.part + (int64_t)blockIdx.x * p.Q * t.D, one);
-    else {                                                              // units without a token
+    if (!BWD || p.per_unit) {                                           // units without a token
       clear();
       for (int u = (int)blockIdx.x; u < p.units; u += (int)gridDim.x) {
         const int b = u / p.splits, sp = u - b * p.splits;
@@ -917,8 +919,14 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
         f4 r[NQB];
 #pragma unroll
         for (int qb = 0; qb < NQB; ++qb) r[qb] = f4{f, f, f, f};
-        store_rows(BWD || p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, r);
+        store_rows(BWD || p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, r, false);
       }
+    } else if (first) {                                                 // no unit of this workgroup had a token
+      clear();
+      f4 r[NQB];
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) r[qb] = f4{0.f, 0.f, 0.f, 0.f};
+      store_rows(p.part + (int64_t)blockIdx.x * p.Q * t.D, r, false);
     }
     mx_wait_vm<0>();                                                    // no load into LDS outlives its wave
   } else {                                                              // ================= weight wave
@@ -955,11 +963,9 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
     bool fresh = true;
     int buf = 0, parity = 0;
     if (BWD) load_scores(cw);
-    for (;;) {
-      const bool more = cw.valid();
-      if (more && fresh) open_unit(cw.b);
+    while (cw.valid()) {
+      if (fresh) open_unit(cw.b);
       mx_barrier();
-      if (!more) break;
       const int b = cw.b, u = cw.u, t0 = cw.tile << 5, len = cw.len;
       if (BWD && fresh && p.Pin) {                                      // delta from the blocks' parts
 #pragma unroll
@@ -1094,6 +1100,7 @@ __global__ __launch_bounds__(64 * mx_pipe_waves<QM>(), mx_pipe_waves<QM>() / 4) 
         }
       }
       buf ^= 1;
+      if (OPENS ? fresh : !cw.valid()) mx_barrier();                    // the sequence's last weights are done
     }
     if constexpr (!BWD) {                                               // units without a token
       for (int u = (int)blockIdx.x; u < p.units; u += (int)gridDim.x) {
@@ -1212,10 +1219,10 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   const int nc = mx_blocks(D), cus = cu_count(), tiles = (N + 31) / 32;
   constexpr int LDS = 160 * 1024;
   int cap;                                                              // workgroups that run at the same time
-  if (nc <= 15) {                                                       // a wave per block and the weight wave: at most 16 (12 at 32 queries)
-    p.qm = Q <= 8 ? 8 : (Q <= 16 || nc > 11 ? 16 : 32);
+  if (nc <= 15) {                                                       // a wave per block and the weight wave
+    p.qm = Q <= 8 ? 8 : 16;
     p.nw = nc; p.cpw = 1; p.groups = 1;
-    const int waves = p.qm == 32 ? 12 : 16;
+    constexpr int waves = 16;                                           // four a SIMD
     p.pipe = true;
     p.lds = mx_pipe_lds(p.qm, nc);
     const int n = (int)(LDS / p.lds);
@@ -1281,8 +1288,7 @@ static int mx_launch(const MxPool& p, const MxPlan& pl, hipStream_t st) {
   if (!pl.pipe) return mx_launch_kernel(ep_mx4_pool_kernel<8, 4, MX_STAGES, BWD>, p, pl, 64 * pl.nw * pl.groups, st);
   const bool opens = BWD || p.qb;
   if (pl.qm == 8) return opens ? mx_launch_kernel(ep_mx4_pipe_kernel<8, BWD, true>, p, pl, threads, st) : mx_launch_kernel(ep_mx4_pipe_kernel<8, BWD, BWD>, p, pl, threads, st);
-  if (pl.qm == 16) return opens ? mx_launch_kernel(ep_mx4_pipe_kernel<16, BWD, true>, p, pl, threads, st) : mx_launch_kernel(ep_mx4_pipe_kernel<16, BWD, BWD>, p, pl, threads, st);
-  return opens ? mx_launch_kernel(ep_mx4_pipe_kernel<32, BWD, true>, p, pl, threads, st) : mx_launch_kernel(ep_mx4_pipe_kernel<32, BWD, BWD>, p, pl, threads, st);
+  return opens ? mx_launch_kernel(ep_mx4_pipe_kernel<16, BWD, true>, p, pl, threads, st) : mx_launch_kernel(ep_mx4_pipe_kernel<16, BWD, BWD>, p, pl, threads, st);
 }
 
 static MxPool mx_pool_params(const ep_mx4_tokens* t, int Q, float scale, const MxPlan& pl) {
