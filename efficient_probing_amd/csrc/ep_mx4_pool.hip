@@ -799,30 +799,49 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
       mx_wait_vm<(NST - 2) * OPS>();
       const char* st = ring + sslot * STAGE;
       char* rec = recs + (buf * nw + wave) * PREC;
-      // lower terms first: only the last addition, the leading term's, rounds at the size of the score
+      mx_u4 w[2];
+      uint32_t sc[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const mx_u4 w = *reinterpret_cast<const mx_u4*>(st + h * 1024 + a_off);
-        const uint32_t sc = *reinterpret_cast<const uint32_t*>(st + 2048 + h * 16 + sc_off) >> (8 * g);
-#pragma unroll
-        for (int qb = 0; qb < NQB; ++qb) {
-          const MxOperand<QM>& o = op[qb];
-          f4 s = {0.f, 0.f, 0.f, 0.f};
-          if constexpr (QM != 8) {
-            s = mx_mfma_codes<1>(w, sc, o.b[4], o.sc[1], s);
-            s = mx_mfma_codes<0>(w, sc, o.b[3], o.sc[1], s);
-          }
-          s = mx_mfma_codes<2>(w, sc, o.b[2], o.sc[0], s);
-          s = mx_mfma_codes<1>(w, sc, o.b[1], o.sc[0], s);
-          s = mx_mfma_codes<0>(w, sc, o.b[0], o.sc[0], s);
-          *reinterpret_cast<f4*>(rec + (2 * qb + h) * 1024 + lane * 16) = s;
-        }
+        w[h] = *reinterpret_cast<const mx_u4*>(st + h * 1024 + a_off);
+        sc[h] = *reinterpret_cast<const uint32_t*>(st + 2048 + h * 16 + sc_off) >> (8 * g);
       }
+      // lower terms first: only the last addition, the leading term's, rounds at the size of the score
+      f4 s[NQB][2];
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb) {
+        const MxOperand<QM>& o = op[qb];
+        s[qb][0] = s[qb][1] = f4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (QM != 8) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) s[qb][h] = mx_mfma_codes<1>(w[h], sc[h], o.b[4], o.sc[1], s[qb][h]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) s[qb][h] = mx_mfma_codes<0>(w[h], sc[h], o.b[3], o.sc[1], s[qb][h]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[qb][h] = mx_mfma_codes<2>(w[h], sc[h], o.b[2], o.sc[0], s[qb][h]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[qb][h] = mx_mfma_codes<1>(w[h], sc[h], o.b[1], o.sc[0], s[qb][h]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[qb][h] = mx_mfma_codes<0>(w[h], sc[h], o.b[0], o.sc[0], s[qb][h]);
+      }
+#pragma unroll
+      for (int qb = 0; qb < NQB; ++qb)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) *reinterpret_cast<f4*>(rec + (2 * qb + h) * 1024 + lane * 16) = s[qb][h];
       sslot = sslot + 1 == NST ? 0 : sslot + 1;
     };
 
-    auto pool = [&]() {                                                 // second contraction of stage pslot with the weights of buffer buf
+    uint32_t w[8], s4[8];
+    auto fetch = [&]() {                                                // the codes and scales of stage pslot: asked for in front of the barrier
       const char* st = ring + pslot * STAGE;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = *reinterpret_cast<const uint32_t*>(st + i * 256 + (p_off ^ ((i & 3) << 4)));
+        s4[i] = *reinterpret_cast<const uint32_t*>(st + 2048 + g * 32 + i * 4);
+      }
+    };
+    auto pool = [&]() {                                                 // second contraction of stage pslot with the weights of buffer buf
       const char* wr = wbuf + buf * WALL;
       mx_u4 wt[NQB][DM::PSETS];
 #pragma unroll
@@ -839,14 +858,9 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
           }
         }
       }
-      uint32_t w[8];
       float sc[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i] = *reinterpret_cast<const uint32_t*>(st + i * 256 + (p_off ^ ((i & 3) << 4)));
-        const uint32_t four = *reinterpret_cast<const uint32_t*>(st + 2048 + g * 32 + i * 4);
-        sc[i] = __uint_as_float(__builtin_amdgcn_alignbit(four, four, rot));
-      }
+      for (int i = 0; i < 8; ++i) sc[i] = __uint_as_float(__builtin_amdgcn_alignbit(s4[i], s4[i], rot));
 #define EP_MX_PAIR(PR)                                                                                                   \
   do {                                                                                                                   \
     uint32_t x[8];                                                                                                       \
@@ -881,6 +895,7 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
       mx_barrier();
       for (;;) {
         const bool more = cs.valid() && (!OPENS || cs.u == unit);
+        fetch();
         if (more) scores();
         mx_barrier();
         buf ^= 1;                                                       // (the parity of the tile before)
@@ -930,6 +945,7 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
     }
     mx_wait_vm<0>();                                                    // no load into LDS outlives its wave
   } else {                                                              // ================= weight wave
+    __builtin_amdgcn_s_setprio(3);                                      // the pool waves wait for it at every barrier
     MxCursor cw = start;
     cw.open(t);
     float m_run[NQB], mz[NQB], l_run[NQB], t_max[NQB], invl[NQB], dml[NQB], sg[NQB][SV];
