@@ -586,5 +586,24 @@ def require_gpu_tensor(t, name: str) -> None:
 
 
 def current_stream_ptr(device=None) -> int:
+    """hipStream_t of torch's current stream (``torch.cuda.current_stream(device).cuda_stream`` without building the Stream object)."""
     import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    index = getattr(device, "index", device)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+def device_guard(device):
+    """Context in which ``device`` is the current one: launches go to the current device."""
+    import torch
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)

@@ -14,6 +14,7 @@ counterpart (its dump keeps float32 tokens, tools/dump_tokens.py:95-98).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -31,6 +32,11 @@ def row_bytes(dim: int) -> Tuple[int, int]:
     """(code bytes, scale bytes) of one token."""
     blocks = -(-dim // BLOCK)
     return blocks * 64, blocks * 4
+
+
+def _check_index(t: torch.Tensor, name: str, n: Optional[int]) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n) or t.shape[0] < 1:
+        raise ValueError(f"{name} must be a contiguous int32 vector" + (f" of {n}" if n else ""))
 
 
 class Mx4Tokens:
@@ -53,8 +59,8 @@ class Mx4Tokens:
             if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]) or (t.shape[0] > 1 and t.stride(0) < t.shape[1] * t.shape[2]):
                 raise ValueError(f"{name}: the rows of an image must be contiguous and images must not overlap (strides {t.stride()})")
         for t, name, n in ((lengths, "lengths", codes.shape[0]), (image_index, "image_index", None)):
-            if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n) or t.shape[0] < 1):
-                raise ValueError(f"{name} must be a contiguous int32 vector" + (f" of {n}" if n else ""))
+            if t is not None:
+                _check_index(t, name, n)
         devices = {t.device for t in (codes, scales, lengths, image_index) if t is not None}
         if len(devices) != 1:
             raise ValueError(f"codes, scales, lengths and image_index must be on one device, got {sorted(map(str, devices))}")
@@ -108,13 +114,17 @@ class Mx4Tokens:
         return Mx4Tokens(mv(self.codes), mv(self.scales), self.dim, mv(self.lengths), mv(self.image_index))
 
     def _args(self, image_index: Optional[torch.Tensor] = None) -> "N.EPMx4Tokens":
+        codes = self.codes
+        N.require_gpu_tensor(codes, "codes")
+        M, n, _ = codes.shape
+        idx = self.image_index
         if image_index is not None:
-            return self.select(image_index)._args()
-        N.require_gpu_tensor(self.codes, "codes")
-        B, n, D = self.shape
-        return N.EPMx4Tokens(codes=self.codes.data_ptr(), scales=self.scales.data_ptr(), codes_bstride=self.codes.stride(0),
-                             scales_bstride=self.scales.stride(0), lengths=F_._ptr(self.lengths), image_index=F_._ptr(self.image_index),
-                             M=self.codes.shape[0], B=B, N=n, D=D)
+            if idx is not None:
+                raise ValueError("this is a batch of a cache already: select from the cache")
+            _check_index(image_index, "image_index", None)
+            idx = image_index
+        return N.EPMx4Tokens(codes.data_ptr(), self.scales.data_ptr(), codes.stride(0), self.scales.stride(0), F_._ptr(self.lengths),
+                             F_._ptr(idx), M, M if idx is None else idx.shape[0], n, self.dim)
 
 
 def empty_cache(images: int, num_tokens: int, dim: int, device, lengths: Optional[torch.Tensor] = None) -> Mx4Tokens:
@@ -148,7 +158,7 @@ def quantize_tokens(x: torch.Tensor, out: Optional[Mx4Tokens] = None, lengths: O
         raise ValueError("lengths belong to a new cache; `out` has its own")
     if tuple(out.shape) != (B, n, D) or out.image_index is not None:
         raise ValueError(f"out must be a cache of {(B, n, D)}, got {tuple(out.shape)}" + (" as a batch" if out.image_index is not None else ""))
-    with torch.cuda.device(_on(x, out.codes)):
+    with N.device_guard(_on(x, out.codes)):
         N.check(N.load().ep_mx4_quantize(x.data_ptr(), _OUT[x.dtype], x.stride(0), x.stride(1), B, n, D, out.codes.data_ptr(),
                                          out.scales.data_ptr(), out.codes.stride(0), out.scales.stride(0),
                                          N.current_stream_ptr(x.device)), "ep_mx4_quantize")
@@ -162,7 +172,7 @@ def dequantize_tokens(cache: Mx4Tokens, dtype: torch.dtype = torch.bfloat16, ima
         raise ValueError(f"dtype must be one of {sorted(map(str, _OUT))}, got {dtype}")
     args = cache._args(image_index)
     out = torch.empty((args.B, args.N, args.D), device=cache.device, dtype=dtype)
-    with torch.cuda.device(_on(out, image_index)):
+    with N.device_guard(_on(out, image_index)):
         N.check(N.load().ep_mx4_dequantize(C.byref(args), out.data_ptr(), _OUT[dtype], N.current_stream_ptr(out.device)), "ep_mx4_dequantize")
     return out
 
@@ -189,8 +199,15 @@ def _padded(n: int) -> int:
     return (n + 3) // 4 * 4
 
 
-def _workspace(B: int, n: int, D: int, Q: int, device) -> torch.Tensor:
-    return torch.empty(N.load().ep_mx4_pool_workspace_bytes(B, n, D, Q), device=device, dtype=torch.uint8)
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(B: int, n: int, D: int, Q: int, device: int) -> int:
+    return N.load().ep_mx4_pool_workspace_bytes(B, n, D, Q)
+
+
+def _workspace(B: int, n: int, D: int, Q: int, device) -> Tuple[Optional[torch.Tensor], int]:
+    """(scratch or None, bytes); to be called with ``device`` current: its compute units decide how the work is cut."""
+    nbytes = _workspace_bytes(B, n, D, Q, device.index)
+    return (torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None), nbytes
 
 
 def pool_forward(cache: Mx4Tokens, queries: torch.Tensor, scale: float, per_image_queries: bool = False,
@@ -205,10 +222,10 @@ def pool_forward(cache: Mx4Tokens, queries: torch.Tensor, scale: float, per_imag
     P = torch.empty((B, Q, D), device=dev, dtype=torch.float32)
     S = torch.empty((B, Q, _padded(n)), device=dev, dtype=torch.float32)[:, :, :n] if need_scores else None
     ML = torch.empty((B, Q, 4), device=dev, dtype=torch.float32)
-    ws = _workspace(B, n, D, Q, dev)
-    with torch.cuda.device(dev):
+    with N.device_guard(dev):
+        ws, nbytes = _workspace(B, n, D, Q, dev)
         N.check(N.load().ep_mx4_pool_forward(C.byref(args), q.data_ptr(), Q * D if per_image_queries else 0, Q, float(scale), P.data_ptr(),
-                                             F_._ptr(S), _padded(n), ML.data_ptr(), ws.data_ptr(), ws.numel(), N.current_stream_ptr(dev)), "ep_mx4_pool_forward")
+                                             F_._ptr(S), _padded(n), ML.data_ptr(), F_._ptr(ws), nbytes, N.current_stream_ptr(dev)), "ep_mx4_pool_forward")
     return P, S, ML
 
 
@@ -242,8 +259,8 @@ def pool_backward(cache: Mx4Tokens, S: torch.Tensor, ML: torch.Tensor, dP: torch
     if accumulate and per_image_queries:
         raise ValueError("accumulate is for shared queries")
     dev = _on(cache.codes, S, ML, dP, P, dq, image_index)
-    ws = _workspace(B, n, D, Q, dev)
-    with torch.cuda.device(dev):
+    with N.device_guard(dev):
+        ws, nbytes = _workspace(B, n, D, Q, dev)
         N.check(N.load().ep_mx4_pool_backward(C.byref(args), Q, float(scale), S.data_ptr(), S.stride(1), ML.data_ptr(), F_._ptr(P), dP.data_ptr(),
                                               dq.data_ptr(), int(per_image_queries), int(accumulate), ws.data_ptr(), ws.numel(),
                                               N.current_stream_ptr(dev)), "ep_mx4_pool_backward")
