@@ -17,6 +17,7 @@ import ctypes as C
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from . import functional as F_
@@ -36,13 +37,13 @@ def _call(lg, val, idx, tail, rows, tgt, temperature, alpha, grad_scale, grad_sc
     R, K = val.shape
     loss = torch.empty((B,), device=lg.device, dtype=torch.float32)
     lib = N.load()
-    ws = torch.empty(lib.ep_distill_workspace_bytes(B, C_, K), device=lg.device, dtype=torch.uint8)
-    args = N.EPDistillArgs(logits=lg.data_ptr(), dtype=_DT[lg.dtype], ldl=lg.stride(0), B=B, C=C_, K=K, R=R, teacher_values=val.data_ptr(),
-                           ldv=val.stride(0), teacher_index=idx.data_ptr(), ldi=idx.stride(0), teacher_tail=F_._ptr(tail),
-                           teacher_rows=F_._ptr(rows), targets=F_._ptr(tgt), temperature=temperature, alpha=alpha, grad_scale=grad_scale,
-                           grad_scale_dev=F_._ptr(grad_scale_dev), loss_rows=loss.data_ptr(), dlogits=F_._ptr(grad), ldd=C_)
-    with torch.cuda.device(lg.device):
-        N.check(lib.ep_distill_topk(C.byref(args), ws.data_ptr(), ws.numel(), N.current_stream_ptr(lg.device)), "ep_distill_topk")
+    nbytes = lib.ep_distill_workspace_bytes(B, C_, K)
+    ws = torch.empty(nbytes, device=lg.device, dtype=torch.uint8) if nbytes else None
+    args = N.EPDistillArgs(lg.data_ptr(), _DT[lg.dtype], lg.stride(0), B, C_, K, R, val.data_ptr(), val.stride(0), idx.data_ptr(), idx.stride(0),
+                           F_._ptr(tail), F_._ptr(rows), F_._ptr(tgt), temperature, alpha, grad_scale, F_._ptr(grad_scale_dev), loss.data_ptr(),
+                           F_._ptr(grad), C_)
+    with N.device_guard(lg.device):
+        N.check(lib.ep_distill_topk(C.byref(args), F_._ptr(ws), nbytes, N.current_stream_ptr(lg.device)), "ep_distill_topk")
     return loss
 
 
@@ -77,17 +78,17 @@ def _checked(logits, teacher_values, teacher_index, targets, teacher_tail, teach
     elif teacher_rows.dtype != torch.int32 or tuple(teacher_rows.shape) != (B,) or not teacher_rows.is_contiguous():
         raise ValueError(f"teacher_rows must be a contiguous int32 vector of {B}")
     dev = logits.device
-    for t, name in ((teacher_values, "teacher_values"), (teacher_index, "teacher_index"), (teacher_tail, "teacher_tail"), (teacher_rows, "teacher_rows"),
-                    (targets, "targets")):
+    for name, t in (("teacher_values", teacher_values), ("teacher_index", teacher_index), ("teacher_tail", teacher_tail), ("teacher_rows", teacher_rows),
+                    ("targets", targets)):
         if t is not None and t.device != dev:
             raise ValueError(f"{name} is on {t.device}, the logits on {dev}")
-    lg = _rows(logits.detach())
-    val = _rows(teacher_values.detach().float())
+    lg = _rows(logits)
+    val = _rows(teacher_values if teacher_values.dtype == torch.float32 else teacher_values.float())
     idx = teacher_index
     if idx.dtype != torch.int32:
         idx = idx.to(torch.int64).clamp(-1, MAX_CLASSES).to(torch.int32)   # (a 64-bit class beyond int32 stays out of range)
     idx = _rows(idx)
-    tail = None if teacher_tail is None else teacher_tail.detach().float().contiguous()
+    tail = None if teacher_tail is None else teacher_tail.float().contiguous()
     tgt = None if targets is None else targets.to(torch.int64).contiguous()
     return lg, val, idx, tail, teacher_rows, tgt, float(temperature), float(alpha)
 
@@ -122,6 +123,7 @@ class _Distillation(torch.autograd.Function):
         return _call(*args, 1.0, None, None).mean()
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         lg = ctx.saved_tensors[0]
         grad = torch.empty(lg.shape, device=lg.device, dtype=lg.dtype)

@@ -223,3 +223,21 @@ def test_refusals(bad):
                                   teacher_tail=torch.zeros(bad["tail"], device=DEV) if "tail" in bad else None,
                                   teacher_rows=torch.zeros(2, device=DEV, dtype=bad["rows"]) if "rows" in bad else None,
                                   temperature=bad.get("T", 1.0), alpha=bad.get("alpha", 1.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C", [50, 1003, 4099, 21841, 40001])
+@pytest.mark.parametrize("gap", [60.0, 90.0, 400.0])
+def test_others_far_below_the_list(C, gap, dtype):
+    """The share of the classes behind the list keeps its logarithm where it has left fp32's range; one row's rest is masked."""
+    B, K = 4, 8
+    val, idx, tail = _teacher(B, C, K, C)
+    z = torch.randn(B, C, generator=torch.Generator().manual_seed(C))
+    z.scatter_add_(1, torch.as_tensor(idx, dtype=torch.long), torch.full((B, K), gap))
+    z[1, C // 2:] -= gap                                           # (long rows: whole pieces far below the others)
+    tgt = np.array([0, C - 1, int(idx[2, 0]), -1])
+    _check(z.to(dtype).to(DEV), val, idx, None, tail)
+    _check(z.to(dtype).to(DEV), val, idx, tgt, tail, T=2.0, alpha=0.5)
+    tail[3] = -np.inf
+    z[3] = torch.where(torch.zeros(C, dtype=torch.bool).scatter(0, torch.as_tensor(idx[3], dtype=torch.long), True), z[3], torch.tensor(-np.inf))
+    _check(z.to(dtype).to(DEV), val, idx, tgt, tail, alpha=0.5)
