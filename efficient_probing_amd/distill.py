@@ -3,6 +3,8 @@ fine-tuned or larger model's K best logits per image instead of (or beside) the 
 
     loss_rows, dlogits = topk_distillation(logits, teacher_values, teacher_index, targets, temperature=2.0, alpha=0.5)
     loss = distillation_loss(logits, teacher_values, teacher_index, ...)          # mean over rows, differentiable in logits
+    values, index, tail = teacher_topk(teacher_logits, k, temperature)            # what a dump keeps of the teacher
+    criterion = TopKDistillation.from_store(store, temperature=2.0, alpha=0.5)    # for engine_finetune.train_one_epoch
 
 Per row, with y = logits / T and p = softmax of the teacher's listed logits / T (and, with ``teacher_tail``, of the mass of all
 classes it does not list, as one more outcome on both sides):
@@ -136,3 +138,64 @@ def distillation_loss(logits: torch.Tensor, teacher_values: torch.Tensor, teache
                       alpha: float = 1.0) -> torch.Tensor:
     """Mean of ``topk_distillation``'s row losses, differentiable in ``logits`` (the teacher takes no gradient)."""
     return _Distillation.apply(logits, teacher_values, teacher_index, targets, teacher_tail, teacher_rows, temperature, alpha)
+
+
+@torch.no_grad()
+def teacher_topk(logits: torch.Tensor, k: int, temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(values (R, k) fp32, index (R, k) int32, tail (R,) fp32) of a teacher's full logits (R, C): its k largest, and the log of the
+    sum of exp(logit / temperature) over the others (-inf where k = C)."""
+    if logits.dim() != 2 or not 1 <= k <= min(logits.shape[1], MAX_K):
+        raise ValueError(f"logits must be (R, C) and k within [1, min(C, {MAX_K})], got {tuple(logits.shape)} and {k}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive, got {temperature}")
+    lg = logits.float()
+    values, index = lg.topk(k, dim=1)
+    tail = (lg / temperature).scatter(1, index, float("-inf")).logsumexp(1)
+    return values, index.to(torch.int32), tail
+
+
+class TopKDistillation(torch.nn.Module):
+    """``distillation_loss`` against a table of teacher rows, as a criterion: ``criterion(logits, targets, image_index)`` with batch row
+    b's teacher in table row ``image_index[b]`` (without it: row b).  ``engine_finetune.train_one_epoch`` hands it the image_index of a
+    resident store's batches.  The table is not part of ``state_dict()``; ``.to(device)`` moves it."""
+
+    def __init__(self, teacher_values: torch.Tensor, teacher_index: torch.Tensor, teacher_tail: Optional[torch.Tensor] = None,
+                 temperature: float = 1.0, alpha: float = 1.0):
+        super().__init__()
+        self.temperature, self.alpha = float(temperature), float(alpha)
+        if not (self.temperature > 0.0 and self.temperature < float("inf")) or not 0.0 <= self.alpha <= 1.0:
+            raise ValueError(f"temperature must be positive and alpha within [0, 1], got {temperature} and {alpha}")
+        if teacher_values.dim() != 2 or teacher_values.shape != teacher_index.shape or min(teacher_values.shape) < 1:
+            raise ValueError(f"teacher_values and teacher_index must be (rows, K), got {tuple(teacher_values.shape)} and {tuple(teacher_index.shape)}")
+        if teacher_tail is not None and tuple(teacher_tail.shape) != (teacher_values.shape[0],):
+            raise ValueError(f"teacher_tail must be ({teacher_values.shape[0]},), got {tuple(teacher_tail.shape)}")
+        self.register_buffer("teacher_values", teacher_values.float(), persistent=False)
+        self.register_buffer("teacher_index", teacher_index.to(torch.int32), persistent=False)
+        self.register_buffer("teacher_tail", None if teacher_tail is None else teacher_tail.float(), persistent=False)
+
+    @classmethod
+    def from_store(cls, store, temperature: Optional[float] = None, alpha: float = 1.0) -> "TopKDistillation":
+        """The teacher that a store carries (``token_store``); the tail belongs to the temperature it was written for."""
+        t = store.teacher
+        if t is None:
+            raise ValueError("this store carries no teacher logits")
+        if temperature is None:
+            temperature = t.temperature
+        if t.tail is not None and temperature != t.temperature:
+            raise ValueError(f"the store's tail was written for temperature {t.temperature}, not {temperature}")
+        return cls(t.values, t.index, t.tail, temperature, alpha)
+
+    def _rows(self, batch: int, image_index: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        if image_index is None and batch != self.teacher_values.shape[0]:
+            raise ValueError(f"a batch of {batch} against a table of {self.teacher_values.shape[0]} teacher rows needs image_index "
+                             "(batches of a token_store.ResidentTokenStore carry it)")
+        return None if image_index is None else image_index.to(torch.int32).contiguous()
+
+    def forward(self, logits: torch.Tensor, targets: Optional[torch.Tensor] = None, image_index: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return distillation_loss(logits, self.teacher_values, self.teacher_index, targets if self.alpha < 1.0 else None, teacher_tail=self.teacher_tail,
+                                 teacher_rows=self._rows(logits.shape[0], image_index), temperature=self.temperature, alpha=self.alpha)
+
+    def rows_and_gradient(self, logits: torch.Tensor, targets: Optional[torch.Tensor], image_index: Optional[torch.Tensor], grad_scale: float):
+        """``topk_distillation`` of the batch: (row losses, gradient), no autograd graph."""
+        return topk_distillation(logits, self.teacher_values, self.teacher_index, targets if self.alpha < 1.0 else None, teacher_tail=self.teacher_tail,
+                                 teacher_rows=self._rows(logits.shape[0], image_index), temperature=self.temperature, alpha=self.alpha, grad_scale=grad_scale)

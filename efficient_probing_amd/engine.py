@@ -24,6 +24,7 @@ import torch.nn as nn
 
 from . import _native as N
 from . import functional as F_
+from . import mx4
 
 OPTIMIZERS = {"lars": 0, "sgd": 1, "adamw": 2}
 
@@ -147,6 +148,7 @@ class ProbeHeadEngine:
         self.grad_norm = torch.zeros(1, device=dev, dtype=torch.float32)
         self._ws = None
         self._ws_key = None
+        self._parts_logits = None                            # of the last step that ran in its parts
         import os as _os
         if _os.environ.get("EP_AUX_STREAM", "1") == "0":     # diagnostics: everything on one stream
             overlap = False
@@ -325,7 +327,11 @@ class ProbeHeadEngine:
                          image_index: Optional[torch.Tensor] = None) -> None:
         """Phase 1: forward + CE + backward into the flat gradient buffer (accumulating across
         micro-steps when accum_iter > 1).  Adds to ``self.stats``.  With ``image_index`` (int32 (B,)),
-        ``x`` is a token store resident in HBM and the batch is read from it in place."""
+        ``x`` is a token store resident in HBM and the batch is read from it in place.  ``x`` may be an ``mx4.Mx4Tokens``
+        cache (the EP head)."""
+        if isinstance(x, mx4.Mx4Tokens):
+            return self.forward_backward_parts(x, targets, image_index)
+        self._parts_logits = None
         self.flush()
         xv, bstride = F_.as_token_view(x)
         _, Nn, D = xv.shape
@@ -528,9 +534,73 @@ class ProbeHeadEngine:
         self._deferred = True
         self._micro = 0
 
+    # ---- the step in its parts: tokens held in 4 bits, and losses other than the cross-entropy ----
+    @property
+    def reads_parts(self) -> bool:
+        """Whether ``mx4.Mx4Tokens`` batches and a ``criterion`` are taken (the EP head)."""
+        return type(self) is ProbeHeadEngine
+
+    @torch.no_grad()
+    def forward_backward_parts(self, x, targets: torch.Tensor, image_index: Optional[torch.Tensor] = None, criterion=None) -> None:
+        """``forward_backward`` as one call per operator instead of one library call: the two token passes run over the 4-bit cache
+        where ``x`` is one, and ``criterion`` (``distill.TopKDistillation``) gives the logits' gradient where it is given.  The
+        arithmetic is fp32 whatever ``arithmetic`` says.  The accuracy counts of ``stats`` are those of ``targets``."""
+        if not self.reads_parts:
+            raise NotImplementedError(f"{type(self).__name__}: 4-bit tokens and a criterion are for the EP head; decode the batch "
+                                      "(mx4.dequantize_tokens) for this one")
+        self.flush()
+        cached = isinstance(x, mx4.Mx4Tokens)
+        pool = self.pool
+        if cached:
+            cache = x if image_index is None else x.select(image_index)
+            if cache.dim != self.dims.D:
+                raise ValueError(f"expected tokens of {self.dims.D} channels, got {cache.dim}")
+            B, n, _ = cache.shape
+            P, S, ML = mx4.pool_forward(cache, pool.cls_token, pool.scale)
+        else:
+            P, S, ML = F_.pool_forward(x, pool.cls_token, pool.scale, image_index=image_index)
+            B, n = P.shape[0], S.shape[2]
+        targets = targets.to(device=self.device, dtype=torch.int64)
+        if tuple(targets.shape) != (B,):
+            raise ValueError(f"{tuple(targets.shape)} targets for a batch of {B}")
+        y = F_.project_forward(P, pool.v.weight)
+        z, rstd = F_.bn_forward_train(y, self.bn.running_mean, self.bn.running_var, self.bn.num_batches_tracked, self.bn.eps, self.bn.momentum)
+        logits = F_.linear_forward(z, self.fc.weight, self.fc.bias)
+        grad_scale = self.loss_scale / self.accum_iter
+        if criterion is None:
+            _, dl, _ = F_.cross_entropy(logits, targets, grad_scale, stats=self.stats)
+        else:
+            rows, dl = criterion.rows_and_gradient(logits, targets, image_index if not cached else cache.image_index, grad_scale)
+            _, _, st = F_.cross_entropy(logits, targets, need_grad=False)
+            st[0] = rows.mean()
+            st[3] = (~torch.isfinite(rows)).sum()
+            self.stats += st
+        if self._scaler is not None:
+            dl = dl * self._scaler_state[2 * self._scaler_slot]
+        acc = self._micro > 0
+        g = [self.flat_g[o:o + p.numel()].view(p.shape) for p, o in zip(self.params_list, self.offsets)]
+        dz, _, _ = F_.linear_backward(dl, z, self.fc.weight, dWc=g[2], dbc=g[3], accumulate=acc)
+        dy = F_.bn_backward(dz, z, rstd)
+        dP, _ = F_.project_backward(dy, y, P, pool.v.weight, ML, dWv=g[1], accumulate=acc)      # (leaves dP . P in ML[..., 2])
+        if cached:
+            mx4.pool_backward(cache, S, ML, dP, pool.scale, dq=g[0][0], accumulate=acc)
+        else:
+            F_.pool_backward(x, S, ML, dP, pool.scale, dcls=g[0][0], accumulate=acc, image_index=image_index)
+        self._workspace(B, n)                                # the optimizer's
+        self._parts_logits = logits
+        self._micro += 1
+
     def train_step(self, x: torch.Tensor, targets: torch.Tensor, lr: Optional[float] = None,
-                   image_index: Optional[torch.Tensor] = None) -> None:
-        """One full iteration (accum_iter == 1): forward/backward, gradient all-reduce, update."""
+                   image_index: Optional[torch.Tensor] = None, criterion=None) -> None:
+        """One full iteration (accum_iter == 1): forward/backward, gradient all-reduce, update.  ``criterion``
+        (``distill.TopKDistillation``) in place of the cross-entropy: the EP head (``reads_parts``)."""
+        self._parts_logits = None
+        if criterion is not None or isinstance(x, mx4.Mx4Tokens):
+            self.forward_backward_parts(x, targets, image_index, criterion)
+            if self._micro >= self.accum_iter:
+                self.all_reduce_grads()
+                self.optimizer_step(lr)
+            return
         if self._pipelined:
             return self._train_step_pipelined(x, targets, lr, image_index)
         if self._one_call_step():
@@ -612,6 +682,15 @@ class ProbeHeadEngine:
     @torch.no_grad()
     def eval_logits(self, x: torch.Tensor, image_index: Optional[torch.Tensor] = None,
                     precision: str = "fp32") -> torch.Tensor:
+        if isinstance(x, mx4.Mx4Tokens):
+            # fp32 under either name: the fp16 mode places the reference's roundings so that its own numbers come out, and the
+            # reference has none on 4-bit tokens
+            if not self.reads_parts:
+                raise NotImplementedError(f"{type(self).__name__}: decode the 4-bit batch (mx4.dequantize_tokens) for this head")
+            self.flush()
+            P, _, _ = mx4.pool_forward(x, self.pool.cls_token, self.pool.scale, image_index=image_index, need_scores=False)
+            z = F_.bn_forward_eval(F_.project_forward(P, self.pool.v.weight), self.bn.running_mean, self.bn.running_var, self.bn.eps)
+            return F_.linear_forward(z, self.fc.weight, self.fc.bias)
         if precision == "fp16_autocast":
             return self.eval_logits_fp16_autocast(x, image_index)
         if precision != "fp32":
@@ -633,6 +712,8 @@ class ProbeHeadEngine:
         diagnostics and tests: the distance of the ``bf16_autocast`` arithmetic from the reference's bf16 head)."""
         fn = {"ProbeHeadEngine": "ep_head_workspace_logits_offset", "CocaHeadEngine": "ep_coca_head_workspace_logits_offset",
               "AbmilpHeadEngine": "ep_abmilp_head_workspace_logits_offset"}.get(type(self).__name__)
+        if self._parts_logits is not None:
+            return self._parts_logits.clone()
         if fn is None or self._ws is None:
             raise RuntimeError("last_train_logits: the EP / CoCa / AbMILP engines after a train step only")
         ldl = C.c_int32(0)

@@ -29,6 +29,8 @@ import torch
 from .util import lr_sched
 from .util import misc
 from .util.misc import AMP_PRECISIONS
+from . import mx4
+from .distill import TopKDistillation
 from .token_store import StoreBatch
 
 
@@ -228,6 +230,24 @@ def _attach_store(engine, batch) -> None:
         engine.attach_store(owner)
 
 
+def _reads_parts(model) -> bool:
+    """Whether the model's head is one whose engine takes 4-bit tokens and a distillation criterion (the EP head)."""
+    from .probe_heads import native_engine_name
+    head = _native_head(model)
+    return head is not None and native_engine_name(head) == "ProbeHeadEngine"
+
+
+def _batch_tokens(samples, image_index, in_place: bool, engine):
+    """(tokens, image_index) as a head reads them: a 4-bit batch in place, or decoded for the heads that take token tensors (bf16 for
+    an engine, which holds the 4-bit values exactly in half the bytes; fp32 for modules, whose weights are fp32)."""
+    if not isinstance(samples, mx4.Mx4Tokens) or in_place:
+        return samples, image_index
+    if samples.lengths is not None:
+        raise ValueError("a 4-bit store with images of fewer tokens needs the EP head: this head has no token mask")
+    dtype = torch.bfloat16 if engine is not None and samples.shape[2] % 8 == 0 else torch.float32
+    return mx4.dequantize_tokens(samples, dtype, image_index), None
+
+
 def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loader: Iterable,
                     optimizer: torch.optim.Optimizer, device: torch.device, epoch: int, loss_scaler,
                     max_norm: float = 0, mixup_fn=None, log_writer=None, args=None,
@@ -235,7 +255,10 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
     """``token_fn(samples) -> (B, N, D) tokens`` (the frozen encoder) enables the fused path for image
     loaders; loaders that already yield 3-D token tensors take it directly.  A loader may also yield
     ``token_store.StoreBatch(store_tensor, image_index, targets)`` (``token_store.ResidentTokenStore.loader``): the batch
-    is then read in place from the HBM-resident store through ``image_index`` -- no gather copy.  Any other batch is read
+    is then read in place from the HBM-resident store through ``image_index`` -- no gather copy.  Tokens held in 4 bits
+    (``mx4.Mx4Tokens``: a store's, or a streaming loader's) are read in place by the EP head and decoded batch by batch for the
+    others.  ``criterion`` may be a ``distill.TopKDistillation``: the store's ``image_index`` names each image's teacher row; the EP
+    head takes it on the fused path.  Any other batch is read
     as the reference reads it: ``batch[0]`` the samples, ``batch[-1]`` the targets (engine_finetune.py:40-41 there)."""
     model.train(True)
     metric_logger = MetricLogger()
@@ -247,7 +270,12 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
     n_iter = len(data_loader)
     # the fused step is plain CE + the optimizer: anything it would silently drop (mixup, gradient clipping, another
     # criterion) takes the module path, which honours it
-    fusable = mixup_fn is None and not max_norm and _plain_cross_entropy(criterion)
+    distill = isinstance(criterion, TopKDistillation)
+    if distill and mixup_fn is not None:
+        raise ValueError("a table of teacher rows belongs to the images as they were stored: no mixup with TopKDistillation")
+    in_place = _reads_parts(model)
+    fusable = mixup_fn is None and not max_norm and (_plain_cross_entropy(criterion) or (distill and in_place))
+    loss_kw = {"criterion": criterion} if distill else {}
     engine = get_engine(model, optimizer, args) if fusable else None
     if engine is not None and hasattr(engine, "defer_update"):
         # inside this loop nothing reads the head's parameters between two steps, so the engine MAY let the large update of a
@@ -290,23 +318,34 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
 
     for step, batch in enumerate(metric_logger.log_every(data_loader, print_freq, header)):
         samples, targets = batch[0], batch[-1]
-        image_index = batch[1] if isinstance(batch, StoreBatch) else None      # resident token store, read in place
+        image_index = rows = batch[1] if isinstance(batch, StoreBatch) else None      # resident token store, read in place
         _attach_store(engine, batch)
         if step % accum_iter == 0:
             lr = lr_sched.adjust_learning_rate(optimizer, step / n_iter + epoch, args)
         samples = samples.to(device, non_blocking=True)
         targets = targets.to(device, non_blocking=True)
-        fused = engine is not None and (samples.dim() == 3 or token_fn is not None)
+        samples, image_index = _batch_tokens(samples, image_index, in_place, engine)
+        cached = isinstance(samples, mx4.Mx4Tokens)
+        fused = engine is not None and (cached or samples.dim() == 3 or token_fn is not None)
+        if cached and mixup_fn is not None:
+            raise ValueError("mixup takes images or token tensors, not tokens held in 4 bits")
+        if not fused and cached and image_index is not None:
+            samples, image_index = samples.select(image_index), None
+        if not fused and distill and image_index is not None:                # (a head without the fused form: a gathered batch)
+            samples, image_index = samples[image_index.long()].float(), None
         if image_index is not None and not fused:
             raise RuntimeError("(store, image_index, targets) batches need the fused engine path (a native head, plain "
                                "cross-entropy, no mixup / gradient clipping)")
         if fused:
-            tokens = samples if samples.dim() == 3 else token_fn(samples)
+            tokens = samples if cached else (samples if samples.dim() == 3 else token_fn(samples)).detach()
             if accum_iter == 1:        # one call: lets a data-parallel EP step overlap its large all-reduce
-                engine.train_step(tokens.detach(), targets, lr=max(g["lr"] for g in optimizer.param_groups),
-                                  image_index=image_index)
+                engine.train_step(tokens, targets, lr=max(g["lr"] for g in optimizer.param_groups),
+                                  image_index=image_index, **loss_kw)
             else:
-                engine.forward_backward(tokens.detach(), targets, image_index)
+                if distill:
+                    engine.forward_backward_parts(tokens, targets, image_index, criterion)
+                else:
+                    engine.forward_backward(tokens, targets, image_index)
                 if (step + 1) % accum_iter == 0:
                     engine.all_reduce_grads()
                     engine.optimizer_step(lr=max(g["lr"] for g in optimizer.param_groups))
@@ -320,7 +359,7 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
                 samples, targets = mixup_fn(samples, targets)
             with torch.autocast("cuda", enabled=(amp != "none" and samples.is_cuda), dtype=AMP_PRECISIONS[amp]):
                 outputs = model(samples)
-                loss = criterion(outputs, targets)
+                loss = criterion(outputs, targets, rows) if distill else criterion(outputs, targets)
             acc1, acc5 = accuracy(outputs.float(), targets if targets.dim() == 1 else targets.argmax(1))
             metric_logger.update(acc1=acc1.item(), acc5=acc5.item())
             loss_value = loss.item()
@@ -373,6 +412,7 @@ def evaluate(data_loader, model, device, *, return_targets_and_preds: bool = Fal
     model.eval()
     metric_logger = MetricLogger()
     engine = get_engine(model)
+    in_place = _reads_parts(model)
     if engine is not None:
         engine.sync_buffers()                      # rank 0's running statistics, as DDP's buffer broadcast gives
     all_t, all_p = [], []
@@ -382,7 +422,10 @@ def evaluate(data_loader, model, device, *, return_targets_and_preds: bool = Fal
         _attach_store(engine, batch)
         if index is not None and engine is None:
             raise RuntimeError("(store, image_index, targets) batches need a native head (the fused engine path)")
-        if engine is not None and (images.dim() == 3 or token_fn is not None):
+        images, index = _batch_tokens(images, index, in_place, engine)
+        if isinstance(images, mx4.Mx4Tokens):                        # (the EP head, at fp32 whatever `precision`: engine.eval_logits)
+            output = engine.eval_logits(images, image_index=index, precision=precision)
+        elif engine is not None and (images.dim() == 3 or token_fn is not None):
             output = engine.eval_logits(images if images.dim() == 3 else token_fn(images), image_index=index, precision=precision)
         else:
             with torch.autocast("cuda", enabled=(precision == "fp16_autocast" and images.is_cuda), dtype=torch.float16):
@@ -413,7 +456,7 @@ def extract_features(data_loader, model, device, *, return_targets_and_preds: bo
     ``stats["targets"]`` / ``stats["features"]`` (CPU tensors) when ``return_targets_and_preds``.
 
     Where the features come from, in this order:
-      * a ``token_store.StoreBatch`` -- the batch's tokens are read in place from the resident store and averaged over the
+      * a ``token_store.StoreBatch`` (or an ``mx4.Mx4Tokens`` batch) -- the tokens are read in place and averaged over the
         token axis by the streaming token pass (``knn.mean_tokens``; the reference takes ``output_feat.mean(dim=1)`` of 3-D
         wrapper outputs, :205-206);
       * ``token_fn(images)`` (the frozen encoder) when given;
@@ -431,6 +474,8 @@ def extract_features(data_loader, model, device, *, return_targets_and_preds: bo
         target = target.to(device, non_blocking=True)
         if isinstance(batch, StoreBatch):
             feat = mean_tokens(images, image_index=batch[1])
+        elif isinstance(images, mx4.Mx4Tokens):
+            feat = mean_tokens(images.to(device, non_blocking=True))
         else:
             images = images.to(device, non_blocking=True)
             if token_fn is not None:

@@ -22,6 +22,7 @@ import torch
 
 from . import _native as N
 from . import functional as F_
+from . import mx4
 
 
 def l2_normalize(x: torch.Tensor, eps: float = 1e-12) -> torch.Tensor:
@@ -36,7 +37,11 @@ def l2_normalize(x: torch.Tensor, eps: float = 1e-12) -> torch.Tensor:
 def mean_tokens(x: torch.Tensor, image_index: Optional[torch.Tensor] = None) -> torch.Tensor:
     """(B, N, D) tokens -> (B, D) mean over tokens (reference extract_features, engine_finetune.py:205-206), computed
     by the streaming token pass: a zero query gives uniform attention, i.e. the mean.  With ``image_index`` (int32 (B,)),
-    ``x`` is a resident token store and the batch is read from it in place."""
+    ``x`` is a resident token store and the batch is read from it in place.  ``x`` may be an ``mx4.Mx4Tokens`` cache: the mean
+    is then over an image's own tokens (0 without any)."""
+    if isinstance(x, mx4.Mx4Tokens):
+        zero = torch.zeros((1, x.dim), device=x.device, dtype=torch.float32)
+        return mx4.pool_forward(x, zero, 1.0, image_index=image_index, need_scores=False)[0][:, 0, :]
     zero = torch.zeros((1, x.shape[-1]), device=x.device, dtype=torch.float32)
     P, _, _ = F_.pool_forward(x, zero, 1.0, image_index=image_index)
     return P[:, 0, :]

@@ -5,6 +5,7 @@
     P, S, ML = pool_forward(cache, queries, scale)              # functional.pool_forward with the cache in place of x
     dq = pool_backward(cache, S, ML, dP, scale, P=P)            # functional.pool_backward / pool_backward_per_image
     P = attention_pool(cache, queries, scale)                   # the two as one differentiable call
+    y = pool_project(cache, queries, v_weight, scale)           # ... with the value projection: what EfficientProbing(cache) runs
 
 A token costs 17/32 byte per channel instead of 4 (fp32) or 2 (bf16); the attention's two passes read just those bytes.  The
 pooled vectors are those of the decoded values at fp32 accuracy; what 4 bits cost is decided when the tokens are written
@@ -18,6 +19,7 @@ import functools
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from . import functional as F_
@@ -262,9 +264,16 @@ def pool_backward(cache: Mx4Tokens, S: torch.Tensor, ML: torch.Tensor, dP: torch
     with N.device_guard(dev):
         ws, nbytes = _workspace(B, n, D, Q, dev)
         N.check(N.load().ep_mx4_pool_backward(C.byref(args), Q, float(scale), S.data_ptr(), S.stride(1), ML.data_ptr(), F_._ptr(P), dP.data_ptr(),
-                                              dq.data_ptr(), int(per_image_queries), int(accumulate), ws.data_ptr(), ws.numel(),
+                                              dq.data_ptr(), int(per_image_queries), int(accumulate), F_._ptr(ws), nbytes,
                                               N.current_stream_ptr(dev)), "ep_mx4_pool_backward")
     return dq
+
+
+def attention(cache: Mx4Tokens, queries: torch.Tensor, scale: float, per_image_queries: bool = False,
+              image_index: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale * queries . x) over the tokens, (B, Q, N): 0 behind an image's length (everywhere for one without tokens)."""
+    _, S, ML = pool_forward(cache, queries, scale, per_image_queries, image_index)
+    return F_.attention_from_scores(S.contiguous(), ML).masked_fill_(ML[..., 1:2] == 0, 0.0)
 
 
 class _AttentionPool(torch.autograd.Function):
@@ -278,6 +287,7 @@ class _AttentionPool(torch.autograd.Function):
         return P
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dP):
         P, S, ML = ctx.saved_tensors
         dq = pool_backward(ctx.cache, S, ML, dP, ctx.scale, P=P, per_image_queries=ctx.per_image)
@@ -290,3 +300,30 @@ def attention_pool(cache: Mx4Tokens, queries: torch.Tensor, scale: float, per_im
     if image_index is not None:
         cache = cache.select(image_index)
     return _AttentionPool.apply(queries, cache, float(scale), per_image_queries)
+
+
+class _PoolProject(torch.autograd.Function):
+    """``functional.ep_pool_project`` over a 4-bit cache."""
+
+    @staticmethod
+    def forward(ctx, queries, v_weight, cache, scale, per_image):
+        need = ctx.needs_input_grad[0]
+        P, S, ML = pool_forward(cache, queries, scale, per_image, need_scores=need)
+        y = F_.project_forward(P, v_weight)
+        ctx.save_for_backward(P, S, ML, y, v_weight)
+        ctx.cache, ctx.scale, ctx.per_image, ctx.qshape = cache, scale, per_image, queries.shape
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        P, S, ML, y, v_weight = ctx.saved_tensors
+        need_q = ctx.needs_input_grad[0]
+        dP, dWv = F_.project_backward(dy.contiguous(), y, P, v_weight, None, need_dP=need_q, need_dWv=ctx.needs_input_grad[1])
+        dq = pool_backward(ctx.cache, S, ML, dP, ctx.scale, P=P, per_image_queries=ctx.per_image).reshape(ctx.qshape) if need_q else None
+        return dq, dWv, None, None, None
+
+
+def pool_project(cache: Mx4Tokens, queries: torch.Tensor, v_weight: torch.Tensor, scale: float, per_image_queries: bool = False) -> torch.Tensor:
+    """``attention_pool``, then the value projection of each query's slice: (B, D') with D' = v_weight.shape[0]."""
+    return _PoolProject.apply(queries, v_weight, cache, float(scale), per_image_queries)

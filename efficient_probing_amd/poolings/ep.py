@@ -6,7 +6,7 @@ created first (kaiming-uniform draw), then ``cls_token = randn(1, Q, dim) * 0.02
 head built under ``torch.manual_seed(s)`` has bit-identical initial weights and a reference
 checkpoint (keys ``v.weight``, ``cls_token``) loads with ``strict=True``.
 
-forward(x: (B, N, C), cls=None) -> (B, C // d_out).  On a GPU the computation runs in the HIP
+forward(x: (B, N, C), cls=None) -> (B, C // d_out); x may also be an ``mx4.Mx4Tokens`` batch (tokens held in 4 bits).  On a GPU the computation runs in the HIP
 kernels (pool-then-project); there is no CPU implementation here.
 """
 from __future__ import annotations
@@ -17,6 +17,7 @@ import torch
 from torch import nn
 
 from .. import functional as F_
+from .. import mx4
 
 
 class EfficientProbing(nn.Module):
@@ -41,6 +42,11 @@ class EfficientProbing(nn.Module):
         self.cls_token = nn.Parameter(torch.randn(1, num_queries, dim) * 0.02)
 
     def forward(self, x: torch.Tensor, cls: Optional[torch.Tensor] = None, **_: Any) -> torch.Tensor:
+        if isinstance(x, mx4.Mx4Tokens):
+            if x.dim != self.v.in_features:
+                raise ValueError(f"expected tokens of {self.v.in_features} channels, got {x.dim}")
+            q = self.cls_token if cls is None else cls
+            return mx4.pool_project(x, q, self.v.weight, self.scale, per_image_queries=cls is not None)
         if x.dim() != 3 or x.shape[-1] != self.v.in_features:
             raise ValueError(f"expected tokens (B, N, {self.v.in_features}), got {tuple(x.shape)}")
         out_dtype = x.dtype
@@ -58,5 +64,7 @@ class EfficientProbing(nn.Module):
     def attention(self, x: torch.Tensor) -> torch.Tensor:
         """softmax((cls_token * scale) @ x^T) as (B, Q, N) -- what reference
         tools/ep_attention_maps.py:52-58 recomputes from a saved head."""
+        if isinstance(x, mx4.Mx4Tokens):
+            return mx4.attention(x, self.cls_token, self.scale)
         _, S, ML = F_.pool_forward(x, self.cls_token, self.scale)
         return F_.attention_from_scores(S, ML)

@@ -9,6 +9,11 @@ keeps the head kernels fed.  This module provides
     + ``labels-XXXXX.npy``; shards are independent, so ranks partition them with no communication.  bf16 storage
     halves disk / HBM footprint (the 1.28 M x 196 x 4096 tokens of a ViT-7B fit 8 GPUs only in bf16); the token
     passes widen bf16 to fp32 on the fly and compute in fp32;
+  * ``mxfp4`` storage (``mx4``): 4-bit codes in ``tokens-XXXXX.bin`` and their scales in ``scales-XXXXX.bin``, 17/32 byte per
+    channel.  The writer quantises on the GPU; a resident store then holds an ``mx4.Mx4Tokens`` cache that the EP head's two token
+    passes read in place.  Images of fewer tokens carry ``lengths-XXXXX.npy``;
+  * a teacher's top logits beside the labels (any dtype of the tokens; ``teacher-XXXXX.npz`` with values / index / tail), which
+    ``distill.TopKDistillation.from_store`` turns into the loss of a probe that learns from them;
   * ``TokenStoreWriter`` / ``read_reference_npz`` (imports the reference's ``.npz`` dump);
   * ``ResidentTokenStore``: a rank's shard loaded ONCE into HBM (288 GB per MI355X: 163 k images of
     256x768 fp32 tokens per GPU, the whole 1.28 M-image ImageNet train set on 8 GPUs) and batches
@@ -21,18 +26,30 @@ from __future__ import annotations
 
 import json
 import os
-from typing import Iterator, List, Optional, Sequence, Tuple
+from typing import Iterator, List, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
+from . import mx4
+
 META = "meta.json"
 
 
+class TeacherRows(NamedTuple):
+    """A teacher's K best logits of every image of a store (``distill.topk_distillation``); ``tail`` (or None) is the log mass of the
+    classes behind them at ``temperature``."""
+    values: torch.Tensor
+    index: torch.Tensor
+    tail: Optional[torch.Tensor]
+    temperature: float
+
+
 class TokenStoreWriter:
-    def __init__(self, out_dir: str, num_tokens: int, dim: int, shard_images: int = 8192, dtype: str = "float32"):
-        if dtype not in ("float32", "bfloat16"):
-            raise NotImplementedError("token store dtype: float32 or bfloat16")
+    def __init__(self, out_dir: str, num_tokens: int, dim: int, shard_images: int = 8192, dtype: str = "float32",
+                 teacher_temperature: float = 1.0):
+        if dtype not in ("float32", "bfloat16", "mxfp4"):
+            raise NotImplementedError("token store dtype: float32, bfloat16 or mxfp4")
         if dtype == "bfloat16" and dim % 8 != 0:
             raise ValueError("bfloat16 token store: dim must be a multiple of 8")
         os.makedirs(out_dir, exist_ok=True)
@@ -40,29 +57,77 @@ class TokenStoreWriter:
         self.shards: List[dict] = []
         self._tok: List[np.ndarray] = []
         self._lab: List[np.ndarray] = []
+        self._more: dict = {}                 # scales, lengths, teacher arrays: what some stores have beside tokens and labels
+        self.teacher_temperature = float(teacher_temperature)
         self._n = 0
 
-    def add(self, tokens: np.ndarray, labels: np.ndarray) -> None:
-        tokens = np.ascontiguousarray(tokens, dtype=np.float32)
-        assert tokens.ndim == 3 and tokens.shape[1:] == (self.N, self.D), tokens.shape
-        assert len(labels) == len(tokens)
-        self._tok.append(tokens); self._lab.append(np.asarray(labels, dtype=np.int64)); self._n += len(tokens)
+    def add(self, tokens, labels: np.ndarray, lengths=None, teacher=None) -> None:
+        """``tokens`` (n, N, D) numpy or torch.  mxfp4: quantised on the GPU (a host array is copied there first), and ``lengths`` (n,)
+        may give images fewer than N tokens.  ``teacher`` = (values (n, K), index (n, K)[, tail (n,)]) of ``distill.teacher_topk`` at
+        this writer's ``teacher_temperature``.  Every ``add`` of a store brings the same parts."""
+        n, dims = len(tokens), tuple(tokens.shape)
+        assert len(dims) == 3 and dims[1:] == (self.N, self.D), dims
+        assert len(labels) == n
+        if n == 0:
+            return
+        more = {}
+        if self.dtype == "mxfp4":
+            x = torch.as_tensor(tokens)
+            cache = mx4.quantize_tokens(x if x.is_cuda else x.to("cuda"))
+            tokens, more["scales"] = cache.codes.cpu().numpy(), cache.scales.cpu().numpy()
+        else:
+            tokens = np.ascontiguousarray(tokens.cpu() if isinstance(tokens, torch.Tensor) else tokens, dtype=np.float32)
+            if lengths is not None:
+                raise ValueError("images of fewer tokens are for mxfp4 stores")
+        host = lambda t, dt: np.ascontiguousarray(t.cpu() if isinstance(t, torch.Tensor) else t, dtype=dt)
+        if lengths is not None:
+            more["lengths"] = host(lengths, np.int32)
+            if more["lengths"].shape != (n,) or more["lengths"].min() < 0 or more["lengths"].max() > self.N:
+                raise ValueError(f"lengths must be ({n},) within [0, {self.N}]")
+        if teacher is not None:
+            if len(teacher) not in (2, 3):
+                raise ValueError("teacher is (values, index) or (values, index, tail)")
+            more["values"], more["index"] = host(teacher[0], np.float32), host(teacher[1], np.int32)
+            if len(teacher) == 3 and teacher[2] is not None:
+                more["tail"] = host(teacher[2], np.float32)
+            if more["values"].ndim != 2 or more["values"].shape != more["index"].shape or any(len(more[k]) != n for k in ("values", "index", "tail") if k in more):
+                raise ValueError(f"teacher arrays must be ({n}, K), ({n}, K) and ({n},)")
+        if (self.shards or self._n) and set(more) != set(self._more):
+            raise ValueError(f"this store's images carry {sorted(self._more)}, these carry {sorted(more)}")
+        if "values" in self._more and self._more["values"] and self._more["values"][0].shape[1] != more["values"].shape[1]:
+            raise ValueError(f"this store's teacher rows have {self._more['values'][0].shape[1]} entries, these have {more['values'].shape[1]}")
+        self._tok.append(tokens); self._lab.append(np.asarray(labels, dtype=np.int64)); self._n += n
+        for k, v in more.items():
+            self._more.setdefault(k, []).append(v)
         while self._n >= self.shard_images:
             self._flush(self.shard_images)
 
     def _flush(self, n: int) -> None:
         tok = np.concatenate(self._tok); lab = np.concatenate(self._lab)
         idx = len(self.shards)
-        _encode(tok[:n], self.dtype).tofile(os.path.join(self.out_dir, f"tokens-{idx:05d}.bin"))
-        np.save(os.path.join(self.out_dir, f"labels-{idx:05d}.npy"), lab[:n])
+        path = lambda name: os.path.join(self.out_dir, name)
+        (tok[:n] if self.dtype == "mxfp4" else _encode(tok[:n], self.dtype)).tofile(path(f"tokens-{idx:05d}.bin"))
+        np.save(path(f"labels-{idx:05d}.npy"), lab[:n])
+        more = {k: np.concatenate(v) for k, v in self._more.items()}
+        if "scales" in more:
+            more["scales"][:n].tofile(path(f"scales-{idx:05d}.bin"))
+        if "lengths" in more:
+            np.save(path(f"lengths-{idx:05d}.npy"), more["lengths"][:n])
+        if "values" in more:
+            np.savez(path(f"teacher-{idx:05d}.npz"), **{k: more[k][:n] for k in ("values", "index", "tail") if k in more})
         self.shards.append({"index": idx, "images": int(n)})
         self._tok, self._lab, self._n = ([tok[n:]] if len(tok) > n else []), ([lab[n:]] if len(lab) > n else []), len(tok) - n
+        self._more = {k: [v[n:]] for k, v in more.items()}          # (an empty rest keeps the widths for the next add)
 
     def close(self) -> dict:
         if self._n:
             self._flush(self._n)
         meta = {"format": "ep-token-store-v1", "num_tokens": self.N, "dim": self.D, "dtype": self.dtype,
                 "shards": self.shards, "total_images": int(sum(s["images"] for s in self.shards))}
+        if "lengths" in self._more:
+            meta["lengths"] = True
+        if "values" in self._more:
+            meta["teacher"] = {"k": int(self._more["values"][0].shape[1]), "tail": "tail" in self._more, "temperature": self.teacher_temperature}
         with open(os.path.join(self.out_dir, META), "w") as f:
             json.dump(meta, f, indent=1)
         return meta
@@ -115,11 +180,45 @@ def steps_per_epoch(meta: dict, world: int, batch_size: int, per_shard: bool = F
 
 
 def open_shard(store_dir: str, meta: dict, shard: dict) -> Tuple[np.memmap, np.ndarray]:
+    if meta.get("dtype") == "mxfp4":
+        raise ValueError("a 4-bit store's shards hold codes and scales: open_shard_arrays")
     tok = np.memmap(os.path.join(store_dir, f"tokens-{shard['index']:05d}.bin"),
                     dtype=np.float32 if meta.get("dtype", "float32") == "float32" else np.int16, mode="r",
                     shape=(shard["images"], meta["num_tokens"], meta["dim"]))
     lab = np.load(os.path.join(store_dir, f"labels-{shard['index']:05d}.npy"))
     return tok, lab
+
+
+def open_shard_arrays(store_dir: str, meta: dict, shard: dict) -> List[np.ndarray]:
+    """What a shard stores of its tokens, one row per image: [tokens], or [codes, scales(, lengths)] of a 4-bit store."""
+    if meta.get("dtype") != "mxfp4":
+        return [open_shard(store_dir, meta, shard)[0]]
+    path = lambda kind, ext: os.path.join(store_dir, f"{kind}-{shard['index']:05d}.{ext}")
+    out = [np.memmap(path(kind, "bin"), dtype=np.uint8, mode="r", shape=(shard["images"], meta["num_tokens"], nb))
+           for kind, nb in zip(("tokens", "scales"), mx4.row_bytes(meta["dim"]))]
+    return out + ([np.load(path("lengths", "npy"))] if meta.get("lengths") else [])
+
+
+def open_shard_labels(store_dir: str, shard: dict) -> np.ndarray:
+    return np.load(os.path.join(store_dir, f"labels-{shard['index']:05d}.npy"))
+
+
+def _buffers(meta: dict, images: int, device, pin: bool = False) -> List[torch.Tensor]:
+    """Empty tensors for the arrays of ``open_shard_arrays``."""
+    n, d = meta["num_tokens"], meta["dim"]
+    dtype = meta.get("dtype", "float32")
+    if dtype == "mxfp4":
+        parts = [((images, n, nb), torch.uint8) for nb in mx4.row_bytes(d)] + ([((images,), torch.int32)] if meta.get("lengths") else [])
+    else:
+        parts = [((images, n, d), torch.float32 if dtype == "float32" else torch.bfloat16)]
+    return [torch.empty(shape, dtype=dt, device=device, pin_memory=pin) for shape, dt in parts]
+
+
+def _tokens(meta: dict, parts: List[torch.Tensor]):
+    """The tensors of ``_buffers`` as what the heads take: a token tensor or an ``mx4.Mx4Tokens``."""
+    if meta.get("dtype") != "mxfp4":
+        return parts[0]
+    return mx4.Mx4Tokens(parts[0], parts[1], meta["dim"], parts[2] if len(parts) > 2 else None)
 
 
 class ResidentTokenStore:
@@ -134,26 +233,38 @@ class ResidentTokenStore:
         self.meta, self.world = meta, world
         self.N, self.D, self.seed, self.rank = meta["num_tokens"], meta["dim"], seed, rank
         self.dtype = meta.get("dtype", "float32")
-        tdt = torch.float32 if self.dtype == "float32" else torch.bfloat16
-        self.tokens = torch.empty((max(n, 1), self.N, self.D), device=device, dtype=tdt)
-        labels = []
+        parts = _buffers(meta, max(n, 1), device)
+        if n == 0 and self.dtype == "mxfp4":                 # (a rank without shards: one image of zeros)
+            for t in parts:
+                t.zero_()
+        labels, teacher = [], []
         off = 0
         for s in mine:
-            tok, lab = open_shard(store_dir, meta, s)
-            self.tokens[off:off + s["images"]].copy_(_to_torch(tok, self.dtype))
-            labels.append(lab); off += s["images"]
+            for t, a in zip(parts, open_shard_arrays(store_dir, meta, s)):
+                t[off:off + s["images"]].copy_(_to_torch(a, self.dtype))
+            labels.append(open_shard_labels(store_dir, s)); off += s["images"]
+            if meta.get("teacher"):
+                teacher.append(np.load(os.path.join(store_dir, f"teacher-{s['index']:05d}.npz")))
+        self.tokens = _tokens(meta, parts)
         self.num_images = n
+        self.teacher: Optional[TeacherRows] = None
+        if teacher:
+            cat = lambda k: torch.from_numpy(np.concatenate([t[k] for t in teacher])).to(device)
+            self.teacher = TeacherRows(cat("values"), cat("index"), cat("tail") if meta["teacher"]["tail"] else None, meta["teacher"]["temperature"])
         self.labels = torch.from_numpy(np.concatenate(labels) if labels else np.zeros(0, np.int64)).to(device)
 
     @classmethod
-    def from_tensors(cls, tokens: torch.Tensor, labels: torch.Tensor, seed: int = 0) -> "ResidentTokenStore":
+    def from_tensors(cls, tokens, labels: torch.Tensor, seed: int = 0, teacher: Optional[TeacherRows] = None) -> "ResidentTokenStore":
         """A resident store around tokens that are already in HBM (synthetic benchmarks, tokens produced by a live encoder
-        pass): ``tokens`` (n, N, D) fp32 / bf16 on the GPU, ``labels`` (n,) int64.  One rank's view (world = 1)."""
+        pass): ``tokens`` (n, N, D) fp32 / bf16 on the GPU or an ``mx4.Mx4Tokens`` cache, ``labels`` (n,) int64.  One rank's view
+        (world = 1)."""
+        if isinstance(tokens, mx4.Mx4Tokens) and tokens.image_index is not None:
+            raise ValueError("a store holds a cache, not a batch of one")
         self = cls.__new__(cls)
         n, N, D = tokens.shape
         self.meta, self.world, self.N, self.D, self.seed, self.rank = {"num_tokens": N, "dim": D}, 1, N, D, seed, 0
-        self.dtype = "float32" if tokens.dtype == torch.float32 else "bfloat16"
-        self.tokens, self.num_images = tokens, n
+        self.dtype = "mxfp4" if isinstance(tokens, mx4.Mx4Tokens) else "float32" if tokens.dtype == torch.float32 else "bfloat16"
+        self.tokens, self.num_images, self.teacher = tokens, n, teacher
         self.labels = labels.to(device=tokens.device, dtype=torch.int64)
         return self
 
@@ -168,6 +279,8 @@ class ResidentTokenStore:
         row (the CLIP head's query input; made from ``"token_stats"`` of the same ``eps``).  ``engine.attach_store(store)`` makes an
         engine look them up (``engine_finetune.train_one_epoch`` / ``evaluate`` do that for a ``StoreBatch``)."""
         from . import functional as F_
+        if self.dtype == "mxfp4":
+            raise ValueError("tables are of float32 / bfloat16 stores: a head that takes them reads a 4-bit store's batches decoded")
         key = (kind, None if eps is None else float(eps))
         cache = self.__dict__.setdefault("_tables", {})
         if key not in cache:
@@ -245,11 +358,9 @@ class StreamingTokenLoader:
         # data parallel: every rank stops after the same number of batches (see steps_per_epoch)
         self.limit = steps_per_epoch(self.meta, world, batch_size, per_shard=True) if world > 1 else None
         self.stream = torch.cuda.Stream(device=device)
-        N, D = self.meta["num_tokens"], self.meta["dim"]
         self.dtype = self.meta.get("dtype", "float32")
-        tdt = torch.float32 if self.dtype == "float32" else torch.bfloat16
-        self.stage = [torch.empty((batch_size, N, D), dtype=tdt).pin_memory() for _ in range(2)]
-        self.dev = [torch.empty((batch_size, N, D), dtype=tdt, device=device) for _ in range(2)]
+        self.stage = [_buffers(self.meta, batch_size, "cpu", pin=True) for _ in range(2)]
+        self.dev = [_buffers(self.meta, batch_size, device) for _ in range(2)]
 
     def __len__(self):
         n = sum(s["images"] // self.B for s in self.shards)
@@ -265,27 +376,29 @@ class StreamingTokenLoader:
         for s in self.shards:
             if k >= total:
                 break
-            tok, lab = open_shard(self.dir, self.meta, s)
+            arrays, lab = open_shard_arrays(self.dir, self.meta, s), open_shard_labels(self.dir, s)
             for lo in range(0, s["images"] - self.B + 1, self.B):
                 if k >= total:
                     break
                 buf = k & 1
                 if copied[buf] is not None:
                     copied[buf].synchronize()                     # previous H2D out of this staging buffer is done
-                self.stage[buf].copy_(_to_torch(tok[lo:lo + self.B], self.dtype))
+                for t, a in zip(self.stage[buf], arrays):
+                    t.copy_(_to_torch(a[lo:lo + self.B], self.dtype))
                 with torch.cuda.stream(self.stream):
                     if consumed[buf] is not None:
                         self.stream.wait_event(consumed[buf])     # consumer finished with this device buffer
-                    self.dev[buf].copy_(self.stage[buf], non_blocking=True)
+                    for t, h in zip(self.dev[buf], self.stage[buf]):
+                        t.copy_(h, non_blocking=True)
                     ev = torch.cuda.Event(); ev.record(self.stream)
                 copied[buf] = ev
                 cur = (buf, torch.from_numpy(lab[lo:lo + self.B]).to(self.device), ev)
                 if pending is not None:
                     main.wait_event(pending[2])
-                    yield self.dev[pending[0]], pending[1]
+                    yield _tokens(self.meta, self.dev[pending[0]]), pending[1]
                     done = torch.cuda.Event(); done.record(main); consumed[pending[0]] = done
                 pending = cur
                 k += 1
         if pending is not None:
             main.wait_event(pending[2])
-            yield self.dev[pending[0]], pending[1]
+            yield _tokens(self.meta, self.dev[pending[0]]), pending[1]

@@ -1,0 +1,280 @@
+"""A probe trained from a compact store: 4-bit tokens and a teacher's top logits, through the dump, the stores, the engine and the
+training and evaluation loops.
+
+Gradients are compared in norm with a float64 statement of the whole step on the decoded tokens.  The step is about ten stages
+(scores, softmax, pooled rows, projection, BatchNorm, classifier, loss, and back); an fp32 stage over K products is off by about
+u sqrt(K) <= 32 u of its result's norm (u = 2^-24, K <= 1024), and BatchNorm's backward, a difference, can enlarge what comes into it a
+few times: 10 * 32 * 4 u = 1280 u.  Parameters after several steps: the updates' errors add up and feed the next gradients, 8192 u."""
+from argparse import Namespace
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import distill_oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+
+
+def _model(D, C, Q=4, head="ep", seed=0, **kw):
+    from efficient_probing_amd import probe_heads
+
+    class Enc(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.head = torch.nn.Linear(D, C)
+
+        def forward(self, x):
+            return self.head(x)
+    torch.manual_seed(seed)
+    m = Enc()
+    probe_heads.build_probe_head(m, Namespace(cls_features=head, ep_queries=Q, d_out=1, nb_classes=C, **kw))
+    return m.to(DEV)
+
+
+def _store(n, N, D, C, K=5, seed=0, lengths=False, tail=True, temperature=2.0):
+    from efficient_probing_amd import distill, mx4, token_store as TS
+    g = torch.Generator().manual_seed(seed)
+    labels = torch.randint(0, C, (n,), generator=g)
+    x = torch.randn(n, N, D, generator=g) + 0.3 * torch.randn(C, 1, D, generator=g)[labels]
+    teacher = torch.randn(n, C, generator=g) + 3 * torch.nn.functional.one_hot(labels, C)
+    v, i, t = distill.teacher_topk(teacher.to(DEV), K, temperature)
+    ln = None
+    if lengths:
+        ln = torch.randint(0, N + 1, (n,), generator=g, dtype=torch.int32)
+        ln[:3] = torch.tensor([0, 1, N])
+        ln = ln.to(DEV)
+    cache = mx4.quantize_tokens(x.to(DEV), lengths=ln)
+    return TS.ResidentTokenStore.from_tensors(cache, labels, teacher=TS.TeacherRows(v, i, t if tail else None, temperature))
+
+
+def _step64(head, x, lengths, targets, teacher=None, T=1.0, alpha=1.0):
+    """Loss and gradients (queries, v, weight, bias) of one training step in float64."""
+    pool, bn, fc = head[0], head[1], head[2]
+    p = [t.detach().double().cpu().requires_grad_() for t in (pool.cls_token, pool.v.weight, fc.weight, fc.bias)]
+    x = x.double().cpu()
+    B, N, D = x.shape
+    S = torch.einsum("qd,bnd->bqn", p[0][0] * pool.scale, x)
+    if lengths is not None:
+        S = S.masked_fill(torch.arange(N) >= lengths.cpu().long()[:, None, None], -torch.inf)
+    A = torch.softmax(S, -1)
+    if lengths is not None:
+        A = torch.where(lengths.cpu()[:, None, None] > 0, A, torch.zeros(()))
+        A = torch.nan_to_num(A)
+    P = torch.einsum("bqn,bnd->bqd", A, x)
+    Q = P.shape[1]
+    W = p[1].view(Q, -1, D)
+    y = torch.einsum("bqd,qkd->bqk", P, W).reshape(B, -1)
+    z = (y - y.mean(0)) / torch.sqrt(y.var(0, unbiased=False) + bn.eps)
+    logits = z @ p[2].t() + p[3]
+    if teacher is None:
+        loss = torch.nn.functional.cross_entropy(logits, targets.cpu())
+        loss.backward()
+        return float(loss.detach()), [t.grad for t in p]
+    rows, g = distill_oracle.distill(logits.detach().numpy(), teacher[0], teacher[1], targets.cpu().numpy(), teacher[2], T, alpha)
+    logits.backward(torch.from_numpy(g / B))
+    return rows.mean(), [t.grad for t in p]
+
+
+def _teacher_rows(store, idx):
+    t = store.teacher
+    pick = lambda a: None if a is None else a[idx.long()].double().cpu().numpy()
+    return pick(t.values), t.index[idx.long()].cpu().numpy(), pick(t.tail)
+
+
+def _close(got, want, lim):
+    err = (got.double().cpu() - want).norm() / want.norm()
+    assert err <= lim, float(err / lim)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("N,D,Q,C", [(33, 128, 4, 20), (20, 384, 1, 101), (50, 768, 8, 64), (9, 2048, 32, 10)])
+def test_engine_step_against_float64(N, D, Q, C, ragged):
+    """Cross-entropy and distillation, on a batch read in place with an image twice."""
+    from efficient_probing_amd import distill, mx4
+    from efficient_probing_amd.engine import ProbeHeadEngine
+    store = _store(40, N, D, C, lengths=ragged)
+    idx = torch.tensor([3, 0, 7, 7, 1, 39, 12, 2, 25, 30, 31, 8], dtype=torch.int32, device=DEV)
+    tgt = store.labels[idx.long()].clone()
+    head = _model(D, C, Q).head.train()
+    x = mx4.dequantize_tokens(store.tokens, torch.float32, idx)
+    ln = None if store.tokens.lengths is None else store.tokens.lengths[idx.long()]
+    for crit in (None, distill.TopKDistillation.from_store(store, alpha=0.6), distill.TopKDistillation(store.teacher.values, store.teacher.index).to(DEV)):
+        eng = ProbeHeadEngine(head, optimizer="sgd", lr=0.0)
+        eng.forward_backward_parts(store.tokens, tgt, idx, crit)
+        teacher = None if crit is None else _teacher_rows(store, idx)[:2] + ((_teacher_rows(store, idx)[2],) if crit.teacher_tail is not None else (None,))
+        loss, want = _step64(head, x, ln, tgt, teacher, *((crit.temperature, crit.alpha) if crit is not None else ()))
+        stats = eng.read_stats()
+        assert abs(stats[0] - loss) <= 1280 * U * max(1.0, abs(loss)) and stats[3] == 0
+        for p, w in zip(eng.params_list, want):
+            _close(p.grad, w, 1280 * U)
+        first = [p.grad.clone() for p in eng.params_list]
+        eng.forward_backward_parts(store.tokens, tgt, idx, crit)            # a second micro-step adds the same again
+        for p, f in zip(eng.params_list, first):
+            assert torch.allclose(p.grad, 2 * f, rtol=4 * U, atol=0) or (p.grad - 2 * f).norm() <= 4 * U * f.norm()
+        assert torch.equal(eng.last_train_logits().argmax(1), eng._parts_logits.argmax(1))
+
+
+@pytest.mark.parametrize("cls", [False, True])
+def test_module_against_float64(cls):
+    """EfficientProbing over a batch of the cache: value and gradients of the queries (shared or per image) and of v."""
+    from efficient_probing_amd import mx4
+    from efficient_probing_amd.poolings.ep import EfficientProbing
+    store = _store(12, 21, 256, 9, lengths=True)
+    torch.manual_seed(1)
+    m = EfficientProbing(256, num_queries=4).to(DEV)
+    idx = torch.tensor([0, 5, 1, 5, 11], dtype=torch.int32, device=DEV)
+    batch = store.tokens.select(idx)
+    q = torch.randn(5, 4, 256, device=DEV, requires_grad=True) if cls else m.cls_token
+    y = m(batch, cls=q) if cls else m(batch)
+    w = torch.randn(y.shape, generator=torch.Generator().manual_seed(2))
+    (y * w.to(DEV)).sum().backward()
+    x, ln = mx4.dequantize_tokens(batch, torch.float32).double().cpu(), store.tokens.lengths[idx.long()].cpu()
+    q64, v64 = q.detach().double().cpu().requires_grad_(), m.v.weight.detach().double().cpu().requires_grad_()
+    S = (q64 * m.scale) @ x.transpose(1, 2)
+    S = S.masked_fill(torch.arange(21) >= ln.long()[:, None, None], -torch.inf)
+    A = torch.nan_to_num(torch.softmax(S, -1).masked_fill(ln[:, None, None] == 0, 0.0))
+    want = torch.einsum("bqd,qkd->bqk", A @ x, v64.view(4, -1, 256)).reshape(5, -1)
+    (want * w.double()).sum().backward()
+    _close(y.detach(), want.detach(), 256 * U)
+    _close(m.v.weight.grad, v64.grad, 256 * U)
+    _close(q.grad, torch.nan_to_num(q64.grad), 512 * U)
+    if not cls:
+        att = m.attention(batch)
+        assert att.shape == (5, 4, 21) and (att.double().cpu() - A.detach()).abs().max() <= 256 * U
+
+
+def _epoch(model, store, criterion=None, epochs=1, **kw):
+    from efficient_probing_amd import engine_finetune as EF
+    from efficient_probing_amd.util.lars import LARS
+    from efficient_probing_amd.util.misc import NativeScalerWithGradNormCount
+    opt = LARS(model.head.parameters(), lr=0.1, weight_decay=0.0)
+    args = Namespace(lr=0.1, min_lr=0.0, warmup_epochs=0, epochs=4, accum_iter=kw.pop("accum_iter", 1), amp="none")
+    scaler = NativeScalerWithGradNormCount() if kw.pop("scaler", False) else kw.pop("loss_scaler", None)
+    out = [EF.train_one_epoch(model, criterion, store.loader(16, epoch=e), opt, torch.device(DEV), e, scaler, args=args, **kw) for e in range(epochs)]
+    return out, scaler
+
+
+@pytest.mark.parametrize("accum,scaler", [(1, False), (2, False), (1, True)])
+def test_training_on_codes_is_training_on_their_values(accum, scaler):
+    """The same epochs on the 4-bit store and on a store of its decoded tokens (the fused step)."""
+    from efficient_probing_amd import mx4, token_store as TS
+    store = _store(64, 19, 256, 12)
+    plain = TS.ResidentTokenStore.from_tensors(mx4.dequantize_tokens(store.tokens, torch.float32), store.labels)
+    m1, m2 = _model(256, 12), _model(256, 12)
+    start = [p.detach().clone() for p in m1.head.parameters()]
+    (a, s1), (b, s2) = _epoch(m1, store, epochs=2, accum_iter=accum, scaler=scaler), _epoch(m2, plain, epochs=2, accum_iter=accum, scaler=scaler)
+    for p, q, s in zip(m1.head.parameters(), m2.head.parameters(), start):
+        assert (p - q).norm() <= 8192 * U * max((q - s).norm(), 1e-3 * q.norm())
+    for x, y in zip(a, b):
+        assert abs(x["loss"] - y["loss"]) <= 8192 * U * abs(y["loss"]) and x["acc1"] == y["acc1"] and x["acc5"] == y["acc5"]
+    if scaler:
+        assert s1.get_scale() == s2.get_scale() and s1._growth_tracker == s2._growth_tracker
+    from efficient_probing_amd import engine_finetune as EF
+    ev = [EF.evaluate(st.loader(16, shuffle=False, drop_last=False), m, torch.device(DEV), precision="fp32", return_targets_and_preds=True)
+          for st, m in ((store, m1), (plain, m2))]
+    assert torch.equal(ev[0]["preds"], ev[1]["preds"]) and abs(ev[0]["loss"] - ev[1]["loss"]) <= 8192 * U * ev[1]["loss"]
+    half = EF.evaluate(store.loader(16, shuffle=False, drop_last=False), m1, torch.device(DEV))
+    assert half["loss"] == ev[0]["loss"]                                    # (fp32 under either name)
+
+
+def test_distillation_epochs_fused_and_through_modules(tmp_path):
+    """Dump with a teacher -> store on disk -> epochs with distillation: the fused step on codes and on plain tokens, and the modules
+    through autograd (a clipping bound that never acts sends them there) give the same head; evaluation and features follow."""
+    from efficient_probing_amd import distill, dump, engine_finetune as EF, mx4, token_store as TS
+    from efficient_probing_amd.util.misc import NativeScalerWithGradNormCount
+    torch.manual_seed(0)
+    proj = torch.nn.Conv2d(3, 128, kernel_size=4, stride=4).to(DEV).eval()
+    big = torch.nn.Linear(3 * 16 * 16, 12).to(DEV)
+    g = torch.Generator().manual_seed(1)
+    imgs, labs = torch.randn(70, 3, 16, 16, generator=g), torch.randint(0, 12, (70,), generator=g)
+    meta = dump.dump_tokens([(imgs[i:i + 16], labs[i:i + 16]) for i in range(0, 70, 16)], lambda x: proj(x).flatten(2).transpose(1, 2), str(tmp_path),
+                            dtype="mx4", shard_images=32, device=torch.device(DEV), max_images=66, teacher_fn=lambda x: 4 * big(x.flatten(1)),
+                            teacher_k=4, teacher_temperature=2.0)
+    assert meta["dtype"] == "mxfp4" and meta["total_images"] == 66 and meta["teacher"] == {"k": 4, "tail": True, "temperature": 2.0}
+    store = TS.ResidentTokenStore(str(tmp_path), torch.device(DEV))
+    with torch.no_grad():
+        want = mx4.quantize_tokens(torch.cat([proj(imgs[i:i + 16].to(DEV)).flatten(2).transpose(1, 2) for i in range(0, 70, 16)])[:66])
+    assert torch.equal(store.tokens.codes, want.codes) and torch.equal(store.tokens.scales, want.scales) and torch.equal(store.labels.cpu(), labs[:66])
+    ld = TS.StreamingTokenLoader(str(tmp_path), torch.device(DEV), batch_size=8)
+    got = [(x.codes.clone(), x.scales.clone(), t.clone()) for x, t in ld]
+    rows = torch.cat([torch.arange(0, 32), torch.arange(32, 64)]).to(DEV)           # whole batches of the two full shards
+    assert len(got) == len(ld) == 8
+    for k, ref in enumerate((want.codes, want.scales, store.labels)):
+        assert torch.equal(torch.cat([b[k] for b in got]), ref[rows])
+
+    plain = TS.ResidentTokenStore.from_tensors(mx4.dequantize_tokens(store.tokens, torch.float32), store.labels, teacher=store.teacher)
+    heads = []
+    for st, kw in ((store, {}), (plain, {}), (store, dict(max_norm=1e9, loss_scaler=NativeScalerWithGradNormCount()))):
+        m = _model(128, 12)
+        out, _ = _epoch(m, st, distill.TopKDistillation.from_store(st, alpha=0.5), epochs=2, **kw)
+        assert out[1]["loss"] < out[0]["loss"] * 1.5 and np.isfinite(out[1]["loss"])
+        heads.append(m)
+    start = _model(128, 12)
+    for m in heads[1:]:
+        for p, q, s in zip(m.head.parameters(), heads[0].head.parameters(), start.head.parameters()):
+            assert (p - q).norm() <= 8192 * U * max((q - s).norm(), 1e-3 * q.norm())
+    ev = EF.evaluate(store.loader(16, shuffle=False, drop_last=False), heads[0], torch.device(DEV))
+    assert np.isfinite(ev["loss"])
+    f = EF.extract_features(store.loader(16, shuffle=False, drop_last=False), None, torch.device(DEV), return_targets_and_preds=True)
+    ref = plain.tokens.double().mean(1).cpu()
+    assert (f["features"].double() - ref).abs().max() <= 64 * U * plain.tokens.abs().max().item()
+    # epochs straight from the streaming loader: no index, so no table of teacher rows
+    out = EF.train_one_epoch(heads[0], None, ld, *_rest(heads[0]))
+    assert np.isfinite(out["loss"])
+    with pytest.raises(ValueError, match="image_index"):
+        EF.train_one_epoch(heads[0], distill.TopKDistillation.from_store(store).to(DEV), ld, *_rest(heads[0]))
+
+
+def _rest(model):
+    from efficient_probing_amd.util.lars import LARS
+    opt = LARS(model.head.parameters(), lr=0.1, weight_decay=0.0)
+    return opt, torch.device(DEV), 0, None, 0, None, None, Namespace(lr=0.1, min_lr=0.0, warmup_epochs=0, epochs=4, accum_iter=1, amp="none")
+
+
+@pytest.mark.parametrize("head", ["simpool", "coca", "aim", "jepa"])
+def test_other_heads_read_the_batch_decoded(head):
+    """A head without the in-place form: one epoch on the 4-bit store equals one on its decoded tokens, with distillation through the
+    modules; images of fewer tokens are refused, because the head would read the rows behind them."""
+    from efficient_probing_amd import distill, engine_finetune as EF, mx4, token_store as TS
+    from efficient_probing_amd.util.misc import NativeScalerWithGradNormCount
+    kw = dict(num_heads=4)
+    store = _store(48, 16, 128, 7)
+    plain = TS.ResidentTokenStore.from_tensors(mx4.dequantize_tokens(store.tokens, torch.bfloat16), store.labels)
+    m1, m2 = _model(128, 7, head=head, **kw), _model(128, 7, head=head, **kw)
+    (a, _), (b, _) = _epoch(m1, store), _epoch(m2, plain)
+    assert np.isfinite(a[0]["loss"]) and abs(a[0]["loss"] - b[0]["loss"]) <= 8192 * U * abs(b[0]["loss"])
+    EF.evaluate(store.loader(16, shuffle=False, drop_last=False), m1, torch.device(DEV))
+    m3 = _model(128, 7, head=head, **kw)
+    out, _ = _epoch(m3, store, distill.TopKDistillation.from_store(store, alpha=0.5), loss_scaler=NativeScalerWithGradNormCount())
+    assert np.isfinite(out[0]["loss"])
+    with pytest.raises(ValueError, match="EP head"):
+        _epoch(_model(128, 7, head=head, **kw), _store(48, 16, 128, 7, lengths=True))
+
+
+def test_refusals():
+    from efficient_probing_amd import distill, engine_finetune as EF
+    from efficient_probing_amd.engine import ProbeHeadEngine, make_engine
+    store = _store(20, 8, 128, 6)
+    crit = distill.TopKDistillation.from_store(store)
+    with pytest.raises(ValueError, match="temperature"):
+        distill.TopKDistillation.from_store(store, temperature=1.0)
+    with pytest.raises(ValueError, match="mixup"):
+        _epoch(_model(128, 6), store, crit, mixup_fn=lambda a, b: (a, b))
+    with pytest.raises(ValueError, match="mixup"):
+        _epoch(_model(128, 6), store, None, mixup_fn=lambda a, b: (a, b))
+    with pytest.raises(ValueError, match="tables"):
+        store.table("channel_stats")
+    eng = ProbeHeadEngine(_model(256, 6).head.train(), optimizer="sgd")
+    with pytest.raises(ValueError, match="256 channels|channels"):
+        eng.forward_backward(store.tokens, store.labels)
+    eng = ProbeHeadEngine(_model(128, 6).head.train(), optimizer="sgd")
+    with pytest.raises(ValueError, match="targets"):
+        eng.forward_backward(store.tokens, store.labels[:3])
+    other = make_engine(_model(128, 6, head="simpool").head.train(), optimizer="sgd")
+    with pytest.raises(NotImplementedError):
+        other.forward_backward(store.tokens, store.labels)
+    with pytest.raises(NotImplementedError):
+        other.eval_logits(store.tokens)
