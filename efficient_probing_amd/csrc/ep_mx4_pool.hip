@@ -85,8 +85,9 @@ __device__ __forceinline__ f4 mx_mfma_codes(const mx_u4& codes, uint32_t scale, 
 template <int QM>
 struct MxOperand { mx_u6 b[MxDims<QM>::SETS]; uint32_t sc[MxDims<QM>::SCB]; };
 
-// the operand of one row block for this lane's column; QM 8: two terms share an operand, columns 8-15 take the odd ones
-template <int QM>
+// the operand of one row block for this lane's column; QM 8: two terms share an operand, columns 8-15 take the odd ones.  FIFTH: the
+// last term (and its scale byte) in all columns, for a caller that puts two blocks' last terms into one operand
+template <int QM, bool FIFTH = false>
 __device__ __forceinline__ void mx_operand(mx_f16 a, mx_f16 b, int c, MxOperand<QM>& o) {       // a, b: the row's even and odd channels
   uint32_t am = 0;
 #pragma unroll
@@ -113,7 +114,7 @@ __device__ __forceinline__ void mx_operand(mx_f16 a, mx_f16 b, int c, MxOperand<
     }
     const uint32_t byte = bad ? 255u : (uint32_t)(s0 - 5 * t);
     if constexpr (QM == 8) {
-      if (t % 2 == 0) { o.b[t / 2] = k; bytes[0] |= (odd ? 0u : byte) << (8 * (t / 2)); }
+      if (t % 2 == 0) { o.b[t / 2] = k; bytes[0] |= (odd && !(FIFTH && t == 4) ? 0u : byte) << (8 * (t / 2)); }
       else {
 #pragma unroll
         for (int i = 0; i < 6; ++i) o.b[t / 2][i] = odd ? k[i] : o.b[t / 2][i];
@@ -125,7 +126,7 @@ __device__ __forceinline__ void mx_operand(mx_f16 a, mx_f16 b, int c, MxOperand<
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  if constexpr (QM == 8) {                                     // there is no sixth term
+  if constexpr (QM == 8 && !FIFTH) {                           // there is no sixth term
 #pragma unroll
     for (int i = 0; i < 6; ++i) o.b[2][i] = odd ? 0u : o.b[2][i];
   }
@@ -171,13 +172,17 @@ struct MxCursor {
   }
 };
 
-template <int QM, int CPW, int NST, bool BWD>
-__global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
-  typedef MxDims<QM> DM;
-  constexpr int NQB = DM::NQB, SV = DM::SV;
-  constexpr int CODES = 2048 * CPW, STAGE = CODES + 256 * ((CPW + 1) / 2), OPS = 2 * CPW + (CPW + 1) / 2;
+// ---- the wide-row form ---------------------------------------------------------------------------------------------------
+// Rows of more than 14 blocks.  A wave owns four blocks of the row for all tokens and up to 8 queries; `groups` such sets of waves share
+// a workgroup and take turns at the tiles (forward: of one image; backward: a group per image).  Every wave makes the weights itself,
+// in the very lanes in which its second contraction wants them.  Accumulators and operand rows of four blocks fill 192 of 256 registers:
+// lane constants are made again where they are used, since a register reloaded from scratch waits for the tiles in flight.
+template <bool BWD, bool OPENS>
+__global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
+  constexpr int QM = 8, CPW = 4, NST = MX_STAGES, REC = 1024;          // REC: bytes of an exchange record, the lane's four scores
+  constexpr int CODES = 2048 * CPW, STAGE = CODES + 128 * CPW, OPS = 2 * CPW + CPW / 2;
   extern __shared__ __align__(16) char lds[];
-  const int lane = lane_id(), c = lane & 15, g = lane >> 4;
+  const int lane = lane_id();
   const int wave = wave_id_uniform();
   const int nw = p.nw, groups = p.groups;
   const int grp = wave / nw, dw = wave - grp * nw;
@@ -188,14 +193,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
   char* ring = lds + wave * (NST * STAGE);
   char* exch = lds + nw * groups * (NST * STAGE);                      // [2][groups][nw][REC]
 
-  // ---- lane constants.  LDS row r of a tile holds token 8 (r % 4) + r / 4, its 16-byte pieces XOR-ed with r / 4: both contractions
-  // then read all banks.
-  const int tok0 = 8 * g + (QM == 8 ? 4 * (c >> 3) : 0);               // first token of the lane's scores in a tile
-  const int sc_off = (8 * (c >> 2) + (c & 3)) * 4;                     // + 16 h: scale dword of the score row
-  const int a_off = (4 * (c & 3) + (c >> 2)) * 64 + ((g ^ (c & 3)) << 4);
-  const int p_off = g * 64 + c * 4;                                    // slot i: (p_off ^ 16 (i % 4)) + 256 i
-  const uint32_t rot = (uint32_t)(8 * (c >> 2) + 9);
-
+  // LDS row r of a tile holds token 8 (r % 4) + r / 4, its 16-byte pieces XOR-ed with r / 4: both contractions then read all banks
   auto issue = [&](const MxCursor& cu, int slot) {
     char* st = ring + slot * STAGE;
     const int t0 = cu.tile << 5, rows = cu.len - t0;
@@ -214,7 +212,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
     }
 #pragma unroll
     for (int k = 0; k < CPW; k += 2) {                                 // lanes 32-63: the second block
-      const int ch0 = chunk0 + k < nc ? chunk0 + k : nc - 1, ch1 = k + 1 < CPW && ch0 + 1 < nc ? ch0 + 1 : ch0;
+      const int ch0 = chunk0 + k < nc ? chunk0 + k : nc - 1, ch1 = ch0 + 1 < nc ? ch0 + 1 : ch0;
       __builtin_amdgcn_global_load_lds((mx_gptr_t)(scl + (offs + (unsigned)(ln < 32 ? ch0 : ch1) * 4u)), (mx_lds_t)(st + CODES + k * 128), 4, 0, 0);
     }
   };
@@ -225,210 +223,172 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
   else { cu.u = (int)blockIdx.x; cu.ustep = (int)gridDim.x; cu.toff = grp; cu.tstep = groups; }
   MxCursor ahead = cu;                                                  // the next tile to load
   ahead.open(t);
-  float sg[NQB][SV];                                                    // backward: saved scores of the next tile
+  f4 sg;                                                                // backward: saved scores of the next tile
   auto load_scores = [&](const MxCursor& cu) {
-    const int ln = mx_fresh(lane), c = ln & 15, tok0 = 8 * (ln >> 4) + (QM == 8 ? 4 * (c >> 3) : 0);
-#pragma unroll
-    for (int qb = 0; qb < NQB; ++qb) {
-      const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-      const float* row = p.S + ((int64_t)cu.b * p.Q + q0) * p.lds_;
-#pragma unroll
-      for (int h = 0; h < SV / 4; ++h) {
-        const int n = (cu.tile << 5) + tok0 + 4 * h;
-        const f4 v = *reinterpret_cast<const f4*>(row + (unsigned)((q < qn ? q : 0) * (int)p.lds_ + (n < p.lds_ ? n : (int)p.lds_ - 4)));
-        sg[qb][4 * h] = v.x; sg[qb][4 * h + 1] = v.y; sg[qb][4 * h + 2] = v.z; sg[qb][4 * h + 3] = v.w;
-      }
-    }
+    const int ln = mx_fresh(lane), q = ln & 7, n = (cu.tile << 5) + 8 * (ln >> 4) + 4 * ((ln >> 3) & 1);
+    const float* row = p.S + ((int64_t)cu.b * p.Q + q0) * p.lds_;
+    sg = *reinterpret_cast<const f4*>(row + (unsigned)((q < qn ? q : 0) * (int)p.lds_ + (n < p.lds_ ? n : (int)p.lds_ - 4)));
   };
   if constexpr (BWD) load_scores(ahead);
 #pragma unroll
   for (int i = 0; i < NST; ++i) { issue(ahead, i); ahead.next(t); }
 
-  // ---- operand rows
-  MxOperand<QM> op[NQB][CPW];
-  auto load_operand = [&](const float* rows, const float* prows, float mul, float (&delta)[NQB]) {
-    const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
+  // ---- operand rows: one block at a time and last to first, the operands moving up by one (as straight code for every block this part
+  // alone would be 11 KiB of instructions that run once)
+  struct { mx_u6 b[2]; uint32_t sc; } op[CPW];
+  mx_u6 fifth[CPW / 2];                                                 // two blocks' last terms, in columns 0-7 and 8-15 (which are added)
+  auto load_operand = [&](const float* rows, const float* prows, float mul) {
+    const int ln = mx_fresh(lane), c = ln & 15, q = c & 7;
+    const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * p.ldq + 32 * (ln >> 4);      // (rows without a query: the first one's, times 0)
+    float d = 0.f;
+    mx_f16 ve, vo;
+    auto load = [&](int k) {
+      const bool in = chunk0 + k < nc;
+      mx_load_row(rows + at + (in ? chunk0 + k : nc - 1) * MX_BLOCK, in && q < qn ? mul : 0.f, ve, vo);
+    };
+    load(CPW - 1);
+#pragma unroll 1
+    for (int k = CPW - 1; k >= 0; --k) {
+      if (BWD && prows) {
+        mx_f16 we, wo;
+        mx_load_row(prows + at + (chunk0 + k < nc ? chunk0 + k : nc - 1) * MX_BLOCK, 1.f, we, wo);
 #pragma unroll
-    for (int qb = 0; qb < NQB; ++qb) {
-      const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-      const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * p.ldq + 32 * g;      // (rows without a query: the first one's, times 0)
-      float d = 0.f;
-#pragma unroll
-      for (int k = 0; k < CPW; ++k) {
-        const bool in = chunk0 + k < nc;
-        const int d0 = (in ? chunk0 + k : nc - 1) * MX_BLOCK;
-        mx_f16 ve, vo;
-        mx_load_row(rows + at + d0, in && q < qn ? mul : 0.f, ve, vo);
-        if (BWD && prows) {
-          mx_f16 we, wo;
-          mx_load_row(prows + at + d0, 1.f, we, wo);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) d = fmaf(vo[i], wo[i], fmaf(ve[i], we[i], d));
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        mx_operand<QM>(ve, vo, c, op[qb][k]);
+        for (int i = 0; i < 16; ++i) d = fmaf(vo[i], wo[i], fmaf(ve[i], we[i], d));
         __builtin_amdgcn_sched_barrier(0);
       }
-      delta[qb] = BWD && prows ? mx_over_groups_sum(d) : 0.f;
-    }
-  };
-  float delta[NQB];
-
-  float m_run[NQB], mz[NQB], l_run[NQB], t_max[NQB], invl[NQB];         // mz: the maximum that weights are taken against
-  auto open_unit = [&](int b) {                                         // backward: dP's rows and the saved statistics
-    const int c = mx_fresh(lane) & 15;
-    load_operand(p.q + (int64_t)b * p.Q * p.ldq, p.Pin ? p.Pin + (int64_t)b * p.Q * p.ldq : nullptr, 1.f, delta);
 #pragma unroll
-    for (int qb = 0; qb < NQB; ++qb) {
-      const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-      f4 ml = {0.f, 0.f, 0.f, 0.f};
-      if (q < qn) ml = *reinterpret_cast<const f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4);
-      mz[qb] = ml.x;
-      invl[qb] = ml.y == 0.f ? 0.f : 1.f / ml.y;
-      if (!p.Pin && dw == 0) delta[qb] = ml.z;                          // (each D-slice takes off its own part of delta)
+      for (int j = CPW - 1; j > 0; --j) op[j] = op[j - 1];
+      const mx_f16 ue = ve, uo = vo;
+      if (k > 0) load(k - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      MxOperand<QM> o;
+      mx_operand<QM, true>(ue, uo, c, o);
+      op[0].b[0] = o.b[0]; op[0].b[1] = o.b[1];
+      const bool up = (c & 8) != 0;
+      op[0].sc = up == ((k & 1) != 0) ? o.sc[0] : o.sc[0] & 0xffffu;     // the other block's columns: times 2^-127
+      if (k & 1) {
+#pragma unroll
+        for (int j = CPW / 2 - 1; j > 0; --j) fifth[j] = fifth[j - 1];
+      }
+#pragma unroll
+      for (int i = 0; i < 6; ++i) fifth[0][i] = up && !(k & 1) ? fifth[0][i] : o.b[2][i];
+      __builtin_amdgcn_sched_barrier(0);
     }
+    return BWD && prows ? mx_over_groups_sum(d) : 0.f;
   };
-  f4 acc[NQB][CPW][8];
+  float delta = 0.f, m_run, mz, l_run, t_max, invl;                     // mz: the maximum that weights are taken against
+  auto open_unit = [&](int b) {                                         // backward: dP's rows and the saved statistics
+    delta = load_operand(p.q + (int64_t)b * p.Q * p.ldq, p.Pin ? p.Pin + (int64_t)b * p.Q * p.ldq : nullptr, 1.f);
+    const int q = mx_fresh(lane) & 7;
+    f4 ml = {0.f, 0.f, 0.f, 0.f};
+    if (q < qn) ml = *reinterpret_cast<const f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4);
+    mz = ml.x;
+    invl = ml.y == 0.f ? 0.f : 1.f / ml.y;
+    if (!p.Pin && dw == 0) delta = ml.z;                                // (each D-slice takes off its own part of delta)
+  };
+  f4 acc[CPW][8];
   auto clear = [&]() {
 #pragma unroll
-    for (int qb = 0; qb < NQB; ++qb)
+    for (int k = 0; k < CPW; ++k)
 #pragma unroll
-      for (int k = 0; k < CPW; ++k)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[qb][k][j] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < 8; ++j) acc[k][j] = f4{0.f, 0.f, 0.f, 0.f};
   };
   clear();
   int slot = 0, buf = 0;
 
-  // acc rows 4 g + i of query block qb are queries qrow(i); multiply each by the value that lane (c = query) holds
-  auto scale_rows = [&](int qb, float f) {
+  // acc rows 4 g + i are queries (4 g + i) % 8; multiply each by the value that lane (c = query) holds
+  auto scale_rows = [&](float f) {
     const int g = mx_fresh(lane) >> 4;
     float r[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __shfl(f, QM == 8 ? (4 * g + i) & 7 : 4 * g + i, 64);
+    for (int i = 0; i < 4; ++i) r[i] = __shfl(f, (4 * g + i) & 7, 64);
 #pragma unroll
     for (int k = 0; k < CPW; ++k)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { acc[qb][k][j].x *= r[0]; acc[qb][k][j].y *= r[1]; acc[qb][k][j].z *= r[2]; acc[qb][k][j].w *= r[3]; }
+      for (int j = 0; j < 8; ++j) { acc[k][j].x *= r[0]; acc[k][j].y *= r[1]; acc[k][j].z *= r[2]; acc[k][j].w *= r[3]; }
   };
 
   auto tile_step = [&](int b, int t0, int len) {
-    float s[NQB][SV];
     const char* st = ring + slot * STAGE;
+    f4 s;
     {
       mx_wait_vm<(NST - 1) * OPS>();
-      // first contraction
-      f4 sa[NQB][2], sl[NQB][2];                                        // leading and lower terms: an addition to a large sum costs its last bit
+      // first contraction, sixteen tokens at a time.  Leading and lower terms are kept apart: an addition to a large sum costs its last bit
+      const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
+      const char* codes = st + (4 * (c & 3) + (c >> 2)) * 64 + ((g ^ (c & 3)) << 4);
+      const char* scl = st + CODES + (8 * (c >> 2) + (c & 3)) * 4;
+      f4 sum[2];
 #pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) sa[qb][0] = sa[qb][1] = sl[qb][0] = sl[qb][1] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int h = 0; h < 2; ++h) {
+        __builtin_amdgcn_sched_barrier(0);
+        f4 sa = {0.f, 0.f, 0.f, 0.f}, sl = sa;
 #pragma unroll
-      for (int k = 0; k < CPW; ++k)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const mx_u4 w = *reinterpret_cast<const mx_u4*>(st + k * 2048 + h * 1024 + a_off);
-          const uint32_t sc = *reinterpret_cast<const uint32_t*>(st + CODES + k * 128 + h * 16 + sc_off) >> (8 * g);
-#pragma unroll
-          for (int qb = 0; qb < NQB; ++qb) {
-            const MxOperand<QM>& o = op[qb][k];
-            sa[qb][h] = mx_mfma_codes<0>(w, sc, o.b[0], o.sc[0], sa[qb][h]);
-            if constexpr (QM != 8) {
-              sl[qb][h] = mx_mfma_codes<1>(w, sc, o.b[4], o.sc[1], sl[qb][h]);
-              sl[qb][h] = mx_mfma_codes<0>(w, sc, o.b[3], o.sc[1], sl[qb][h]);
-            }
-            sl[qb][h] = mx_mfma_codes<2>(w, sc, o.b[2], o.sc[0], sl[qb][h]);
-            sl[qb][h] = mx_mfma_codes<1>(w, sc, o.b[1], o.sc[0], sl[qb][h]);
-          }
+        for (int k = 0; k < CPW; ++k) {
+          const mx_u4 w = *reinterpret_cast<const mx_u4*>(codes + k * 2048 + h * 1024);
+          const uint32_t sc = *reinterpret_cast<const uint32_t*>(scl + k * 128 + h * 16) >> (8 * g);
+          sa = mx_mfma_codes<0>(w, sc, op[k].b[0], op[k].sc, sa);
+          sl = mx_mfma_codes<2>(w, sc, fifth[k / 2], op[k].sc, sl);
+          sl = mx_mfma_codes<1>(w, sc, op[k].b[1], op[k].sc, sl);
         }
+        sum[h] = sa + sl;
+      }
+      const bool up = (c & 8) != 0;                                    // columns q and q + 8 are terms of one query
 #pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) {
-        sa[qb][0] += sl[qb][0]; sa[qb][1] += sl[qb][1];
-        if constexpr (QM == 8) {                                        // columns q and q + 8 are terms of one query
-          const bool up = (c & 8) != 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float own = up ? sa[qb][1][i] : sa[qb][0][i], oth = up ? sa[qb][0][i] : sa[qb][1][i];
-            s[qb][i] = own + mx_ror8(oth) - (BWD ? delta[qb] : 0.f);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { s[qb][i] = sa[qb][0][i] - (BWD ? delta[qb] : 0.f); s[qb][4 + i] = sa[qb][1][i] - (BWD ? delta[qb] : 0.f); }
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float own = up ? sum[1][i] : sum[0][i], oth = up ? sum[0][i] : sum[1][i];
+        s[i] = own + mx_ror8(oth) - (BWD ? delta : 0.f);
       }
     }
     __builtin_amdgcn_sched_barrier(0);
     if (nw > 1) {                                                       // add the D-slices
-      char* ex = exch + (buf * groups + grp) * nw * DM::REC;
-      {
-#pragma unroll
-        for (int qb = 0; qb < NQB; ++qb)
-#pragma unroll
-          for (int h = 0; h < SV / 4; ++h)
-            *reinterpret_cast<f4*>(ex + dw * DM::REC + ((qb * (SV / 4) + h) * 64 + lane) * 16) = f4{s[qb][4 * h], s[qb][4 * h + 1], s[qb][4 * h + 2], s[qb][4 * h + 3]};
-      }
+      char* ex = exch + (buf * groups + grp) * nw * REC + mx_fresh(lane) * 16;
+      *reinterpret_cast<f4*>(ex + dw * REC) = s;
       mx_barrier();
       buf ^= 1;
-      {
-#pragma unroll
-        for (int qb = 0; qb < NQB; ++qb)
-#pragma unroll
-          for (int h = 0; h < SV / 4; ++h) {
-            f4 v = *reinterpret_cast<const f4*>(ex + ((qb * (SV / 4) + h) * 64 + lane) * 16);
-            for (int o = 1; o < nw; ++o) v += *reinterpret_cast<const f4*>(ex + o * DM::REC + ((qb * (SV / 4) + h) * 64 + lane) * 16);
-            s[qb][4 * h] = v.x; s[qb][4 * h + 1] = v.y; s[qb][4 * h + 2] = v.z; s[qb][4 * h + 3] = v.w;
-          }
-      }
+      s = *reinterpret_cast<const f4*>(ex);
+#pragma unroll 4
+      for (int o = 1; o < nw; ++o) s += *reinterpret_cast<const f4*>(ex + o * REC);
     }
     const bool tail = t0 + 32 > len;
     // weights
-    mx_u4 wt[NQB][DM::PSETS];
-#pragma unroll
-    for (int qb = 0; qb < NQB; ++qb) {
-      float pv[SV];
+    mx_u4 wt[2];
+    {
+      const int ln = mx_fresh(lane), c = ln & 15, tok0 = 8 * (ln >> 4) + 4 * (c >> 3);      // the lane's first token in the tile
+      float pv[4];
       if constexpr (!BWD) {
         if (tail) {
 #pragma unroll
-          for (int i = 0; i < SV; ++i) s[qb][i] = t0 + tok0 + i < len ? s[qb][i] : -INFINITY;
+          for (int i = 0; i < 4; ++i) s[i] = t0 + tok0 + i < len ? s[i] : -INFINITY;
         }
         if (p.S && dw == 0) {
-          const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-          if (q < qn) {
-            float* sp = p.S + ((int64_t)b * p.Q + q0 + q) * p.lds_ + t0 + tok0;
-#pragma unroll
-            for (int h = 0; h < SV / 4; ++h)
-              if (t0 + tok0 + 4 * h < t.N) *reinterpret_cast<f4*>(sp + 4 * h) = f4{s[qb][4 * h], s[qb][4 * h + 1], s[qb][4 * h + 2], s[qb][4 * h + 3]};
-          }
+          const int q = c & 7;
+          if (q < qn && t0 + tok0 < t.N) *reinterpret_cast<f4*>(p.S + ((int64_t)b * p.Q + q0 + q) * p.lds_ + t0 + tok0) = s;
         }
-        float mx = s[qb][0];
-#pragma unroll
-        for (int i = 1; i < SV; ++i) mx = fmaxf(mx, s[qb][i]);
-        t_max[qb] = fmaxf(t_max[qb], mx);
-        if (__any(mx > m_run[qb] + MX_LAZY)) {
-          if (QM == 8) mx = fmaxf(mx, mx_ror8(mx));
-          mx = mx_over_groups_max(mx);
-          const float mn = fmaxf(m_run[qb], mx);
-          const float f = mn == m_run[qb] ? 1.f : __builtin_amdgcn_exp2f((m_run[qb] - mn) * MX_LOG2E);
-          m_run[qb] = mn;
-          mz[qb] = mn == -INFINITY ? 0.f : mn;
-          l_run[qb] *= f;
-          scale_rows(qb, f);
+        float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        t_max = fmaxf(t_max, mx);
+        if (__any(mx > m_run + MX_LAZY)) {
+          mx = mx_over_groups_max(fmaxf(mx, mx_ror8(mx)));
+          const float mn = fmaxf(m_run, mx);
+          const float f = mn == m_run ? 1.f : __builtin_amdgcn_exp2f((m_run - mn) * MX_LOG2E);
+          m_run = mn;
+          mz = mn == -INFINITY ? 0.f : mn;
+          l_run *= f;
+          scale_rows(f);
         }
 #pragma unroll
-        for (int i = 0; i < SV; ++i) { pv[i] = __builtin_amdgcn_exp2f((s[qb][i] - mz[qb]) * MX_LOG2E); l_run[qb] += pv[i]; }
+        for (int i = 0; i < 4; ++i) { pv[i] = __builtin_amdgcn_exp2f((s[i] - mz) * MX_LOG2E); l_run += pv[i]; }
       } else {
 #pragma unroll
-        for (int i = 0; i < SV; ++i) {
-          const float a = __builtin_amdgcn_exp2f((sg[qb][i] - mz[qb]) * MX_LOG2E) * invl[qb];
-          pv[i] = a * s[qb][i];
-        }
+        for (int i = 0; i < 4; ++i) pv[i] = __builtin_amdgcn_exp2f((sg[i] - mz) * MX_LOG2E) * invl * s[i];
         if (tail) {
 #pragma unroll
-          for (int i = 0; i < SV; ++i) pv[i] = t0 + tok0 + i < len ? pv[i] : 0.f;
+          for (int i = 0; i < 4; ++i) pv[i] = t0 + tok0 + i < len ? pv[i] : 0.f;
         }
       }
       // three bf16 terms, exact: the upper half of the bits, of what is left, and of what is left then
-      uint32_t H[SV / 2], M[SV / 2], L[SV / 2];
+      uint32_t H[2], M[2], L[2];
 #pragma unroll
-      for (int i = 0; i < SV / 2; ++i) {
+      for (int i = 0; i < 2; ++i) {
         const float a = pv[2 * i], b2 = pv[2 * i + 1];
         const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), rb = b2 - __uint_as_float(__float_as_uint(b2) & 0xffff0000u);
         const float la = ra - __uint_as_float(__float_as_uint(ra) & 0xffff0000u), lb = rb - __uint_as_float(__float_as_uint(rb) & 0xffff0000u);
@@ -436,33 +396,32 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
         M[i] = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), 0x07060302u);
         L[i] = __builtin_amdgcn_perm(__float_as_uint(lb), __float_as_uint(la), 0x07060302u);
       }
-      if constexpr (QM == 8) {                                          // rows 0-7: first and third term, rows 8-15: second; 8 slots = both halves
-        const bool up = (c & 8) != 0;
+      const bool up = (c & 8) != 0;                                     // rows 0-7: first and third term, rows 8-15: second; 8 slots = both halves
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t r1 = mx_ror8u(up ? H[i] : M[i]), r2 = mx_ror8u(L[i]);
-          wt[qb][0][i] = up ? r1 : H[i];
-          wt[qb][0][2 + i] = up ? M[i] : r1;
-          wt[qb][1][i] = up ? 0u : L[i];
-          wt[qb][1][2 + i] = up ? 0u : r2;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { wt[qb][0][i] = H[i]; wt[qb][1][i] = M[i]; wt[qb][2][i] = L[i]; }
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t r1 = mx_ror8u(up ? H[i] : M[i]), r2 = mx_ror8u(L[i]);
+        wt[0][i] = up ? r1 : H[i];
+        wt[0][2 + i] = up ? M[i] : r1;
+        wt[1][i] = up ? 0u : L[i];
+        wt[1][2 + i] = up ? 0u : r2;
       }
     }
     // second contraction
     __builtin_amdgcn_sched_barrier(0);
+    {
+      const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
+      const int p_off = g * 64 + c * 4;                                 // slot i: (p_off ^ 16 (i % 4)) + 256 i
+      const uint32_t rot = (uint32_t)(8 * (c >> 2) + 9);
 #pragma unroll
-    for (int k = 0; k < CPW; ++k) {
-      uint32_t w[8];
-      float sc[8];
+      for (int k = 0; k < CPW; ++k) {
+        uint32_t w[8];
+        float sc[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i] = *reinterpret_cast<const uint32_t*>(st + k * 2048 + i * 256 + (p_off ^ ((i & 3) << 4)));
-        const uint32_t four = *reinterpret_cast<const uint32_t*>(st + CODES + k * 128 + g * 32 + i * 4);
-        sc[i] = __uint_as_float(__builtin_amdgcn_alignbit(four, four, rot));
-      }
+        for (int i = 0; i < 8; ++i) {
+          w[i] = *reinterpret_cast<const uint32_t*>(st + k * 2048 + i * 256 + (p_off ^ ((i & 3) << 4)));
+          const uint32_t four = *reinterpret_cast<const uint32_t*>(st + CODES + k * 128 + g * 32 + i * 4);
+          sc[i] = __uint_as_float(__builtin_amdgcn_alignbit(four, four, rot));
+        }
 #define EP_MX_PAIR(PR)                                                                                                   \
   do {                                                                                                                   \
     uint32_t x[8];                                                                                                       \
@@ -472,14 +431,15 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
       ev[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05040100u);                                                \
       od[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);                                                \
     }                                                                                                                    \
-    _Pragma("unroll") for (int qb = 0; qb < NQB; ++qb) _Pragma("unroll") for (int z = DM::PSETS - 1; z >= 0; --z) {     \
-      acc[qb][k][2 * PR] = mx_mfma(wt[qb][z], ev, acc[qb][k][2 * PR]);                                                   \
-      acc[qb][k][2 * PR + 1] = mx_mfma(wt[qb][z], od, acc[qb][k][2 * PR + 1]);                                           \
+    _Pragma("unroll") for (int z = 1; z >= 0; --z) {                                                                    \
+      acc[k][2 * PR] = mx_mfma(wt[z], ev, acc[k][2 * PR]);                                                               \
+      acc[k][2 * PR + 1] = mx_mfma(wt[z], od, acc[k][2 * PR + 1]);                                                       \
     }                                                                                                                    \
   } while (0)
-      EP_MX_PAIR(0); EP_MX_PAIR(1); EP_MX_PAIR(2); EP_MX_PAIR(3);
-      __builtin_amdgcn_sched_barrier(0);
+        EP_MX_PAIR(0); EP_MX_PAIR(1); EP_MX_PAIR(2); EP_MX_PAIR(3);
+        __builtin_amdgcn_sched_barrier(0);
 #undef EP_MX_PAIR
+      }
     }
   };
   // the stage is read: load the tile NST further on into it.  The loads always are the same number (at the end of the sequence they
@@ -493,43 +453,36 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
     slot = slot + 1 == NST ? 0 : slot + 1;
   };
 
-  // store (or add) acc times r(query) as rows of out (row stride D): QM 8 adds the two term rows first
-  auto store_rows = [&](float* out, const float (&inv)[NQB], bool add) {
+  // store (or add) acc times inv(query) as rows of out (row stride D), the two term rows added first
+  auto store_rows = [&](float* out, float inv, bool add) {
     const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
+    float r[4];
 #pragma unroll
-    for (int qb = 0; qb < NQB; ++qb) {
-      float r[4];
+    for (int i = 0; i < 4; ++i) r[i] = __shfl(inv, 4 * (g & 1) + i, 64);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = __shfl(inv[qb], QM == 8 ? 4 * (g & 1) + i : 4 * g + i, 64);
+    for (int k = 0; k < CPW; ++k)
 #pragma unroll
-      for (int k = 0; k < CPW; ++k)
+      for (int i = 0; i < 4; ++i) {
+        const int q = 4 * (g & 1) + i;
+        float* o = out + (int64_t)(q0 + q) * t.D;
+        __builtin_amdgcn_sched_barrier(0);                               // row by row: the added values of all rows at once would not fit
+        f4 x;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int q = QM == 8 ? 4 * (g & 1) + i : qb * 16 + 4 * g + i;
-          float* o = out + (int64_t)(q0 + q) * t.D;
-          __builtin_amdgcn_sched_barrier(0);                             // row by row: the added values of all rows at once would not fit
-          constexpr int NV = QM == 8 ? 1 : 2;
-#pragma unroll
-          for (int v = 0; v < NV; ++v) {
-            f4 x;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = (QM == 8 ? fold32(acc[qb][k][j][i], acc[qb][k][j + 4][i]) : acc[qb][k][4 * v + j][i]) * r[i];
-            const int d = (chunk0 + k) * MX_BLOCK + 8 * c + (QM == 8 ? 4 * (g >> 1) : 4 * v);
-            if (q < qn && chunk0 + k < nc) {
-              if (p.veco) {
-                if (d < t.D) {
-                  if (BWD && add) x += *reinterpret_cast<const f4*>(o + d);
-                  *reinterpret_cast<f4*>(o + d) = x;
-                }
-              } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (d + j < t.D) o[d + j] = BWD && add ? o[d + j] + x[j] : x[j];
-              }
+        for (int j = 0; j < 4; ++j) x[j] = fold32(acc[k][j][i], acc[k][j + 4][i]) * r[i];
+        const int d = (chunk0 + k) * MX_BLOCK + 8 * c + 4 * (g >> 1);
+        if (q < qn && chunk0 + k < nc) {
+          if (p.veco) {
+            if (d < t.D) {
+              if (BWD && add) x += *reinterpret_cast<const f4*>(o + d);
+              *reinterpret_cast<f4*>(o + d) = x;
             }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (d + j < t.D) o[d + j] = BWD && add ? o[d + j] + x[j] : x[j];
           }
         }
-    }
+      }
   };
   // add the groups' accumulators into group 0's, half a row block at a time, through the exchange records (2 groups nw of them, at
   // least 4 KiB a wave of a group)
@@ -537,34 +490,32 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
     const int ln = mx_fresh(lane);
     for (int o = 1; o < groups; ++o) {
 #pragma unroll
-      for (int qb = 0; qb < NQB; ++qb)
+      for (int k = 0; k < CPW; ++k)
 #pragma unroll
-        for (int k = 0; k < CPW; ++k)
+        for (int j0 = 0; j0 < 8; j0 += 4) {
+          if (grp == o) {
 #pragma unroll
-          for (int j0 = 0; j0 < 8; j0 += 4) {
-            if (grp == o) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) *reinterpret_cast<f4*>(exch + (dw * 4 + j) * 1024 + ln * 16) = acc[qb][k][j0 + j];
-            }
-            mx_barrier();
-            if (grp == 0) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[qb][k][j0 + j] += *reinterpret_cast<const f4*>(exch + (dw * 4 + j) * 1024 + ln * 16);
-            }
-            mx_barrier();
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<f4*>(exch + (dw * 4 + j) * 1024 + ln * 16) = acc[k][j0 + j];
           }
+          mx_barrier();
+          if (grp == 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[k][j0 + j] += *reinterpret_cast<const f4*>(exch + (dw * 4 + j) * 1024 + ln * 16);
+          }
+          mx_barrier();
+        }
     }
   };
 
   if constexpr (!BWD) {
+    if constexpr (!OPENS) load_operand(p.q, nullptr, p.scale);
     for (int u = (int)blockIdx.x; u < p.units; u += (int)gridDim.x) {
       const int b = u / p.splits, sp = u - b * p.splits;
       int len;
       const int img = mx_image_uniform(t, b, len);
       const int n = (len + 31) >> 5, lo = sp * p.tps, hi = (sp + 1) * p.tps < n ? (sp + 1) * p.tps : n;
-      if (p.qb || u == (int)blockIdx.x) load_operand(p.q + (int64_t)b * p.qb, nullptr, p.scale, delta);
-#pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) { m_run[qb] = t_max[qb] = -INFINITY; mz[qb] = l_run[qb] = 0.f; }
+      if constexpr (OPENS) load_operand(p.q + (int64_t)b * p.qb, nullptr, p.scale);
+      m_run = t_max = -INFINITY; mz = l_run = 0.f;
       clear();
       int tl = lo;
       for (; tl + grp < hi; tl += groups) {
@@ -577,60 +528,42 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
         for (int q = 0; q < qn; ++q)
           for (int i = (n << 5) + ln; i < t.N; i += 64) p.S[((int64_t)b * p.Q + q0 + q) * p.lds_ + i] = img < 0 ? __uint_as_float(0x7fc00000u) : -INFINITY;
       }
-      float f[NQB];
-#pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) {                                // over the lanes of a query
-        if (QM == 8) { l_run[qb] += mx_ror8(l_run[qb]); t_max[qb] = fmaxf(t_max[qb], mx_ror8(t_max[qb])); }
-        l_run[qb] = mx_over_groups_sum(l_run[qb]);
-        t_max[qb] = mx_over_groups_max(t_max[qb]);
-      }
+      l_run = mx_over_groups_sum(l_run + mx_ror8(l_run));               // over the lanes of a query
+      t_max = mx_over_groups_max(fmaxf(t_max, mx_ror8(t_max)));
       if (groups > 1) {
-        float* ml = reinterpret_cast<float*>(exch);                     // [groups][NQB][16][3]
+        float* ml = reinterpret_cast<float*>(exch);                     // [groups][16][3]
         mx_barrier();
         if (dw == 0 && g == 0) {
-#pragma unroll
-          for (int qb = 0; qb < NQB; ++qb) {
-            float* e = ml + ((grp * NQB + qb) * 16 + c) * 3;
-            e[0] = m_run[qb]; e[1] = l_run[qb]; e[2] = t_max[qb];
-          }
+          float* e = ml + (grp * 16 + c) * 3;
+          e[0] = m_run; e[1] = l_run; e[2] = t_max;
         }
         mx_barrier();
-#pragma unroll
-        for (int qb = 0; qb < NQB; ++qb) {
-          float M = -INFINITY, T = -INFINITY, l = 0.f;
-          for (int o = 0; o < groups; ++o) { const float* e = ml + ((o * NQB + qb) * 16 + c) * 3; M = fmaxf(M, e[0]); T = fmaxf(T, e[2]); }
-          for (int o = 0; o < groups; ++o) {
-            const float* e = ml + ((o * NQB + qb) * 16 + c) * 3;
-            l += e[0] == M ? e[1] : e[1] * __builtin_amdgcn_exp2f((e[0] - M) * MX_LOG2E);
-          }
-          const float own = m_run[qb] == M ? 1.f : __builtin_amdgcn_exp2f((m_run[qb] - M) * MX_LOG2E);
-          scale_rows(qb, own);
-          m_run[qb] = M; l_run[qb] = l; t_max[qb] = T;
-          mz[qb] = M == -INFINITY ? 0.f : M;
+        float M = -INFINITY, T = -INFINITY, l = 0.f;
+        for (int o = 0; o < groups; ++o) { const float* e = ml + (o * 16 + c) * 3; M = fmaxf(M, e[0]); T = fmaxf(T, e[2]); }
+        for (int o = 0; o < groups; ++o) {
+          const float* e = ml + (o * 16 + c) * 3;
+          l += e[0] == M ? e[1] : e[1] * __builtin_amdgcn_exp2f((e[0] - M) * MX_LOG2E);
         }
+        const float own = m_run == M ? 1.f : __builtin_amdgcn_exp2f((m_run - M) * MX_LOG2E);
+        scale_rows(own);
+        m_run = M; l_run = l; t_max = T;
+        mz = M == -INFINITY ? 0.f : M;
+        mx_barrier();                                                   // (the records are read: they carry accumulators next)
         add_groups();
       }
       if (grp == 0) {
         const float bad = img < 0 ? __uint_as_float(0x7fc00000u) : 0.f;
-#pragma unroll
-        for (int qb = 0; qb < NQB; ++qb) {
-          const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-          const bool none = t_max[qb] == -INFINITY && l_run[qb] == 0.f;                       // no token
-          const float m = none ? (p.splits > 1 ? -INFINITY : 0.f) : t_max[qb];
-          const float e = none ? 0.f : __builtin_amdgcn_exp2f((mz[qb] - m) * MX_LOG2E);       // from the running to the true maximum
-          if (dw == 0 && g == 0 && (QM != 8 || c < 8) && q < qn) {
-            if (p.splits > 1) *reinterpret_cast<f2*>(p.part_ml + ((int64_t)u * p.Q + q0 + q) * 2) = f2{m + bad, l_run[qb] * e + bad};
-            else *reinterpret_cast<f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4) = f4{m + bad, l_run[qb] * e + bad, 0.f, 0.f};
-          }
-          f[qb] = (p.splits > 1 ? e : (none ? 0.f : 1.f / l_run[qb])) + bad;
+        const bool none = t_max == -INFINITY && l_run == 0.f;                                 // no token
+        const float m = none ? (p.splits > 1 ? -INFINITY : 0.f) : t_max;
+        const float e = none ? 0.f : __builtin_amdgcn_exp2f((mz - m) * MX_LOG2E);             // from the running to the true maximum
+        if (dw == 0 && g == 0 && c < 8 && c < qn) {
+          if (p.splits > 1) *reinterpret_cast<f2*>(p.part_ml + ((int64_t)u * p.Q + q0 + c) * 2) = f2{m + bad, l_run * e + bad};
+          else *reinterpret_cast<f4*>(p.ML + ((int64_t)b * p.Q + q0 + c) * 4) = f4{m + bad, l_run * e + bad, 0.f, 0.f};
         }
-        store_rows(p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, f, false);
+        store_rows(p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, (p.splits > 1 ? e : (none ? 0.f : 1.f / l_run)) + bad, false);
       }
     }
   } else {
-    float one[NQB];
-#pragma unroll
-    for (int qb = 0; qb < NQB; ++qb) one[qb] = p.scale;
     const int rounds = (p.units + cu.ustep - 1) / cu.ustep;
     int u = cu.u;
     cu.open(t);
@@ -646,10 +579,10 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_pool_kernel(MxPool p) {
       if (nw > 1)
         for (; it < p.tps; ++it) mx_barrier();                          // groups with fewer tiles keep the others' barriers
       if (p.per_unit) {                                                 // one gradient per image (and split)
-        if (u < p.units) store_rows(p.part + (int64_t)u * p.Q * t.D, one, false);
+        if (u < p.units) store_rows(p.part + (int64_t)u * p.Q * t.D, p.scale, false);
       } else {
         if (groups > 1) { mx_barrier(); add_groups(); }
-        if (grp == 0) store_rows(p.part + (int64_t)blockIdx.x * p.Q * t.D, one, r > 0);
+        if (grp == 0) store_rows(p.part + (int64_t)blockIdx.x * p.Q * t.D, p.scale, r > 0);
       }
     }
   }
@@ -1240,7 +1173,7 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   const int nc = mx_blocks(D), cus = cu_count(), tiles = (N + 31) / 32;
   constexpr int LDS = 160 * 1024;
   int cap;                                                              // workgroups that run at the same time
-  if (nc <= 15) {                                                       // a wave per block and the weight wave
+  if (nc <= 14) {                                                       // a wave per block and the weight wave: what 160 KiB of LDS hold
     p.qm = Q <= 8 ? 8 : 16;
     p.nw = nc; p.cpw = 1; p.groups = 1;
     constexpr int waves = 16;                                           // four a SIMD
@@ -1300,14 +1233,14 @@ template <typename K>
 static int mx_launch_kernel(K* fn, const MxPool& p, const MxPlan& pl, int threads, hipStream_t st) {
   if (pl.lds > 64 * 1024) EP_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, (int)pl.lds));
   hipLaunchKernelGGL(fn, dim3((unsigned)pl.grid, (unsigned)pl.yblk), dim3((unsigned)threads), pl.lds, st, p);
-  EP_LAUNCH_CHECK("ep_mx4_pool_kernel");
+  EP_LAUNCH_CHECK("MX4 attention kernel");
   return 0;
 }
 template <bool BWD>
 static int mx_launch(const MxPool& p, const MxPlan& pl, hipStream_t st) {
   const int threads = 64 * (pl.nw + 1);
-  if (!pl.pipe) return mx_launch_kernel(ep_mx4_pool_kernel<8, 4, MX_STAGES, BWD>, p, pl, 64 * pl.nw * pl.groups, st);
   const bool opens = BWD || p.qb;
+  if (!pl.pipe) return mx_launch_kernel(opens ? ep_mx4_wide_kernel<BWD, true> : ep_mx4_wide_kernel<BWD, BWD>, p, pl, 64 * pl.nw * pl.groups, st);
   if (pl.qm == 8) return opens ? mx_launch_kernel(ep_mx4_pipe_kernel<8, BWD, true>, p, pl, threads, st) : mx_launch_kernel(ep_mx4_pipe_kernel<8, BWD, BWD>, p, pl, threads, st);
   return opens ? mx_launch_kernel(ep_mx4_pipe_kernel<16, BWD, true>, p, pl, threads, st) : mx_launch_kernel(ep_mx4_pipe_kernel<16, BWD, BWD>, p, pl, threads, st);
 }

@@ -150,6 +150,22 @@ def test_attention(B, N, D, Q, per_image):
     _check(c, x, q, D ** -0.5, per_image, seed=N)
 
 
+@pytest.mark.parametrize("D", [1536, 1664, 1665, 1792, 1793, 1920, 1921, 2049, 2560, 2700, 3584, 3970, 4096])
+@pytest.mark.parametrize("Q", [3, 13])
+def test_every_cut_of_wide_rows(D, Q):
+    """Rows around the border between the two forms of the kernel and around their slices, images of different lengths."""
+    lengths = [0, 97, 1, 64, 33]
+    c, x = _cache(5, 97, D, D, lengths)
+    q = torch.randn(Q, D, generator=torch.Generator().manual_seed(Q)) * 1.5
+    _check(c, x, q, D ** -0.5, False, [1, 4, 0, 3, 2, 1], lengths)
+
+
+def test_more_images_than_compute_units_of_wide_rows():
+    c, x = _cache(20, 40, 2100, 7)
+    q = torch.randn(5, 2100, generator=torch.Generator().manual_seed(2))
+    _check(c, x, q, 2100 ** -0.5, False, [i % 20 for i in range(600)])
+
+
 @pytest.mark.parametrize("B,N,D,Q", [(6, 1, 64, 2), (7, 40, 130, 8), (6, 197, 384, 12), (5, 257, 1152, 8), (4, 90, 768, 32), (3, 40, 4096, 2)])
 @pytest.mark.parametrize("per_image", [False, True])
 def test_ragged_and_indexed(B, N, D, Q, per_image):
