@@ -37,13 +37,10 @@ constexpr int MX_NT = 2;                         // cache policy of the code loa
 constexpr float MX_LAZY = 12.0f;                 // the running maximum follows a score only when it lies this far above it
 
 template <int QM> struct MxDims {
-  static constexpr int NQB = QM == 32 ? 2 : 1;   // blocks of query rows
-  static constexpr int ROWS = QM == 8 ? 8 : 16;  // queries of a block
   static constexpr int SETS = QM == 8 ? 3 : 5;   // matrix operands of the fp32 rows: five terms, two of them in one operand at QM 8
   static constexpr int SCB = QM == 8 ? 1 : 2;    // dwords of their scale bytes
-  static constexpr int SV = QM == 8 ? 4 : 8;     // scores per lane, tile and query block
+  static constexpr int SV = QM == 8 ? 4 : 8;     // scores per lane and tile
   static constexpr int PSETS = QM == 8 ? 2 : 3;  // operands of the weights
-  static constexpr int REC = 64 * 4 * SV * NQB;  // bytes of an exchange record
 };
 
 // the lane number once more, opaque to the compiler: what is derived from it is made where it is used and not kept in registers
@@ -599,9 +596,9 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
 template <int QM, bool BWD, bool OPENS>
 __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
   typedef MxDims<QM> DM;
-  constexpr int NQB = DM::NQB, SV = DM::SV, PREC = 2048 * NQB;            // a record: the accumulators as they are
+  constexpr int SV = DM::SV, PREC = 2048;            // a record: the accumulators as they are
   constexpr int NST = MX_PIPE_STAGES, STAGE = 2048 + 128, OPS = 3;
-  constexpr int WREC = NQB * DM::PSETS * 1024, WALL = WREC + 2 * NQB * 64 + 64;      // weights, rescaling factors, row factors, flags
+  constexpr int WREC = DM::PSETS * 1024, WALL = WREC + 128 + 64;      // weights, rescaling factors, row factors, flags
   extern __shared__ __align__(16) char lds[];
   const int lane = lane_id(), c = lane & 15, g = lane >> 4;
   const int wave = wave_id_uniform();
@@ -610,7 +607,7 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
   const int q0 = (int)blockIdx.y * p.qblk, qn = p.Q - q0 < p.qblk ? p.Q - q0 : p.qblk;      // queries of this workgroup
   char* recs = lds + nw * (NST * STAGE);                                // [2][nw][REC]
   char* wbuf = recs + 2 * nw * PREC;                                 // [2][WALL]
-  float* dbuf = reinterpret_cast<float*>(wbuf + 2 * WALL);              // [2][nw][NQB][16]: the blocks' parts of delta, by parity of the unit
+  float* dbuf = reinterpret_cast<float*>(wbuf + 2 * WALL);              // [2][nw][16]: the blocks' parts of delta, by parity of the unit
   const int tok0 = 8 * g + (QM == 8 ? 4 * (c >> 3) : 0);                // first token of the lane's scores in a tile
   const float NANF = __uint_as_float(0x7fc00000u);
 
@@ -660,71 +657,64 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
     for (int i = 0; i < NST; ++i) load_tile(i);
     MxCursor cp = cs;                                                   // the tile to pool
 
-    MxOperand<QM> op[NQB];
+    MxOperand<QM> op;
     int parity = 0;
     auto open_unit = [&](int b) {                                       // the operand rows; backward: this block's part of delta = dP . P
       const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
       const float* rows = p.q + (BWD ? (int64_t)b * p.Q * p.ldq : (int64_t)b * p.qb);
+      const int q = QM == 8 ? c & 7 : c;
+      const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * p.ldq + wave * MX_BLOCK + 32 * g;    // (rows without a query: the first one's, times 0)
+      mx_f16 ve, vo;
+      mx_load_row(rows + at, q < qn ? (BWD ? 1.f : p.scale) : 0.f, ve, vo);
+      if (BWD && p.Pin) {
+        float d = 0.f;
+        mx_f16 we, wo;
+        mx_load_row(p.Pin + (int64_t)b * p.Q * p.ldq + at, 1.f, we, wo);
 #pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) {
-        const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-        const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * p.ldq + wave * MX_BLOCK + 32 * g;    // (rows without a query: the first one's, times 0)
-        mx_f16 ve, vo;
-        mx_load_row(rows + at, q < qn ? (BWD ? 1.f : p.scale) : 0.f, ve, vo);
-        if (BWD && p.Pin) {
-          float d = 0.f;
-          mx_f16 we, wo;
-          mx_load_row(p.Pin + (int64_t)b * p.Q * p.ldq + at, 1.f, we, wo);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) d = fmaf(vo[i], wo[i], fmaf(ve[i], we[i], d));
-          d = mx_over_groups_sum(d);
-          if (g == 0) dbuf[((parity * nw + wave) * NQB + qb) * 16 + c] = d;
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        mx_operand<QM>(ve, vo, c, op[qb]);
+        for (int i = 0; i < 16; ++i) d = fmaf(vo[i], wo[i], fmaf(ve[i], we[i], d));
+        d = mx_over_groups_sum(d);
+        if (g == 0) dbuf[((parity * nw + wave)) * 16 + c] = d;
         __builtin_amdgcn_sched_barrier(0);
       }
+      mx_operand<QM>(ve, vo, c, op);
+      __builtin_amdgcn_sched_barrier(0);
       parity ^= 1;
     };
 
-    f4 acc[NQB][8];
+    f4 acc[8];
     auto clear = [&]() {
 #pragma unroll
-      for (int qb = 0; qb < NQB; ++qb)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[qb][j] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < 8; ++j) acc[j] = f4{0.f, 0.f, 0.f, 0.f};
     };
     // acc times r (one factor per row 4 g + i) as rows of out: QM 8 adds the two term rows first
-    auto store_rows = [&](float* out, const f4 (&r)[NQB], bool add) {
+    auto store_rows = [&](float* out, const f4 (&r), bool add) {
       const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
 #pragma unroll
-      for (int qb = 0; qb < NQB; ++qb)
+      for (int i = 0; i < 4; ++i) {
+        const int q = QM == 8 ? 4 * (g & 1) + i : 4 * g + i;
+        float* o = out + (int64_t)(q0 + q) * t.D;
+        __builtin_amdgcn_sched_barrier(0);
+        constexpr int NV = QM == 8 ? 1 : 2;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int q = QM == 8 ? 4 * (g & 1) + i : qb * 16 + 4 * g + i;
-          float* o = out + (int64_t)(q0 + q) * t.D;
-          __builtin_amdgcn_sched_barrier(0);
-          constexpr int NV = QM == 8 ? 1 : 2;
+        for (int v = 0; v < NV; ++v) {
+          f4 x;
 #pragma unroll
-          for (int v = 0; v < NV; ++v) {
-            f4 x;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = (QM == 8 ? fold32(acc[qb][j][i], acc[qb][j + 4][i]) : acc[qb][4 * v + j][i]) * r[qb][i];
-            const int d = wave * MX_BLOCK + 8 * c + (QM == 8 ? 4 * (g >> 1) : 4 * v);
-            if (q < qn) {
-              if (p.veco) {
-                if (d < t.D) {
-                  if (BWD && add) x += *reinterpret_cast<const f4*>(o + d);
-                  *reinterpret_cast<f4*>(o + d) = x;
-                }
-              } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (d + j < t.D) o[d + j] = BWD && add ? o[d + j] + x[j] : x[j];
+          for (int j = 0; j < 4; ++j) x[j] = (QM == 8 ? fold32(acc[j][i], acc[j + 4][i]) : acc[4 * v + j][i]) * r[i];
+          const int d = wave * MX_BLOCK + 8 * c + (QM == 8 ? 4 * (g >> 1) : 4 * v);
+          if (q < qn) {
+            if (p.veco) {
+              if (d < t.D) {
+                if (BWD && add) x += *reinterpret_cast<const f4*>(o + d);
+                *reinterpret_cast<f4*>(o + d) = x;
               }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (d + j < t.D) o[d + j] = BWD && add ? o[d + j] + x[j] : x[j];
             }
           }
         }
+      }
     };
     int sslot = 0, pslot = 0, buf = 0;
 
@@ -740,28 +730,23 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
         sc[h] = *reinterpret_cast<const uint32_t*>(st + 2048 + h * 16 + sc_off) >> (8 * g);
       }
       // lower terms first: only the last addition, the leading term's, rounds at the size of the score
-      f4 s[NQB][2];
+      f4 s[2];
+      const MxOperand<QM>& o = op;
+      s[0] = s[1] = f4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (QM != 8) {
 #pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) {
-        const MxOperand<QM>& o = op[qb];
-        s[qb][0] = s[qb][1] = f4{0.f, 0.f, 0.f, 0.f};
-        if constexpr (QM != 8) {
+        for (int h = 0; h < 2; ++h) s[h] = mx_mfma_codes<1>(w[h], sc[h], o.b[4], o.sc[1], s[h]);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) s[qb][h] = mx_mfma_codes<1>(w[h], sc[h], o.b[4], o.sc[1], s[qb][h]);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) s[qb][h] = mx_mfma_codes<0>(w[h], sc[h], o.b[3], o.sc[1], s[qb][h]);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s[qb][h] = mx_mfma_codes<2>(w[h], sc[h], o.b[2], o.sc[0], s[qb][h]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s[qb][h] = mx_mfma_codes<1>(w[h], sc[h], o.b[1], o.sc[0], s[qb][h]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s[qb][h] = mx_mfma_codes<0>(w[h], sc[h], o.b[0], o.sc[0], s[qb][h]);
+        for (int h = 0; h < 2; ++h) s[h] = mx_mfma_codes<0>(w[h], sc[h], o.b[3], o.sc[1], s[h]);
       }
 #pragma unroll
-      for (int qb = 0; qb < NQB; ++qb)
+      for (int h = 0; h < 2; ++h) s[h] = mx_mfma_codes<2>(w[h], sc[h], o.b[2], o.sc[0], s[h]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) *reinterpret_cast<f4*>(rec + (2 * qb + h) * 1024 + lane * 16) = s[qb][h];
+      for (int h = 0; h < 2; ++h) s[h] = mx_mfma_codes<1>(w[h], sc[h], o.b[1], o.sc[0], s[h]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) s[h] = mx_mfma_codes<0>(w[h], sc[h], o.b[0], o.sc[0], s[h]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) *reinterpret_cast<f4*>(rec + h * 1024 + lane * 16) = s[h];
       sslot = sslot + 1 == NST ? 0 : sslot + 1;
     };
 
@@ -776,19 +761,14 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
     };
     auto pool = [&]() {                                                 // second contraction of stage pslot with the weights of buffer buf
       const char* wr = wbuf + buf * WALL;
-      mx_u4 wt[NQB][DM::PSETS];
+      mx_u4 wt[DM::PSETS];
 #pragma unroll
-      for (int qb = 0; qb < NQB; ++qb)
-#pragma unroll
-        for (int z = 0; z < DM::PSETS; ++z) wt[qb][z] = *reinterpret_cast<const mx_u4*>(wr + (qb * DM::PSETS + z) * 1024 + lane * 16);
+      for (int z = 0; z < DM::PSETS; ++z) wt[z] = *reinterpret_cast<const mx_u4*>(wr + z * 1024 + lane * 16);
       if constexpr (!BWD) {
-        if (__builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(wr + WREC + 2 * NQB * 64))) {        // the running maximum has moved
+        if (__builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(wr + WREC + 128))) {        // the running maximum has moved
+          const f4 r = *reinterpret_cast<const f4*>(wr + WREC + (QM == 8 ? 16 * (g & 1) : 16 * g));
 #pragma unroll
-          for (int qb = 0; qb < NQB; ++qb) {
-            const f4 r = *reinterpret_cast<const f4*>(wr + WREC + qb * 64 + (QM == 8 ? 16 * (g & 1) : 16 * g));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[qb][j] *= r;
-          }
+          for (int j = 0; j < 8; ++j) acc[j] *= r;
         }
       }
       float sc[8];
@@ -803,9 +783,9 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
       ev[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05040100u);                                                \
       od[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);                                                \
     }                                                                                                                    \
-    _Pragma("unroll") for (int qb = 0; qb < NQB; ++qb) _Pragma("unroll") for (int z = DM::PSETS - 1; z >= 0; --z) {     \
-      acc[qb][2 * PR] = mx_mfma(wt[qb][z], ev, acc[qb][2 * PR]);                                                         \
-      acc[qb][2 * PR + 1] = mx_mfma(wt[qb][z], od, acc[qb][2 * PR + 1]);                                                 \
+    _Pragma("unroll") for (int z = DM::PSETS - 1; z >= 0; --z) {     \
+      acc[2 * PR] = mx_mfma(wt[z], ev, acc[2 * PR]);                                                         \
+      acc[2 * PR + 1] = mx_mfma(wt[z], od, acc[2 * PR + 1]);                                                 \
     }                                                                                                                    \
   } while (0)
       EP_MX_PAIR(0); EP_MX_PAIR(1); EP_MX_PAIR(2); EP_MX_PAIR(3);
@@ -837,9 +817,8 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
         const bool done = cp.next(t);                                   // that was the unit's last tile
         if constexpr (!BWD) {
           if (done) {
-            f4 r[NQB];
-#pragma unroll
-            for (int qb = 0; qb < NQB; ++qb) r[qb] = *reinterpret_cast<const f4*>(wbuf + buf * WALL + WREC + NQB * 64 + qb * 64 + (QM == 8 ? 16 * (g & 1) : 16 * g));
+            f4 r;
+            r = *reinterpret_cast<const f4*>(wbuf + buf * WALL + WREC + 64 + (QM == 8 ? 16 * (g & 1) : 16 * g));
             store_rows(p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, r, false);
             if (!OPENS) clear();
           }
@@ -849,9 +828,8 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
       }
       buf ^= 1;
       if constexpr (BWD) {
-        f4 one[NQB];
-#pragma unroll
-        for (int qb = 0; qb < NQB; ++qb) one[qb] = f4{p.scale, p.scale, p.scale, p.scale};
+        f4 one;
+        one = f4{p.scale, p.scale, p.scale, p.scale};
         store_rows(p.part + (int64_t)(p.per_unit ? unit : (int)blockIdx.x) * p.Q * t.D, one, !p.per_unit && !first);
       }
       first = false;
@@ -864,16 +842,14 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
         const int img = mx_image_uniform(t, b, len);
         if (sp * p.tps < (len + 31) >> 5) continue;
         const float f = !BWD && img < 0 ? NANF : 0.f;
-        f4 r[NQB];
-#pragma unroll
-        for (int qb = 0; qb < NQB; ++qb) r[qb] = f4{f, f, f, f};
+        f4 r;
+        r = f4{f, f, f, f};
         store_rows(BWD || p.splits > 1 ? p.part + (int64_t)u * p.Q * t.D : p.P + (int64_t)b * p.Q * t.D, r, false);
       }
     } else if (first) {                                                 // no unit of this workgroup had a token
       clear();
-      f4 r[NQB];
-#pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) r[qb] = f4{0.f, 0.f, 0.f, 0.f};
+      f4 r;
+      r = f4{0.f, 0.f, 0.f, 0.f};
       store_rows(p.part + (int64_t)blockIdx.x * p.Q * t.D, r, false);
     }
     mx_wait_vm<0>();                                                    // no load into LDS outlives its wave
@@ -881,32 +857,26 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
     __builtin_amdgcn_s_setprio(3);                                      // the pool waves wait for it at every barrier
     MxCursor cw = start;
     cw.open(t);
-    float m_run[NQB], mz[NQB], l_run[NQB], t_max[NQB], invl[NQB], dml[NQB], sg[NQB][SV];
+    float m_run, mz, l_run, t_max, invl, dml, sg[SV];
     auto load_scores = [&](const MxCursor& cu) {                        // backward: the saved scores of a tile
+      const int q = QM == 8 ? c & 7 : c;
+      const float* row = p.S + ((int64_t)cu.b * p.Q + q0) * p.lds_;
 #pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) {
-        const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-        const float* row = p.S + ((int64_t)cu.b * p.Q + q0) * p.lds_;
-#pragma unroll
-        for (int h = 0; h < SV / 4; ++h) {
-          const int n = (cu.tile << 5) + tok0 + 4 * h;
-          const f4 v = *reinterpret_cast<const f4*>(row + (unsigned)((q < qn ? q : 0) * (int)p.lds_ + (n < p.lds_ ? n : (int)p.lds_ - 4)));
-          sg[qb][4 * h] = v.x; sg[qb][4 * h + 1] = v.y; sg[qb][4 * h + 2] = v.z; sg[qb][4 * h + 3] = v.w;
-        }
+      for (int h = 0; h < SV / 4; ++h) {
+        const int n = (cu.tile << 5) + tok0 + 4 * h;
+        const f4 v = *reinterpret_cast<const f4*>(row + (unsigned)((q < qn ? q : 0) * (int)p.lds_ + (n < p.lds_ ? n : (int)p.lds_ - 4)));
+        sg[4 * h] = v.x; sg[4 * h + 1] = v.y; sg[4 * h + 2] = v.z; sg[4 * h + 3] = v.w;
       }
     };
     auto open_unit = [&](int b) {
-#pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) {
-        m_run[qb] = t_max[qb] = -INFINITY; mz[qb] = l_run[qb] = 0.f;
-        if constexpr (BWD) {
-          const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-          f4 ml = {0.f, 0.f, 0.f, 0.f};
-          if (q < qn) ml = *reinterpret_cast<const f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4);
-          mz[qb] = ml.x;
-          invl[qb] = ml.y == 0.f ? 0.f : 1.f / ml.y;
-          dml[qb] = ml.z;
-        }
+      m_run = t_max = -INFINITY; mz = l_run = 0.f;
+      if constexpr (BWD) {
+        const int q = QM == 8 ? c & 7 : c;
+        f4 ml = {0.f, 0.f, 0.f, 0.f};
+        if (q < qn) ml = *reinterpret_cast<const f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4);
+        mz = ml.x;
+        invl = ml.y == 0.f ? 0.f : 1.f / ml.y;
+        dml = ml.z;
       }
     };
     bool fresh = true;
@@ -917,131 +887,122 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
       mx_barrier();
       const int b = cw.b, u = cw.u, t0 = cw.tile << 5, len = cw.len;
       if (BWD && fresh && p.Pin) {                                      // delta from the blocks' parts
-#pragma unroll
-        for (int qb = 0; qb < NQB; ++qb) {
-          float d = 0.f;
-          for (int o = 0; o < nw; ++o) d += dbuf[((parity * nw + o) * NQB + qb) * 16 + c];
-          dml[qb] = d;
-        }
+        float d = 0.f;
+        for (int o = 0; o < nw; ++o) d += dbuf[((parity * nw + o)) * 16 + c];
+        dml = d;
         parity ^= 1;
       }
       const bool tail = t0 + 32 > len;
       char* wr = wbuf + buf * WALL;
       bool moved = false;
+      const int q = QM == 8 ? c & 7 : c;
+      float s[SV], pv[SV];
+      f4 v[2];
 #pragma unroll
-      for (int qb = 0; qb < NQB; ++qb) {
-        const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-        float s[SV], pv[SV];
-        f4 v[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) v[h] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int h = 0; h < 2; ++h) v[h] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int o = 0; o < nw; ++o) {                                  // the blocks' parts, in their order
-          const char* r = recs + (buf * nw + o) * PREC + qb * 2048 + lane * 16;
-          v[0] += *reinterpret_cast<const f4*>(r);
-          v[1] += *reinterpret_cast<const f4*>(r + 1024);
-        }
-        if constexpr (QM == 8) {                                        // columns q and q + 8 are terms of one query; a lane keeps one half
-          const bool up = (c & 8) != 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float own = up ? v[1][i] : v[0][i], oth = up ? v[0][i] : v[1][i];
-            s[i] = own + mx_ror8(oth);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < SV; ++i) s[i] = v[i / 4][i % 4];
-        }
-        if constexpr (!BWD) {
-          if (tail) {
-#pragma unroll
-            for (int i = 0; i < SV; ++i) s[i] = t0 + tok0 + i < len ? s[i] : -INFINITY;
-          }
-          if (p.S && q < qn) {
-            float* sp = p.S + ((int64_t)b * p.Q + q0 + q) * p.lds_ + t0 + tok0;
-#pragma unroll
-            for (int h = 0; h < SV / 4; ++h)
-              if (t0 + tok0 + 4 * h < t.N) *reinterpret_cast<f4*>(sp + 4 * h) = f4{s[4 * h], s[4 * h + 1], s[4 * h + 2], s[4 * h + 3]};
-          }
-          float mx = s[0];
-#pragma unroll
-          for (int i = 1; i < SV; ++i) mx = fmaxf(mx, s[i]);
-          t_max[qb] = fmaxf(t_max[qb], mx);
-          float f = 1.f;
-          if (__any(mx > m_run[qb] + MX_LAZY)) {
-            if (QM == 8) mx = fmaxf(mx, mx_ror8(mx));
-            mx = mx_over_groups_max(mx);
-            const float mn = fmaxf(m_run[qb], mx);
-            f = mn == m_run[qb] ? 1.f : __builtin_amdgcn_exp2f((m_run[qb] - mn) * MX_LOG2E);
-            m_run[qb] = mn;
-            mz[qb] = mn == -INFINITY ? 0.f : mn;
-            l_run[qb] *= f;
-            moved = !fresh;                                             // (nothing is accumulated in front of the first tile)
-          }
-          if (g == 0 && (QM != 8 || c < 8)) *reinterpret_cast<float*>(wr + WREC + qb * 64 + c * 4) = f;
-#pragma unroll
-          for (int i = 0; i < SV; ++i) { pv[i] = __builtin_amdgcn_exp2f((s[i] - mz[qb]) * MX_LOG2E); l_run[qb] += pv[i]; }
-        } else {
-#pragma unroll
-          for (int i = 0; i < SV; ++i) {
-            const float a = __builtin_amdgcn_exp2f((sg[qb][i] - mz[qb]) * MX_LOG2E) * invl[qb];
-            pv[i] = a * (s[i] - dml[qb]);
-          }
-          if (tail) {
-#pragma unroll
-            for (int i = 0; i < SV; ++i) pv[i] = t0 + tok0 + i < len ? pv[i] : 0.f;
-          }
-        }
-        // three bf16 terms, exact: the upper half of the bits, of what is left, and of what is left then
-        uint32_t H[SV / 2], M[SV / 2], L[SV / 2];
-#pragma unroll
-        for (int i = 0; i < SV / 2; ++i) {
-          const float x = pv[2 * i], y = pv[2 * i + 1];
-          const float rx = x - __uint_as_float(__float_as_uint(x) & 0xffff0000u), ry = y - __uint_as_float(__float_as_uint(y) & 0xffff0000u);
-          const float lx = rx - __uint_as_float(__float_as_uint(rx) & 0xffff0000u), ly = ry - __uint_as_float(__float_as_uint(ry) & 0xffff0000u);
-          H[i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
-          M[i] = __builtin_amdgcn_perm(__float_as_uint(ry), __float_as_uint(rx), 0x07060302u);
-          L[i] = __builtin_amdgcn_perm(__float_as_uint(ly), __float_as_uint(lx), 0x07060302u);
-        }
-        mx_u4 wt[DM::PSETS];
-        if constexpr (QM == 8) {                                        // rows 0-7: first and third term, rows 8-15: second; 8 slots = both halves
-          const bool up = (c & 8) != 0;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t r1 = mx_ror8u(up ? H[i] : M[i]), r2 = mx_ror8u(L[i]);
-            wt[0][i] = up ? r1 : H[i];
-            wt[0][2 + i] = up ? M[i] : r1;
-            wt[1][i] = up ? 0u : L[i];
-            wt[1][2 + i] = up ? 0u : r2;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { wt[0][i] = H[i]; wt[1][i] = M[i]; wt[DM::PSETS - 1][i] = L[i]; }
-        }
-#pragma unroll
-        for (int z = 0; z < DM::PSETS; ++z) *reinterpret_cast<mx_u4*>(wr + (qb * DM::PSETS + z) * 1024 + lane * 16) = wt[z];
+      for (int o = 0; o < nw; ++o) {                                  // the blocks' parts, in their order
+        const char* r = recs + (buf * nw + o) * PREC + lane * 16;
+        v[0] += *reinterpret_cast<const f4*>(r);
+        v[1] += *reinterpret_cast<const f4*>(r + 1024);
       }
+      if constexpr (QM == 8) {                                        // columns q and q + 8 are terms of one query; a lane keeps one half
+        const bool up = (c & 8) != 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float own = up ? v[1][i] : v[0][i], oth = up ? v[0][i] : v[1][i];
+          s[i] = own + mx_ror8(oth);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < SV; ++i) s[i] = v[i / 4][i % 4];
+      }
+      if constexpr (!BWD) {
+        if (tail) {
+#pragma unroll
+          for (int i = 0; i < SV; ++i) s[i] = t0 + tok0 + i < len ? s[i] : -INFINITY;
+        }
+        if (p.S && q < qn) {
+          float* sp = p.S + ((int64_t)b * p.Q + q0 + q) * p.lds_ + t0 + tok0;
+#pragma unroll
+          for (int h = 0; h < SV / 4; ++h)
+            if (t0 + tok0 + 4 * h < t.N) *reinterpret_cast<f4*>(sp + 4 * h) = f4{s[4 * h], s[4 * h + 1], s[4 * h + 2], s[4 * h + 3]};
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < SV; ++i) mx = fmaxf(mx, s[i]);
+        t_max = fmaxf(t_max, mx);
+        float f = 1.f;
+        if (__any(mx > m_run + MX_LAZY)) {
+          if (QM == 8) mx = fmaxf(mx, mx_ror8(mx));
+          mx = mx_over_groups_max(mx);
+          const float mn = fmaxf(m_run, mx);
+          f = mn == m_run ? 1.f : __builtin_amdgcn_exp2f((m_run - mn) * MX_LOG2E);
+          m_run = mn;
+          mz = mn == -INFINITY ? 0.f : mn;
+          l_run *= f;
+          moved = !fresh;                                             // (nothing is accumulated in front of the first tile)
+        }
+        if (g == 0 && (QM != 8 || c < 8)) *reinterpret_cast<float*>(wr + WREC + c * 4) = f;
+#pragma unroll
+        for (int i = 0; i < SV; ++i) { pv[i] = __builtin_amdgcn_exp2f((s[i] - mz) * MX_LOG2E); l_run += pv[i]; }
+      } else {
+#pragma unroll
+        for (int i = 0; i < SV; ++i) {
+          const float a = __builtin_amdgcn_exp2f((sg[i] - mz) * MX_LOG2E) * invl;
+          pv[i] = a * (s[i] - dml);
+        }
+        if (tail) {
+#pragma unroll
+          for (int i = 0; i < SV; ++i) pv[i] = t0 + tok0 + i < len ? pv[i] : 0.f;
+        }
+      }
+      // three bf16 terms, exact: the upper half of the bits, of what is left, and of what is left then
+      uint32_t H[SV / 2], M[SV / 2], L[SV / 2];
+#pragma unroll
+      for (int i = 0; i < SV / 2; ++i) {
+        const float x = pv[2 * i], y = pv[2 * i + 1];
+        const float rx = x - __uint_as_float(__float_as_uint(x) & 0xffff0000u), ry = y - __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+        const float lx = rx - __uint_as_float(__float_as_uint(rx) & 0xffff0000u), ly = ry - __uint_as_float(__float_as_uint(ry) & 0xffff0000u);
+        H[i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+        M[i] = __builtin_amdgcn_perm(__float_as_uint(ry), __float_as_uint(rx), 0x07060302u);
+        L[i] = __builtin_amdgcn_perm(__float_as_uint(ly), __float_as_uint(lx), 0x07060302u);
+      }
+      mx_u4 wt[DM::PSETS];
+      if constexpr (QM == 8) {                                        // rows 0-7: first and third term, rows 8-15: second; 8 slots = both halves
+        const bool up = (c & 8) != 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t r1 = mx_ror8u(up ? H[i] : M[i]), r2 = mx_ror8u(L[i]);
+          wt[0][i] = up ? r1 : H[i];
+          wt[0][2 + i] = up ? M[i] : r1;
+          wt[1][i] = up ? 0u : L[i];
+          wt[1][2 + i] = up ? 0u : r2;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { wt[0][i] = H[i]; wt[1][i] = M[i]; wt[DM::PSETS - 1][i] = L[i]; }
+      }
+#pragma unroll
+      for (int z = 0; z < DM::PSETS; ++z) *reinterpret_cast<mx_u4*>(wr + z * 1024 + lane * 16) = wt[z];
       fresh = cw.next(t);
       if constexpr (BWD) load_scores(cw);
       else {
-        if (lane == 0) *reinterpret_cast<int*>(wr + WREC + 2 * NQB * 64) = moved;
+        if (lane == 0) *reinterpret_cast<int*>(wr + WREC + 128) = moved;
         if (fresh) {                                                    // the unit is done: statistics, row factors, the scores behind its tiles
           const int spl = u - b * p.splits;
-#pragma unroll
-          for (int qb = 0; qb < NQB; ++qb) {
-            const int q = qb * 16 + (QM == 8 ? (c & 7) : c);
-            float l = l_run[qb], tm = t_max[qb];
-            if (QM == 8) { l += mx_ror8(l); tm = fmaxf(tm, mx_ror8(tm)); }
-            l = mx_over_groups_sum(l);
-            tm = mx_over_groups_max(tm);
-            const float e = __builtin_amdgcn_exp2f((mz[qb] - tm) * MX_LOG2E);               // from the running to the true maximum
-            if (g == 0 && (QM != 8 || c < 8)) {
-              if (q < qn) {
-                if (p.splits > 1) *reinterpret_cast<f2*>(p.part_ml + ((int64_t)u * p.Q + q0 + q) * 2) = f2{tm, l * e};
-                else *reinterpret_cast<f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4) = f4{tm, l * e, 0.f, 0.f};
-              }
-              *reinterpret_cast<float*>(wr + WREC + NQB * 64 + qb * 64 + c * 4) = p.splits > 1 ? e : 1.f / l;
+          const int q = QM == 8 ? c & 7 : c;
+          float l = l_run, tm = t_max;
+          if (QM == 8) { l += mx_ror8(l); tm = fmaxf(tm, mx_ror8(tm)); }
+          l = mx_over_groups_sum(l);
+          tm = mx_over_groups_max(tm);
+          const float e = __builtin_amdgcn_exp2f((mz - tm) * MX_LOG2E);               // from the running to the true maximum
+          if (g == 0 && (QM != 8 || c < 8)) {
+            if (q < qn) {
+              if (p.splits > 1) *reinterpret_cast<f2*>(p.part_ml + ((int64_t)u * p.Q + q0 + q) * 2) = f2{tm, l * e};
+              else *reinterpret_cast<f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4) = f4{tm, l * e, 0.f, 0.f};
             }
+            *reinterpret_cast<float*>(wr + WREC + 64 + c * 4) = p.splits > 1 ? e : 1.f / l;
           }
           if (p.S && spl == p.splits - 1)
             for (int q = 0; q < qn; ++q)
@@ -1164,8 +1125,8 @@ struct MxPlan {
 };
 
 static size_t mx_pipe_lds(int qm, int nw) {
-  const size_t nqb = qm == 32 ? 2 : 1, rec = 2048 * nqb, wall = nqb * (qm == 8 ? 2 : 3) * 1024 + 2 * nqb * 64 + 64;
-  return (size_t)nw * MX_PIPE_STAGES * 2176 + 2 * (size_t)nw * rec + 2 * wall + 2 * (size_t)nw * nqb * 64;
+  const size_t wall = (qm == 8 ? 2 : 3) * 1024 + 2 * 64 + 64;
+  return (size_t)nw * MX_PIPE_STAGES * 2176 + 2 * (size_t)nw * 2048 + 2 * wall + 2 * (size_t)nw * 64;
 }
 
 static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
