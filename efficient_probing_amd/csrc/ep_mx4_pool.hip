@@ -2,22 +2,25 @@
 //     S = scale q.x     A = softmax over the image's tokens     P = A x
 //     dA = dP.x         dS = A (dA - dP.P)                       dq = scale sum dS x
 //
-// ONE kernel for both passes: they are the same two contractions with a per-token weight between them.  Every byte of the cache is
-// read once per pass.  A wave owns CPW 128-channel blocks of the row for all tokens and queries (a D-slice); a tile is 32 tokens.
+// Both passes are the same two contractions with a per-token weight between them, and every byte of the cache is read once in each.  A
+// wave owns one 128-channel block of the rows (pipelined form, up to 14 blocks) or four (wide-row form) for all tokens of a tile of 32.
 //
-//   * Tiles come HBM -> LDS by LDS-DMA into a ring of NST stages that the wave keeps to itself (no barrier on the data path).
+//   * Tiles come HBM -> LDS by LDS-DMA into a ring of stages that the wave keeps to itself (no barrier on the data path).
 //   * First contraction (scores / dA), on the matrix cores in the cache's own format: v_mfma_scale_f32_16x16x128_f8f6f4 takes the
 //     E2M1 codes and their E8M0 scale bytes as they lie in LDS, no decoding.  The fp32 operand (queries, dP) becomes five E2M3
 //     terms with block scales 2^-5 apart: below 2 that type is a fixed-point grid of 1/8, so every term takes five more bits and
 //     at most 2^-24 of a block's largest value is left over.  All products are exact, the sums fp32.
-//   * D-slices are added through LDS, one record per wave and tile, in wave order, one barrier per tile; every wave then holds the
-//     scores in the very lanes in which the second contraction wants its weights.
+//   * The blocks' parts of a score are added through LDS in block order.
 //   * Weights (exp(S - max), or dS) are split into three bf16 terms, exactly.
 //   * Second contraction: codes are decoded to bf16 (exact; v_cvt_scalef32_pk_bf16_fp4 applies the token's own scale, which is why
 //     this side cannot stay in 4 bits: the contraction runs over tokens and every token has its own scale), transposed between
 //     token pairs by v_perm, v_mfma_f32_16x16x32_bf16.
 //
-// QM 8: up to 8 queries, rows of a 16-row matrix instruction = 8 queries x 2 terms.  QM 16 / 32: one / two blocks of 16 queries.
+// QM 8: up to 8 queries, rows of a 16-row matrix instruction = 8 queries x 2 terms.  QM 16: up to 16.  More: blockIdx.y.
+//
+// Bound: HBM, then decoding.  Reading 107 MB of codes takes 20 us at the rate this ring streams them, decoding and both contractions 23 us
+// of the matrix and vector units beside it (1024 x 256 x 768, 8 queries: 37 us in all forward, of them about 10 before the first tile
+// and behind the last; 2048 images: 66 us, 3.2 TB/s).
 #include "ep_mx4.h"
 #include "ep_mx4_pool.h"
 
@@ -173,7 +176,9 @@ struct MxCursor {
 // Rows of more than 14 blocks.  A wave owns four blocks of the row for all tokens and up to 8 queries; `groups` such sets of waves share
 // a workgroup and take turns at the tiles (forward: of one image; backward: a group per image).  Every wave makes the weights itself,
 // in the very lanes in which its second contraction wants them.  Accumulators and operand rows of four blocks fill 192 of 256 registers:
-// lane constants are made again where they are used, since a register reloaded from scratch waits for the tiles in flight.
+// lane constants are made again where they are used, since a register reloaded from scratch waits for the tiles in flight.  Bound:
+// matrix and vector units with two waves a SIMD (256 x 784 x 4096, 4 queries: 131 us forward, 3.3 TB/s), and about 25 us for the operand
+// rows, the first tile and the way out (128 x 196 x 4096: 36 us and 8 us to join two runs an image).
 template <bool BWD, bool OPENS>
 __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
   constexpr int QM = 8, CPW = 4, NST = MX_STAGES, REC = 1024;          // REC: bytes of an exchange record, the lane's four scores
@@ -591,7 +596,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
 //     pool waves   first contraction of tile j -> record j | barrier j | second contraction of tile j - 1, refill its stage
 //     weight wave                                          | barrier j | sums the records of tile j, softmax (or dS), weights j
 // so that the long chain exchange -> maximum -> exponentials -> split runs beside the contractions of other tiles, once per tile
-// instead of once per wave, and the pool waves' registers (accumulators and operand of one block) leave room for 3 - 4 waves a SIMD.
+// instead of once per wave, and the pool waves' registers (accumulators and operand of one block) leave room for 4 waves a SIMD.
 // OPENS: the operand rows change with the image (backward, per-image queries); else they are made once.
 template <int QM, bool BWD, bool OPENS>
 __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
@@ -1134,7 +1139,9 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   const int nc = mx_blocks(D), cus = cu_count(), tiles = (N + 31) / 32;
   constexpr int LDS = 160 * 1024;
   int cap;                                                              // workgroups that run at the same time
-  if (nc <= 14) {                                                       // a wave per block and the weight wave: what 160 KiB of LDS hold
+  if (nc <= 14) {                                                       // a wave per block and the weight wave: what 160 KiB of LDS hold.
+    // (512 x 256 x 1792, 8 queries: 42 us forward and 61 backward; wide-row form 55 and 69.  Narrower rows gain more.)  More than 8
+    // queries: blocks of 16 (512 x 256 x 768: 16 queries 30 us forward, as two blocks of 8 43; 8 queries as a block of 16 27, of 8 25.5)
     p.qm = Q <= 8 ? 8 : 16;
     p.nw = nc; p.cpw = 1; p.groups = 1;
     constexpr int waves = 16;                                           // four a SIMD
@@ -1153,8 +1160,10 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   }
   p.yblk = (Q + p.qm - 1) / p.qm;
   p.qblk = (Q + p.yblk - 1) / p.yblk;
-  // few images: their token axis is cut into runs.  Forward the runs have to be joined by a second launch, so they are kept longer.
-  const int per = p.pipe ? 1 : p.groups, least = bwd ? 2 : (p.pipe ? 8 : 2 * per);
+  // few images: their token axis is cut into runs of at least `least` tiles.  Forward the runs have to be joined by a second launch, so
+  // they are kept longer (64 x 257 x 768, 8 queries: 8 tiles 17 us, 4 22 us); backward every run opens its operand rows (128 x 196 x
+  // 768: 4 tiles 19 us, 2 25 us), which wide rows still gain from (128 x 196 x 4096: 2 tiles 44 us, 4 54 us)
+  const int per = p.pipe ? 1 : p.groups, least = p.pipe ? (bwd ? 4 : 8) : (bwd ? 2 : 2 * per);
   p.splits = B < cap * (bwd ? per : 1) ? (cap * (bwd ? per : 1)) / B : 1;
   if (p.splits > tiles / least) p.splits = tiles / least;
   if (p.splits < 1) p.splits = 1;
@@ -1227,6 +1236,7 @@ int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bst
   p.lds_ = s_stride;
   EP_TRY(mx_launch<false>(p, pl, st));
   if (pl.splits > 1) {
+    // few runs: one chain (128 x 196 x 4096, two runs: 45 us in all, sixteen chains 74); many: sixteen (2 x 50001 x 1024: 34 us, one 86)
     if (pl.splits <= 4)
       hipLaunchKernelGGL(ep_mx4_join_kernel<1>, dim3((unsigned)t->B * Q, (unsigned)((t->D + 1023) / 1024)), dim3(256), 0, st, p.part, p.part_ml, pl.splits, Q, t->D, P, ML);
     else
@@ -1283,7 +1293,7 @@ static int mx_pool_check(const ep_mx4_tokens* t, int Q, void* ws, size_t bytes, 
   EP_TRY(mx4_check(t, what));
   EP_REQUIRE(Q > 0, EP_E_ARG, "%s: Q = %d", what, Q);
   EP_REQUIRE(t->D <= MX_MAX_D, EP_E_SHAPE, "%s: D = %d > %d", what, t->D, MX_MAX_D);
-  EP_REQUIRE((int64_t)t->B * Q <= 2147483647, EP_E_SHAPE, "%s: %d x %d rows in one call", what, t->B, Q);
+  EP_REQUIRE((int64_t)t->B * Q <= 1 << 30, EP_E_SHAPE, "%s: %d x %d rows in one call", what, t->B, Q);
   const size_t need = ep_mx4_pool_workspace_bytes(t->B, t->N, t->D, Q);
   EP_REQUIRE(bytes >= need, EP_E_WORKSPACE, "%s: workspace %zu < %zu", what, bytes, need);
   EP_REQUIRE(!need || (ws && aligned16(ws)), EP_E_ARG, "%s: the workspace must be given and 16-byte aligned", what);
