@@ -19,6 +19,7 @@ namespace ep {
 constexpr int DIST_MAX_K = 1024;
 constexpr int DIST_MAX_C = 1 << 20;               // (256 pieces, one for each thread that joins them)
 constexpr int DIST_PIECE = 4096;                  // classes of a workgroup where a row is cut
+constexpr int DIST_SLICE = 1 << 22;               // workgroups of a launch (HIP takes less than 2^32 threads)
 constexpr float DIST_LOW = 1e-30f;                // a sum of exponentials below this has lost bits
 constexpr float DIST_LOG2E = 1.4426950408889634f;
 
@@ -358,12 +359,12 @@ __device__ __forceinline__ void dist_stores_done() { asm volatile("s_waitcnt vmc
 
 // ---- a row in the registers of TH threads ---------------------------------------------------------------------------------
 template <int DT, int TH, int NV, bool LABEL>
-__global__ __launch_bounds__(TH < 256 ? 256 : TH, TH == 256 ? 8 : NV * DistElem<DT>::VEC > 32 && DT == 0 ? 4 : 6) void ep_distill_rows_kernel(ep_distill_args a, int row_lds) {
+__global__ __launch_bounds__(TH < 256 ? 256 : TH, TH == 256 ? 8 : NV * DistElem<DT>::VEC > 32 && DT == 0 ? 4 : 6) void ep_distill_rows_kernel(ep_distill_args a, int row0, int row_lds) {
   extern __shared__ __align__(16) char dyn[];
   typedef typename DistElem<DT>::T T;
   constexpr int RPW = TH < 256 ? 256 / TH : 1;                          // rows of a workgroup
   const int sub = TH < 256 ? (int)threadIdx.x / TH : 0, tid = (int)threadIdx.x - sub * TH;
-  const int b = (int)blockIdx.x * RPW + sub;
+  const int b = row0 + (int)blockIdx.x * RPW + sub;
   if (b >= a.B) return;                                                 // (a whole wave: nothing below waits for it)
   char* mine = dyn + sub * row_lds;
   float* red = reinterpret_cast<float*>(mine);                          // 48 floats
@@ -397,13 +398,13 @@ __global__ __launch_bounds__(TH < 256 ? 256 : TH, TH == 256 ? 8 : NV * DistElem<
 struct DistPart { float m, s0, s2, mo, s1; };     // a piece's maximum and sums; the sum over its unlisted classes is relative to mo
 
 template <int DT, bool LABEL>
-__global__ __launch_bounds__(256) void ep_distill_part_kernel(ep_distill_args a, int pieces, DistPart* __restrict__ part) {
+__global__ __launch_bounds__(256) void ep_distill_part_kernel(ep_distill_args a, int row0, int pieces, DistPart* __restrict__ part) {
   extern __shared__ __align__(16) char dyn[];
   typedef typename DistElem<DT>::T T;
   constexpr int NV = DIST_PIECE / 256 / DistElem<DT>::VEC;
   float* red = reinterpret_cast<float*>(dyn);
   uint32_t* bits = reinterpret_cast<uint32_t*>(dyn + 256);
-  const int b = (int)(blockIdx.x / (unsigned)pieces), pc = (int)(blockIdx.x % (unsigned)pieces), tid = (int)threadIdx.x;
+  const int b = row0 + (int)(blockIdx.x / (unsigned)pieces), pc = (int)(blockIdx.x % (unsigned)pieces), tid = (int)threadIdx.x;
   const int lo = pc * DIST_PIECE, n = a.C - lo < DIST_PIECE ? a.C - lo : DIST_PIECE;
   const T* z = static_cast<const T*>(a.logits) + (int64_t)b * a.ldl + lo;
   DistRun<DT, 256, NV> run;
@@ -425,18 +426,18 @@ __global__ __launch_bounds__(256) void ep_distill_part_kernel(ep_distill_args a,
   dist_sums<256, 3>(s, red);
   float mo = m == -INFINITY ? 0.f : m;
   if (a.teacher_tail && s[1] < DIST_LOW) dist_run_others(run, tid, DIST_LOG2E / a.temperature, bits, red, mo, s[1]);
-  if (tid == 0) part[blockIdx.x] = DistPart{m, s[0], s[2], mo, s[1]};
+  if (tid == 0) part[(int64_t)b * pieces + pc] = DistPart{m, s[0], s[2], mo, s[1]};
 }
 
 template <int DT, bool LABEL>
-__global__ __launch_bounds__(256) void ep_distill_join_kernel(ep_distill_args a, int pieces, const DistPart* __restrict__ part) {
+__global__ __launch_bounds__(256) void ep_distill_join_kernel(ep_distill_args a, int row0, int pieces, const DistPart* __restrict__ part) {
   extern __shared__ __align__(16) char dyn[];
   typedef typename DistElem<DT>::T T;
   constexpr int NV = DIST_PIECE / 256 / DistElem<DT>::VEC;
   float* red = reinterpret_cast<float*>(dyn);
   int* flag = reinterpret_cast<int*>(dyn + 192);
   const DistEntries e = dist_entries(reinterpret_cast<int*>(dyn + 256), a.K);
-  const int b = (int)blockIdx.x, pc = (int)blockIdx.y, tid = (int)threadIdx.x;
+  const int b = row0 + (int)blockIdx.x, pc = (int)blockIdx.y, tid = (int)threadIdx.x;
   const int lo = pc * DIST_PIECE, n = a.C - lo < DIST_PIECE ? a.C - lo : DIST_PIECE;
   const T* row = static_cast<const T*>(a.logits) + (int64_t)b * a.ldl;
   DistRun<DT, 256, NV> run;
@@ -480,7 +481,11 @@ static int dist_launch(const ep_distill_args& a, void* ws, hipStream_t st) {
 #define EP_DIST_ROWS(TH, NV)                                                                                              \
   do {                                                                                                                    \
     constexpr int rpw = TH < 256 ? 256 / TH : 1;                                                                          \
-    hipLaunchKernelGGL((ep_distill_rows_kernel<DT, TH, NV, LABEL>), dim3((a.B + rpw - 1) / rpw), dim3(TH < 256 ? 256 : TH), rpw * lds, st, a, (int)lds); \
+    for (int64_t row = 0; row < a.B; row += (int64_t)rpw * DIST_SLICE) {                                                  \
+      const int64_t n = a.B - row < (int64_t)rpw * DIST_SLICE ? a.B - row : (int64_t)rpw * DIST_SLICE;                    \
+      hipLaunchKernelGGL((ep_distill_rows_kernel<DT, TH, NV, LABEL>), dim3((unsigned)((n + rpw - 1) / rpw)), dim3(TH < 256 ? 256 : TH), rpw * lds, st, a, \
+                         (int)row, (int)lds);                                                                             \
+    }                                                                                                                     \
   } while (0)
     if (th == 64) EP_DIST_ROWS(64, 16 / VEC);
     else if (th == 256) EP_DIST_ROWS(256, 16 / VEC);
@@ -490,12 +495,16 @@ static int dist_launch(const ep_distill_args& a, void* ws, hipStream_t st) {
     EP_LAUNCH_CHECK("ep_distill_rows_kernel");
     return 0;
   }
-  const int pieces = dist_pieces(a.C);
-  EP_REQUIRE((int64_t)a.B * pieces <= 2147483647, EP_E_SHAPE, "ep_distill_topk: %d rows of %d classes in one call", a.B, a.C);
-  hipLaunchKernelGGL((ep_distill_part_kernel<DT, LABEL>), dim3((unsigned)a.B * pieces), dim3(256), 256 + DIST_PIECE / 8, st, a, pieces, static_cast<DistPart*>(ws));
-  EP_LAUNCH_CHECK("ep_distill_part_kernel");
-  hipLaunchKernelGGL((ep_distill_join_kernel<DT, LABEL>), dim3(a.B, a.dlogits ? pieces : 1), dim3(256), 256 + (size_t)dist_quads(a.K) * 48, st, a, pieces, static_cast<const DistPart*>(ws));
-  EP_LAUNCH_CHECK("ep_distill_join_kernel");
+  const int pieces = dist_pieces(a.C), most = DIST_SLICE / pieces;
+  for (int64_t row = 0; row < a.B; row += most) {
+    const int n = a.B - row < most ? (int)(a.B - row) : most;
+    hipLaunchKernelGGL((ep_distill_part_kernel<DT, LABEL>), dim3((unsigned)(n * pieces)), dim3(256), 256 + DIST_PIECE / 8, st, a, (int)row, pieces,
+                       static_cast<DistPart*>(ws));
+    EP_LAUNCH_CHECK("ep_distill_part_kernel");
+    hipLaunchKernelGGL((ep_distill_join_kernel<DT, LABEL>), dim3((unsigned)n, a.dlogits ? pieces : 1), dim3(256), 256 + (size_t)dist_quads(a.K) * 48, st, a, (int)row,
+                       pieces, static_cast<const DistPart*>(ws));
+    EP_LAUNCH_CHECK("ep_distill_join_kernel");
+  }
   return 0;
 }
 

@@ -50,10 +50,10 @@ __device__ __forceinline__ int mx_exponent(float amax) {
 
 // one lane per eight channels; grid.x over B * N * Dp / 8
 template <int DT, bool VEC>
-__global__ __launch_bounds__(256) void ep_mx4_quantize_kernel(const typename MxElem<DT>::T* __restrict__ x, int64_t xb, int64_t xt, int64_t total,
+__global__ __launch_bounds__(256) void ep_mx4_quantize_kernel(const typename MxElem<DT>::T* __restrict__ x, int64_t xb, int64_t xt, int64_t first, int64_t total,
                                                               int N, int D, int words, uint8_t* __restrict__ codes,
                                                               uint8_t* __restrict__ scales, int64_t cb, int64_t sb) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t id = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
   const bool in = id < total;
   const int64_t row = in ? id / words : 0;
   const int j = in ? (int)(id - row * words) : 0;
@@ -96,8 +96,8 @@ __device__ __forceinline__ uint32_t mx_out_pair(uint32_t bf2) {      // two bf16
 
 // one lane per eight channels of the output; VEC: D % 8 == 0
 template <int DT, bool VEC>
-__global__ __launch_bounds__(256) void ep_mx4_dequantize_kernel(ep_mx4_tokens t, int64_t total, int words, int words_out, typename MxElem<DT>::T* __restrict__ out) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void ep_mx4_dequantize_kernel(ep_mx4_tokens t, int64_t first, int64_t total, int words, int words_out, typename MxElem<DT>::T* __restrict__ out) {
+  const int64_t id = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= total) return;
   const int64_t row = id / words_out;
   const int j = (int)(id - row * words_out);
@@ -132,9 +132,12 @@ __global__ __launch_bounds__(256) void ep_mx4_dequantize_kernel(ep_mx4_tokens t,
   }
 }
 
+constexpr int64_t MX_SLICE = 1 << 30;            // threads of a launch (HIP takes less than 2^32)
+static unsigned mx_slice(int64_t first, int64_t total) { return (unsigned)(((total - first < MX_SLICE ? total - first : MX_SLICE) + 255) / 256); }
+
 int mx4_check(const ep_mx4_tokens* t, const char* what) {
   EP_REQUIRE(t && t->codes && t->scales, EP_E_ARG, "%s: null pointer", what);
-  EP_REQUIRE(t->B > 0 && t->N > 0 && t->D > 0 && t->M > 0 && t->M <= 2147483647, EP_E_ARG, "%s: B %d, N %d, D %d, M %lld must be positive", what, t->B, t->N,
+  EP_REQUIRE(t->B > 0 && t->N > 0 && t->D > 0 && t->M > 0 && t->M <= 2147483647 && t->N <= 1 << 30, EP_E_ARG, "%s: B %d, N %d, D %d, M %lld must be positive", what, t->B, t->N,
              t->D, (long long)t->M);
   EP_REQUIRE(t->image_index || t->B <= t->M, EP_E_ARG, "%s: a batch of %d images from a cache of %lld needs an image_index", what, t->B, (long long)t->M);
   const int64_t nb = mx_blocks(t->D);
@@ -160,19 +163,20 @@ int ep_mx4_quantize(const void* x, int x_dtype, int64_t x_bstride, int64_t x_tst
   EP_REQUIRE(x_dtype >= EP_DTYPE_F32 && x_dtype <= EP_DTYPE_F16, EP_E_UNSUPPORTED, "ep_mx4_quantize: dtype %d", x_dtype);
   EP_REQUIRE((N == 1 || x_tstride >= 0) && (B == 1 || x_bstride >= 0), EP_E_ARG, "ep_mx4_quantize: negative stride");
   const int words = mx_blocks(D) * 16;
-  const int64_t total = (int64_t)B * N * words, grid = (total + 255) / 256;
-  EP_REQUIRE(grid <= 2147483647, EP_E_SHAPE, "ep_mx4_quantize: %d x %d x %d tokens in one call", B, N, D);
+  const int64_t total = (int64_t)B * N * words;
   const int per16 = x_dtype == EP_DTYPE_F32 ? 4 : 8;
   const bool vec = D % 8 == 0 && aligned16(x) && (B == 1 || x_bstride % per16 == 0) && (N == 1 || x_tstride % per16 == 0);
   hipStream_t st = (hipStream_t)stream;
 #define EP_MXQ(DT, V)                                                                                                                    \
-  hipLaunchKernelGGL((ep_mx4_quantize_kernel<DT, V>), dim3((unsigned)grid), dim3(256), 0, st, (const MxElem<DT>::T*)x, x_bstride, x_tstride, total, \
-                     N, D, words, codes, scales, codes_bstride, scales_bstride)
-  if (x_dtype == EP_DTYPE_F32) { if (vec) EP_MXQ(0, true); else EP_MXQ(0, false); }
-  else if (x_dtype == EP_DTYPE_BF16) { if (vec) EP_MXQ(1, true); else EP_MXQ(1, false); }
-  else { if (vec) EP_MXQ(2, true); else EP_MXQ(2, false); }
+  hipLaunchKernelGGL((ep_mx4_quantize_kernel<DT, V>), dim3(mx_slice(first, total)), dim3(256), 0, st, (const MxElem<DT>::T*)x, x_bstride, x_tstride, first, \
+                     total, N, D, words, codes, scales, codes_bstride, scales_bstride)
+  for (int64_t first = 0; first < total; first += MX_SLICE) {
+    if (x_dtype == EP_DTYPE_F32) { if (vec) EP_MXQ(0, true); else EP_MXQ(0, false); }
+    else if (x_dtype == EP_DTYPE_BF16) { if (vec) EP_MXQ(1, true); else EP_MXQ(1, false); }
+    else { if (vec) EP_MXQ(2, true); else EP_MXQ(2, false); }
 #undef EP_MXQ
-  EP_LAUNCH_CHECK("ep_mx4_quantize_kernel");
+    EP_LAUNCH_CHECK("ep_mx4_quantize_kernel");
+  }
   return 0;
 }
 
@@ -182,17 +186,18 @@ int ep_mx4_dequantize(const ep_mx4_tokens* t, void* out, int out_dtype, ep_strea
   EP_REQUIRE(aligned16(out), EP_E_ALIGN, "ep_mx4_dequantize: out must be 16-byte aligned");
   EP_REQUIRE(out_dtype >= EP_DTYPE_F32 && out_dtype <= EP_DTYPE_F16, EP_E_UNSUPPORTED, "ep_mx4_dequantize: dtype %d", out_dtype);
   const int words = mx_blocks(t->D) * 16, words_out = (t->D + 7) / 8;
-  const int64_t total = (int64_t)t->B * t->N * words_out, grid = (total + 255) / 256;
-  EP_REQUIRE(grid <= 2147483647, EP_E_SHAPE, "ep_mx4_dequantize: %d x %d x %d tokens in one call", t->B, t->N, t->D);
+  const int64_t total = (int64_t)t->B * t->N * words_out;
   const bool vec = t->D % 8 == 0;
   hipStream_t st = (hipStream_t)stream;
 #define EP_MXD(DT, V) \
-  hipLaunchKernelGGL((ep_mx4_dequantize_kernel<DT, V>), dim3((unsigned)grid), dim3(256), 0, st, *t, total, words, words_out, (MxElem<DT>::T*)out)
-  if (out_dtype == EP_DTYPE_F32) { if (vec) EP_MXD(0, true); else EP_MXD(0, false); }
-  else if (out_dtype == EP_DTYPE_BF16) { if (vec) EP_MXD(1, true); else EP_MXD(1, false); }
-  else { if (vec) EP_MXD(2, true); else EP_MXD(2, false); }
+  hipLaunchKernelGGL((ep_mx4_dequantize_kernel<DT, V>), dim3(mx_slice(first, total)), dim3(256), 0, st, *t, first, total, words, words_out, (MxElem<DT>::T*)out)
+  for (int64_t first = 0; first < total; first += MX_SLICE) {
+    if (out_dtype == EP_DTYPE_F32) { if (vec) EP_MXD(0, true); else EP_MXD(0, false); }
+    else if (out_dtype == EP_DTYPE_BF16) { if (vec) EP_MXD(1, true); else EP_MXD(1, false); }
+    else { if (vec) EP_MXD(2, true); else EP_MXD(2, false); }
 #undef EP_MXD
-  EP_LAUNCH_CHECK("ep_mx4_dequantize_kernel");
+    EP_LAUNCH_CHECK("ep_mx4_dequantize_kernel");
+  }
   return 0;
 }
 

@@ -1116,11 +1116,11 @@ __global__ __launch_bounds__(256) void ep_mx4_sum_kernel(const float* __restrict
 
 // rows of D channels -> rows of whole 128-channel blocks, zero-filled
 __global__ __launch_bounds__(256) void ep_mx4_pad_rows_kernel(const float* __restrict__ src, int64_t rows, int D, int Dp, float* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * Dp) return;
-  const int64_t r = i / Dp;
-  const int d = (int)(i - r * Dp);
-  out[i] = d < D ? src[r * D + d] : 0.f;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * Dp; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / Dp;
+    const int d = (int)(i - r * Dp);
+    out[i] = d < D ? src[r * D + d] : 0.f;
+  }
 }
 
 struct MxPlan {
@@ -1166,7 +1166,7 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   const int per = p.pipe ? 1 : p.groups, least = p.pipe ? (bwd ? 4 : 8) : (bwd ? 2 : 2 * per);
   p.splits = B < cap * (bwd ? per : 1) ? (cap * (bwd ? per : 1)) / B : 1;
   if (p.splits > tiles / least) p.splits = tiles / least;
-  if (p.splits < 1) p.splits = 1;
+  if (p.splits < 1 || (int64_t)B * Q > 1 << 22) p.splits = 1;            // (the joining launch has a workgroup per row)
   p.tps = (tiles + p.splits - 1) / p.splits;
   p.splits = (tiles + p.tps - 1) / p.tps;
   p.units = B * p.splits;
@@ -1191,8 +1191,7 @@ static int mx_rows(const float* src, int64_t rows, int D, char*& ws, const float
   if (D % MX_BLOCK == 0) return 0;
   const int Dp = mx_blocks(D) * MX_BLOCK;
   const int64_t grid = (rows * Dp + 255) / 256;
-  EP_REQUIRE(grid <= 2147483647, EP_E_SHAPE, "MX4 attention: %lld rows of %d channels in one call", (long long)rows, D);
-  hipLaunchKernelGGL(ep_mx4_pad_rows_kernel, dim3((unsigned)grid), dim3(256), 0, st, src, rows, D, Dp, reinterpret_cast<float*>(ws));
+  hipLaunchKernelGGL(ep_mx4_pad_rows_kernel, dim3((unsigned)(grid < 1 << 20 ? grid : 1 << 20)), dim3(256), 0, st, src, rows, D, Dp, reinterpret_cast<float*>(ws));
   EP_LAUNCH_CHECK("ep_mx4_pad_rows_kernel");
   *out = reinterpret_cast<float*>(ws);
   ws += (size_t)rows * Dp * 4;
@@ -1293,6 +1292,7 @@ static int mx_pool_check(const ep_mx4_tokens* t, int Q, void* ws, size_t bytes, 
   EP_TRY(mx4_check(t, what));
   EP_REQUIRE(Q > 0, EP_E_ARG, "%s: Q = %d", what, Q);
   EP_REQUIRE(t->D <= MX_MAX_D, EP_E_SHAPE, "%s: D = %d > %d", what, t->D, MX_MAX_D);
+  EP_REQUIRE(Q <= 65535 * 8 && (int64_t)Q * t->D < 1 << 28, EP_E_SHAPE, "%s: %d queries of %d channels in one call", what, Q, t->D);
   EP_REQUIRE((int64_t)t->B * Q <= 1 << 30, EP_E_SHAPE, "%s: %d x %d rows in one call", what, t->B, Q);
   const size_t need = ep_mx4_pool_workspace_bytes(t->B, t->N, t->D, Q);
   EP_REQUIRE(bytes >= need, EP_E_WORKSPACE, "%s: workspace %zu < %zu", what, bytes, need);

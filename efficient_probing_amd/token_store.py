@@ -71,15 +71,15 @@ class TokenStoreWriter:
         if n == 0:
             return
         more = {}
+        host = lambda t, dt: np.ascontiguousarray(t.detach().cpu() if isinstance(t, torch.Tensor) else t, dtype=dt)
         if self.dtype == "mxfp4":
-            x = torch.as_tensor(tokens)
+            x = torch.as_tensor(tokens).detach()
             cache = mx4.quantize_tokens(x if x.is_cuda else x.to("cuda"))
             tokens, more["scales"] = cache.codes.cpu().numpy(), cache.scales.cpu().numpy()
         else:
-            tokens = np.ascontiguousarray(tokens.cpu() if isinstance(tokens, torch.Tensor) else tokens, dtype=np.float32)
+            tokens = host(tokens, np.float32)
             if lengths is not None:
                 raise ValueError("images of fewer tokens are for mxfp4 stores")
-        host = lambda t, dt: np.ascontiguousarray(t.cpu() if isinstance(t, torch.Tensor) else t, dtype=dt)
         if lengths is not None:
             more["lengths"] = host(lengths, np.int32)
             if more["lengths"].shape != (n,) or more["lengths"].min() < 0 or more["lengths"].max() > self.N:

@@ -241,3 +241,16 @@ def test_others_far_below_the_list(C, gap, dtype):
     tail[3] = -np.inf
     z[3] = torch.where(torch.zeros(C, dtype=torch.bool).scatter(0, torch.as_tensor(idx[3], dtype=torch.long), True), z[3], torch.tensor(-np.inf))
     _check(z.to(dtype).to(DEV), val, idx, tgt, tail, alpha=0.5)
+
+
+def test_more_rows_than_a_launch():
+    from efficient_probing_amd import distill
+    B, R = 4 * 2 ** 22 + 5, 7
+    z = torch.randn(R, 2, generator=torch.Generator().manual_seed(0)).to(DEV)
+    val, idx = torch.tensor([[1.0], [2.0], [0.5], [-1.0], [0.0], [3.0], [1.5]], device=DEV), torch.tensor([0, 1, 0, 1, -1, 0, 1], device=DEV, dtype=torch.int32)[:, None]
+    rows = (torch.arange(B, device=DEV) % R).to(torch.int32)
+    small, g = distill.topk_distillation(z, val, idx)
+    loss, grad = distill.topk_distillation(z.repeat(B // R + 1, 1)[:B], val, idx, teacher_rows=rows, grad_scale=float(B) / R)
+    assert torch.equal(loss, small.repeat(B // R + 1)[:B])
+    want = g.repeat(B // R + 1, 1)[:B]
+    assert ((grad - want).abs() <= 4 * U * want.abs()).all()

@@ -356,3 +356,19 @@ def test_wide_rows_are_refused_by_the_attention():
     c = mx4.quantize_tokens(torch.randn(1, 2, 4104, device=DEV))
     with pytest.raises(ValueError, match="4096"):
         mx4.pool_forward(c, torch.zeros(1, 4104, device=DEV), 1.0)
+
+
+def test_calls_larger_than_a_launch():
+    """More than 2^30 pieces of eight channels in one call (images of one broadcast tensor; a cache read through an index)."""
+    from efficient_probing_amd import mx4
+    B, N, D = 530000, 4, 4096
+    x = _tokens(1, N, D, 3)
+    codes, scales = (torch.from_numpy(a).to(DEV) for a in O.quantize(x.numpy()))
+    c = mx4.quantize_tokens(x.to(torch.float32).to(DEV).expand(B, N, D))
+    for lo in (0, 2 ** 30 // (N * 512) - 1, B - 2):
+        assert bool((c.codes[lo:lo + 2] == codes).all()) and bool((c.scales[lo:lo + 2] == scales).all())
+    del c
+    back = mx4.dequantize_tokens(mx4.Mx4Tokens(codes, scales, D), torch.bfloat16, torch.zeros(B, dtype=torch.int32, device=DEV))
+    want = mx4.dequantize_tokens(mx4.Mx4Tokens(codes, scales, D), torch.bfloat16)
+    for lo in (0, 2 ** 30 // (N * 512) - 1, B - 2):
+        assert bool((back[lo:lo + 2] == want).all())
