@@ -372,3 +372,22 @@ def test_calls_larger_than_a_launch():
     want = mx4.dequantize_tokens(mx4.Mx4Tokens(codes, scales, D), torch.bfloat16)
     for lo in (0, 2 ** 30 // (N * 512) - 1, B - 2):
         assert bool((back[lo:lo + 2] == want).all())
+
+
+@pytest.mark.parametrize("D,Q", [(1152, 12), (2048, 5)])
+def test_captured_with_large_shared_memory(D, Q):
+    from efficient_probing_amd import mx4
+    c, x = _cache(3, 70, D, D)
+    q, dP = torch.randn(Q, D, device=DEV), torch.randn(3, Q, D, device=DEV)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        P, S, ML = mx4.pool_forward(c, q, 0.05)
+        dq = mx4.pool_backward(c, S, ML, dP, 0.05, P=P)
+    for _ in range(3):
+        q.normal_()
+        Pe, Se, MLe = mx4.pool_forward(c, q, 0.05)
+        de = mx4.pool_backward(c, Se, MLe, dP, 0.05, P=Pe)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(P, Pe) and torch.equal(S, Se) and torch.equal(dq, de)
