@@ -1059,16 +1059,20 @@ __global__ __launch_bounds__(256) void ep_mx4_join_kernel(const float* __restric
   if (threadIdx.x == 0 && blockIdx.y == 0) *reinterpret_cast<f4*>(ML + ((int64_t)b * Q + q) * 4) = f4{l == 0.f ? 0.f : m, l, 0.f, 0.f};
   const int x = (int)threadIdx.x % LN, y = (int)threadIdx.x / LN, d = ((int)blockIdx.y * LN + x) * 4;
   f4 a = {0.f, 0.f, 0.f, 0.f};
+  // (a run without tokens has sum 0 and rows of zeros; nothing here waits for a comparison, so that several rows are on their way)
+#pragma unroll 4
   for (int s = y; s < splits; s += CH) {
-    if (e[(int64_t)s * 2 * Q + 1] == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f((e[(int64_t)s * 2 * Q] - m) * MX_LOG2E);
+    const f2 st = *reinterpret_cast<const f2*>(e + (int64_t)s * 2 * Q);
+    const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f((st.x - m) * MX_LOG2E);
     const float* row = part + (((int64_t)b * splits + s) * Q + q) * D + d;
-    if (D % 4 == 0) { if (d < D) a += f * *reinterpret_cast<const f4*>(row); }
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+    if (D % 4 == 0) { if (d < D) v = *reinterpret_cast<const f4*>(row); }
     else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (d + j < D) a[j] += f * row[j];
+        if (d + j < D) v[j] = row[j];
     }
+    a += f * v;
   }
   red[y][x] = a;
   __syncthreads();
