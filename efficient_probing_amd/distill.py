@@ -34,6 +34,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
 
 
+def _int32(t: torch.Tensor, most: int) -> torch.Tensor:
+    """Indices as the kernels read them: a 64-bit one beyond int32 stays out of range instead of wrapping into it."""
+    return t if t.dtype == torch.int32 else t.to(torch.int64).clamp(-1, most).to(torch.int32)
+
+
 def _call(lg, val, idx, tail, rows, tgt, temperature, alpha, grad_scale, grad_scale_dev, grad) -> torch.Tensor:
     B, C_ = lg.shape
     R, K = val.shape
@@ -86,10 +91,7 @@ def _checked(logits, teacher_values, teacher_index, targets, teacher_tail, teach
             raise ValueError(f"{name} is on {t.device}, the logits on {dev}")
     lg = _rows(logits)
     val = _rows(teacher_values if teacher_values.dtype == torch.float32 else teacher_values.float())
-    idx = teacher_index
-    if idx.dtype != torch.int32:
-        idx = idx.to(torch.int64).clamp(-1, MAX_CLASSES).to(torch.int32)   # (a 64-bit class beyond int32 stays out of range)
-    idx = _rows(idx)
+    idx = _rows(_int32(teacher_index, MAX_CLASSES))
     tail = None if teacher_tail is None else teacher_tail.float().contiguous()
     tgt = None if targets is None else targets.to(torch.int64).contiguous()
     return lg, val, idx, tail, teacher_rows, tgt, float(temperature), float(alpha)
@@ -170,7 +172,9 @@ class TopKDistillation(torch.nn.Module):
         if teacher_tail is not None and tuple(teacher_tail.shape) != (teacher_values.shape[0],):
             raise ValueError(f"teacher_tail must be ({teacher_values.shape[0]},), got {tuple(teacher_tail.shape)}")
         self.register_buffer("teacher_values", teacher_values.float(), persistent=False)
-        self.register_buffer("teacher_index", teacher_index.to(torch.int32), persistent=False)
+        if teacher_index.dtype.is_floating_point or teacher_index.dtype == torch.bool:
+            raise ValueError(f"teacher_index must hold integers, got {teacher_index.dtype}")
+        self.register_buffer("teacher_index", _int32(teacher_index, MAX_CLASSES), persistent=False)
         self.register_buffer("teacher_tail", None if teacher_tail is None else teacher_tail.float(), persistent=False)
 
     @classmethod
@@ -189,7 +193,7 @@ class TopKDistillation(torch.nn.Module):
         if image_index is None and batch != self.teacher_values.shape[0]:
             raise ValueError(f"a batch of {batch} against a table of {self.teacher_values.shape[0]} teacher rows needs image_index "
                              "(batches of a token_store.ResidentTokenStore carry it)")
-        return None if image_index is None else image_index.to(torch.int32).contiguous()
+        return None if image_index is None else _int32(image_index, 2 ** 31 - 1).contiguous()
 
     def forward(self, logits: torch.Tensor, targets: Optional[torch.Tensor] = None, image_index: Optional[torch.Tensor] = None) -> torch.Tensor:
         return distillation_loss(logits, self.teacher_values, self.teacher_index, targets if self.alpha < 1.0 else None, teacher_tail=self.teacher_tail,

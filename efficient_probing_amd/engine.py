@@ -66,7 +66,7 @@ class ProbeHeadEngine:
     def _bind_store_tables(self, xv, image_index) -> None:
         self._bound_tables = {}
         st = getattr(self, "_store", None)
-        if st is None or image_index is None or not self._store_kinds:
+        if st is None or image_index is None or not self._store_kinds or isinstance(st.tokens, mx4.Mx4Tokens):
             return
         # the tables are indexed [image][token] with the STORE's token count: a view with the same base pointer but another
         # token count / row width / batch stride (store.tokens[:, :K]) must not bind them (it would read them with the wrong

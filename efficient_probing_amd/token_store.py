@@ -87,7 +87,10 @@ class TokenStoreWriter:
         if teacher is not None:
             if len(teacher) not in (2, 3):
                 raise ValueError("teacher is (values, index) or (values, index, tail)")
-            more["values"], more["index"] = host(teacher[0], np.float32), host(teacher[1], np.int32)
+            more["values"], index = host(teacher[0], np.float32), host(teacher[1], np.int64)
+            if index.size and (index.min() < -2 ** 31 or index.max() >= 2 ** 31):
+                raise ValueError("teacher classes must fit 32 bits")
+            more["index"] = index.astype(np.int32)
             if len(teacher) == 3 and teacher[2] is not None:
                 more["tail"] = host(teacher[2], np.float32)
             if more["values"].ndim != 2 or more["values"].shape != more["index"].shape or any(len(more[k]) != n for k in ("values", "index", "tail") if k in more):

@@ -57,7 +57,7 @@ def test_writer_refusals(tmp_path):
     tok, lab = np.zeros((4, 2, 8), np.float32), np.zeros(4, np.int64)
     w = TS.TokenStoreWriter(str(tmp_path), 2, 8)
     for bad in ((np.zeros((4, 3)),), (np.zeros((4, 3)), np.zeros((4, 2))), (np.zeros((3, 3)), np.zeros((3, 3))), (np.zeros(4), np.zeros(4)),
-                (np.zeros((4, 3)), np.zeros((4, 3)), np.zeros(3))):
+                (np.zeros((4, 3)), np.zeros((4, 3)), np.zeros(3)), (np.zeros((4, 3)), np.full((4, 3), 2 ** 32 + 1))):
         with pytest.raises(ValueError):
             w.add(tok, lab, teacher=bad)
     with pytest.raises(ValueError, match="mxfp4"):
@@ -119,6 +119,22 @@ def test_criterion_refusals():
     with pytest.raises(ValueError, match="image_index"):
         c._rows(4, None)
     assert c._rows(6, None) is None and c._rows(2, torch.tensor([5, 5])).dtype == torch.int32
+    assert c._rows(2, torch.tensor([2 ** 32 + 5, -2 ** 40])).tolist() == [2 ** 31 - 1, -1]          # out of range, not wrapped into it
+    i[0, 0] = 2 ** 32 + 1
+    assert distill.TopKDistillation(v, i).teacher_index[0, 0] == distill.MAX_CLASSES
+    with pytest.raises(ValueError, match="integers"):
+        distill.TopKDistillation(v, v)
+
+
+def test_tables_are_not_looked_up_in_a_store_of_codes():
+    """An engine that has seen a 4-bit store is then called with a batch of its own."""
+    from efficient_probing_amd.engine import CaeHeadEngine
+    cache = mx4.Mx4Tokens(torch.zeros(3, 2, 64, dtype=torch.uint8), torch.zeros(3, 2, 4, dtype=torch.uint8), 100)
+    eng = CaeHeadEngine.__new__(CaeHeadEngine)
+    eng._store = TS.ResidentTokenStore.from_tensors(cache, torch.zeros(3))
+    assert eng._store_kinds
+    eng._bind_store_tables(torch.zeros(3, 2, 100), torch.zeros(2, dtype=torch.int32))
+    assert eng._bound_tables == {}
 
 
 def test_who_reads_codes():
