@@ -42,7 +42,7 @@ def _int32(t: torch.Tensor, most: int) -> torch.Tensor:
 def _call(lg, val, idx, tail, rows, tgt, temperature, alpha, grad_scale, grad_scale_dev, grad) -> torch.Tensor:
     B, C_ = lg.shape
     R, K = val.shape
-    loss = torch.empty((B,), device=lg.device, dtype=torch.float32)
+    loss = val.new_empty((B,))
     lib = N.load()
     nbytes = lib.ep_distill_workspace_bytes(B, C_, K)
     ws = torch.empty(nbytes, device=lg.device, dtype=torch.uint8) if nbytes else None
@@ -110,7 +110,7 @@ def topk_distillation(logits: torch.Tensor, teacher_values: torch.Tensor, teache
     one takes no label term.  A row whose teacher lists nothing has no distillation term.  A class, target or row out of range
     makes that row's loss and gradient NaN."""
     args = _checked(logits, teacher_values, teacher_index, targets, teacher_tail, teacher_rows, temperature, alpha)
-    grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype) if need_grad else None
+    grad = torch.empty_like(logits, memory_format=torch.contiguous_format) if need_grad else None
     return _call(*args, float(grad_scale), None, grad), grad
 
 

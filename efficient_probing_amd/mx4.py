@@ -234,9 +234,9 @@ def pool_forward(cache: Mx4Tokens, queries: torch.Tensor, scale: float, per_imag
     B, n, D = args.B, args.N, args.D
     q, Q = _queries(cache, queries, per_image_queries, B)
     dev = _on(cache.codes, q, image_index)
-    P = torch.empty((B, Q, D), device=dev, dtype=torch.float32)
-    S = torch.empty((B, Q, _padded(n)), device=dev, dtype=torch.float32)[:, :, :n] if need_scores else None
-    ML = torch.empty((B, Q, 4), device=dev, dtype=torch.float32)
+    P = q.new_empty((B, Q, D))
+    S = q.new_empty((B, Q, _padded(n)))[:, :, :n] if need_scores else None
+    ML = q.new_empty((B, Q, 4))
     with N.device_guard(dev):
         ws, nbytes = _workspace(B, n, D, Q, dev)
         N.check(N.load().ep_mx4_pool_forward(C.byref(args), q.data_ptr(), Q * D if per_image_queries else 0, Q, float(scale), P.data_ptr(),
