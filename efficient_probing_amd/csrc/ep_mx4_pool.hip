@@ -85,10 +85,9 @@ __device__ __forceinline__ f4 mx_mfma_codes(const mx_u4& codes, uint32_t scale, 
 template <int QM>
 struct MxOperand { mx_u6 b[MxDims<QM>::SETS]; uint32_t sc[MxDims<QM>::SCB]; };
 
-// the operand of one row block for this lane's column; QM 8: two terms share an operand, columns 8-15 take the odd ones.  FIFTH: the
-// last term (and its scale byte) in all columns, for a caller that puts two blocks' last terms into one operand
-template <int QM, bool FIFTH = false>
-__device__ __forceinline__ void mx_operand(mx_f16 a, mx_f16 b, int c, MxOperand<QM>& o) {       // a, b: the row's even and odd channels
+// `take` gets each term with its scale byte (255 where the row holds an infinity or a NaN: its scores become NaN)
+template <typename F>
+__device__ __forceinline__ void mx_terms(mx_f16 a, mx_f16 b, F&& take) {                     // a, b: the row's even and odd channels
   uint32_t am = 0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -97,10 +96,8 @@ __device__ __forceinline__ void mx_operand(mx_f16 a, mx_f16 b, int c, MxOperand<
     am = y > am ? y : am;
   }
   const int ex = (int)(am >> 23);
-  const bool bad = ex == 255;                                  // an infinity or a NaN in the row: the scale byte 255 makes its scores NaN
+  const bool bad = ex == 255;
   const int s0 = bad ? 252 : (ex < 24 ? 24 : ex);              // the row lies below 2 * 2^(s0 - 127)
-  const bool odd = QM == 8 && (c & 8) != 0;
-  uint32_t bytes[2] = {0, 0};
 #pragma unroll
   for (int t = 0; t < 5; ++t) {
     const float sc = __uint_as_float((uint32_t)(s0 - 5 * t) << 23);
@@ -112,9 +109,19 @@ __device__ __forceinline__ void mx_operand(mx_f16 a, mx_f16 b, int c, MxOperand<
 #pragma unroll
       for (int i = 0; i < 16; ++i) { a[i] -= d[2 * i]; b[i] -= d[2 * i + 1]; }
     }
-    const uint32_t byte = bad ? 255u : (uint32_t)(s0 - 5 * t);
+    take(t, k, bad ? 255u : (uint32_t)(s0 - 5 * t));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// the operand of one row block for this lane's column; QM 8: two terms share an operand, columns 8-15 take the odd ones
+template <int QM>
+__device__ __forceinline__ void mx_operand(const mx_f16& a, const mx_f16& b, int c, MxOperand<QM>& o) {
+  const bool odd = QM == 8 && (c & 8) != 0;
+  uint32_t bytes[2] = {0, 0};
+  mx_terms(a, b, [&](int t, const mx_u6& k, uint32_t byte) {
     if constexpr (QM == 8) {
-      if (t % 2 == 0) { o.b[t / 2] = k; bytes[0] |= (odd && !(FIFTH && t == 4) ? 0u : byte) << (8 * (t / 2)); }
+      if (t % 2 == 0) { o.b[t / 2] = k; bytes[0] |= (odd ? 0u : byte) << (8 * (t / 2)); }
       else {
 #pragma unroll
         for (int i = 0; i < 6; ++i) o.b[t / 2][i] = odd ? k[i] : o.b[t / 2][i];
@@ -124,9 +131,8 @@ __device__ __forceinline__ void mx_operand(mx_f16 a, mx_f16 b, int c, MxOperand<
       o.b[t] = k;
       bytes[t / 3] |= byte << (8 * (t % 3));
     }
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  if constexpr (QM == 8 && !FIFTH) {                           // there is no sixth term
+  });
+  if constexpr (QM == 8) {                                     // there is no sixth term
 #pragma unroll
     for (int i = 0; i < 6; ++i) o.b[2][i] = odd ? 0u : o.b[2][i];
   }
@@ -177,8 +183,8 @@ struct MxCursor {
 // a workgroup and take turns at the tiles (forward: of one image; backward: a group per image).  Every wave makes the weights itself,
 // in the very lanes in which its second contraction wants them.  Accumulators and operand rows of four blocks fill 192 of 256 registers:
 // lane constants are made again where they are used, since a register reloaded from scratch waits for the tiles in flight.  Bound:
-// matrix and vector units with two waves a SIMD (256 x 784 x 4096, 4 queries: 131 us forward, 3.3 TB/s), and about 25 us for the operand
-// rows, the first tile and the way out (128 x 196 x 4096: 36 us and 8 us to join two runs an image).
+// matrix and vector units with two waves a SIMD (256 x 784 x 4096, 4 queries: 126 us forward, 3.5 TB/s), and about 20 us for the operand
+// rows, the first tile and the way out (128 x 196 x 4096: 35 us and 8 us to join two runs an image).
 template <bool BWD, bool OPENS>
 __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
   constexpr int QM = 8, CPW = 4, NST = MX_STAGES, REC = 1024;          // REC: bytes of an exchange record, the lane's four scores
@@ -235,48 +241,61 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
 #pragma unroll
   for (int i = 0; i < NST; ++i) { issue(ahead, i); ahead.next(t); }
 
-  // ---- operand rows: one block at a time and last to first, the operands moving up by one (as straight code for every block this part
-  // alone would be 11 KiB of instructions that run once)
+  // ---- operand rows.  Columns q and q + 8 belong to one query: lanes of the first make blocks 0 and 1, of the second blocks 2 and 3,
+  // and they exchange the terms that the other's columns take.  The last terms of blocks i and i + 2 share an operand.  One block at a time
+  // (as straight code this part would be several KiB of instructions that run once), the operands moving up by one.
   struct { mx_u6 b[2]; uint32_t sc; } op[CPW];
-  mx_u6 fifth[CPW / 2];                                                 // two blocks' last terms, in columns 0-7 and 8-15 (which are added)
+  mx_u6 fifth[CPW / 2];
   auto load_operand = [&](const float* rows, const float* prows, float mul) {
     const int ln = mx_fresh(lane), c = ln & 15, q = c & 7;
+    const bool up = (c & 8) != 0;
     const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * p.ldq + 32 * (ln >> 4);      // (rows without a query: the first one's, times 0)
+    const int mine = chunk0 + (up ? 2 : 0);
     float d = 0.f;
     mx_f16 ve, vo;
-    auto load = [&](int k) {
-      const bool in = chunk0 + k < nc;
-      mx_load_row(rows + at + (in ? chunk0 + k : nc - 1) * MX_BLOCK, in && q < qn ? mul : 0.f, ve, vo);
+    auto load = [&](int i) {
+      const bool in = mine + i < nc;
+      mx_load_row(rows + at + (in ? mine + i : nc - 1) * MX_BLOCK, in && q < qn ? mul : 0.f, ve, vo);
     };
-    load(CPW - 1);
+    load(1);
 #pragma unroll 1
-    for (int k = CPW - 1; k >= 0; --k) {
+    for (int i = 1; i >= 0; --i) {
       if (BWD && prows) {
         mx_f16 we, wo;
-        mx_load_row(prows + at + (chunk0 + k < nc ? chunk0 + k : nc - 1) * MX_BLOCK, 1.f, we, wo);
+        mx_load_row(prows + at + (mine + i < nc ? mine + i : nc - 1) * MX_BLOCK, 1.f, we, wo);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) d = fmaf(vo[i], wo[i], fmaf(ve[i], we[i], d));
+        for (int j = 0; j < 16; ++j) d = fmaf(vo[j], wo[j], fmaf(ve[j], we[j], d));
         __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int j = CPW - 1; j > 0; --j) op[j] = op[j - 1];
+      op[1] = op[0]; op[3] = op[2]; fifth[1] = fifth[0];
       const mx_f16 ue = ve, uo = vo;
-      if (k > 0) load(k - 1);
+      if (i > 0) load(0);
       __builtin_amdgcn_sched_barrier(0);
-      MxOperand<QM> o;
-      mx_operand<QM, true>(ue, uo, c, o);
-      op[0].b[0] = o.b[0]; op[0].b[1] = o.b[1];
-      const bool up = (c & 8) != 0;
-      op[0].sc = up == ((k & 1) != 0) ? o.sc[0] : o.sc[0] & 0xffffu;     // the other block's columns: times 2^-127
-      if (k & 1) {
+      mx_u6 even;
+      uint32_t eb = 0;
+      op[0].sc = op[2].sc = 0;
+      mx_terms(ue, uo, [&](int t, const mx_u6& k, uint32_t byte) {
+        if (t == 4) {
+          fifth[0] = k;                                                 // the other block's columns: times 2^-127
+          op[0].sc |= (up ? 0u : byte) << 16;
+          op[2].sc |= (up ? byte : 0u) << 16;
+        } else if (t % 2 == 0) {
+          even = k; eb = byte;
+        } else {                                                        // columns 0-7 take the even term, 8-15 the odd one
 #pragma unroll
-        for (int j = CPW / 2 - 1; j > 0; --j) fifth[j] = fifth[j - 1];
-      }
-#pragma unroll
-      for (int i = 0; i < 6; ++i) fifth[0][i] = up && !(k & 1) ? fifth[0][i] : o.b[2][i];
+          for (int w = 0; w < 6; ++w) {
+            const uint32_t other = mx_ror8u(up ? even[w] : k[w]);
+            op[0].b[t / 2][w] = up ? other : even[w];
+            op[2].b[t / 2][w] = up ? k[w] : other;
+          }
+          const uint32_t other = mx_ror8u(up ? eb : byte);
+          op[0].sc |= (up ? other : eb) << (8 * (t / 2));
+          op[2].sc |= (up ? byte : other) << (8 * (t / 2));
+        }
+      });
       __builtin_amdgcn_sched_barrier(0);
     }
-    return BWD && prows ? mx_over_groups_sum(d) : 0.f;
+    return BWD && prows ? mx_over_groups_sum(d + mx_ror8(d)) : 0.f;
   };
   float delta = 0.f, m_run, mz, l_run, t_max, invl;                     // mz: the maximum that weights are taken against
   auto open_unit = [&](int b) {                                         // backward: dP's rows and the saved statistics
@@ -329,7 +348,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
           const mx_u4 w = *reinterpret_cast<const mx_u4*>(codes + k * 2048 + h * 1024);
           const uint32_t sc = *reinterpret_cast<const uint32_t*>(scl + k * 128 + h * 16) >> (8 * g);
           sa = mx_mfma_codes<0>(w, sc, op[k].b[0], op[k].sc, sa);
-          sl = mx_mfma_codes<2>(w, sc, fifth[k / 2], op[k].sc, sl);
+          sl = mx_mfma_codes<2>(w, sc, fifth[k % 2], op[k].sc, sl);
           sl = mx_mfma_codes<1>(w, sc, op[k].b[1], op[k].sc, sl);
         }
         sum[h] = sa + sl;
@@ -1144,7 +1163,7 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   constexpr int LDS = 160 * 1024;
   int cap;                                                              // workgroups that run at the same time
   if (nc <= 14) {                                                       // a wave per block and the weight wave: what 160 KiB of LDS hold.
-    // (512 x 256 x 1792, 8 queries: 42 us forward and 61 backward; wide-row form 55 and 69.  Narrower rows gain more.)  More than 8
+    // (512 x 256 x 1792, 8 queries: 42 us forward and 60 backward; wide-row form 50 and 63.  Narrower rows gain more.)  More than 8
     // queries: blocks of 16 (512 x 256 x 768: 16 queries 30 us forward, as two blocks of 8 43; 8 queries as a block of 16 27, of 8 25.5)
     p.qm = Q <= 8 ? 8 : 16;
     p.nw = nc; p.cpw = 1; p.groups = 1;
@@ -1169,7 +1188,7 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   cap = cap / p.yblk > 1 ? cap / p.yblk : 1;
   // few images: their token axis is cut into runs of at least `least` tiles.  Forward the runs have to be joined by a second launch, so
   // they are kept longer (64 x 257 x 768, 8 queries: 8 tiles 17 us, 4 22 us); backward every run opens its operand rows (128 x 196 x
-  // 768: 4 tiles 19 us, 2 25 us), which wide rows still gain from (128 x 196 x 4096: 2 tiles 44 us, 4 54 us)
+  // 768: 4 tiles 19 us, 2 25 us), which wide rows still gain from (128 x 196 x 4096: 2 tiles 40 us, 4 49 us)
   const int per = p.pipe ? 1 : p.groups, least = p.pipe ? (bwd ? 4 : 8) : (bwd ? 2 : 2 * per);
   p.splits = B < cap * (bwd ? per : 1) ? (cap * (bwd ? per : 1)) / B : 1;
   if (p.splits > tiles / least) p.splits = tiles / least;
@@ -1242,7 +1261,7 @@ int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bst
   p.lds_ = s_stride;
   EP_TRY(mx_launch<false>(p, pl, st));
   if (pl.splits > 1) {
-    // few runs: one chain (128 x 196 x 4096, two runs: 45 us in all, sixteen chains 74); many: sixteen (2 x 50001 x 1024: 34 us, one 86)
+    // few runs: one chain (128 x 196 x 4096, two runs: 41 us in all, sixteen chains 70); many: sixteen (2 x 50001 x 1024: 34 us, one 86)
     if (pl.splits <= 4)
       hipLaunchKernelGGL(ep_mx4_join_kernel<1>, dim3((unsigned)t->B * Q, (unsigned)((t->D + 1023) / 1024)), dim3(256), 0, st, p.part, p.part_ml, pl.splits, Q, t->D, P, ML);
     else
