@@ -10,7 +10,8 @@ Two execution paths, chosen per call:
     BatchNorm1d, Linear)`` and the loader yields token tensors ``(B, N, D)`` (live encoder output
     via ``token_fn`` or pre-dumped tokens): one ``ProbeHeadEngine`` step per batch -- forward, loss,
     backward, [one all-reduce], optimizer in the HIP kernels, no host sync inside the step; loss /
-    accuracy are read back every ``print_freq`` steps instead of three ``.item()`` per step.
+    accuracy are read back every ``print_freq`` steps instead of three ``.item()`` per step.  Tokens held in 4 bits
+    (``mx4.Mx4Tokens``) and a ``distill.TopKDistillation`` criterion stay on this path for the EP head.
   * MODULE -- anything else: the reference's loop (autocast, criterion, loss scaler, optimizer)
     driving whatever modules ``model`` contains; the native modules run their kernels through
     autograd.  Non-finite loss stops the run with exit code 1 like the reference
