@@ -7,9 +7,11 @@
 //
 //   * Tiles come HBM -> LDS by LDS-DMA into a ring of stages that the wave keeps to itself (no barrier on the data path).
 //   * First contraction (scores / dA), on the matrix cores in the cache's own format: v_mfma_scale_f32_16x16x128_f8f6f4 takes the
-//     E2M1 codes and their E8M0 scale bytes as they lie in LDS, no decoding.  The fp32 operand (queries, dP) becomes five E2M3
-//     terms with block scales 2^-5 apart: below 2 that type is a fixed-point grid of 1/8, so every term takes five more bits and
-//     at most 2^-24 of a block's largest value is left over.  All products are exact, the sums fp32.
+//     E2M1 codes and their E8M0 scale bytes as they lie in LDS, no decoding.  The fp32 operand (queries, dP) becomes seven (wide
+//     rows: six) E2M3 terms with a scale per 32 channels, 2^-5 apart.  The grid of a term is 1/8 below 2 and 1/4 up to 4, so every term
+//     takes five more bits: values down to 2^-11 (2^-6) of the largest of their 32 channels are exact, of smaller ones at most 2^-35
+//     (2^-30) of that largest is left over.  (Five terms would leave 2^-25: rows whose channels differ by 100 to 10000, which meet
+//     tokens sized inversely, then give scores up to 4e-4 off.)  All products of codes and terms are exact, the sums fp32.
 //   * The blocks' parts of a score are added through LDS in block order.
 //   * Weights (exp(S - max), or dS) are split into three bf16 terms, exactly.
 //   * Second contraction: codes are decoded to bf16 (exact; v_cvt_scalef32_pk_bf16_fp4 applies the token's own scale, which is why
@@ -39,9 +41,14 @@ constexpr float MX_LOG2E = 1.4426950408889634f;
 constexpr int MX_NT = 2;                         // cache policy of the code loads: streamed once
 constexpr float MX_LAZY = 12.0f;                 // the running maximum follows a score only when it lies this far above it
 
+// Terms of an fp32 operand row.  Pipelined form: seven (five cost 2 - 7 % less: 1024 x 256 x 768, 8 queries: 40 us forward and 50 backward
+// instead of 42 and 53).  Wide rows: six, what the registers hold (five: 1 % less).
+constexpr int MX_TERMS = 7, MX_WIDE_TERMS = 6;
+
 template <int QM> struct MxDims {
-  static constexpr int SETS = QM == 8 ? 3 : 5;   // matrix operands of the fp32 rows: five terms, two of them in one operand at QM 8
-  static constexpr int SCB = QM == 8 ? 1 : 2;    // dwords of their scale bytes
+  static_assert(MX_TERMS <= 7, "scores() multiplies up to seven operands");
+  static constexpr int SETS = QM == 8 ? (MX_TERMS + 1) / 2 : MX_TERMS;       // matrix operands of the fp32 rows: two terms in one at QM 8
+  static constexpr int SCB = (SETS + 3) / 4;     // dwords of their scale bytes
   static constexpr int SV = QM == 8 ? 4 : 8;     // scores per lane and tile
   static constexpr int PSETS = QM == 8 ? 2 : 3;  // operands of the weights
 };
@@ -78,15 +85,16 @@ __device__ __forceinline__ f4 mx_mfma_codes(const mx_u4& codes, uint32_t scale, 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4 /* E2M1 */, 2 /* E2M3 */, 0, (int)scale, BYTE, (int)row_scales);
 }
 
-// 32 consecutive fp32 values of an operand row -> six E2M3 terms; term t has scale byte s0 - 4 t.  The conversion's two sources are
-// the even and the odd values.  It and its inverse write their results before they have read all of their sources (the scale among
+// 32 consecutive fp32 values of an operand row -> TERMS E2M3 terms; term t has scale byte s0 - 5 t.  The row's largest value lies in
+// [2, 4) times the first scale; what a term leaves is at most 1/8 of its scale (1/16 of values up to 2), which is 4 (2) of the next
+// one's.  The conversion's two sources are the even and the odd values.  It and its inverse write their results before they have read all of their sources (the scale among
 // them), which the compiler does not allow for: it may place the result over a source that dies there, and the low terms then differ
 // from run to run.  So every source is kept alive behind the instruction by an empty asm.
 template <int QM>
 struct MxOperand { mx_u6 b[MxDims<QM>::SETS]; uint32_t sc[MxDims<QM>::SCB]; };
 
 // `take` gets each term with its scale byte (255 where the row holds an infinity or a NaN: its scores become NaN)
-template <typename F>
+template <int TERMS, typename F>
 __device__ __forceinline__ void mx_terms(mx_f16 a, mx_f16 b, F&& take) {                     // a, b: the row's even and odd channels
   uint32_t am = 0;
 #pragma unroll
@@ -97,13 +105,13 @@ __device__ __forceinline__ void mx_terms(mx_f16 a, mx_f16 b, F&& take) {        
   }
   const int ex = (int)(am >> 23);
   const bool bad = ex == 255;
-  const int s0 = bad ? 252 : (ex < 24 ? 24 : ex);              // the row lies below 2 * 2^(s0 - 127)
+  const int s0 = bad ? 252 : (ex <= 5 * TERMS ? 5 * TERMS : ex - 1);      // (every term's scale is a normal number)
 #pragma unroll
-  for (int t = 0; t < 5; ++t) {
+  for (int t = 0; t < TERMS; ++t) {
     const float sc = __uint_as_float((uint32_t)(s0 - 5 * t) << 23);
     const mx_u6 k = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, sc);
     asm volatile("" ::"v"(a), "v"(b), "v"(sc), "v"(k));
-    if (t < 4) {
+    if (t < TERMS - 1) {
       const mx_f32 d = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(k, sc);
       asm volatile("" ::"v"(k), "v"(sc), "v"(d));
 #pragma unroll
@@ -119,7 +127,7 @@ template <int QM>
 __device__ __forceinline__ void mx_operand(const mx_f16& a, const mx_f16& b, int c, MxOperand<QM>& o) {
   const bool odd = QM == 8 && (c & 8) != 0;
   uint32_t bytes[2] = {0, 0};
-  mx_terms(a, b, [&](int t, const mx_u6& k, uint32_t byte) {
+  mx_terms<MX_TERMS>(a, b, [&](int t, const mx_u6& k, uint32_t byte) {
     if constexpr (QM == 8) {
       if (t % 2 == 0) { o.b[t / 2] = k; bytes[0] |= (odd ? 0u : byte) << (8 * (t / 2)); }
       else {
@@ -129,15 +137,15 @@ __device__ __forceinline__ void mx_operand(const mx_f16& a, const mx_f16& b, int
       }
     } else {
       o.b[t] = k;
-      bytes[t / 3] |= byte << (8 * (t % 3));
+      bytes[t / 4] |= byte << (8 * (t % 4));
     }
   });
-  if constexpr (QM == 8) {                                     // there is no sixth term
+  if constexpr (QM == 8 && MX_TERMS % 2 != 0) {                // the last operand has one term
 #pragma unroll
-    for (int i = 0; i < 6; ++i) o.b[2][i] = odd ? 0u : o.b[2][i];
+    for (int i = 0; i < 6; ++i) o.b[MX_TERMS / 2][i] = odd ? 0u : o.b[MX_TERMS / 2][i];
   }
   o.sc[0] = bytes[0];
-  if constexpr (QM != 8) o.sc[1] = bytes[1];
+  if constexpr (MxDims<QM>::SCB > 1) o.sc[1] = bytes[1];
 }
 
 // 32 values of an operand row (16-byte aligned, whole 128-channel blocks: other rows are padded first), times mul
@@ -181,8 +189,9 @@ struct MxCursor {
 // ---- the wide-row form ---------------------------------------------------------------------------------------------------
 // Rows of more than 14 blocks.  A wave owns four blocks of the row for all tokens and up to 8 queries; `groups` such sets of waves share
 // a workgroup and take turns at the tiles (forward: of one image; backward: a group per image).  Every wave makes the weights itself,
-// in the very lanes in which its second contraction wants them.  Accumulators and operand rows of four blocks fill 192 of 256 registers:
-// lane constants are made again where they are used, since a register reloaded from scratch waits for the tiles in flight.  Bound:
+// in the very lanes in which its second contraction wants them.  Accumulators and operand rows of four blocks fill 200 of 256 registers:
+// lane constants are made again where they are used and the operands' scale bytes lie in LDS, since a register reloaded from scratch waits
+// for the tiles in flight.  Bound:
 // matrix and vector units with two waves a SIMD (256 x 784 x 4096, 4 queries: 126 us forward, 3.5 TB/s), and about 20 us for the operand
 // rows, the first tile and the way out (128 x 196 x 4096: 35 us and 8 us to join two runs an image).
 template <bool BWD, bool OPENS>
@@ -200,6 +209,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
   const int q0 = (int)blockIdx.y * p.qblk, qn = p.Q - q0 < p.qblk ? p.Q - q0 : p.qblk;      // queries of this workgroup
   char* ring = lds + wave * (NST * STAGE);
   char* exch = lds + nw * groups * (NST * STAGE);                      // [2][groups][nw][REC]
+  char* opsc = exch + (2 * nw * groups + wave) * REC;                  // the wave's own: scale bytes of its operands, a dword a block
 
   // LDS row r of a tile holds token 8 (r % 4) + r / 4, its 16-byte pieces XOR-ed with r / 4: both contractions then read all banks
   auto issue = [&](const MxCursor& cu, int slot) {
@@ -242,16 +252,17 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
   for (int i = 0; i < NST; ++i) { issue(ahead, i); ahead.next(t); }
 
   // ---- operand rows.  Columns q and q + 8 belong to one query: lanes of the first make blocks 0 and 1, of the second blocks 2 and 3,
-  // and they exchange the terms that the other's columns take.  The last terms of blocks i and i + 2 share an operand.  One block at a time
-  // (as straight code this part would be several KiB of instructions that run once), the operands moving up by one.
-  struct { mx_u6 b[2]; uint32_t sc; } op[CPW];
-  mx_u6 fifth[CPW / 2];
+  // and they exchange the terms that the other's columns take.  One block at a time (as straight code this part would be several KiB of
+  // instructions that run once), the operands moving up by one.
+  struct { mx_u6 b[MX_WIDE_TERMS / 2]; } op[CPW];
+  static_assert(MX_WIDE_TERMS == 6, "two terms an operand, as tile_step multiplies them");
   auto load_operand = [&](const float* rows, const float* prows, float mul) {
     const int ln = mx_fresh(lane), c = ln & 15, q = c & 7;
     const bool up = (c & 8) != 0;
     const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * p.ldq + 32 * (ln >> 4);      // (rows without a query: the first one's, times 0)
     const int mine = chunk0 + (up ? 2 : 0);
     float d = 0.f;
+    uint32_t sc[CPW];
     mx_f16 ve, vo;
     auto load = [&](int i) {
       const bool in = mine + i < nc;
@@ -267,19 +278,15 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
         for (int j = 0; j < 16; ++j) d = fmaf(vo[j], wo[j], fmaf(ve[j], we[j], d));
         __builtin_amdgcn_sched_barrier(0);
       }
-      op[1] = op[0]; op[3] = op[2]; fifth[1] = fifth[0];
+      op[1] = op[0]; op[3] = op[2]; sc[1] = sc[0]; sc[3] = sc[2];
       const mx_f16 ue = ve, uo = vo;
       if (i > 0) load(0);
       __builtin_amdgcn_sched_barrier(0);
       mx_u6 even;
       uint32_t eb = 0;
-      op[0].sc = op[2].sc = 0;
-      mx_terms(ue, uo, [&](int t, const mx_u6& k, uint32_t byte) {
-        if (t == 4) {
-          fifth[0] = k;                                                 // the other block's columns: times 2^-127
-          op[0].sc |= (up ? 0u : byte) << 16;
-          op[2].sc |= (up ? byte : 0u) << 16;
-        } else if (t % 2 == 0) {
+      sc[0] = sc[2] = 0;
+      mx_terms<MX_WIDE_TERMS>(ue, uo, [&](int t, const mx_u6& k, uint32_t byte) {
+        if (t % 2 == 0) {
           even = k; eb = byte;
         } else {                                                        // columns 0-7 take the even term, 8-15 the odd one
 #pragma unroll
@@ -289,12 +296,13 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
             op[2].b[t / 2][w] = up ? k[w] : other;
           }
           const uint32_t other = mx_ror8u(up ? eb : byte);
-          op[0].sc |= (up ? other : eb) << (8 * (t / 2));
-          op[2].sc |= (up ? byte : other) << (8 * (t / 2));
+          sc[0] |= (up ? other : eb) << (8 * (t / 2));
+          sc[2] |= (up ? byte : other) << (8 * (t / 2));
         }
       });
       __builtin_amdgcn_sched_barrier(0);
     }
+    *reinterpret_cast<mx_u4*>(opsc + ln * 16) = mx_u4{sc[0], sc[1], sc[2], sc[3]};
     return BWD && prows ? mx_over_groups_sum(d + mx_ror8(d)) : 0.f;
   };
   float delta = 0.f, m_run, mz, l_run, t_max, invl;                     // mz: the maximum that weights are taken against
@@ -338,6 +346,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
       const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
       const char* codes = st + (4 * (c & 3) + (c >> 2)) * 64 + ((g ^ (c & 3)) << 4);
       const char* scl = st + CODES + (8 * (c >> 2) + (c & 3)) * 4;
+      const mx_u4 osc = *reinterpret_cast<const mx_u4*>(opsc + ln * 16);
       f4 sum[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -347,9 +356,9 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
         for (int k = 0; k < CPW; ++k) {
           const mx_u4 w = *reinterpret_cast<const mx_u4*>(codes + k * 2048 + h * 1024);
           const uint32_t sc = *reinterpret_cast<const uint32_t*>(scl + k * 128 + h * 16) >> (8 * g);
-          sa = mx_mfma_codes<0>(w, sc, op[k].b[0], op[k].sc, sa);
-          sl = mx_mfma_codes<2>(w, sc, fifth[k % 2], op[k].sc, sl);
-          sl = mx_mfma_codes<1>(w, sc, op[k].b[1], op[k].sc, sl);
+          sa = mx_mfma_codes<0>(w, sc, op[k].b[0], osc[k], sa);
+          sl = mx_mfma_codes<2>(w, sc, op[k].b[2], osc[k], sl);
+          sl = mx_mfma_codes<1>(w, sc, op[k].b[1], osc[k], sl);
         }
         sum[h] = sa + sl;
       }
@@ -616,7 +625,8 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
 //     weight wave                                          | barrier j | sums the records of tile j, softmax (or dS), weights j
 // so that the long chain exchange -> maximum -> exponentials -> split runs beside the contractions of other tiles, once per tile
 // instead of once per wave, and the pool waves' registers (accumulators and operand of one block) leave room for 4 waves a SIMD.
-// OPENS: the operand rows change with the image (backward, per-image queries); else they are made once.
+// OPENS: the operand rows change with the image (backward, per-image queries); else they are made once.  QM 16 makes the lane constants of a
+// step where they are used: with seven terms there are no registers to keep them in.
 template <int QM, bool BWD, bool OPENS>
 __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
   typedef MxDims<QM> DM;
@@ -641,11 +651,6 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
 
   if (wave < nw) {                                                      // ================= pool waves
     char* ring = lds + wave * (NST * STAGE);
-    const int sc_off = (8 * (c >> 2) + (c & 3)) * 4;                    // + 16 h: scale dword of the score row
-    const int a_off = (4 * (c & 3) + (c >> 2)) * 64 + ((g ^ (c & 3)) << 4);
-    const int p_off = g * 64 + c * 4;                                   // slot i: (p_off ^ 16 (i % 4)) + 256 i
-    const uint32_t rot = (uint32_t)(8 * (c >> 2) + 9);
-
     // lane offsets of a whole tile; rows behind an image's end repeat its last one
     const int dtok = 8 * ((lane >> 2) & 3) + g;
     const unsigned dseg = (unsigned)(((lane & 3) ^ g) * 16);
@@ -744,6 +749,9 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
 
     auto scores = [&]() {                                               // first contraction of the ring's stage sslot -> record
       mx_wait_vm<(NST - 2) * OPS>();
+      const int ln = QM == 8 ? lane : mx_fresh(lane), c = ln & 15, g = ln >> 4;
+      const int sc_off = (8 * (c >> 2) + (c & 3)) * 4;                  // + 16 h: scale dword of the score row
+      const int a_off = (4 * (c & 3) + (c >> 2)) * 64 + ((g ^ (c & 3)) << 4);
       const char* st = ring + sslot * STAGE;
       char* rec = recs + (buf * nw + wave) * PREC;
       mx_u4 w[2];
@@ -757,26 +765,22 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
       f4 s[2];
       const MxOperand<QM>& o = op;
       s[0] = s[1] = f4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (QM != 8) {
+#define EP_MX_TERM(Z)                                                                                                    \
+  if constexpr (DM::SETS > Z) {                                                                                          \
+    _Pragma("unroll") for (int h = 0; h < 2; ++h) s[h] = mx_mfma_codes<Z % 4>(w[h], sc[h], o.b[Z], o.sc[Z / 4], s[h]);   \
+  }
+      EP_MX_TERM(6) EP_MX_TERM(5) EP_MX_TERM(4) EP_MX_TERM(3) EP_MX_TERM(2) EP_MX_TERM(1) EP_MX_TERM(0)
+#undef EP_MX_TERM
 #pragma unroll
-        for (int h = 0; h < 2; ++h) s[h] = mx_mfma_codes<1>(w[h], sc[h], o.b[4], o.sc[1], s[h]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s[h] = mx_mfma_codes<0>(w[h], sc[h], o.b[3], o.sc[1], s[h]);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) s[h] = mx_mfma_codes<2>(w[h], sc[h], o.b[2], o.sc[0], s[h]);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) s[h] = mx_mfma_codes<1>(w[h], sc[h], o.b[1], o.sc[0], s[h]);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) s[h] = mx_mfma_codes<0>(w[h], sc[h], o.b[0], o.sc[0], s[h]);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) *reinterpret_cast<f4*>(rec + h * 1024 + lane * 16) = s[h];
+      for (int h = 0; h < 2; ++h) *reinterpret_cast<f4*>(rec + h * 1024 + ln * 16) = s[h];
       sslot = sslot + 1 == NST ? 0 : sslot + 1;
     };
 
     uint32_t w[8], s4[8];
     auto fetch = [&]() {                                                // the codes and scales of stage pslot: asked for in front of the barrier
       const char* st = ring + pslot * STAGE;
+      const int ln = QM == 8 ? lane : mx_fresh(lane), c = ln & 15, g = ln >> 4;
+      const int p_off = g * 64 + c * 4;                                 // slot i: (p_off ^ 16 (i % 4)) + 256 i
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         w[i] = *reinterpret_cast<const uint32_t*>(st + i * 256 + (p_off ^ ((i & 3) << 4)));
@@ -785,9 +789,11 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
     };
     auto pool = [&]() {                                                 // second contraction of stage pslot with the weights of buffer buf
       const char* wr = wbuf + buf * WALL;
+      const int ln = QM == 8 ? lane : mx_fresh(lane), c = ln & 15, g = ln >> 4;
+      const uint32_t rot = (uint32_t)(8 * (c >> 2) + 9);
       mx_u4 wt[DM::PSETS];
 #pragma unroll
-      for (int z = 0; z < DM::PSETS; ++z) wt[z] = *reinterpret_cast<const mx_u4*>(wr + z * 1024 + lane * 16);
+      for (int z = 0; z < DM::PSETS; ++z) wt[z] = *reinterpret_cast<const mx_u4*>(wr + z * 1024 + ln * 16);
       if constexpr (!BWD) {
         if (__builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(wr + WREC + 128))) {        // the running maximum has moved
           const f4 r = *reinterpret_cast<const f4*>(wr + WREC + (QM == 8 ? 16 * (g & 1) : 16 * g));
@@ -1177,7 +1183,7 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
     p.nw = (nc + 3) / 4; p.cpw = 4;
     p.groups = bwd || B <= cus ? 8 / p.nw : 1;
     const int waves = p.nw * p.groups;
-    p.lds = (size_t)waves * (MX_STAGES * (2048 * 4 + 512)) + 2 * (size_t)waves * 1024;
+    p.lds = (size_t)waves * (MX_STAGES * (2048 * 4 + 512)) + 3 * (size_t)waves * 1024;
     const int n = (int)(LDS / p.lds);
     cap = cus * (8 / waves < n ? 8 / waves : n);
   }

@@ -8,8 +8,10 @@
     y = pool_project(cache, queries, v_weight, scale)           # ... with the value projection: what EfficientProbing(cache) runs
 
 A token costs 17/32 byte per channel instead of 4 (fp32) or 2 (bf16); the attention's two passes read just those bytes.  The
-pooled vectors are those of the decoded values at fp32 accuracy; what 4 bits cost is decided when the tokens are written
-(11 - 13 % of their root mean square for Gaussian to Laplace-distributed channels).  No CPU path; the reference has no
+pooled vectors are those of the decoded values at fp32 accuracy (queries and gradients enter the products exactly down to 2^-11 of
+the largest of their 32 channels, 2^-6 in rows of more than 1792 channels; of a smaller one at most 2^-35, 2^-30, of that largest is
+lost); what 4 bits cost is decided when the tokens are written (11 - 13 % of their root mean square for Gaussian to
+Laplace-distributed channels).  No CPU path; the reference has no
 counterpart (its dump keeps float32 tokens, tools/dump_tokens.py:95-98).
 """
 from __future__ import annotations
