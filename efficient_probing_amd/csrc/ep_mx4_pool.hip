@@ -85,11 +85,23 @@ __device__ __forceinline__ f4 mx_mfma_codes(const mx_u4& codes, uint32_t scale, 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4 /* E2M1 */, 2 /* E2M3 */, 0, (int)scale, BYTE, (int)row_scales);
 }
 
+// 16 + 16 consecutive fp32 values (the even and the odd channels) -> E2M3 at a scale, and back.  Both instructions write their results
+// before they have read all of their sources (the scale among them), which the compiler's own form of them does not say: a result placed
+// over a source that dies there makes the low terms differ from run to run.  Hence early-clobber results; and since a matrix instruction
+// may read the result of the inline assembly next, its two wait states come along.
+__device__ __forceinline__ mx_u6 mx_to_fp6(const mx_f16& even, const mx_f16& odd, float scale) {
+  mx_u6 k;
+  asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3\n\ts_nop 1" : "=&v"(k) : "v"(even), "v"(odd), "v"(scale));
+  return k;
+}
+__device__ __forceinline__ mx_f32 mx_from_fp6(const mx_u6& k, float scale) {
+  mx_f32 d;
+  asm("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2\n\ts_nop 1" : "=&v"(d) : "v"(k), "v"(scale));
+  return d;
+}
+
 // 32 consecutive fp32 values of an operand row -> TERMS E2M3 terms; term t has scale byte s0 - 5 t.  The row's largest value lies in
-// [2, 4) times the first scale; what a term leaves is at most 1/8 of its scale (1/16 of values up to 2), which is 4 (2) of the next
-// one's.  The conversion's two sources are the even and the odd values.  It and its inverse write their results before they have read all of their sources (the scale among
-// them), which the compiler does not allow for: it may place the result over a source that dies there, and the low terms then differ
-// from run to run.  So every source is kept alive behind the instruction by an empty asm.
+// [2, 4) times the first scale; what a term leaves is at most 1/8 of its scale (1/16 of values up to 2), which is 4 (2) of the next one's.
 template <int QM>
 struct MxOperand { mx_u6 b[MxDims<QM>::SETS]; uint32_t sc[MxDims<QM>::SCB]; };
 
@@ -109,11 +121,9 @@ __device__ __forceinline__ void mx_terms(mx_f16 a, mx_f16 b, F&& take) {        
 #pragma unroll
   for (int t = 0; t < TERMS; ++t) {
     const float sc = __uint_as_float((uint32_t)(s0 - 5 * t) << 23);
-    const mx_u6 k = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, sc);
-    asm volatile("" ::"v"(a), "v"(b), "v"(sc), "v"(k));
+    const mx_u6 k = mx_to_fp6(a, b, sc);
     if (t < TERMS - 1) {
-      const mx_f32 d = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(k, sc);
-      asm volatile("" ::"v"(k), "v"(sc), "v"(d));
+      const mx_f32 d = mx_from_fp6(k, sc);
 #pragma unroll
       for (int i = 0; i < 16; ++i) { a[i] -= d[2 * i]; b[i] -= d[2 * i + 1]; }
     }
@@ -625,8 +635,8 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
 //     weight wave                                          | barrier j | sums the records of tile j, softmax (or dS), weights j
 // so that the long chain exchange -> maximum -> exponentials -> split runs beside the contractions of other tiles, once per tile
 // instead of once per wave, and the pool waves' registers (accumulators and operand of one block) leave room for 4 waves a SIMD.
-// OPENS: the operand rows change with the image (backward, per-image queries); else they are made once.  QM 16 makes the lane constants of a
-// step where they are used: with seven terms there are no registers to keep them in.
+// OPENS: the operand rows change with the image (backward, per-image queries); else they are made once.  QM 16 and the backward pass make the
+// lane constants of a step where they are used: with seven terms there are no registers to keep them in.
 template <int QM, bool BWD, bool OPENS>
 __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
   typedef MxDims<QM> DM;
@@ -749,7 +759,7 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
 
     auto scores = [&]() {                                               // first contraction of the ring's stage sslot -> record
       mx_wait_vm<(NST - 2) * OPS>();
-      const int ln = QM == 8 ? lane : mx_fresh(lane), c = ln & 15, g = ln >> 4;
+      const int ln = QM == 8 && !BWD ? lane : mx_fresh(lane), c = ln & 15, g = ln >> 4;
       const int sc_off = (8 * (c >> 2) + (c & 3)) * 4;                  // + 16 h: scale dword of the score row
       const int a_off = (4 * (c & 3) + (c >> 2)) * 64 + ((g ^ (c & 3)) << 4);
       const char* st = ring + sslot * STAGE;
@@ -779,7 +789,7 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
     uint32_t w[8], s4[8];
     auto fetch = [&]() {                                                // the codes and scales of stage pslot: asked for in front of the barrier
       const char* st = ring + pslot * STAGE;
-      const int ln = QM == 8 ? lane : mx_fresh(lane), c = ln & 15, g = ln >> 4;
+      const int ln = QM == 8 && !BWD ? lane : mx_fresh(lane), c = ln & 15, g = ln >> 4;
       const int p_off = g * 64 + c * 4;                                 // slot i: (p_off ^ 16 (i % 4)) + 256 i
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -789,7 +799,7 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
     };
     auto pool = [&]() {                                                 // second contraction of stage pslot with the weights of buffer buf
       const char* wr = wbuf + buf * WALL;
-      const int ln = QM == 8 ? lane : mx_fresh(lane), c = ln & 15, g = ln >> 4;
+      const int ln = QM == 8 && !BWD ? lane : mx_fresh(lane), c = ln & 15, g = ln >> 4;
       const uint32_t rot = (uint32_t)(8 * (c >> 2) + 9);
       mx_u4 wt[DM::PSETS];
 #pragma unroll
