@@ -435,7 +435,7 @@ __global__ __launch_bounds__(256) void ep_ce_kernel(const float* __restrict__ lo
   const int lane = threadIdx.x & 63;
   const float* row = logits + (int64_t)b * ldl;
   // a label outside [0, C) (an ignore_index, a wrong nb_classes) must not become an out-of-bounds read: the row is
-  // flagged (rowstat[3], which stops the training loop like a non-finite loss), contributes no loss and no gradient
+  // flagged (rowstat[3], which stops the training loop like a non-finite loss), contributes no loss, no gradient and no hit
   const int64_t tgt64 = targets[b];
   const bool tgt_ok = tgt64 >= 0 && tgt64 < (int64_t)C;
   const int tgt = tgt_ok ? (int)tgt64 : 0;
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(256) void ep_ce_kernel(const float* __restrict__ lo
     if (rowstat) {
       const float isbad = (fb > 0.5f || !(fabsf(loss) <= 3.4028234664e38f)) ? 1.f : 0.f;
       *reinterpret_cast<f4*>(rowstat + (int64_t)b * 4) =
-          f4{loss / (float)B, fr < 0.5f ? 1.f : 0.f, fr < 4.5f ? 1.f : 0.f, isbad};
+          f4{loss / (float)B, tgt_ok && fr < 0.5f ? 1.f : 0.f, tgt_ok && fr < 4.5f ? 1.f : 0.f, isbad};
     }
   }
 }

@@ -544,7 +544,8 @@ class ProbeHeadEngine:
     def forward_backward_parts(self, x, targets: torch.Tensor, image_index: Optional[torch.Tensor] = None, criterion=None) -> None:
         """``forward_backward`` as one call per operator instead of one library call: the two token passes run over the 4-bit cache
         where ``x`` is one, and ``criterion`` (``distill.TopKDistillation``) gives the logits' gradient where it is given.  The
-        arithmetic is fp32 whatever ``arithmetic`` says.  The accuracy counts of ``stats`` are those of ``targets``."""
+        arithmetic is fp32 whatever ``arithmetic`` says.  The accuracy counts of ``stats`` are those of ``targets`` (an image without a
+        label, a negative target, is no hit)."""
         if not self.reads_parts:
             raise NotImplementedError(f"{type(self).__name__}: 4-bit tokens and a criterion are for the EP head; decode the batch "
                                       "(mx4.dequantize_tokens) for this one")
