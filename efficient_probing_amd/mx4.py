@@ -127,6 +127,13 @@ class Mx4Tokens:
         mv = lambda t: None if t is None else t.to(device, non_blocking=non_blocking)
         return Mx4Tokens(mv(self.codes), mv(self.scales), self.dim, mv(self.lengths), mv(self.image_index))
 
+    def _parts(self) -> Tuple[Optional[torch.Tensor], ...]:
+        return self.codes, self.scales, self.lengths, self.image_index
+
+    def _versions(self) -> Tuple[Optional[int], ...]:
+        """What changes when any of the tensors is written (those of inference mode keep no count)."""
+        return tuple(None if t is None or t.is_inference() else t._version for t in self._parts())
+
     def _args(self, image_index: Optional[torch.Tensor] = None) -> "N.EPMx4Tokens":
         codes = self.codes
         N.require_gpu_tensor(codes, "codes")
@@ -169,7 +176,8 @@ def quantize_tokens(x: torch.Tensor, out: Optional[Mx4Tokens] = None, lengths: O
         x = x.float()
     if x.stride(2) != 1 or min(x.stride()) < 0:
         x = x.contiguous()
-    if out is None:
+    given = out is not None
+    if not given:
         out = empty_cache(B, n, D, x.device, lengths)
     elif lengths is not None:
         raise ValueError("lengths belong to a new cache; `out` has its own")
@@ -179,6 +187,8 @@ def quantize_tokens(x: torch.Tensor, out: Optional[Mx4Tokens] = None, lengths: O
         N.check(N.load().ep_mx4_quantize(x.data_ptr(), _OUT[x.dtype], x.stride(0), x.stride(1), B, n, D, out.codes.data_ptr(),
                                          out.scales.data_ptr(), out.codes.stride(0), out.scales.stride(0),
                                          N.current_stream_ptr(x.device)), "ep_mx4_quantize")
+    if given:                                                   # (the kernel's writes are not seen by torch's own count)
+        torch.autograd.graph.increment_version((out.codes, out.scales))
     return out
 
 
@@ -291,6 +301,18 @@ def attention(cache: Mx4Tokens, queries: torch.Tensor, scale: float, per_image_q
     return F_.attention_from_scores(S.contiguous(), ML).masked_fill_(ML[..., 1:2] == 0, 0.0)
 
 
+def _keep_cache(ctx, cache: Mx4Tokens) -> None:
+    """For the backward pass, with the versions that its tensors have now."""
+    ctx.cache, ctx.versions = Mx4Tokens._made(cache.codes, cache.scales, cache.dim, cache.lengths, cache.image_index), cache._versions()
+
+
+def _kept_cache(ctx) -> Mx4Tokens:
+    if ctx.cache._versions() != ctx.versions:
+        raise RuntimeError("one of the 4-bit cache's tensors needed for gradient computation has been modified since the forward pass "
+                           "(quantize_tokens(out=...) or an in-place operation)")
+    return ctx.cache
+
+
 class _AttentionPool(torch.autograd.Function):
     @staticmethod
     def forward(ctx, queries, cache, scale, per_image):
@@ -298,20 +320,22 @@ class _AttentionPool(torch.autograd.Function):
         P, S, ML = pool_forward(cache, queries, scale, per_image, need_scores=need)
         if need:
             ctx.save_for_backward(P, S, ML)
-        ctx.cache, ctx.scale, ctx.per_image, ctx.qshape = cache, scale, per_image, queries.shape
+        _keep_cache(ctx, cache)
+        ctx.scale, ctx.per_image, ctx.qshape = scale, per_image, queries.shape
         return P
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dP):
         P, S, ML = ctx.saved_tensors
-        dq = pool_backward(ctx.cache, S, ML, dP, ctx.scale, P=P, per_image_queries=ctx.per_image)
+        dq = pool_backward(_kept_cache(ctx), S, ML, dP, ctx.scale, P=P, per_image_queries=ctx.per_image)
         return dq.reshape(ctx.qshape), None, None, None
 
 
 def attention_pool(cache: Mx4Tokens, queries: torch.Tensor, scale: float, per_image_queries: bool = False,
                    image_index: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """softmax(scale * queries . x) x over the cache's tokens, differentiable in ``queries`` (the tokens are frozen): (B, Q, D)."""
+    """softmax(scale * queries . x) x over the cache's tokens, differentiable in ``queries`` (the tokens are frozen): (B, Q, D).  The
+    backward pass reads the cache again: one that was written in between is an error."""
     if image_index is not None:
         cache = cache.select(image_index)
     return _AttentionPool.apply(queries, cache, float(scale), per_image_queries)
@@ -326,7 +350,8 @@ class _PoolProject(torch.autograd.Function):
         P, S, ML = pool_forward(cache, queries, scale, per_image, need_scores=need)
         y = F_.project_forward(P, v_weight)
         ctx.save_for_backward(P, S, ML, y, v_weight)
-        ctx.cache, ctx.scale, ctx.per_image, ctx.qshape = cache, scale, per_image, queries.shape
+        _keep_cache(ctx, cache)
+        ctx.scale, ctx.per_image, ctx.qshape = scale, per_image, queries.shape
         return y
 
     @staticmethod
@@ -335,7 +360,7 @@ class _PoolProject(torch.autograd.Function):
         P, S, ML, y, v_weight = ctx.saved_tensors
         need_q = ctx.needs_input_grad[0]
         dP, dWv = F_.project_backward(dy.contiguous(), y, P, v_weight, None, need_dP=need_q, need_dWv=ctx.needs_input_grad[1])
-        dq = pool_backward(ctx.cache, S, ML, dP, ctx.scale, P=P, per_image_queries=ctx.per_image).reshape(ctx.qshape) if need_q else None
+        dq = pool_backward(_kept_cache(ctx), S, ML, dP, ctx.scale, P=P, per_image_queries=ctx.per_image).reshape(ctx.qshape) if need_q else None
         return dq, dWv, None, None, None
 
 
