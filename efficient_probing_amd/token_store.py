@@ -62,16 +62,21 @@ class TokenStoreWriter:
         self._n = 0
 
     def add(self, tokens, labels: np.ndarray, lengths=None, teacher=None) -> None:
-        """``tokens`` (n, N, D) numpy or torch.  mxfp4: quantised on the GPU (a host array is copied there first), and ``lengths`` (n,)
+        """``tokens`` (n, N, D): numpy, torch (any floating type, any device) or nested lists.  mxfp4: quantised on the GPU (a host array is copied there first), and ``lengths`` (n,)
         may give images fewer than N tokens.  ``teacher`` = (values (n, K), index (n, K)[, tail (n,)]) of ``distill.teacher_topk`` at
         this writer's ``teacher_temperature``.  Every ``add`` of a store brings the same parts."""
+        if not isinstance(tokens, torch.Tensor):
+            tokens = np.asarray(tokens)
         n, dims = len(tokens), tuple(tokens.shape)
         assert len(dims) == 3 and dims[1:] == (self.N, self.D), dims
         assert len(labels) == n
         if n == 0:
             return
         more = {}
-        host = lambda t, dt: np.ascontiguousarray(t.detach().cpu() if isinstance(t, torch.Tensor) else t, dtype=dt)
+        def host(t, dt):
+            if isinstance(t, torch.Tensor):                    # (numpy has no bfloat16)
+                t = (t.detach().float() if t.dtype == torch.bfloat16 else t.detach()).cpu().numpy()
+            return np.ascontiguousarray(t, dtype=dt)
         if self.dtype == "mxfp4":
             x = torch.as_tensor(tokens).detach()
             cache = mx4.quantize_tokens(x if x.is_cuda else x.to("cuda"))

@@ -154,3 +154,23 @@ def test_who_reads_codes():
         EF._batch_tokens(cache, idx, False, None)
     x = torch.zeros(2, 3, 4)
     assert EF._batch_tokens(x, idx, False, None) == (x, idx)
+
+
+def test_writer_takes_what_it_took(tmp_path):
+    """Tokens as nested lists, as integers or doubles, and torch tensors of any floating type; teacher rows likewise."""
+    tok = [[[1.0, 2.0, 3.0, 4.0, 5.0, 6.0, 7.0, 8.0]], [[0.5] * 8]]
+    x = torch.tensor(tok)
+    w = TS.TokenStoreWriter(str(tmp_path / "a"), 1, 8)
+    for t in (tok, np.array(tok, np.float64), np.array(tok).astype(np.int32), x, x.double(), x.to(torch.bfloat16), x.half(), x.transpose(0, 1).contiguous().transpose(0, 1)):
+        w.add(t, [3, 4])
+    assert w.close()["total_images"] == 16
+    st = TS.ResidentTokenStore(str(tmp_path / "a"), "cpu")
+    for lo in range(0, 16, 2):
+        assert torch.equal(st.tokens[lo:lo + 2], x if lo != 4 else x.floor())
+    w = TS.TokenStoreWriter(str(tmp_path / "b"), 1, 8)
+    w.add(x.to(torch.bfloat16), [0, 1], teacher=(torch.tensor([[2.0, 1.0], [0.5, 0.25]], dtype=torch.bfloat16), [[4, 2], [0, 1]], torch.zeros(2, dtype=torch.bfloat16)))
+    w.close()
+    t = TS.ResidentTokenStore(str(tmp_path / "b"), "cpu").teacher
+    assert t.values.tolist() == [[2.0, 1.0], [0.5, 0.25]] and t.index.tolist() == [[4, 2], [0, 1]] and t.tail.tolist() == [0.0, 0.0]
+    with pytest.raises(AssertionError):
+        w.add([[1.0] * 8], [0])
