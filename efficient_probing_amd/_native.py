@@ -585,10 +585,18 @@ def require_gpu_tensor(t, name: str) -> None:
                            f"(got device {t.device})")
 
 
+def _device_index(device):
+    """Of a torch.device, an index or a name; None for the current device."""
+    if isinstance(device, str):
+        import torch
+        device = torch.device(device)
+    return device if device is None or isinstance(device, int) else device.index
+
+
 def current_stream_ptr(device=None) -> int:
     """hipStream_t of torch's current stream (``torch.cuda.current_stream(device).cuda_stream`` without building the Stream object)."""
     import torch
-    index = getattr(device, "index", device)
+    index = _device_index(device)
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
