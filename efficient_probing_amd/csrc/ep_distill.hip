@@ -20,7 +20,9 @@ constexpr int DIST_MAX_K = 1024;
 constexpr int DIST_MAX_C = 1 << 20;               // (256 pieces, one for each thread that joins them)
 constexpr int DIST_PIECE = 4096;                  // classes of a workgroup where a row is cut
 constexpr int DIST_SLICE = 1 << 22;               // workgroups of a launch (HIP takes less than 2^32 threads)
-constexpr float DIST_LOW = 1e-30f;                // a sum of exponentials below this has lost bits
+// A sum of exponentials below this is taken again relative to its own maximum: an exponential below 2^-126 is zero, which a sum of 1e-30
+// would still feel (classes 20 below it, with shares of 1e-8 of the tail, took no gradient); of 1e-16 it loses shares below 1e-22.
+constexpr float DIST_LOW = 1e-16f;
 constexpr float DIST_LOG2E = 1.4426950408889634f;
 
 template <int DT> struct DistElem { typedef float T; static constexpr int VEC = 4; };

@@ -41,3 +41,33 @@ def distill(z, values, index, targets=None, tail=None, T=1.0, alpha=1.0):
             h[targets[b]] -= 1
             grad[b] += (1 - alpha) * h
     return loss, grad
+
+
+def sizes(z, values, index, targets=None, tail=None, T=1.0, alpha=1.0):
+    """Of every component of ``distill``'s gradient: the size of the terms that it is a sum of, and how far its exponents lie from the
+    row's maximum, |z - max z| / min(T, 1) (what an error of the exponents' arguments is relative to)."""
+    z = np.asarray(z, np.float64)
+    B, C = z.shape
+    mag, far = np.zeros((B, C)), np.zeros((B, C))
+    for b in range(B):
+        keep = index[b] >= 0
+        idx, t = index[b][keep], np.asarray(values[b], np.float64)[keep] / T
+        listed = np.zeros(C, bool)
+        listed[idx] = True
+        y = z[b] / T
+        far[b] = (z[b].max() - z[b]) / min(T, 1.0)
+        rest = -np.inf if tail is None else float(tail[b])
+        ends = np.append(t, rest)
+        lt = _lse(ends)
+        if lt > -np.inf:
+            p = np.exp(ends - lt)
+            m = np.exp(y - _lse(y))
+            np.add.at(m, idx, p[:-1])
+            if tail is not None and p[-1] > 0:
+                m[~listed] += p[-1] * np.exp(y[~listed] - _lse(y[~listed]))
+            mag[b] += alpha * T * m
+        if alpha < 1.0 and targets[b] >= 0:
+            h = np.exp(z[b] - _lse(z[b]))
+            h[targets[b]] += 1
+            mag[b] += (1 - alpha) * h
+    return mag, far

@@ -1,0 +1,64 @@
+"""The distillation's gradient class by class: most of a long row are classes that the teacher does not list, each with a share far below
+the largest component, and each has to be right relative to its own terms.
+
+Bound of a component (u = 2^-24), on the sizes of the terms that it is a sum of (oracle ``sizes``): an exponential is off by 4 u (the
+instruction, its sum's and its quotient's rounding) plus 4 u times its argument (the difference's rounding, the factor log2(e) / T and the
+product's), and arguments that count in a sum are log C <= 14 in the mean: 64 u for a sum; the teacher's side likewise with arguments of
+the size of its logits over T.  r = 192 u + 8 u (|argument| + teacher's).  Then one rounding to the logits' type (half a step), half of
+its smallest subnormal, and 2^-126 per term, below which an exponential is zero."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import distill_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
+
+
+def _teacher(R, C, K, seed):
+    rng = np.random.default_rng(seed)
+    start, step = rng.integers(0, C, (R, 1)), max(1, C // K)
+    idx = np.stack([(start[r] + step * rng.permutation(K)) % C for r in range(R)]).astype(np.int32)
+    return (6 + 3 * rng.standard_normal((R, K))).astype(np.float32), idx, (4 + rng.standard_normal(R)).astype(np.float32)
+
+
+def _check(z, val, idx, tgt, tail, T, alpha, gs):
+    from efficient_probing_amd import distill
+    B, C = z.shape
+    dev = lambda a: None if a is None else torch.as_tensor(a, device=DEV)
+    zf = z.double().cpu().numpy()
+    want = O.distill(zf, val, idx, tgt, tail, T, alpha)[1] * (gs / B)
+    mag, far = O.sizes(zf, val, idx, tgt, tail, T, alpha)
+    _, grad = distill.topk_distillation(z, dev(val), dev(idx), dev(tgt), teacher_tail=dev(tail), temperature=T, alpha=alpha, grad_scale=gs)
+    t = np.abs(val).max() / T + (0.0 if tail is None else np.abs(tail).max()) + 14.0
+    lim = (gs / B) * (mag * (192 * U + 8 * U * (far + t)) + 4 * T * 2.0 ** -126) + np.abs(want) * torch.finfo(z.dtype).eps / 2 + TINY[z.dtype]
+    err = np.abs(grad.double().cpu().numpy() - want)
+    assert (err <= lim).all(), (float((err / lim).max()), np.unravel_index((err / lim).argmax(), err.shape), float((err > lim).mean()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,C,K", [(3, 2, 1), (5, 63, 5), (4, 1000, 32), (3, 4099, 100), (2, 10000, 16), (2, 21841, 64), (1, 32768, 64), (2, 65537, 256),
+                                   (2, 131071, 128), (1, 1 << 20, 1024)])
+@pytest.mark.parametrize("mode", ["soft", "soft+label", "tail", "tail+label"])
+def test_every_class_by_its_own_terms(B, C, K, dtype, mode):
+    """(the loss scale keeps the shares of unlisted classes within fp16's range)"""
+    z = (2 * torch.randn(B, C, generator=torch.Generator().manual_seed(C))).to(dtype).to(DEV)
+    val, idx, tail = _teacher(B, C, K, C + K)
+    label = "label" in mode
+    tgt = np.random.default_rng(B + C).integers(0, C, B) if label else None
+    _check(z, val, idx, tgt, tail if "tail" in mode else None, 2.0 if label else 1.0, 0.4 if label else 1.0, 4096.0)
+
+
+@pytest.mark.parametrize("C", [50, 3000, 21841, 40001])
+@pytest.mark.parametrize("gap", [30.0, 45.0, 60.0, 66.0, 75.0, 200.0])
+def test_shares_far_below_the_list(C, gap):
+    """The classes behind the list from near its logits to beyond fp32's range below them, with a spread of their own."""
+    B, K = 3, 8
+    val, idx, tail = _teacher(B, C, K, C)
+    z = 3 * torch.randn(B, C, generator=torch.Generator().manual_seed(C))
+    z.scatter_add_(1, torch.as_tensor(idx, dtype=torch.long), torch.full((B, K), gap))
+    _check(z.to(DEV), val, idx, None, tail, 1.0, 1.0, 1.0)
+    _check(z.to(DEV), val, idx, np.array([0, int(idx[1, 0]), -1]), tail, 1.0, 0.5, 1.0)
