@@ -50,8 +50,9 @@ __device__ __forceinline__ void dist_store(typename DistElem<DT>::T* p, float v)
   if constexpr (DT == 1) { const __bf16 h = (__bf16)v; *p = __builtin_bit_cast(uint16_t, h); }
   else *p = (typename DistElem<DT>::T)v;
 }
+typedef uint32_t dist_u4 __attribute__((ext_vector_type(4)));
 template <int DT>
-__device__ __forceinline__ void dist_unpack(const uint4& r, float (&v)[DistElem<DT>::VEC]) {
+__device__ __forceinline__ void dist_unpack(const dist_u4& r, float (&v)[DistElem<DT>::VEC]) {
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -246,9 +247,10 @@ template <int DT, int TH, int NV>
 struct DistRun {
   typedef typename DistElem<DT>::T T;
   static constexpr int VEC = DistElem<DT>::VEC;
-  struct __attribute__((packed, aligned(sizeof(T)))) Piece { uint4 v; };
+  struct __attribute__((packed, aligned(sizeof(T)))) Piece { dist_u4 v; };
+  static_assert(alignof(Piece) == sizeof(T), "(a class type such as uint4 would not be packed, and 16 bytes promised to the compiler)");
   int nv, edge;                 // pieces, single classes
-  uint4 raw[NV];
+  dist_u4 raw[NV];
   float one;                    // the thread's single class (thread < edge)
   __device__ __forceinline__ int edge_class(int t) const { return nv * VEC + t; }
   __device__ __forceinline__ void load(const T* z, int n, int tid) {
@@ -258,7 +260,7 @@ struct DistRun {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int i = tid + v * TH;
-      raw[v] = i < nv ? p[i].v : uint4{0u, 0u, 0u, 0u};
+      raw[v] = i < nv ? p[i].v : dist_u4{0u, 0u, 0u, 0u};
     }
     one = tid < edge ? dist_load<DT>(z + edge_class(tid)) : 0.f;
   }
@@ -349,9 +351,9 @@ __device__ __forceinline__ void dist_run_grad(const DistRun<DT, TH, NV>& r, int 
     dist_unpack<DT>(r.raw[v], f);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) f[i] = dist_grad_plain<LABEL>(g, f[i]);
-    uint4 w;
-    if constexpr (DT == 0) w = uint4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
-    else w = uint4{dist_pair<DT>(f[0], f[1]), dist_pair<DT>(f[2], f[3]), dist_pair<DT>(f[4], f[5]), dist_pair<DT>(f[6], f[7])};
+    dist_u4 w;
+    if constexpr (DT == 0) w = dist_u4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+    else w = dist_u4{dist_pair<DT>(f[0], f[1]), dist_pair<DT>(f[2], f[3]), dist_pair<DT>(f[4], f[5]), dist_pair<DT>(f[6], f[7])};
     reinterpret_cast<typename DistRun<DT, TH, NV>::Piece*>(dz)[p].v = w;
   }
   if (tid < r.edge) dist_store<DT>(dz + r.edge_class(tid), dist_grad_plain<LABEL>(g, r.one));
