@@ -106,7 +106,7 @@ struct DistEntries {            // in LDS, K entries and the label, padded to wh
 struct DistRow {
   int64_t r;                    // row of the teacher's tables
   int tg;                       // label, or -1
-  bool bad, soft;               // something out of range; the teacher lists anything
+  bool bad, soft;               // something out of range; there is a distillation term
   float tail, tl, ptail;        // log mass behind the list; logsumexp over list and tail; the tail's probability
   float ml, ms;                 // student's statistics: maximum of the logits; log of the sum of exp((z - ml) / T)
   float mo;                     // what the sum over the classes behind the list is relative to
@@ -154,7 +154,7 @@ __device__ __forceinline__ void dist_teacher(const ep_distill_args& a, int b, in
   dist_sync<TH>();
   const int f = *flag;
   d.bad = (f & 1) || !row_ok || tg_bad;
-  d.soft = tm > -INFINITY || (f & 2) || d.tail != d.tail;
+  d.soft = a.alpha > 0.f && (tm > -INFINITY || (f & 2) || d.tail != d.tail);   // (no 0 times infinity)
   float ts[1] = {0.f};
   _Pragma("unroll 1") for (int k = tid; k < a.K; k += TH) ts[0] += d.soft && e.idx[k] >= 0 ? __builtin_amdgcn_exp2f((e.pk[k] - tm) * DIST_LOG2E) : 0.f;
   dist_sums<TH, 1>(ts, red);

@@ -23,7 +23,7 @@ def distill(z, values, index, targets=None, tail=None, T=1.0, alpha=1.0):
         rest = -np.inf if tail is None else float(tail[b])
         ends = np.append(t, rest)
         lt = _lse(ends)
-        if lt > -np.inf:
+        if alpha > 0 and lt > -np.inf:
             logp = ends - lt
             p = np.exp(logp)
             logq = np.append(y[idx] - ly, (_lse(y[~listed]) - ly) if tail is not None else 0.0)
@@ -59,7 +59,7 @@ def sizes(z, values, index, targets=None, tail=None, T=1.0, alpha=1.0):
         rest = -np.inf if tail is None else float(tail[b])
         ends = np.append(t, rest)
         lt = _lse(ends)
-        if lt > -np.inf:
+        if alpha > 0 and lt > -np.inf:
             p = np.exp(ends - lt)
             m = np.exp(y - _lse(y))
             np.add.at(m, idx, p[:-1])

@@ -62,3 +62,27 @@ def test_shares_far_below_the_list(C, gap):
     z.scatter_add_(1, torch.as_tensor(idx, dtype=torch.long), torch.full((B, K), gap))
     _check(z.to(DEV), val, idx, None, tail, 1.0, 1.0, 1.0)
     _check(z.to(DEV), val, idx, np.array([0, int(idx[1, 0]), -1]), tail, 1.0, 0.5, 1.0)
+
+
+@pytest.mark.parametrize("C", [40, 5000, 40001])
+@pytest.mark.parametrize("tail_on", [False, True])
+def test_without_weight_the_teacher_does_not_count(C, tail_on):
+    """alpha = 0 is the cross-entropy alone, also where the distillation term would be infinite or not a number: the student gives a
+    listed class no mass, nothing is left for the tail, the teacher's logits are NaN."""
+    from efficient_probing_amd import distill
+    B, K = 5, 6
+    val, idx, tail = _teacher(B, C, K, C)
+    z = torch.randn(B, C, generator=torch.Generator().manual_seed(C))
+    z[0, int(idx[0, 0])] = -np.inf
+    z[1] = torch.where(torch.zeros(C, dtype=torch.bool).scatter(0, torch.as_tensor(idx[1], dtype=torch.long), True), z[1], torch.tensor(-np.inf))
+    val[2, 1], val[3, 0] = np.nan, np.inf
+    tail[4] = np.nan
+    tgt = torch.tensor([int(idx[b, 3]) for b in range(B)])
+    ref = z.double().requires_grad_(True)
+    want = torch.nn.functional.cross_entropy(ref, tgt, reduction="none")
+    want.sum().backward()
+    dev = lambda a: torch.as_tensor(a, device=DEV)
+    loss, grad = distill.topk_distillation(z.to(DEV), dev(val), dev(idx), tgt.to(DEV), teacher_tail=dev(tail) if tail_on else None, temperature=2.0, alpha=0.0, grad_scale=float(B))
+    assert (loss.double().cpu() - want.detach()).abs().max() <= 192 * U * 20
+    one = torch.nn.functional.one_hot(tgt, C)
+    assert ((grad.double().cpu() - ref.grad).abs() <= 320 * U * (ref.grad.abs() + 2 * one) + 2.0 ** -126).all()
