@@ -18,6 +18,7 @@ namespace ep {
 
 constexpr int DIST_MAX_K = 1024;
 constexpr int DIST_MAX_C = 1 << 20;               // (256 pieces, one for each thread that joins them)
+constexpr float DIST_MIN_T = 1e-15f, DIST_MAX_T = 1e15f;      // T^2, and a logit over T, stay within fp32
 constexpr int DIST_PIECE = 4096;                  // classes of a workgroup where a row is cut
 constexpr int DIST_SLICE = 1 << 22;               // workgroups of a launch (HIP takes less than 2^32 threads)
 // A sum of exponentials below this is taken again relative to its own maximum: an exponential below 2^-126 is zero, which a sum of 1e-30
@@ -532,8 +533,8 @@ int ep_distill_topk(const ep_distill_args* a, void* workspace, size_t workspace_
   EP_REQUIRE(a->teacher_rows || a->R >= a->B, EP_E_ARG, "ep_distill_topk: %lld teacher rows for a batch of %d need teacher_rows", (long long)a->R, a->B);
   EP_REQUIRE((a->B == 1 || (a->ldl >= a->C && (!a->dlogits || a->ldd >= a->C))) && (a->R == 1 || (a->ldv >= a->K && a->ldi >= a->K)), EP_E_SHAPE,
              "ep_distill_topk: a row stride is below its row");
-  EP_REQUIRE(a->temperature > 0.f && a->temperature <= 3.0e38f && a->alpha >= 0.f && a->alpha <= 1.f, EP_E_ARG,
-             "ep_distill_topk: temperature %g must be positive and alpha %g within [0, 1]", (double)a->temperature, (double)a->alpha);
+  EP_REQUIRE(a->temperature >= DIST_MIN_T && a->temperature <= DIST_MAX_T && a->alpha >= 0.f && a->alpha <= 1.f, EP_E_ARG,
+             "ep_distill_topk: temperature %g must lie within [1e-15, 1e15] and alpha %g within [0, 1]", (double)a->temperature, (double)a->alpha);
   EP_REQUIRE(a->targets || a->alpha == 1.f, EP_E_ARG, "ep_distill_topk: alpha < 1 needs targets");
   const size_t need = ep_distill_workspace_bytes(a->B, a->C, a->K);
   EP_REQUIRE(workspace_bytes >= need, EP_E_WORKSPACE, "ep_distill_topk: workspace %zu < %zu", workspace_bytes, need);

@@ -29,6 +29,16 @@ MAX_CLASSES = 1 << 20
 _DT = {torch.float32: N.EP_DTYPE_F32, torch.bfloat16: N.EP_DTYPE_BF16, torch.float16: N.EP_DTYPE_F16}
 
 
+def _check_temperature(T: float) -> None:
+    if not 1e-15 <= T <= 1e15:                                  # (its square and its inverse times a logit stay within fp32)
+        raise ValueError(f"temperature must lie within [1e-15, 1e15], got {T}")
+
+
+def _check_alpha(alpha: float) -> None:
+    if not 0.0 <= alpha <= 1.0:
+        raise ValueError(f"alpha must lie within [0, 1], got {alpha}")
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """Rows with contiguous elements that do not overlap, as the kernels read them."""
     return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
@@ -69,8 +79,8 @@ def _checked(logits, teacher_values, teacher_index, targets, teacher_tail, teach
         raise ValueError(f"at most {MAX_K} teacher entries and {MAX_CLASSES} classes, got {K} and {C_}")
     if teacher_index.dtype.is_floating_point or teacher_index.dtype == torch.bool:
         raise ValueError(f"teacher_index must hold integers, got {teacher_index.dtype}")
-    if not (temperature > 0.0 and temperature < float("inf")) or not 0.0 <= alpha <= 1.0:
-        raise ValueError(f"temperature must be positive and alpha within [0, 1], got {temperature} and {alpha}")
+    _check_temperature(temperature)
+    _check_alpha(alpha)
     if alpha < 1.0 and targets is None:
         raise ValueError("alpha < 1 needs targets")
     if targets is not None and tuple(targets.shape) != (B,):
@@ -148,8 +158,7 @@ def teacher_topk(logits: torch.Tensor, k: int, temperature: float = 1.0) -> Tupl
     sum of exp(logit / temperature) over the others (-inf where k = C)."""
     if logits.dim() != 2 or not 1 <= k <= min(logits.shape[1], MAX_K):
         raise ValueError(f"logits must be (R, C) and k within [1, min(C, {MAX_K})], got {tuple(logits.shape)} and {k}")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive, got {temperature}")
+    _check_temperature(temperature)
     lg = logits.float()
     values, index = lg.topk(k, dim=1)
     tail = (lg / temperature).scatter(1, index, float("-inf")).logsumexp(1)
@@ -165,8 +174,8 @@ class TopKDistillation(torch.nn.Module):
                  temperature: float = 1.0, alpha: float = 1.0):
         super().__init__()
         self.temperature, self.alpha = float(temperature), float(alpha)
-        if not (self.temperature > 0.0 and self.temperature < float("inf")) or not 0.0 <= self.alpha <= 1.0:
-            raise ValueError(f"temperature must be positive and alpha within [0, 1], got {temperature} and {alpha}")
+        _check_temperature(self.temperature)
+        _check_alpha(self.alpha)
         if teacher_values.dim() != 2 or teacher_values.shape != teacher_index.shape or min(teacher_values.shape) < 1:
             raise ValueError(f"teacher_values and teacher_index must be (rows, K), got {tuple(teacher_values.shape)} and {tuple(teacher_index.shape)}")
         if teacher_tail is not None and tuple(teacher_tail.shape) != (teacher_values.shape[0],):

@@ -1214,7 +1214,7 @@ int ep_mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float
  * with r = teacher_rows[b] (int32, into a table of R rows read in place), or b.  A class listed more than once takes the sum of
  * its entries; entries with a negative index are skipped; a row without any entry has no distillation term, nor has any row with alpha == 0.  targets may be NULL
  * when alpha == 1; a negative target takes no label term.  A row index, class or target out of range makes the row's loss and gradient
- * NaN and is never read through.  K <= 1024, C <= 2^20.  dlogits (same type and row stride rules as logits, not overlapping them) may
+ * NaN and is never read through.  K <= 1024, C <= 2^20, T within [1e-15, 1e15].  dlogits (same type and row stride rules as logits, not overlapping them) may
  * be NULL. */
 typedef struct ep_distill_args {
   const void* logits; int32_t dtype; int64_t ldl;       /* fp32 / bf16 / fp16; row stride in elements, >= C */

@@ -174,3 +174,19 @@ def test_writer_takes_what_it_took(tmp_path):
     assert t.values.tolist() == [[2.0, 1.0], [0.5, 0.25]] and t.index.tolist() == [[4, 2], [0, 1]] and t.tail.tolist() == [0.0, 0.0]
     with pytest.raises(AssertionError):
         w.add([[1.0] * 8], [0])
+
+
+@pytest.mark.parametrize("T", [1e-20, 1e-40, 1e20, 3e38])
+def test_temperatures_whose_square_or_inverse_leaves_fp32(T):
+    """They gave losses of 0 times infinity."""
+    import ctypes as C
+    from efficient_probing_amd import _native as N
+    v, i = torch.zeros(6, 3), torch.zeros(6, 3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="temperature"):
+        distill.TopKDistillation(v, i, temperature=T)
+    with pytest.raises(ValueError, match="temperature"):
+        distill.teacher_topk(torch.zeros(2, 5), 3, T)
+    buf = torch.zeros(64)
+    a = N.EPDistillArgs(logits=buf.data_ptr(), dtype=0, ldl=10, B=2, C=10, K=3, R=2, teacher_values=buf.data_ptr(), ldv=3, teacher_index=buf.data_ptr(), ldi=3,
+                        temperature=T, alpha=1.0, grad_scale=1.0, loss_rows=buf.data_ptr())
+    assert N.load().ep_distill_topk(C.byref(a), buf.data_ptr(), 1 << 20, 0) == -1
