@@ -113,11 +113,12 @@ def topk_distillation(logits: torch.Tensor, teacher_values: torch.Tensor, teache
     """(loss of every row (B,) fp32, d(mean loss)/dlogits * grad_scale in the logits' type, or None without ``need_grad``).
 
     ``logits`` (B, C) fp32 / bf16 / fp16, any row stride.  ``teacher_values`` / ``teacher_index`` (R, K): the teacher's logits and their
-    classes, in any order; entries with a negative class are skipped, a class listed twice takes both entries.  ``teacher_tail``
+    classes, in any order; entries with a negative class are skipped, a class listed twice counts as two entries (the loss sums
+    p (log p - log q) of each, the gradient takes the sum of their p).  ``teacher_tail``
     (R,): log of the sum of exp(logit / temperature) over the classes not listed (-inf: none); without it the listed classes are
     the teacher's whole distribution.  ``teacher_rows`` (B,) int32: batch row b reads row ``teacher_rows[b]`` of the tables in place
     (a store's table and the batch's image_index); without it row b.  ``targets`` (B,) class indices for ``alpha`` < 1; a negative
-    one takes no label term.  A row whose teacher lists nothing has no distillation term.  A class, target or row out of range
+    one takes no label term.  A row whose teacher lists nothing, and any row with ``alpha`` 0, has no distillation term.  A class, target or row out of range
     makes that row's loss and gradient NaN."""
     args = _checked(logits, teacher_values, teacher_index, targets, teacher_tail, teacher_rows, temperature, alpha)
     grad = torch.empty_like(logits, memory_format=torch.contiguous_format) if need_grad else None

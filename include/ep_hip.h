@@ -1211,11 +1211,12 @@ int ep_mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float
  *   log q_k = y[idx_k] - logsumexp(y),   log q_tail = logsumexp(y over the classes not listed) - logsumexp(y)
  *   loss_rows[b] = alpha * T^2 * sum p (log p - log q)  +  (1 - alpha) * (logsumexp(logits) - logits[target])
  *   dlogits[b, :] = grad_scale / B * d loss_rows[b] / d logits[b, :]      (grad_scale times *grad_scale_dev where given)
- * with r = teacher_rows[b] (int32, into a table of R rows read in place), or b.  A class listed more than once takes the sum of
- * its entries; entries with a negative index are skipped; a row without any entry has no distillation term, nor has any row with alpha == 0.  targets may be NULL
- * when alpha == 1; a negative target takes no label term.  A row index, class or target out of range makes the row's loss and gradient
- * NaN and is never read through.  K <= 1024, C <= 2^20, T within [1e-15, 1e15].  dlogits (same type and row stride rules as logits, not overlapping them) may
- * be NULL. */
+ * with r = teacher_rows[b] (int32, into a table of R rows read in place), or b.  A class listed more than once counts entry by entry:
+ * the loss sums p (log p - log q) of each, the gradient takes the sum of their p.  Entries with a negative index are skipped; a row
+ * without any entry has no distillation term, nor has any row with alpha == 0.  targets may be NULL when alpha == 1; a negative target
+ * takes no label term.  A row index, class or target out of range makes the row's loss and gradient NaN and is never read through.
+ * K <= 1024, C <= 2^20, T within [1e-15, 1e15].  dlogits (same type and row stride rules as logits, not overlapping them) may be
+ * NULL. */
 typedef struct ep_distill_args {
   const void* logits; int32_t dtype; int64_t ldl;       /* fp32 / bf16 / fp16; row stride in elements, >= C */
   int32_t B, C, K; int64_t R;                           /* R: rows of the teacher's tables */
