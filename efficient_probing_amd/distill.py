@@ -150,7 +150,8 @@ def distillation_loss(logits: torch.Tensor, teacher_values: torch.Tensor, teache
                       teacher_tail: Optional[torch.Tensor] = None, teacher_rows: Optional[torch.Tensor] = None, temperature: float = 1.0,
                       alpha: float = 1.0) -> torch.Tensor:
     """Mean of ``topk_distillation``'s row losses, differentiable in ``logits`` (the teacher takes no gradient)."""
-    return _Distillation.apply(logits, teacher_values, teacher_index, targets, teacher_tail, teacher_rows, temperature, alpha)
+    tail = None if teacher_tail is None else teacher_tail.detach()
+    return _Distillation.apply(logits, teacher_values.detach(), teacher_index, targets, tail, teacher_rows, temperature, alpha)
 
 
 @torch.no_grad()

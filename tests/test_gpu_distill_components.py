@@ -86,3 +86,19 @@ def test_without_weight_the_teacher_does_not_count(C, tail_on):
     assert (loss.double().cpu() - want.detach()).abs().max() <= 192 * U * 20
     one = torch.nn.functional.one_hot(tgt, C)
     assert ((grad.double().cpu() - ref.grad).abs() <= 320 * U * (ref.grad.abs() + 2 * one) + 2.0 ** -126).all()
+
+
+def test_a_teacher_that_requires_gradients():
+    """The teacher's logits of a model that trains elsewhere: it takes no gradient, the student does; without a student that trains the loss
+    is a constant."""
+    from efficient_probing_amd import distill
+    B, C, K = 4, 50, 6
+    val, idx, tail = _teacher(B, C, K, 1)
+    v, t = torch.as_tensor(val, device=DEV).requires_grad_(), torch.as_tensor(tail, device=DEV).requires_grad_()
+    i, z = torch.as_tensor(idx, device=DEV), torch.randn(B, C, device=DEV)
+    assert not distill.distillation_loss(z, v, i, teacher_tail=t).requires_grad
+    q = z.clone().requires_grad_()
+    loss = distill.distillation_loss(q, v * 1.0, i, teacher_tail=t * 1.0)
+    loss.backward()
+    rows, grad = distill.topk_distillation(z, v, i, teacher_tail=t)
+    assert v.grad is None and t.grad is None and torch.equal(q.grad, grad) and not rows.requires_grad and not grad.requires_grad
