@@ -238,6 +238,13 @@ def _reads_parts(model) -> bool:
     return head is not None and native_engine_name(head) == "ProbeHeadEngine"
 
 
+def _token_model(model, stored: bool):
+    """What a batch of the module path goes through: a store's tokens are the native head's, whatever the model does in front of it (as
+    on the fused path).  A data-parallel wrapper is called itself, or its gradients would not be averaged."""
+    head = _native_head(model) if stored and not hasattr(model, "module") else None
+    return model if head is None else head
+
+
 def _batch_tokens(samples, image_index, in_place: bool, engine):
     """(tokens, image_index) as a head reads them: a 4-bit batch in place, or decoded for the heads that take token tensors (bf16 for
     an engine, which holds the 4-bit values exactly in half the bytes; fp32 for modules, whose weights are fp32)."""
@@ -359,7 +366,7 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
             if mixup_fn is not None:
                 samples, targets = mixup_fn(samples, targets)
             with torch.autocast("cuda", enabled=(amp != "none" and samples.is_cuda), dtype=AMP_PRECISIONS[amp]):
-                outputs = model(samples)
+                outputs = _token_model(model, cached or rows is not None)(samples)
                 loss = criterion(outputs, targets, rows) if distill else criterion(outputs, targets)
             acc1, acc5 = accuracy(outputs.float(), targets if targets.dim() == 1 else targets.argmax(1))
             metric_logger.update(acc1=acc1.item(), acc5=acc5.item())

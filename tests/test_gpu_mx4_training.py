@@ -278,3 +278,32 @@ def test_refusals():
         other.forward_backward(store.tokens, store.labels)
     with pytest.raises(NotImplementedError):
         other.eval_logits(store.tokens)
+
+
+@pytest.mark.parametrize("head", ["ep", "simpool"])
+@pytest.mark.parametrize("codes", [True, False])
+def test_stored_tokens_go_to_the_head_of_an_encoder(head, codes):
+    """A model whose forward starts from images: what a store holds are its tokens, which are the head's on the module path as on the
+    fused one (distillation of a head without the fused form; a clipping bound with the EP head)."""
+    from efficient_probing_amd import distill, mx4, token_store as TS
+    from efficient_probing_amd.util.misc import NativeScalerWithGradNormCount
+    store = _store(48, 16, 128, 7)
+    if not codes:
+        store = TS.ResidentTokenStore.from_tensors(mx4.dequantize_tokens(store.tokens, torch.float32), store.labels, teacher=store.teacher)
+
+    class Encoder(torch.nn.Module):
+        def __init__(self, head):
+            super().__init__()
+            self.patch_embed = torch.nn.Conv2d(3, 128, 4, 4)
+            for p in self.parameters():
+                p.requires_grad_(False)
+            self.head = head
+
+        def forward(self, images):
+            return self.head(self.patch_embed(images).flatten(2).transpose(1, 2))
+    plain, full = _model(128, 7, head=head, num_heads=4), _model(128, 7, head=head, num_heads=4)
+    full = Encoder(full.head).to(DEV)
+    out = [_epoch(m, store, distill.TopKDistillation.from_store(store, alpha=0.5), max_norm=1e9, loss_scaler=NativeScalerWithGradNormCount())[0][0] for m in (plain, full)]
+    assert out[0]["loss"] == out[1]["loss"] and np.isfinite(out[0]["loss"])
+    for p, q in zip(plain.head.parameters(), full.head.parameters()):
+        assert torch.equal(p, q)
