@@ -256,7 +256,10 @@ class ResidentTokenStore:
         self.tokens = _tokens(meta, parts)
         self.num_images = n
         self.teacher: Optional[TeacherRows] = None
-        if teacher:
+        if meta.get("teacher"):
+            if not teacher:                                  # (a rank without shards: one row that lists nothing)
+                k = meta["teacher"]["k"]
+                teacher = [{"values": np.zeros((1, k), np.float32), "index": np.full((1, k), -1, np.int32), "tail": np.full(1, -np.inf, np.float32)}]
             cat = lambda k: torch.from_numpy(np.concatenate([t[k] for t in teacher])).to(device)
             self.teacher = TeacherRows(cat("values"), cat("index"), cat("tail") if meta["teacher"]["tail"] else None, meta["teacher"]["temperature"])
         self.labels = torch.from_numpy(np.concatenate(labels) if labels else np.zeros(0, np.int64)).to(device)

@@ -190,3 +190,17 @@ def test_temperatures_whose_square_or_inverse_leaves_fp32(T):
     a = N.EPDistillArgs(logits=buf.data_ptr(), dtype=0, ldl=10, B=2, C=10, K=3, R=2, teacher_values=buf.data_ptr(), ldv=3, teacher_index=buf.data_ptr(), ldi=3,
                         temperature=T, alpha=1.0, grad_scale=1.0, loss_rows=buf.data_ptr())
     assert N.load().ep_distill_topk(C.byref(a), buf.data_ptr(), 1 << 20, 0) == -1
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_a_rank_without_shards_has_a_teacher_too(tmp_path, tail):
+    """More ranks than shards: every rank builds the same criterion; the empty one's table lists nothing."""
+    w = TS.TokenStoreWriter(str(tmp_path), 2, 8, teacher_temperature=3.0)
+    w.add(np.zeros((4, 2, 8)), np.zeros(4), teacher=(np.ones((4, 5)), np.ones((4, 5))) + ((np.ones(4),) if tail else ()))
+    w.close()
+    st = TS.ResidentTokenStore(str(tmp_path), "cpu", world=3, rank=2)
+    assert st.num_images == 0 and st.num_batches(2) == 0
+    crit = distill.TopKDistillation.from_store(st, alpha=0.5)
+    assert crit.temperature == 3.0 and crit.teacher_values.shape == (1, 5) and (crit.teacher_index == -1).all() and (crit.teacher_tail is not None) == tail
+    if tail:
+        assert torch.isneginf(crit.teacher_tail).all()
