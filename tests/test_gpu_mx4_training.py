@@ -307,3 +307,31 @@ def test_stored_tokens_go_to_the_head_of_an_encoder(head, codes):
     assert out[0]["loss"] == out[1]["loss"] and np.isfinite(out[0]["loss"])
     for p, q in zip(plain.head.parameters(), full.head.parameters()):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("codes", [True, False])
+def test_logits_of_a_step_in_its_parts(codes):
+    """``last_train_logits`` after such a step are the train-mode logits of its batch (BatchNorm over the batch), and those of a later step
+    through the one library call are not these any more."""
+    from efficient_probing_amd import distill, mx4
+    from efficient_probing_amd.engine import ProbeHeadEngine
+    store = _store(40, 25, 256, 13, lengths=codes)
+    idx = torch.arange(3, 27, dtype=torch.int32, device=DEV)
+    head = _model(256, 13, 8).head.train()
+    x = mx4.dequantize_tokens(store.tokens, torch.float32)
+    ln = store.tokens.lengths[idx.long()] if codes else None
+    eng = ProbeHeadEngine(head, optimizer="sgd", lr=0.0)
+    eng.forward_backward_parts(store.tokens if codes else x, store.labels[idx.long()], idx, distill.TopKDistillation.from_store(store))
+    got = eng.last_train_logits()
+    pool, bn, fc = head[0], head[1], head[2]
+    xb = x[idx.long()].double().cpu()
+    S = torch.einsum("qd,bnd->bqn", pool.cls_token.detach().double().cpu()[0] * pool.scale, xb)
+    if codes:
+        S = S.masked_fill(torch.arange(25) >= ln.cpu().long()[:, None, None], -torch.inf)
+    P = torch.einsum("bqn,bnd->bqd", torch.nan_to_num(torch.softmax(S, -1)), xb)
+    y = torch.einsum("bqd,qkd->bqk", P, pool.v.weight.detach().double().cpu().view(8, -1, 256)).reshape(24, -1)
+    want = ((y - y.mean(0)) / torch.sqrt(y.var(0, unbiased=False) + bn.eps)) @ fc.weight.detach().double().cpu().t() + fc.bias.detach().double().cpu()
+    _close(got, want, 1280 * U)
+    eng.optimizer_step(0.0)
+    eng.train_step(x[:8].contiguous(), store.labels[:8])
+    assert eng.last_train_logits().shape == (8, 13)
