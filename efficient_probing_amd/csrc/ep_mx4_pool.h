@@ -19,7 +19,7 @@ struct MxPool {
   int nc, nw, groups;                    // 128-channel blocks of a row; waves a row is cut over; such groups of waves in a workgroup
   int splits, tps, units;                // an image's tiles are cut into `splits` runs of `tps`; unit = image * splits + run
   int per_unit;                          // backward: a gradient per unit instead of per workgroup
-  int ldq;                               // row stride of the operand rows
+  int vecq;                              // how the operand rows lie: 2 whole blocks, 1 whole 16-byte pieces, 0 anything
   int veco;                              // 16-byte stores to the outputs
 };
 

@@ -158,11 +158,22 @@ __device__ __forceinline__ void mx_operand(const mx_f16& a, const mx_f16& b, int
   if constexpr (MxDims<QM>::SCB > 1) o.sc[1] = bytes[1];
 }
 
-// 32 values of an operand row (16-byte aligned, whole 128-channel blocks: other rows are padded first), times mul
-__device__ __forceinline__ void mx_load_row(const float* row, float mul, mx_f16& a, mx_f16& b) {
+// 32 values of an operand row from `row` on, times mul; `valid` of them exist, the others are 0.  vec (uniform) says how they lie: 2 rows
+// of whole 128-channel blocks, 1 whole 16-byte pieces, 0 anything
+__device__ __forceinline__ void mx_load_row(const float* row, int valid, int vec, float mul, mx_f16& a, mx_f16& b) {
   f4 x[8];
+  if (vec == 2) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const f4*>(row)[i];
+    for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const f4*>(row)[i];
+  } else if (vec == 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 4 * i < valid ? reinterpret_cast<const f4*>(row)[i] : f4{0.f, 0.f, 0.f, 0.f};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i][j] = 4 * i + j < valid ? row[4 * i + j] : 0.f;
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     a[2 * i] = x[i][0] * mul; b[2 * i] = x[i][1] * mul;
@@ -269,23 +280,25 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
   auto load_operand = [&](const float* rows, const float* prows, float mul) {
     const int ln = mx_fresh(lane), c = ln & 15, q = c & 7;
     const bool up = (c & 8) != 0;
-    const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * p.ldq + 32 * (ln >> 4);      // (rows without a query: the first one's, times 0)
+    const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * t.D;          // (rows without a query: the first one's, times 0)
     const int mine = chunk0 + (up ? 2 : 0);
-    float d = 0.f;
+    float sum = 0.f;
     uint32_t sc[CPW];
     mx_f16 ve, vo;
     auto load = [&](int i) {
       const bool in = mine + i < nc;
-      mx_load_row(rows + at + (in ? mine + i : nc - 1) * MX_BLOCK, in && q < qn ? mul : 0.f, ve, vo);
+      const int d = (in ? mine + i : nc - 1) * MX_BLOCK + 32 * (ln >> 4);
+      mx_load_row(rows + at + d, t.D - d, p.vecq, in && q < qn ? mul : 0.f, ve, vo);
     };
     load(1);
 #pragma unroll 1
     for (int i = 1; i >= 0; --i) {
       if (BWD && prows) {
         mx_f16 we, wo;
-        mx_load_row(prows + at + (mine + i < nc ? mine + i : nc - 1) * MX_BLOCK, 1.f, we, wo);
+        const int d = (mine + i < nc ? mine + i : nc - 1) * MX_BLOCK + 32 * (ln >> 4);
+        mx_load_row(prows + at + d, t.D - d, p.vecq, 1.f, we, wo);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) d = fmaf(vo[j], wo[j], fmaf(ve[j], we[j], d));
+        for (int j = 0; j < 16; ++j) sum = fmaf(vo[j], wo[j], fmaf(ve[j], we[j], sum));
         __builtin_amdgcn_sched_barrier(0);
       }
       op[1] = op[0]; op[3] = op[2]; sc[1] = sc[0]; sc[3] = sc[2];
@@ -313,11 +326,11 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
       __builtin_amdgcn_sched_barrier(0);
     }
     *reinterpret_cast<mx_u4*>(opsc + ln * 16) = mx_u4{sc[0], sc[1], sc[2], sc[3]};
-    return BWD && prows ? mx_over_groups_sum(d + mx_ror8(d)) : 0.f;
+    return BWD && prows ? mx_over_groups_sum(sum + mx_ror8(sum)) : 0.f;
   };
   float delta = 0.f, m_run, mz, l_run, t_max, invl;                     // mz: the maximum that weights are taken against
   auto open_unit = [&](int b) {                                         // backward: dP's rows and the saved statistics
-    delta = load_operand(p.q + (int64_t)b * p.Q * p.ldq, p.Pin ? p.Pin + (int64_t)b * p.Q * p.ldq : nullptr, 1.f);
+    delta = load_operand(p.q + (int64_t)b * p.Q * t.D, p.Pin ? p.Pin + (int64_t)b * p.Q * t.D : nullptr, 1.f);
     const int q = mx_fresh(lane) & 7;
     f4 ml = {0.f, 0.f, 0.f, 0.f};
     if (q < qn) ml = *reinterpret_cast<const f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4);
@@ -700,15 +713,16 @@ __global__ __launch_bounds__(1024, 4) void ep_mx4_pipe_kernel(MxPool p) {
     int parity = 0;
     auto open_unit = [&](int b) {                                       // the operand rows; backward: this block's part of delta = dP . P
       const int ln = mx_fresh(lane), c = ln & 15, g = ln >> 4;
-      const float* rows = p.q + (BWD ? (int64_t)b * p.Q * p.ldq : (int64_t)b * p.qb);
+      const float* rows = p.q + (BWD ? (int64_t)b * p.Q * t.D : (int64_t)b * p.qb);
       const int q = QM == 8 ? c & 7 : c;
-      const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * p.ldq + wave * MX_BLOCK + 32 * g;    // (rows without a query: the first one's, times 0)
+      const int lo = wave * MX_BLOCK + 32 * g;
+      const int64_t at = (int64_t)(q0 + (q < qn ? q : 0)) * t.D + lo;   // (rows without a query: the first one's, times 0)
       mx_f16 ve, vo;
-      mx_load_row(rows + at, q < qn ? (BWD ? 1.f : p.scale) : 0.f, ve, vo);
+      mx_load_row(rows + at, t.D - lo, p.vecq, q < qn ? (BWD ? 1.f : p.scale) : 0.f, ve, vo);
       if (BWD && p.Pin) {
         float d = 0.f;
         mx_f16 we, wo;
-        mx_load_row(p.Pin + (int64_t)b * p.Q * p.ldq + at, 1.f, we, wo);
+        mx_load_row(p.Pin + (int64_t)b * p.Q * t.D + at, t.D - lo, p.vecq, 1.f, we, wo);
 #pragma unroll
         for (int i = 0; i < 16; ++i) d = fmaf(vo[i], wo[i], fmaf(ve[i], we[i], d));
         d = mx_over_groups_sum(d);
@@ -1153,19 +1167,10 @@ __global__ __launch_bounds__(256) void ep_mx4_sum_kernel(const float* __restrict
   }
 }
 
-// rows of D channels -> rows of whole 128-channel blocks, zero-filled
-__global__ __launch_bounds__(256) void ep_mx4_pad_rows_kernel(const float* __restrict__ src, int64_t rows, int D, int Dp, float* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * Dp; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / Dp;
-    const int d = (int)(i - r * Dp);
-    out[i] = d < D ? src[r * D + d] : 0.f;
-  }
-}
-
 struct MxPlan {
-  int qm, cpw, nw, groups, splits, tps, units, grid, yblk, qblk;
+  int qm, nw, groups, splits, tps, units, grid, yblk, qblk;
   bool pipe;                                                            // the pipelined form, or the wide-row form
-  size_t lds, ws, pad;                                                  // ws: bytes, of them pad for padded operand rows
+  size_t lds, ws;                                                       // bytes
 };
 
 static size_t mx_pipe_lds(int qm, int nw) {
@@ -1182,7 +1187,7 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
     // (512 x 256 x 1792, 8 queries: 42 us forward and 60 backward; wide-row form 50 and 63.  Narrower rows gain more.)  More than 8
     // queries: blocks of 16 (512 x 256 x 768: 16 queries 30 us forward, as two blocks of 8 43; 8 queries as a block of 16 27, of 8 25.5)
     p.qm = Q <= 8 ? 8 : 16;
-    p.nw = nc; p.cpw = 1; p.groups = 1;
+    p.nw = nc; p.groups = 1;
     constexpr int waves = 16;                                           // four a SIMD
     p.pipe = true;
     p.lds = mx_pipe_lds(p.qm, nc);
@@ -1190,7 +1195,7 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
     cap = cus * (waves / (nc + 1) < n ? waves / (nc + 1) : n);
   } else {                                                              // four blocks per wave
     p.qm = 8;
-    p.nw = (nc + 3) / 4; p.cpw = 4;
+    p.nw = (nc + 3) / 4;
     p.groups = bwd || B <= cus ? 8 / p.nw : 1;
     const int waves = p.nw * p.groups;
     p.lds = (size_t)waves * (MX_STAGES * (2048 * 4 + 512)) + 3 * (size_t)waves * 1024;
@@ -1221,24 +1226,11 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   }
   if (bwd) p.ws = !per_image ? (size_t)p.grid * Q * D * 4 : p.splits > 1 ? (size_t)p.units * Q * D * 4 : 0;
   else p.ws = p.splits > 1 ? (size_t)p.units * Q * (D + 2) * 4 : 0;
-  const size_t rows = (size_t)(bwd ? 2 * (int64_t)B * Q : per_image ? (int64_t)B * Q : Q);
-  p.pad = D % MX_BLOCK ? round_up(rows * nc * MX_BLOCK * 4, 256) : 0;
-  p.ws += p.pad;
   return p;
 }
 
-// operand rows as the kernel reads them
-static int mx_rows(const float* src, int64_t rows, int D, char*& ws, const float** out, hipStream_t st) {
-  *out = src;
-  if (D % MX_BLOCK == 0) return 0;
-  const int Dp = mx_blocks(D) * MX_BLOCK;
-  const int64_t grid = (rows * Dp + 255) / 256;
-  hipLaunchKernelGGL(ep_mx4_pad_rows_kernel, dim3((unsigned)(grid < 1 << 20 ? grid : 1 << 20)), dim3(256), 0, st, src, rows, D, Dp, reinterpret_cast<float*>(ws));
-  EP_LAUNCH_CHECK("ep_mx4_pad_rows_kernel");
-  *out = reinterpret_cast<float*>(ws);
-  ws += (size_t)rows * Dp * 4;
-  return 0;
-}
+// how the operand rows lie (mx_load_row)
+static int mx_rows(int D, const float* a, const float* b) { return D % 4 || !aligned16(a) || !aligned16(b) ? 0 : D % MX_BLOCK ? 1 : 2; }
 
 template <typename K>
 static int mx_launch_kernel(K* fn, const MxPool& p, const MxPlan& pl, int threads, hipStream_t st) {
@@ -1260,7 +1252,6 @@ static MxPool mx_pool_params(const ep_mx4_tokens* t, int Q, float scale, const M
   MxPool p{};
   p.t = *t; p.Q = Q; p.scale = scale; p.nc = mx_blocks(t->D);
   p.nw = pl.nw; p.groups = pl.groups; p.splits = pl.splits; p.tps = pl.tps; p.units = pl.units; p.qblk = pl.qblk;
-  p.ldq = p.nc * MX_BLOCK;
   return p;
 }
 
@@ -1269,10 +1260,8 @@ int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bst
   const MxPlan pl = mx_plan(t->B, t->N, t->D, Q, false, q_bstride != 0);
   EP_REQUIRE(ws_bytes >= pl.ws, EP_E_WORKSPACE, "ep_mx4_pool_forward: workspace %zu < %zu", ws_bytes, pl.ws);
   MxPool p = mx_pool_params(t, Q, scale, pl);
-  char* w = static_cast<char*>(ws);
-  p.qb = q_bstride ? (int64_t)Q * p.ldq : 0; p.P = P; p.S = S; p.ML = ML;
-  EP_TRY(mx_rows(queries, q_bstride ? (int64_t)t->B * Q : Q, t->D, w, &p.q, st));
-  p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + pl.pad); p.part_ml = p.part + (size_t)pl.units * Q * t->D;
+  p.q = queries; p.qb = q_bstride; p.vecq = mx_rows(t->D, queries, nullptr); p.P = P; p.S = S; p.ML = ML;
+  p.part = static_cast<float*>(ws); p.part_ml = p.part + (size_t)pl.units * Q * t->D;
   p.veco = t->D % 4 == 0 && aligned16(pl.splits > 1 ? (const void*)p.part : (const void*)P);
   p.lds_ = s_stride;
   EP_TRY(mx_launch<false>(p, pl, st));
@@ -1292,12 +1281,10 @@ int mx4_pool_backward(const ep_mx4_tokens* t, int Q, float scale, const float* S
   const MxPlan pl = mx_plan(t->B, t->N, t->D, Q, true, per_image != 0);
   EP_REQUIRE(ws_bytes >= pl.ws, EP_E_WORKSPACE, "ep_mx4_pool_backward: workspace %zu < %zu", ws_bytes, pl.ws);
   MxPool p = mx_pool_params(t, Q, scale, pl);
-  char* w = static_cast<char*>(ws);
-  EP_TRY(mx_rows(dP, (int64_t)t->B * Q, t->D, w, &p.q, st));
-  if (P) EP_TRY(mx_rows(P, (int64_t)t->B * Q, t->D, w, &p.Pin, st));
+  p.q = dP; p.Pin = P; p.vecq = mx_rows(t->D, dP, P);
   p.S = const_cast<float*>(S); p.ML = const_cast<float*>(ML);
   p.per_unit = per_image != 0;
-  p.part = per_image && pl.splits == 1 ? dq : reinterpret_cast<float*>(static_cast<char*>(ws) + pl.pad);
+  p.part = per_image && pl.splits == 1 ? dq : static_cast<float*>(ws);
   p.veco = t->D % 4 == 0 && aligned16(p.part);
   p.lds_ = s_stride;
   const int64_t QD = (int64_t)Q * t->D;

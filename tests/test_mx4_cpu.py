@@ -146,3 +146,14 @@ def test_attention_oracle_against_differences():
         qp[pos] += h; qm[pos] -= h
         d = ((mx4_oracle.attention(x, ln, qp, 0.4)[0] - mx4_oracle.attention(x, ln, qm, 0.4)[0]) * dP).sum() / (2 * h)
         assert abs(d - dq[pos]) < 1e-8
+
+
+@pytest.mark.parametrize("D", [100, 192, 1000, 1088, 2500, 4090])
+def test_workspace_does_not_grow_with_the_batch(D):
+    """Operand rows are read where they lie, also where a row is not whole 128-channel blocks: what is left is the workgroups' partial
+    gradients (at most 16 waves on each of a chip's compute units, taken as 304 at most)."""
+    from efficient_probing_amd import _native as N
+    lib = N.load()
+    for Q in (1, 8, 32):
+        sizes = {lib.ep_mx4_pool_workspace_bytes(B, 20, D, Q) for B in (8192, 16384, 65536)}
+        assert len(sizes) == 1 and 0 < sizes.pop() <= 304 * 8 * Q * D * 4 + 256
