@@ -125,6 +125,16 @@ def topk_distillation(logits: torch.Tensor, teacher_values: torch.Tensor, teache
     return _call(*args, float(grad_scale), None, grad), grad
 
 
+def mean_rows(rows: torch.Tensor) -> torch.Tensor:
+    """Mean of row losses, by sums of at most 65536 at a time: a library reduction over several workgroups clears its counters by a memset,
+    which a captured graph does not repeat, and gives the first replay's mean ever after."""
+    n = rows.shape[0]
+    while rows.shape[0] > 65536:
+        whole = rows.shape[0] // 1024 * 1024
+        rows = torch.cat((rows[:whole].view(-1, 1024).sum(1), rows[whole:]))
+    return rows.sum() / n
+
+
 class _Distillation(torch.autograd.Function):
     """The backward pass runs the rows again with the incoming gradient as its scale: no second buffer of the logits' size is kept or
     rescaled, and a loss scale acts before the gradient is rounded to a 16-bit type."""
@@ -135,7 +145,7 @@ class _Distillation(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             ctx.save_for_backward(*args[:6])
             ctx.t, ctx.alpha = args[6:]
-        return _call(*args, 1.0, None, None).mean()
+        return mean_rows(_call(*args, 1.0, None, None))
 
     @staticmethod
     @once_differentiable

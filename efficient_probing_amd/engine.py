@@ -25,6 +25,7 @@ import torch.nn as nn
 from . import _native as N
 from . import functional as F_
 from . import mx4
+from .distill import mean_rows
 
 OPTIMIZERS = {"lars": 0, "sgd": 1, "adamw": 2}
 
@@ -573,7 +574,7 @@ class ProbeHeadEngine:
         else:
             rows, dl = criterion.rows_and_gradient(logits, targets, image_index if not cached else cache.image_index, grad_scale)
             _, _, st = F_.cross_entropy(logits, targets, need_grad=False)
-            st[0] = rows.mean()
+            st[0] = mean_rows(rows)
             st[3] = (~torch.isfinite(rows)).sum()
             self.stats += st
         if self._scaler is not None:

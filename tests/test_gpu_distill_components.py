@@ -102,3 +102,27 @@ def test_a_teacher_that_requires_gradients():
     loss.backward()
     rows, grad = distill.topk_distillation(z, v, i, teacher_tail=t)
     assert v.grad is None and t.grad is None and torch.equal(q.grad, grad) and not rows.requires_grad and not grad.requires_grad
+
+
+def test_captured_means_of_growing_batches():
+    """One graph after another, up to batches whose mean would take several workgroups: replays follow the logits, with eager work between."""
+    from efficient_probing_amd import distill
+    for B in (1000, 20000, 100000, 300000, 2000000):
+        g = torch.Generator(device=DEV).manual_seed(1)
+        z, v = torch.randn(B, 4, device=DEV, generator=g), torch.randn(B, 2, device=DEV, generator=g)
+        i = torch.randint(0, 4, (B, 2), device=DEV, generator=g, dtype=torch.int32)
+        zs = z.clone()
+        distill.distillation_loss(zs, v, i)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = distill.distillation_loss(zs, v, i)
+        for k in range(6):
+            zs.copy_(z * (k + 1))
+            want = distill.distillation_loss(zs, v, i)
+            torch.randn(1000000, device=DEV).sum().item()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert float(out) == float(want), (B, k)
+        exact = float(distill.topk_distillation(zs, v, i)[0].double().mean())
+        assert abs(float(want) - exact) <= 64 * U * abs(exact)
