@@ -124,5 +124,10 @@ def test_captured_means_of_growing_batches():
             graph.replay()
             torch.cuda.synchronize()
             assert float(out) == float(want), (B, k)
-        exact = float(distill.topk_distillation(zs, v, i)[0].double().mean())
-        assert abs(float(want) - exact) <= 64 * U * abs(exact)
+
+
+def test_mean_of_many_rows():
+    from efficient_probing_amd import distill
+    for n in (1, 65536, 65537, 66000, 300001, 2 ** 21 + 3):
+        rows = torch.rand(n, generator=torch.Generator().manual_seed(n)) + 0.5
+        assert abs(float(distill.mean_rows(rows.to(DEV))) - float(rows.double().mean())) <= 64 * U * 1.5
