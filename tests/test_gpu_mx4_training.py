@@ -335,3 +335,57 @@ def test_logits_of_a_step_in_its_parts(codes):
     eng.optimizer_step(0.0)
     eng.train_step(x[:8].contiguous(), store.labels[:8])
     assert eng.last_train_logits().shape == (8, 13)
+
+
+def test_loss_scale_skips_a_step_in_its_parts():
+    """A loss scale that overflows the gradients: the update is skipped and the scale halved, on codes as on plain tokens; the next steps go on."""
+    from efficient_probing_amd import mx4
+    from efficient_probing_amd.engine import ProbeHeadEngine
+    from efficient_probing_amd.util.misc import NativeScalerWithGradNormCount
+    store = _store(16, 9, 128, 7, tail=False)
+    x = mx4.dequantize_tokens(store.tokens, torch.float32)
+    out = []
+    for tokens in (store.tokens, x):
+        head = _model(128, 7).head.train()
+        with torch.no_grad():
+            head[2].weight *= 1e4                                          # (gradients of y are 10^4 times the logits')
+        scaler = NativeScalerWithGradNormCount()
+        scaler._scale = 2.0 ** 120
+        eng = ProbeHeadEngine(head, optimizer="sgd")
+        eng.attach_scaler(scaler)
+        start = eng.flat_p.clone()
+        scales, moved = [], []
+        for _ in range(8):
+            before = eng.flat_p.clone()
+            eng.train_step(tokens, store.labels, lr=1e-3)
+            scales.append(scaler.get_scale())
+            moved.append(not torch.equal(before, eng.flat_p))
+        assert bool(torch.isfinite(eng.flat_p).all()) and not moved[0] and any(moved)
+        out.append((scales, moved, eng.flat_p - start))
+    assert out[0][0] == out[1][0] and out[0][1] == out[1][1]
+    assert (out[0][2] - out[1][2]).norm() <= 8192 * U * out[1][2].norm()
+
+
+def test_two_streams_at_once():
+    """Forward and backward over one cache on two streams, interleaved from the host: workspaces are each call's own."""
+    from efficient_probing_amd import mx4
+    store = _store(64, 197, 384, 9)
+    g = torch.Generator().manual_seed(3)
+    qs = [torch.randn(12, 384, generator=g).to(DEV) for _ in range(2)]
+    dP = torch.randn(64, 12, 384, generator=g).to(DEV)
+    def call(q):
+        P, S, ML = mx4.pool_forward(store.tokens, q, 0.05)
+        return P, mx4.pool_backward(store.tokens, S, ML, dP, 0.05, P=P)
+    want = [call(q) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(10):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(call(qs[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for P, dq in got[k]:
+            assert torch.equal(P, want[k][0]) and torch.equal(dq, want[k][1])
