@@ -72,3 +72,36 @@ def test_rows_of_uneven_channels(B, N, D, Q, kind, per_image):
     if not per_image:
         lim, want = lim.sum(0), want.sum(0)
     assert over(dq, want, lim) <= 1.0, over(dq, want, lim)
+
+
+@pytest.mark.parametrize("B,N,D,Q", [(2, 70, 256, 8), (2, 70, 200, 16), (2, 70, 2048, 5)])
+def test_powers_of_two_pass_through(B, N, D, Q):
+    """Gradients and queries times a power of two: the same bits, moved (terms, weights and sums all scale)."""
+    from efficient_probing_amd import mx4
+    g = torch.Generator().manual_seed(D)
+    c = mx4.quantize_tokens(torch.randn(B, N, D, generator=g).to(DEV))
+    q, dP = torch.randn(Q, D, generator=g).to(DEV), torch.randn(B, Q, D, generator=g).to(DEV)
+    P, S, ML = mx4.pool_forward(c, q, 0.125)
+    dq = mx4.pool_backward(c, S, ML, dP, 0.125, P=P)
+    for k in (-60, -20, 20, 60):
+        assert torch.equal(mx4.pool_backward(c, S, ML, dP * 2.0 ** k, 0.125, P=P), dq * 2.0 ** k)
+        for a, b in zip(mx4.pool_forward(c, q * 2.0 ** k, 0.125 * 2.0 ** -k), (P, S, ML)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D", [256, 2048])
+def test_rows_at_the_ends_of_fp32(D):
+    """Rows near fp32's largest and smallest values stay finite and right; a row with an infinity or a NaN spoils its own query alone."""
+    from efficient_probing_amd import mx4
+    x = torch.zeros(1, 40, D)
+    x[0, :, 5] = torch.arange(40) % 5 - 2.0
+    c = mx4.quantize_tokens(x.to(DEV))
+    q = torch.zeros(6, D)
+    q[0, 5], q[1, 5], q[2, 5], q[3, 5], q[4, 7], q[5, 9] = 3.0e38, 2.0 ** -120, 1.5 * 2.0 ** -126, 1.0, float("inf"), float("nan")
+    P, S, ML = mx4.pool_forward(c, q.to(DEV), 0.25)
+    want = (q[:4, 5].double() * 0.25)[:, None] * x[0, :, 5].double()
+    got = S[0, :4].double().cpu()
+    # a term's scale is a normal number, 2^(5 t - 127) at least for the t-th last: the last term's grid is 2^(5 - 127) / 8 = 2^-125 (wide rows
+    # alike), so that up to 2^-126 of a channel is lost whatever its size; times |x| <= 2
+    assert ((got - want).abs() <= 2.0 ** -23 * want.abs() + 2.0 ** -126 * 2.0).all()
+    assert bool(torch.isfinite(P[0, :4]).all()) and bool(torch.isnan(P[0, 4:]).all())
