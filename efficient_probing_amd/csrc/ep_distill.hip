@@ -4,8 +4,8 @@
 // (a wave for up to 1024 classes, four rows a workgroup; 4 or 8 waves above): one read, then maximum, sums of exponentials, gradient.
 // Longer rows are cut into pieces of 4096 over many workgroups in two launches: partial maxima and sums, then each piece's gradient.
 // Measured with 64 listed classes and a tail (bytes read and written per second; a copy of the same size reaches 4.7 TB/s):
-// 2048 x 32768 bf16 57 us (4.7 TB/s), 2048 x 21841 bf16 46 us (3.9), 4096 x 10000 fp32 67 us (4.9), 16384 x 1000 fp32 31 us (4.2);
-// in pieces 512 x 100000 fp32 111 us (3.7: the second launch reads the logits again), 6 x 131071 fp32 14 us (one workgroup a row:
+// 2048 x 32768 bf16 61 us (4.4 TB/s), 2048 x 21841 bf16 48 us (3.7), 4096 x 10000 fp32 68 us (4.8), 16384 x 1000 fp32 36 us (3.6);
+// in pieces 512 x 100000 fp32 129 us (3.2: the second launch reads the logits again), 6 x 131071 fp32 14 us (one workgroup a row:
 // 310 us).  bf16 rows are also near the vector unit's rate: about 16 instructions a class, two of them exponentials.
 //
 // The classes that the teacher lists are marked in an LDS bit map, so that the mass of all others is summed without them and not formed

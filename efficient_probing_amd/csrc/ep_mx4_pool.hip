@@ -20,9 +20,10 @@
 //
 // QM 8: up to 8 queries, rows of a 16-row matrix instruction = 8 queries x 2 terms.  QM 16: up to 16.  More: blockIdx.y.
 //
-// Bound: HBM, then decoding.  Reading 107 MB of codes takes 20 us at the rate this ring streams them, decoding and both contractions 23 us
-// of the matrix and vector units beside it (1024 x 256 x 768, 8 queries: 37 us in all forward, of them about 10 before the first tile
-// and behind the last; 2048 images: 66 us, 3.2 TB/s).
+// Bound: the chain from a tile's arrival to its weights, and the start of a launch, more than any one unit.  1024 x 256 x 768, 8 queries:
+// forward 42 us (38 back to back), 142 MB from and to HBM at 3.4 TB/s, matrix units busy 17 % of the time, waves waiting 43 % of their
+// cycles (barriers and loads) and stalled at issue 27 %; backward 51 us, 208 MB at 4.1 TB/s, 14 %, 49 % and 25 %.  Twice the images take
+// 67 and 99 us back to back: some 10 us a launch lie before the first tile and behind the last.
 #include "ep_mx4.h"
 #include "ep_mx4_pool.h"
 
@@ -214,7 +215,7 @@ struct MxCursor {
 // lane constants are made again where they are used and the operands' scale bytes lie in LDS, since a register reloaded from scratch waits
 // for the tiles in flight.  Bound:
 // matrix and vector units with two waves a SIMD (256 x 784 x 4096, 4 queries: 126 us forward, 3.5 TB/s), and about 20 us for the operand
-// rows, the first tile and the way out (128 x 196 x 4096: 35 us and 8 us to join two runs an image).
+// rows, the first tile and the way out (128 x 196 x 4096: 36 us and 8 us to join two runs an image).
 template <bool BWD, bool OPENS>
 __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
   constexpr int QM = 8, CPW = 4, NST = MX_STAGES, REC = 1024;          // REC: bytes of an exchange record, the lane's four scores
@@ -1184,8 +1185,8 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   constexpr int LDS = 160 * 1024;
   int cap;                                                              // workgroups that run at the same time
   if (nc <= 14) {                                                       // a wave per block and the weight wave: what 160 KiB of LDS hold.
-    // (512 x 256 x 1792, 8 queries: 42 us forward and 60 backward; wide-row form 50 and 63.  Narrower rows gain more.)  More than 8
-    // queries: blocks of 16 (512 x 256 x 768: 16 queries 30 us forward, as two blocks of 8 43; 8 queries as a block of 16 27, of 8 25.5)
+    // (512 x 256 x 1792, 8 queries: 44 us forward and 60 backward; wide-row form 53 and 64.  Narrower rows gain more.)  More than 8
+    // queries: blocks of 16 (512 x 256 x 768: 16 queries 31 us forward, as two blocks of 8 37; 8 queries as a block of 16 28, of 8 25)
     p.qm = Q <= 8 ? 8 : 16;
     p.nw = nc; p.groups = 1;
     constexpr int waves = 16;                                           // four a SIMD
@@ -1205,11 +1206,11 @@ static MxPlan mx_plan(int B, int N, int D, int Q, bool bwd, bool per_image) {
   p.yblk = (Q + p.qm - 1) / p.qm;
   p.qblk = (Q + p.yblk - 1) / p.yblk;
   // ... for each block of queries: a second round of workgroups would make its operands and fill its ring once more (256 x 196 x 1024, 32
-  // queries: 36.7 us forward instead of 42.4, 48.6 backward instead of 51)
+  // queries: 36 us forward instead of 43, 50 backward instead of 58)
   cap = cap / p.yblk > 1 ? cap / p.yblk : 1;
   // few images: their token axis is cut into runs of at least `least` tiles.  Forward the runs have to be joined by a second launch, so
-  // they are kept longer (64 x 257 x 768, 8 queries: 8 tiles 17 us, 4 22 us); backward every run opens its operand rows (128 x 196 x
-  // 768: 4 tiles 19 us, 2 25 us), which wide rows still gain from (128 x 196 x 4096: 2 tiles 40 us, 4 49 us)
+  // they are kept longer (64 x 257 x 768, 8 queries: 8 tiles 15.8 us, 4 17 us); backward every run opens its operand rows (128 x 196 x
+  // 768: 4 tiles 20 us, 2 25 us), which wide rows still gain from (128 x 196 x 4096: 2 tiles 40 us, 4 49 us)
   const int per = p.pipe ? 1 : p.groups, least = p.pipe ? (bwd ? 4 : 8) : (bwd ? 2 : 2 * per);
   p.splits = B < cap * (bwd ? per : 1) ? (cap * (bwd ? per : 1)) / B : 1;
   if (p.splits > tiles / least) p.splits = tiles / least;
@@ -1266,7 +1267,7 @@ int mx4_pool_forward(const ep_mx4_tokens* t, const float* queries, int64_t q_bst
   p.lds_ = s_stride;
   EP_TRY(mx_launch<false>(p, pl, st));
   if (pl.splits > 1) {
-    // few runs: one chain (128 x 196 x 4096, two runs: 41 us in all, sixteen chains 70); many: sixteen (2 x 50001 x 1024: 34 us, one 86)
+    // few runs: one chain (128 x 196 x 4096, two runs: 41 us in all, sixteen chains 70); many: sixteen (2 x 50001 x 1024: 43 us, one 83)
     if (pl.splits <= 4)
       hipLaunchKernelGGL(ep_mx4_join_kernel<1>, dim3((unsigned)t->B * Q, (unsigned)((t->D + 1023) / 1024)), dim3(256), 0, st, p.part, p.part_ml, pl.splits, Q, t->D, P, ML);
     else
