@@ -329,13 +329,14 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
     *reinterpret_cast<mx_u4*>(opsc + ln * 16) = mx_u4{sc[0], sc[1], sc[2], sc[3]};
     return BWD && prows ? mx_over_groups_sum(sum + mx_ror8(sum)) : 0.f;
   };
-  float delta = 0.f, m_run, mz, l_run, t_max, invl;                     // mz: the maximum that weights are taken against
+  float delta = 0.f, m_run, l_run, t_max, invl;                         // m_run: what weights are taken against (-inf: no token yet)
+  auto base = [](float m) { return m == -INFINITY ? 0.f : m; };
   auto open_unit = [&](int b) {                                         // backward: dP's rows and the saved statistics
     delta = load_operand(p.q + (int64_t)b * p.Q * t.D, p.Pin ? p.Pin + (int64_t)b * p.Q * t.D : nullptr, 1.f);
     const int q = mx_fresh(lane) & 7;
     f4 ml = {0.f, 0.f, 0.f, 0.f};
     if (q < qn) ml = *reinterpret_cast<const f4*>(p.ML + ((int64_t)b * p.Q + q0 + q) * 4);
-    mz = ml.x;
+    m_run = ml.x;
     invl = ml.y == 0.f ? 0.f : 1.f / ml.y;
     if (!p.Pin && dw == 0) delta = ml.z;                                // (each D-slice takes off its own part of delta)
   };
@@ -425,15 +426,14 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
           const float mn = fmaxf(m_run, mx);
           const float f = mn == m_run ? 1.f : __builtin_amdgcn_exp2f((m_run - mn) * MX_LOG2E);
           m_run = mn;
-          mz = mn == -INFINITY ? 0.f : mn;
           l_run *= f;
           scale_rows(f);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { pv[i] = __builtin_amdgcn_exp2f((s[i] - mz) * MX_LOG2E); l_run += pv[i]; }
+        for (int i = 0; i < 4; ++i) { pv[i] = __builtin_amdgcn_exp2f((s[i] - base(m_run)) * MX_LOG2E); l_run += pv[i]; }
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pv[i] = __builtin_amdgcn_exp2f((sg[i] - mz) * MX_LOG2E) * invl * s[i];
+        for (int i = 0; i < 4; ++i) pv[i] = __builtin_amdgcn_exp2f((sg[i] - m_run) * MX_LOG2E) * invl * s[i];
         if (tail) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) pv[i] = t0 + tok0 + i < len ? pv[i] : 0.f;
@@ -569,7 +569,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
       const int img = mx_image_uniform(t, b, len);
       const int n = (len + 31) >> 5, lo = sp * p.tps, hi = (sp + 1) * p.tps < n ? (sp + 1) * p.tps : n;
       if constexpr (OPENS) load_operand(p.q + (int64_t)b * p.qb, nullptr, p.scale);
-      m_run = t_max = -INFINITY; mz = l_run = 0.f;
+      m_run = t_max = -INFINITY; l_run = 0.f;
       clear();
       int tl = lo;
       for (; tl + grp < hi; tl += groups) {
@@ -601,7 +601,6 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
         const float own = m_run == M ? 1.f : __builtin_amdgcn_exp2f((m_run - M) * MX_LOG2E);
         scale_rows(own);
         m_run = M; l_run = l; t_max = T;
-        mz = M == -INFINITY ? 0.f : M;
         mx_barrier();                                                   // (the records are read: they carry accumulators next)
         add_groups();
       }
@@ -609,7 +608,7 @@ __global__ __launch_bounds__(512, 2) void ep_mx4_wide_kernel(MxPool p) {
         const float bad = img < 0 ? __uint_as_float(0x7fc00000u) : 0.f;
         const bool none = t_max == -INFINITY && l_run == 0.f;                                 // no token
         const float m = none ? (p.splits > 1 ? -INFINITY : 0.f) : t_max;
-        const float e = none ? 0.f : __builtin_amdgcn_exp2f((mz - m) * MX_LOG2E);             // from the running to the true maximum
+        const float e = none ? 0.f : __builtin_amdgcn_exp2f((base(m_run) - m) * MX_LOG2E);             // from the running to the true maximum
         if (dw == 0 && g == 0 && c < 8 && c < qn) {
           if (p.splits > 1) *reinterpret_cast<f2*>(p.part_ml + ((int64_t)u * p.Q + q0 + c) * 2) = f2{m + bad, l_run * e + bad};
           else *reinterpret_cast<f4*>(p.ML + ((int64_t)b * p.Q + q0 + c) * 4) = f4{m + bad, l_run * e + bad, 0.f, 0.f};
