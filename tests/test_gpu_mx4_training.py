@@ -389,3 +389,37 @@ def test_two_streams_at_once():
     for k in range(2):
         for P, dq in got[k]:
             assert torch.equal(P, want[k][0]) and torch.equal(dq, want[k][1])
+
+
+def test_ragged_images_through_disk_and_stream(tmp_path):
+    """Images of fewer tokens: written on the GPU, read back resident and as a stream (whose buffers are used in turn), one epoch each on the
+    same batches, and an epoch through the modules (a clipping bound), whose backward pass reads the stream's buffers again."""
+    from efficient_probing_amd import engine_finetune as EF, token_store as TS
+    from efficient_probing_amd.util.lars import LARS
+    from efficient_probing_amd.util.misc import NativeScalerWithGradNormCount
+    g = torch.Generator().manual_seed(0)
+    n, N, D, C = 64, 11, 200, 6
+    x, lab, ln = torch.randn(n, N, D, generator=g), torch.randint(0, C, (n,), generator=g), torch.randint(0, N + 1, (n,), generator=g)
+    w = TS.TokenStoreWriter(str(tmp_path), N, D, shard_images=32, dtype="mxfp4")
+    for lo in range(0, n, 24):
+        w.add(x[lo:lo + 24].to(DEV) if lo else x[lo:lo + 24].numpy(), lab[lo:lo + 24], lengths=ln[lo:lo + 24])
+    w.close()
+    store = TS.ResidentTokenStore(str(tmp_path), torch.device(DEV))
+    stream = TS.StreamingTokenLoader(str(tmp_path), torch.device(DEV), batch_size=8)
+    assert torch.equal(store.tokens.lengths.cpu(), ln.to(torch.int32)) and len(stream) == 8
+    for k, (b, t) in enumerate(stream):
+        assert torch.equal(b.codes, store.tokens.codes[8 * k:8 * k + 8]) and torch.equal(b.lengths.cpu(), ln[8 * k:8 * k + 8].to(torch.int32)) and torch.equal(t.cpu(), lab[8 * k:8 * k + 8])
+    heads = []
+    for loader, kw in ((store.loader(8, shuffle=False), {}), (stream, {}), (stream, dict(max_norm=1e9))):
+        m = _model(D, C)
+        opt = LARS(m.head.parameters(), lr=0.1, weight_decay=0.0)
+        args = Namespace(lr=0.1, min_lr=0.0, warmup_epochs=0, epochs=4, accum_iter=1, amp="none")
+        EF.train_one_epoch(m, torch.nn.CrossEntropyLoss(), loader, opt, torch.device(DEV), 0, NativeScalerWithGradNormCount() if kw else None, args=args, **kw)
+        heads.append(m)
+    start = _model(D, C)
+    for p, q in zip(heads[0].head.parameters(), heads[1].head.parameters()):
+        assert torch.equal(p, q)
+    for p, q, s in zip(heads[2].head.parameters(), heads[0].head.parameters(), start.head.parameters()):
+        assert (p - q).norm() <= 8192 * U * max((q - s).norm(), 1e-3 * q.norm())
+    ev = [EF.evaluate(ld, heads[0], torch.device(DEV)) for ld in (store.loader(8, shuffle=False, drop_last=False), stream)]
+    assert ev[0]["loss"] == ev[1]["loss"] and ev[0]["acc1"] == ev[1]["acc1"]
