@@ -327,6 +327,8 @@ def train_one_epoch(model: torch.nn.Module, criterion: torch.nn.Module, data_loa
     for step, batch in enumerate(metric_logger.log_every(data_loader, print_freq, header)):
         samples, targets = batch[0], batch[-1]
         image_index = rows = batch[1] if isinstance(batch, StoreBatch) else None      # resident token store, read in place
+        if distill and rows is None:
+            raise ValueError("TopKDistillation needs each batch's image_index (batches of a token_store.ResidentTokenStore carry it)")
         _attach_store(engine, batch)
         if step % accum_iter == 0:
             lr = lr_sched.adjust_learning_rate(optimizer, step / n_iter + epoch, args)

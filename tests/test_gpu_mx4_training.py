@@ -423,3 +423,19 @@ def test_ragged_images_through_disk_and_stream(tmp_path):
         assert (p - q).norm() <= 8192 * U * max((q - s).norm(), 1e-3 * q.norm())
     ev = [EF.evaluate(ld, heads[0], torch.device(DEV)) for ld in (store.loader(8, shuffle=False, drop_last=False), stream)]
     assert ev[0]["loss"] == ev[1]["loss"] and ev[0]["acc1"] == ev[1]["acc1"]
+
+
+def test_a_teacher_table_needs_the_images_of_a_batch():
+    """A loader whose batches carry no image_index, with a batch as large as the table: which row belongs to which image is not known."""
+    from efficient_probing_amd import distill, mx4
+    store = _store(16, 9, 128, 7)
+    x = mx4.dequantize_tokens(store.tokens, torch.float32)
+    order = torch.randperm(16, generator=torch.Generator().manual_seed(1)).to(DEV)
+
+    class Shuffled(list):
+        def loader(self, *a, **k):
+            return self
+    for batch in ((x[order], store.labels[order]), (store.tokens.select(order.to(torch.int32)), store.labels[order])):
+        for head in ("ep", "simpool"):
+            with pytest.raises(ValueError, match="image_index"):
+                _epoch(_model(128, 7, head=head, num_heads=4), Shuffled([batch]), distill.TopKDistillation.from_store(store))
