@@ -118,7 +118,7 @@ __device__ __forceinline__ void mx_terms(mx_f16 a, mx_f16 b, F&& take) {        
   }
   const int ex = (int)(am >> 23);
   const bool bad = ex == 255;
-  const int s0 = bad ? 252 : (ex <= 5 * TERMS ? 5 * TERMS : ex - 1);      // (every term's scale is a normal number: what is lost is at least 2^-126)
+  const int s0 = bad ? 252 : (ex <= 5 * TERMS ? 5 * TERMS : ex - 1);      // (every term has a normal scale: below 2^-91 a row keeps what lies above 2^-126)
 #pragma unroll
   for (int t = 0; t < TERMS; ++t) {
     const float sc = __uint_as_float((uint32_t)(s0 - 5 * t) << 23);
